@@ -49,7 +49,7 @@
 extern "C" {
 #endif
 
-#define FA_ABI_VERSION 8
+#define FA_ABI_VERSION 9
 
 /* Error codes returned before any HIP call is made. */
 #define FA_OK 0
@@ -367,6 +367,112 @@ int fa_fwd_noalloc(const fa_half_t* q, const fa_half_t* k, const fa_half_t* v,
                    float scale, int causal, void* stream);
 /* Bytes of the device array fa_fwd_noalloc uses (the largest workspace it serves). */
 int64_t fa_fwd_noalloc_max_workspace_bytes(void);
+
+/* ---- The operators around the attention call ------------------------------------------
+ * No counterpart in the reference. Conventions as above, except where said: tensors may be
+ * strided (strides in elements, multiples of 8 for 16-bit tensors, whose last dimension is
+ * contiguous), head sizes D are multiples of 8 up to 128, and what page tables, lengths,
+ * slots and positions hold is read and checked on the GPU. */
+
+#define FA_ROPE_INTERLEAVED 1     /* pairs are the values 2 i and 2 i + 1, not i and i + R / 2 */
+#define FA_ROPE_WEIGHT_F32 2      /* norm weights (and their gradients) are float32            */
+#define FA_ROPE_POSITIONS_I64 4   /* positions are int64, not int32                            */
+
+/* RMS norm of each head's queries and keys and rotation by position, in one launch:
+ *   y = x / sqrt(mean(x^2) + eps) * weight   (y = x when both weights are NULL)
+ *   q_out, k_out = y with its first R values rotated in pairs by the token's R / 2 angles
+ * q, q_out: [B, Hq, N, D]; k, k_out: [B, Hkv, N, D]; the outputs are contiguous. cos, sin:
+ * float32 [P, R / 2], contiguous; R a multiple of 16 up to D. positions [B, N]: the row of cos
+ * and sin of each token, or NULL for 0 .. N - 1; a token whose position is not in [0, P) has
+ * NaN for its rows. Weights [D]: of the element type or float32. `strides` holds the batch,
+ * head and row stride of q, those of k, and the batch and token stride of positions. Arithmetic
+ * in float32, rounded once. */
+int fa_qk_norm_rope(const fa_half_t* q, const fa_half_t* k, fa_half_t* q_out, fa_half_t* k_out,
+                    const float* cos, const float* sin, const void* positions,
+                    const void* q_weight, const void* k_weight, const int64_t* strides,
+                    int64_t B, int64_t Hq, int64_t Hkv, int64_t N, int64_t D, int64_t R,
+                    int64_t P, float eps, int flags, void* stream);
+int fa_qk_norm_rope_bf16(const fa_half_t* q, const fa_half_t* k, fa_half_t* q_out,
+                         fa_half_t* k_out, const float* cos, const float* sin,
+                         const void* positions, const void* q_weight, const void* k_weight,
+                         const int64_t* strides, int64_t B, int64_t Hq, int64_t Hkv, int64_t N,
+                         int64_t D, int64_t R, int64_t P, float eps, int flags, void* stream);
+
+/* Its backward: gq, gk the gradients of q_out, k_out; dq, dk (contiguous) those of q, k, and
+ * dq_weight, dk_weight [D] those of the weights, each of which may be NULL to leave it out.
+ * Without weights q and k are not read and may be NULL. `strides` holds the batch, head and row
+ * stride of gq, gk, q and k, and the batch and token stride of positions. The weights' gradients
+ * are fp32 sums in a fixed order over a workspace of fa_qk_norm_rope_bwd_workspace_bytes
+ * (needed for them only); concurrent calls need separate workspaces. */
+int64_t fa_qk_norm_rope_bwd_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t N,
+                                            int64_t D);
+int fa_qk_norm_rope_bwd(const fa_half_t* gq, const fa_half_t* gk, const fa_half_t* q,
+                        const fa_half_t* k, fa_half_t* dq, fa_half_t* dk, void* dq_weight,
+                        void* dk_weight, const float* cos, const float* sin,
+                        const void* positions, const void* q_weight, const void* k_weight,
+                        const int64_t* strides, int64_t B, int64_t Hq, int64_t Hkv, int64_t N,
+                        int64_t D, int64_t R, int64_t P, float eps, int flags, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+int fa_qk_norm_rope_bwd_bf16(const fa_half_t* gq, const fa_half_t* gk, const fa_half_t* q,
+                             const fa_half_t* k, fa_half_t* dq, fa_half_t* dk, void* dq_weight,
+                             void* dk_weight, const float* cos, const float* sin,
+                             const void* positions, const void* q_weight, const void* k_weight,
+                             const int64_t* strides, int64_t B, int64_t Hq, int64_t Hkv,
+                             int64_t N, int64_t D, int64_t R, int64_t P, float eps, int flags,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/* A paged key/value cache: pages of S tokens (a multiple of 16), k_cache and v_cache
+ * [pages, H, S, D] with one layout (page, head and row stride). Token p of sequence b lies in
+ * row p % S of page page_table[b, p / S]; its slot is page * S + p % S.
+ *
+ * fa_paged_plan places a step's new tokens: sequence b holds lengths[b] tokens and gets
+ * new_tokens[b] more (both below 2^30; negative ones count as 0). Pages come from
+ * free_pages[F], from place free_start[0] on (NULL: 0), in the order of the sequences. Writes
+ * the new pages' entries of page_table [B, M] (rows table_stride apart; no other entry), and
+ *   slots, positions [T]  of the tokens in the order of the sequences; slot -1 and position 0
+ *                         behind the last one
+ *   starts [B + 1]        a sequence's first token, and their number
+ *   lengths_out [B]       lengths + new_tokens
+ *   free_start_out [1]    the place behind the last page taken
+ * Tokens past T get neither a slot nor a page table entry. When the free pages run out, the
+ * entries of the missing ones are -1 and so are their tokens' slots (free_start_out counts them:
+ * it is above F); tokens behind a sequence's M pages have slot -1. The outputs must not overlap
+ * the inputs. */
+int fa_paged_plan(int32_t* page_table, int64_t table_stride, const int32_t* lengths,
+                  const int32_t* new_tokens, const int32_t* free_pages, const int32_t* free_start,
+                  int64_t* slots, int32_t* positions, int32_t* starts, int32_t* lengths_out,
+                  int32_t* free_start_out, int64_t B, int64_t M, int64_t S, int64_t F, int64_t T,
+                  void* stream);
+
+/* Rows t of key and value [T, H, D] (16-bit elements of any type) into slots[t] of the caches;
+ * slots that are negative or behind the last page are left out. The other slots must differ
+ * from each other. `strides`: token and head stride of key, those of value, and page, head and
+ * row stride of the caches. */
+int fa_paged_store(const fa_half_t* key, const fa_half_t* value, fa_half_t* k_cache,
+                   fa_half_t* v_cache, const int64_t* slots, const int64_t* strides, int64_t T,
+                   int64_t H, int64_t D, int64_t pages, int64_t S, void* stream);
+
+/* Attention of the newest N tokens of each sequence over the cache, o = softmax(scale q K^T) V:
+ * lengths[b] counts the cached tokens, the N ones of q [B, Hq, N, D] included, and query n sees
+ * keys j <= lengths[b] - N + n (the last query sees all: a causal mask from the end, unlike the
+ * top-left one above). Rows that see no key are 0. A sequence whose length is not in [0, M * S],
+ * or of whose pages one is not in [0, pages), has NaN for its rows. o [B, Hq, N, D] is
+ * contiguous. `strides`: batch, head and row stride of q, page, head and row stride of the
+ * caches, and the row stride of page_table. The workspace (fa_paged_fwd_workspace_bytes) holds
+ * partial results of key ranges, fp32; they are joined in a fixed order, so results do not vary
+ * from call to call. Concurrent calls need separate workspaces. */
+int64_t fa_paged_fwd_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t N, int64_t D,
+                                     int64_t M, int64_t S);
+int fa_paged_fwd(const fa_half_t* q, const fa_half_t* k_cache, const fa_half_t* v_cache,
+                 const int32_t* page_table, const int32_t* lengths, fa_half_t* o,
+                 const int64_t* strides, int64_t B, int64_t Hq, int64_t Hkv, int64_t N,
+                 int64_t D, int64_t pages, int64_t M, int64_t S, float scale, void* workspace,
+                 int64_t workspace_bytes, void* stream);
+int fa_paged_fwd_bf16(const fa_half_t* q, const fa_half_t* k_cache, const fa_half_t* v_cache,
+                      const int32_t* page_table, const int32_t* lengths, fa_half_t* o,
+                      const int64_t* strides, int64_t B, int64_t Hq, int64_t Hkv, int64_t N,
+                      int64_t D, int64_t pages, int64_t M, int64_t S, float scale,
+                      void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Thread-local description of the last failure on the calling thread
  * ("" if none). The pointer stays valid until the next call on the thread. */

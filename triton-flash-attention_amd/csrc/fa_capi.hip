@@ -18,6 +18,7 @@
 
 #include "../../include/fa_gfx950.h"
 #include "fa_kernels.hpp"
+#include "fa_layer.hpp"
 
 // Device-resident scratch of fa_fwd_noalloc: the split-KV forward's fp32
 // partials ([nsplit, B, Hq, N_q, D + 1]) for callers that cannot allocate.
@@ -54,6 +55,20 @@ int launch_result(hipError_t e, const char* name) {
   if (e == hipSuccess) return hip_result(e, name);
   return fail((int)e, "%s launch: %s (hipError %d)", name, hipGetErrorString(e), (int)e);
 }
+
+}  // namespace
+
+// The same for the entry points of fa_capi_layer.hip.
+int fa::capi_fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
+  va_end(ap);
+  return code;
+}
+int fa::capi_launch_result(hipError_t e, const char* name) { return launch_result(e, name); }
+
+namespace {
 
 // Process-wide tiling choice per (kernel, D index, causal); -1 = table default.
 // fa_set_tiling may run on one thread while others launch: every entry is an

@@ -1,0 +1,707 @@
+// fa_paged.hip — the paged key/value cache (gfx950): pages and slots of a step's new tokens
+// (paged_plan_kernel), their keys and values into the cache (paged_store_kernel), and the
+// attention of new tokens over it (paged_fwd_kernel, paged_join_kernel).
+//
+// The cache holds pages of S tokens (a multiple of 16), [pages, Hkv, S, d]; a sequence's tokens
+// 0, 1, ... lie in the pages that its row of the page table names. What the tables, lengths,
+// slots and positions hold is on the GPU and is checked here, entry by entry, before an address
+// is made of it.
+#include <algorithm>
+
+#include "fa_common.hpp"
+#include "fa_layer.hpp"
+
+namespace fa {
+
+namespace {
+
+// Inclusive sum over the lanes of a wave, up to this one.
+template <class T>
+__device__ __forceinline__ T wave_scan(T x, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const T y = __shfl_up(x, d, 64);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
+
+// Sum over the threads before this one of a block of 256, and the block's total. `sums` holds
+// one value a wave; ends with every thread past the barrier that publishes them.
+template <class T>
+__device__ __forceinline__ T block_scan(T x, T* sums, T* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const T incl = wave_scan(x, lane);
+  if (lane == 63) sums[wave] = incl;
+  __syncthreads();
+  T before = incl - x, all = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < wave) before += sums[w];
+    all += sums[w];
+  }
+  *total = all;
+  return before;
+}
+
+}  // namespace
+
+// ---- plan -------------------------------------------------------------------------------
+// Sequence b holds len_b tokens in ceil(len_b / S) pages and gets new_b more: the pages that
+// these need come from the list of free ones, in the order of the sequences, so two running
+// sums over the sequences place everything: of new tokens (a token's row in the step) and of
+// new pages. Every block takes kPlanTokens tokens and computes the running sums itself, 1024
+// sequences at a time in LDS, then finds each token's sequence by bisection: one launch, and
+// no block waits for another. The first token on a new page writes the page's table entry.
+// A step's plan is bound by its chain of loads (lengths, then page ids), a prompt's by writing
+// 12 bytes a token.
+constexpr int kPlanSeqs = 1024;
+constexpr int kPlanTokens = 1024;
+constexpr int kPlanMost = (1 << 30) - 1;  // largest length and number of new tokens
+
+__global__ __launch_bounds__(256) void paged_plan_kernel(PlanArgs a) {
+  __shared__ int64_t first[kPlanSeqs];  // a sequence's first token in the step
+  __shared__ int64_t page0[kPlanSeqs];  // its first new page's place in the free list
+  __shared__ int length[kPlanSeqs];
+  __shared__ int64_t sums[2][4];
+  const int tid = threadIdx.x;
+  const bool head = blockIdx.x == 0;
+  const int64_t t0 = (int64_t)blockIdx.x * kPlanTokens;
+  const int64_t t1 = min(a.T, t0 + kPlanTokens);
+  int64_t tokens = 0;                                  // before this group of sequences
+  int64_t pages = a.free_start ? a.free_start[0] : 0;  // place of its first new page
+  for (int b0 = 0; b0 < a.B; b0 += kPlanSeqs) {
+    if (tokens >= t1 && !head) return;  // the rest belongs to later blocks
+    int len[4], add[4], need[4];
+    int64_t n = 0, g = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int b = b0 + 4 * tid + i;
+      len[i] = add[i] = need[i] = 0;
+      if (b < a.B) {
+        len[i] = min(max(a.lengths[b], 0), kPlanMost);
+        add[i] = min(max(a.new_tokens[b], 0), kPlanMost);
+        const int held = (int)(((unsigned)len[i] + a.S - 1) / a.S);
+        const int then = (int)(((unsigned)(len[i] + add[i]) + a.S - 1) / a.S);
+        need[i] = max(min(then, a.M) - held, 0);  // a row of the table holds M pages
+      }
+      n += add[i];
+      g += need[i];
+    }
+    int64_t n_all, g_all;
+    int64_t n_at = tokens + block_scan(n, sums[0], &n_all);
+    int64_t g_at = pages + block_scan(g, sums[1], &g_all);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int b = b0 + 4 * tid + i;
+      first[4 * tid + i] = n_at;
+      page0[4 * tid + i] = g_at;
+      length[4 * tid + i] = len[i];
+      if (head && b < a.B) {
+        a.starts[b] = (int)min(n_at, (int64_t)INT32_MAX);
+        a.lengths_out[b] = len[i] + add[i];
+      }
+      n_at += add[i];
+      g_at += need[i];
+    }
+    __syncthreads();
+    const int64_t end = min(t1, tokens + n_all);
+    for (int64_t t = max(t0, tokens) + tid; t < end; t += 256) {
+      int lo = 0, hi = kPlanSeqs;  // the last sequence with first <= t holds it
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first[mid] <= t) lo = mid;
+        else hi = mid;
+      }
+      const int pos = length[lo] + (int)(t - first[lo]);
+      const int j = pos / a.S, held = (int)(((unsigned)length[lo] + a.S - 1) / a.S);
+      int page = -1;
+      if (j < a.M) {
+        int* entry = a.table + (int64_t)(b0 + lo) * a.table_stride + j;
+        if (j < held) {
+          page = *entry;
+        } else {
+          const int64_t at = page0[lo] + (j - held);
+          if (at >= 0 && at < a.F) page = a.free_pages[at];
+          if (pos == j * a.S) *entry = page;
+        }
+      }
+      a.slots[t] = page < 0 ? -1 : (int64_t)page * a.S + (pos - j * a.S);
+      a.positions[t] = pos;
+    }
+    tokens += n_all;
+    pages += g_all;
+    __syncthreads();
+  }
+  for (int64_t t = max(t0, tokens) + tid; t < t1; t += 256) {  // padding
+    a.slots[t] = -1;
+    a.positions[t] = 0;
+  }
+  if (head && tid == 0) {
+    a.starts[a.B] = (int)min(tokens, (int64_t)INT32_MAX);
+    a.free_out[0] = (int)min(max(pages, (int64_t)0), (int64_t)INT32_MAX);
+  }
+}
+
+hipError_t launch_paged_plan(const PlanArgs& a, hipStream_t stream) {
+  const int64_t blocks = std::max<int64_t>(1, (a.T + kPlanTokens - 1) / kPlanTokens);
+  if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+  hipLaunchKernelGGL(paged_plan_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+// ---- store ------------------------------------------------------------------------------
+// Row t of the keys and values to slot t's row of every head: a copy in 16-byte pieces, bound
+// by memory. W neighbouring threads share a token and walk over its 2 H chunks pieces; each
+// thread has kStoreTokens tokens in flight. Slots outside the cache are left out.
+constexpr int kStoreTokens = 4;
+
+template <int W>
+__global__ __launch_bounds__(256) void paged_store_kernel(StoreArgs a) {
+  constexpr int TPP = 256 / W;  // tokens of a pass
+  const int item = threadIdx.x % W;
+  const int64_t t0 = (int64_t)blockIdx.x * (TPP * kStoreTokens) + threadIdx.x / W;
+  int64_t page[kStoreTokens];
+  int row[kStoreTokens];
+#pragma unroll
+  for (int i = 0; i < kStoreTokens; ++i) {
+    const int64_t t = t0 + i * TPP;
+    const int64_t slot = t < a.T ? a.slots[t] : -1;
+    page[i] = slot < 0 || slot >= a.pages * a.S ? -1 : slot / a.S;
+    row[i] = (int)(slot - page[i] * a.S);
+  }
+  const int per_side = a.H * a.chunks;
+  for (int p = item; p < 2 * per_side; p += W) {
+    const int side = p >= per_side;
+    const int r = p - side * per_side;
+    const int h = r / a.chunks, c = r - h * a.chunks;
+    const half_t* src = a.src[side] + h * a.ss[side][1] + 8 * c;
+    half_t* dst = a.dst[side] + h * a.ds[1] + 8 * c;
+    u32x4 v[kStoreTokens];
+#pragma unroll
+    for (int i = 0; i < kStoreTokens; ++i)
+      if (page[i] >= 0)
+        v[i] = *reinterpret_cast<const u32x4*>(src + (t0 + i * TPP) * a.ss[side][0]);
+#pragma unroll
+    for (int i = 0; i < kStoreTokens; ++i)
+      if (page[i] >= 0)
+        *reinterpret_cast<u32x4*>(dst + page[i] * a.ds[0] + row[i] * a.ds[2]) = v[i];
+  }
+}
+
+hipError_t launch_paged_store(const StoreArgs& a, hipStream_t stream) {
+  const int pieces = 2 * a.H * a.chunks;
+  const int W = pieces > 128 ? 256 : pieces > 64 ? 128 : pieces > 32 ? 64 : 32;
+  const int64_t tokens = 256 / W * kStoreTokens;
+  const int64_t blocks = (a.T + tokens - 1) / tokens;
+  if (blocks <= 0 || blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+  const dim3 grid((unsigned)blocks), block(256);
+  switch (W) {
+    case 256: hipLaunchKernelGGL(paged_store_kernel<256>, grid, block, 0, stream, a); break;
+    case 128: hipLaunchKernelGGL(paged_store_kernel<128>, grid, block, 0, stream, a); break;
+    case 64: hipLaunchKernelGGL(paged_store_kernel<64>, grid, block, 0, stream, a); break;
+    default: hipLaunchKernelGGL(paged_store_kernel<32>, grid, block, 0, stream, a); break;
+  }
+  return hipGetLastError();
+}
+
+// ---- attention --------------------------------------------------------------------------
+// o = softmax(scale q K^T) V of the group * N query rows that read one key/value head, in
+// blocks of 16 rows (one MFMA block): query n of a sequence of len keys sees keys
+// j <= len - N + n. K and V are read once a row block and next to nothing is computed, so
+// what bounds the kernel is the bytes in flight.
+//
+// Work is dealt by units of 32 keys. The units of all (sequence, head, row block) triples lie
+// on one line, each triple's together; the grid is what the chip holds at once, and every
+// work-group takes an equal stretch of that line, found from the lengths on the GPU (the call
+// reads no length on the host, so it can be captured). A stretch covers whole triples, which
+// are written as they end, and at most one piece at each end of a triple that it shares with
+// its neighbours: those go to the workspace as a normalised partial O and a base-2 log-sum-exp,
+// and paged_join_kernel joins them. Sequences of any mix of lengths load the chip evenly.
+//
+// Within a stretch a work-group's four waves take every fourth unit, each on its own, and
+// merge through LDS at the end of a piece. K and V of the next unit are on their way to a
+// wave's registers while it works on one (16 KiB a wave at D = 128); K rows come in the layout
+// of the MFMA operand, V rows go through a tile in LDS for the transposing reads. A page holds a multiple of 16 tokens, so each half unit of 16
+// keys lies in one page and is read through a buffer descriptor of its own, made of its page's
+// 64-bit address, with the half's rows that exist as its range: rows past the length read
+// zeros and never reach memory. The pages of a wave's next 32 units are kept one a lane.
+//
+// MFMA layouts (16x16x32, lane l, c16 = l % 16, G = l / 16) as in fa_fwd_decode.hip:
+//   S^T block kb: lane holds row c16 and keys 16 kb + 4 G + j of the unit;
+//   O^T block dd: lane holds row c16, d = 16 dd + 4 G + j.
+// Row r of the triple is query r % N of the group's head r / N.
+
+// A row's probabilities are taken against a reference max that moves only when their sum over
+// a unit exceeds this, far below where fp16 ends.
+constexpr float kPagedSumLimit = 256.0f;
+
+template <int D>
+struct PagedTile {
+  static constexpr int NW = 4;
+  static constexpr int KD = D / 32, DD = D / 16;
+  static constexpr int TILE = kPagedUnit * D;          // halves of a unit's K (or V) rows
+  static constexpr int VI = TILE * 2 / 1024;           // 1 KiB loads of a unit's V
+  static constexpr int VROWS = 512 / D;                // rows of one of them
+};
+
+namespace {
+
+// Units of one (head, row block) of a sequence: at least one, which writes the rows of an
+// empty sequence. A length that the table cannot hold has one unit too, marked bad.
+__device__ __forceinline__ int paged_units(const PagedArgs& a, int len) {
+  return len > 0 && len <= a.M * a.S ? (len + kPagedUnit - 1) / kPagedUnit : 1;
+}
+
+// A place on the line of units: unit `unit` of triple `triple` (head-major) of sequence `b`.
+struct PagedPlace {
+  int b, triple, unit;
+};
+
+// The line's length, and the place of its unit `at` (defined where at < the length). `want`
+// is computed from the length. Ends with a barrier.
+template <class Want>
+__device__ __forceinline__ int paged_find(const PagedArgs& a, int* lds, PagedPlace* place,
+                                          Want want) {
+  const int HB = a.Hkv * a.blocks;
+  const int per = (a.B + 255) / 256;
+  const int b0 = threadIdx.x * per, b1 = min(a.B, b0 + per);
+  int mine = 0;
+  for (int b = b0; b < b1; ++b) mine += paged_units(a, a.lengths[b]) * HB;
+  int total;
+  const int before = block_scan(mine, lds, &total);
+  const int at = want(total);
+  if (at >= before && at < before + mine) {
+    int rest = at - before, b = b0, units = 1;
+    for (; b < b1; ++b) {
+      units = paged_units(a, a.lengths[b]);
+      if (rest < units * HB) break;
+      rest -= units * HB;
+    }
+    lds[4] = b;
+    lds[5] = rest / units;
+    lds[6] = rest % units;
+  }
+  __syncthreads();
+  place->b = uniform(lds[4]);
+  place->triple = uniform(lds[5]);
+  place->unit = uniform(lds[6]);
+  return total;
+}
+
+// Units of a work-group's stretch: a multiple of the four waves.
+__device__ __forceinline__ int paged_stretch(int total, int grid) {
+  return ((total + grid - 1) / grid + 3) / 4 * 4;
+}
+
+// A wave's units of a piece: where the half units of its next 32 units lie, one a lane
+// (lane 2 k + half for unit k).
+struct PagedHalves {
+  uint32_t lo, hi;  // byte offset of the half's first row from its head's rows in page 0
+  int rows;         // rows that exist
+};
+
+}  // namespace
+
+template <int D, class E>
+__global__ __launch_bounds__(256, 2) void paged_fwd_kernel(PagedArgs a) {
+  using T = PagedTile<D>;
+  constexpr int KD = T::KD, DD = T::DD, NW = T::NW;
+  constexpr int LDS_FLOATS = NW * DD * 256 + 2 * NW * kPagedRows;
+  static_assert(NW * T::TILE * 2 <= LDS_FLOATS * 4, "the V tiles and the merge share it");
+  __shared__ __attribute__((aligned(16))) float lds[LDS_FLOATS];
+  __shared__ int find[8];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = uniform(tid >> 6);
+  const int c16 = lane & 15;
+  const int G = lane >> 4;
+
+  PagedPlace at;
+  int stretch = 0;
+  const int total = paged_find(a, find, &at, [&](int n) __attribute__((always_inline)) {
+    stretch = paged_stretch(n, a.grid);
+    return (int)min((int64_t)blockIdx.x * stretch, (int64_t)n);
+  });
+  const int64_t x0 = (int64_t)blockIdx.x * stretch;
+  if (x0 >= total) return;
+  int left = min(stretch, (int)(total - x0));
+  bool opening = true;  // the stretch's first piece
+
+  half_t* const vt = reinterpret_cast<half_t*>(lds) + wave * T::TILE;
+  const int row_bytes = (int)a.ks[2] * 2;
+  uint32_t k_off[KD], v_off[T::VI], v_at[T::VI];
+#pragma unroll
+  for (int kd = 0; kd < KD; ++kd) {
+    const int col = 32 * kd + 8 * G;
+    k_off[kd] = col < a.d ? (uint32_t)(c16 * row_bytes + col * 2) : kOutOfRange;
+  }
+#pragma unroll
+  for (int i = 0; i < T::VI; ++i) {
+    const int row = i * T::VROWS + lane / (D / 8), chunk = lane % (D / 8);
+    v_off[i] = 8 * chunk < a.d ? (uint32_t)((row & 15) * row_bytes + chunk * 16) : kOutOfRange;
+    v_at[i] = (uint32_t)swz_offset<D>(row, chunk);
+  }
+  int t_off[DD];
+#pragma unroll
+  for (int dd = 0; dd < DD; ++dd) {
+    const int row = 4 * G + (c16 >> 2), col = 16 * dd + 4 * (c16 & 3);
+    t_off[dd] = row * D + 8 * swz_chunk<D>(row, col >> 3) + (col & 7);
+  }
+
+  while (left > 0) {
+    const int len = uniform(a.lengths[at.b]);
+    const bool fits = len >= 0 && len <= a.M * a.S;
+    const int keys = fits ? len : 0;
+    const int units = paged_units(a, len);
+    const int u0 = at.unit, u1 = min(units, u0 + left);
+    const int kvh = at.triple / a.blocks, block = at.triple - kvh * a.blocks;
+    const int rows = a.group * a.N;
+
+    // The lane's row.
+    const int r = block * kPagedRows + c16;
+    const bool row_ok = r < rows;
+    const int h = r / a.N, n = r - h * a.N;
+    // It sees the keys below this. Rows that do not exist score 0 everywhere: masked, they
+    // would move the reference max in every unit.
+    const int see = row_ok ? keys - a.N + n + 1 : INT32_MAX;
+    const int all_see = keys - a.N + 1;               // every row does
+    half8 qf[KD];
+    {
+      const half_t* q = a.q + at.b * a.qs[0] + (int64_t)(kvh * a.group + h) * a.qs[1] + n * a.qs[2];
+#pragma unroll
+      for (int kd = 0; kd < KD; ++kd) {
+        u32x4 v = {0u, 0u, 0u, 0u};
+        const int col = 32 * kd + 8 * G;
+        if (row_ok && col < a.d) v = *reinterpret_cast<const u32x4*>(q + col);
+        qf[kd] = __builtin_bit_cast(half8, v);
+      }
+    }
+
+    // Unit i of the wave is u0 + wave + 4 i.
+    const int mine = u1 - u0 > wave ? (u1 - u0 - wave + NW - 1) / NW : 0;
+    const half_t* const k_head = a.k + kvh * a.ks[1];
+    const half_t* const v_head = a.v + kvh * a.ks[1];
+    bool bad = !fits;
+    // The page of half unit lane & 1 of unit i0 + lane / 2, and from it where that half lies.
+    auto half_key = [&](int i0) __attribute__((always_inline)) {
+      const int i = i0 + (lane >> 1);
+      return i < mine ? (u0 + wave + NW * i) * kPagedUnit + 16 * (lane & 1) : keys;
+    };
+    auto half_page = [&](int i0) __attribute__((always_inline)) {
+      const int key = half_key(i0);
+      return key < keys ? a.table[at.b * a.table_stride + key / a.S] : 0;
+    };
+    auto halves = [&](int i0, int page) __attribute__((always_inline)) {
+      const int key = half_key(i0);
+      PagedHalves p = {0u, 0u, 0};
+      if (key >= keys) return p;
+      if (page < 0 || page >= a.pages) {
+        p.rows = -1;  // no such page
+        return p;
+      }
+      const int64_t off = (page * a.ks[0] + key % a.S * a.ks[2]) * 2;
+      p.lo = (uint32_t)off;
+      p.hi = (uint32_t)(off >> 32);
+      p.rows = min(16, keys - key);
+      return p;
+    };
+    PagedHalves now = halves(0, half_page(0));
+    int next_page = half_page(32);
+
+    u32x4 kx[2][KD], vx[T::VI];
+    int64_t off[2];
+    uint32_t bytes[2];
+    // Where unit i lies; its K and its V on their way to the registers.
+    auto turn_to = [&](int i) __attribute__((always_inline)) {
+      if ((i & 31) == 0 && i > 0) {
+        now = halves(i, next_page);
+        next_page = half_page(i + 32);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int from = 2 * (i & 31) + e;
+        const uint32_t lo = __builtin_amdgcn_readlane(now.lo, from);
+        const uint32_t hi = __builtin_amdgcn_readlane(now.hi, from);
+        const int n_rows = __builtin_amdgcn_readlane(now.rows, from);
+        off[e] = (int64_t)((uint64_t)hi << 32 | lo);
+        bytes[e] = n_rows > 0 ? (uint32_t)((n_rows - 1) * row_bytes + a.d * 2) : 0u;
+        bad |= n_rows < 0;
+      }
+    };
+    auto load_k = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const rsrc_t r_k = make_rsrc(reinterpret_cast<const char*>(k_head) + off[e], bytes[e]);
+#pragma unroll
+        for (int kd = 0; kd < KD; ++kd) kx[e][kd] = buf_load_b128(r_k, k_off[kd]);
+      }
+    };
+    auto load_v = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < T::VI; ++j) {
+        const int e = j * T::VROWS / 16;
+        const rsrc_t r_v = make_rsrc(reinterpret_cast<const char*>(v_head) + off[e], bytes[e]);
+        vx[j] = buf_load_b128(r_v, v_off[j]);
+      }
+    };
+
+    float4v o[DD];
+#pragma unroll
+    for (int dd = 0; dd < DD; ++dd) o[dd] = {0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    const float c = a.c;
+
+    turn_to(0);
+    load_k();
+    load_v();
+    for (int i = 0; i < mine; ++i) {
+      const int ka = (u0 + wave + NW * i) * kPagedUnit;
+      float4v s[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        s[kb] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kd = 0; kd < KD; ++kd)
+          s[kb] = mma16<E>(__builtin_bit_cast(half8, kx[kb][kd]), qf[kd], s[kb]);
+      }
+      turn_to(i + 1);  // past the last unit: no rows
+      load_k();
+#pragma unroll
+      for (int j = 0; j < T::VI; ++j) *reinterpret_cast<u32x4*>(vt + v_at[j]) = vx[j];
+      load_v();
+      if (ka + kPagedUnit > all_see) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (ka + 16 * kb + 4 * G + j >= see) s[kb][j] = -INFINITY;
+      }
+      half8 pa;
+      auto probs = [&](float ref) __attribute__((always_inline)) {
+        float sum = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float p = exp2_fast(fmaf(s[kb][j], c, -ref));
+            sum += p;
+            pa[4 * kb + j] = to_elem<E>(p);
+          }
+        return sum;
+      };
+      float l_u = probs(m);
+      if (__builtin_amdgcn_ballot_w64(!(l_u <= kPagedSumLimit)) != 0) {
+        float mt = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mt = __builtin_fmaxf(mt, s[kb][j]);
+        const float m_new = __builtin_fmaxf(m, quarters_max(mt) * c);
+        const float ref = exp_reference(m_new);
+        const float alpha = exp2_fast(m - ref);
+        l *= alpha;
+#pragma unroll
+        for (int dd = 0; dd < DD; ++dd) o[dd] *= alpha;
+        m = m_new;
+        l_u = probs(ref);
+      }
+      l += l_u;
+#pragma unroll
+      for (int dd = 0; dd < DD; ++dd) {
+        const half4 lo = __builtin_bit_cast(
+            half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(vt + t_off[dd])));
+        const half4 hi = __builtin_bit_cast(
+            half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(vt + t_off[dd] + 16 * D)));
+        half8 va;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          va[e] = lo[e];
+          va[4 + e] = hi[e];
+        }
+        o[dd] = mma16<E>(va, pa, o[dd]);
+      }
+    }
+
+    // Merge of the waves' results: O, and per row m and l.
+    __syncthreads();
+    float* const xo = lds;                    // [wave][dd][lane][4]
+    float* const xm = lds + NW * DD * 256;    // [wave][row], m then l
+    float lw = quarters_sum(l);
+    if (bad) {  // NaN, whatever the other waves and pieces hold
+      lw = __builtin_nanf("");
+      m = m == -INFINITY ? 0.f : m;
+    }
+#pragma unroll
+    for (int dd = 0; dd < DD; ++dd)
+      *reinterpret_cast<float4v*>(xo + ((wave * DD + dd) * 64 + lane) * 4) = o[dd];
+    if (G == 0) {
+      xm[wave * kPagedRows + c16] = m;
+      xm[(NW + wave) * kPagedRows + c16] = lw;
+    }
+    __syncthreads();
+    float mt = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) mt = __builtin_fmaxf(mt, xm[w * kPagedRows + c16]);
+    float wt[NW], lt = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float mw = xm[w * kPagedRows + c16];
+      wt[w] = mw == -INFINITY ? 0.f : exp2_fast(mw - mt);  // a wave that saw no key weighs 0
+      lt += wt[w] * xm[(NW + w) * kPagedRows + c16];
+    }
+    const float inv = lt == 0.f ? 0.f : 1.0f / lt;  // a row that saw no key is 0
+    const bool whole = u0 == 0 && u1 == units;
+    const int64_t slot = (int64_t)blockIdx.x * 2 + (opening ? 0 : 1);
+    float* const part = a.part + slot * (kPagedRows * (D + 1));
+    half_t* const out =
+        a.o + (((int64_t)at.b * a.Hkv * a.group + kvh * a.group + h) * a.N + n) * a.d;
+#pragma unroll
+    for (int dd = wave; dd < DD; dd += NW) {
+      float4v v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < NW; ++w)
+        v += *reinterpret_cast<const float4v*>(xo + ((w * DD + dd) * 64 + lane) * 4) * wt[w];
+      v *= inv;
+      const int col = 16 * dd + 4 * G;
+      if (!row_ok) continue;
+      if (!whole) *reinterpret_cast<float4v*>(part + c16 * D + col) = v;
+      else if (col < a.d)
+        *reinterpret_cast<u32x2*>(out + col) = pack4<E>(v[0], v[1], v[2], v[3]);
+    }
+    if (!whole && wave == 0 && G == 0 && row_ok)
+      part[kPagedRows * D + c16] = lt == 0.f ? -INFINITY : mt + log2_fast(lt);
+    __syncthreads();
+
+    left -= u1 - u0;
+    opening = false;
+    at.unit = 0;
+    if (++at.triple == a.Hkv * a.blocks) {
+      at.triple = 0;
+      ++at.b;
+    }
+  }
+}
+
+// Joins the pieces of the triples that the stretches' borders cut: block w the triple that the
+// border between stretches w and w + 1 cuts, if that is its first. Piece s of a row weighs
+// exp2(lse_s) against the others'. A lane holds four columns of a row; the four waves take every
+// fourth piece and merge through LDS, in a fixed order.
+template <int D, class E>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
+  constexpr int COLS = D / 4;                     // 4-column pieces of a row
+  constexpr int RPP = 64 / COLS;                  // rows of a pass
+  __shared__ int find[8];
+  __shared__ __attribute__((aligned(16))) float acc_s[4][64][4];
+  __shared__ float m_s[4][64], l_s[4][64];
+  PagedPlace at;
+  int stretch = 0;
+  const int total = paged_find(a, find, &at, [&](int n) __attribute__((always_inline)) {
+    stretch = paged_stretch(n, a.grid);
+    return (int)min(((int64_t)blockIdx.x + 1) * stretch, (int64_t)n);
+  });
+  const int64_t border = ((int64_t)blockIdx.x + 1) * stretch;
+  if (border >= total || at.unit == 0) return;          // it cuts no triple
+  if (at.unit > stretch) return;                        // not the triple's first border
+  const int units = paged_units(a, uniform(a.lengths[at.b]));
+  const int more = (units - at.unit + stretch - 1) / stretch;  // pieces after the first
+  // The first piece is its stretch's only one if the triple starts with the stretch.
+  const int64_t first = (int64_t)blockIdx.x * 2 + (at.unit == stretch ? 0 : 1);
+  const int kvh = at.triple / a.blocks, block = at.triple - kvh * a.blocks;
+  const int rows = min(kPagedRows, a.group * a.N - block * kPagedRows);
+  constexpr int SLOT = kPagedRows * (D + 1);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = 4 * (lane % COLS);
+  for (int r0 = blockIdx.y * RPP; r0 < rows; r0 += gridDim.y * RPP) {
+    const int row = r0 + lane / COLS;
+    float m = -INFINITY, l = 0.f;
+    float4v acc = {0.f, 0.f, 0.f, 0.f};
+    if (row < rows) {
+      for (int p0 = wave; p0 <= more; p0 += 4 * 8) {
+        float ls[8];
+        float4v v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int p = p0 + 4 * i;
+          ls[i] = -INFINITY;
+          v[i] = {0.f, 0.f, 0.f, 0.f};
+          if (p <= more) {
+            const int64_t slot = p == 0 ? first : ((int64_t)blockIdx.x + p) * 2;
+            const float* part = a.part + slot * SLOT;
+            ls[i] = part[kPagedRows * D + row];
+            v[i] = *reinterpret_cast<const float4v*>(part + row * D + col);
+          }
+        }
+        float mx = m;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx = __builtin_fmaxf(mx, ls[i]);
+        const float ref = exp_reference(mx);
+        const float keep = m == -INFINITY ? 0.f : exp2_fast(m - ref);
+        l *= keep;
+        acc *= keep;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float w = ls[i] == -INFINITY ? 0.f : exp2_fast(ls[i] - ref);
+          l += w;
+          acc += v[i] * w;
+        }
+        m = mx;
+      }
+    }
+    __syncthreads();
+    *reinterpret_cast<float4v*>(acc_s[wave][lane]) = acc;
+    m_s[wave][lane] = m;
+    l_s[wave][lane] = l;
+    __syncthreads();
+    if (wave == 0 && row < rows && col < a.d) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mx = __builtin_fmaxf(mx, m_s[w][lane]);
+      float lt = 0.f;
+      float4v v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float mw = m_s[w][lane];
+        const float f = mw == -INFINITY ? 0.f : exp2_fast(mw - mx);
+        lt += f * l_s[w][lane];
+        v += *reinterpret_cast<const float4v*>(acc_s[w][lane]) * f;
+      }
+      v *= lt == 0.f ? 0.f : 1.0f / lt;
+      const int r = block * kPagedRows + row;
+      const int h = r / a.N, n = r - h * a.N;
+      half_t* out = a.o + (((int64_t)at.b * a.Hkv * a.group + kvh * a.group + h) * a.N + n) * a.d;
+      *reinterpret_cast<u32x2*>(out + col) = pack4<E>(v[0], v[1], v[2], v[3]);
+    }
+  }
+}
+
+// Two work-groups a CU, at most one for each four units that the tables could hold.
+int paged_grid(int64_t B, int64_t Hkv, int64_t blocks, int64_t keys) {
+  const int64_t units = B * Hkv * blocks * ((keys + kPagedUnit - 1) / kPagedUnit);
+  return (int)std::clamp<int64_t>((units + 3) / 4, 1, 512);
+}
+
+template <int D, class E>
+hipError_t paged_start(const PagedArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL((paged_fwd_kernel<D, E>), dim3((unsigned)a.grid), dim3(256), 0, stream, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.grid == 1) return e;
+  constexpr int RPP = 64 / (D / 4);
+  const int rows = std::min(kPagedRows, a.group * a.N);
+  const dim3 grid((unsigned)(a.grid - 1), (unsigned)((rows + RPP - 1) / RPP));
+  hipLaunchKernelGGL((paged_join_kernel<D, E>), grid, dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_paged_fwd(const PagedArgs& a, int D, int dtype, hipStream_t stream) {
+  const bool bf = dtype == kBF16;
+  switch (D) {
+    case 32: return bf ? paged_start<32, BF16>(a, stream) : paged_start<32, F16>(a, stream);
+    case 64: return bf ? paged_start<64, BF16>(a, stream) : paged_start<64, F16>(a, stream);
+    case 128: return bf ? paged_start<128, BF16>(a, stream) : paged_start<128, F16>(a, stream);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+}  // namespace fa

@@ -14,7 +14,7 @@ from pathlib import Path
 
 from ._build import LIB_PATH
 
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 FA_OK = 0
 FA_ERR_NULL_POINTER = -1
@@ -101,6 +101,18 @@ del _view
 # Forward without allocation (device-resident scratch): fa_fwd_kv's arguments.
 SIGNATURES["fa_fwd_noalloc"] = SIGNATURES["fa_fwd_kv"]
 SIGNATURES["fa_fwd_noalloc_max_workspace_bytes"] = (_I64, ())
+# The operators around the attention call.
+SIGNATURES["fa_qk_norm_rope"] = (_INT, (_P,) * 10 + (_I64,) * 7 + (_F32, _INT, _P))
+SIGNATURES["fa_qk_norm_rope_bwd_workspace_bytes"] = (_I64, (_I64,) * 5)
+SIGNATURES["fa_qk_norm_rope_bwd"] = (
+    _INT, (_P,) * 14 + (_I64,) * 7 + (_F32, _INT, _P, _I64, _P))
+SIGNATURES["fa_paged_plan"] = (_INT, (_P, _I64) + (_P,) * 9 + (_I64,) * 5 + (_P,))
+SIGNATURES["fa_paged_store"] = (_INT, (_P,) * 6 + (_I64,) * 5 + (_P,))
+SIGNATURES["fa_paged_fwd_workspace_bytes"] = (_I64, (_I64,) * 7)
+SIGNATURES["fa_paged_fwd"] = (_INT, (_P,) * 7 + (_I64,) * 8 + (_F32, _P, _I64, _P))
+for _name in ("fa_qk_norm_rope", "fa_qk_norm_rope_bwd", "fa_paged_fwd"):
+    SIGNATURES[_name + "_bf16"] = SIGNATURES[_name]
+del _name
 
 
 class FlashAttentionError(RuntimeError):

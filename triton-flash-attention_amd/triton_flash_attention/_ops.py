@@ -359,3 +359,180 @@ def flash_bwd(
             ws.data_ptr() if ws is not None else None, ws_bytes, _stream(q),
         ))
     return dq, dk, dv
+
+
+# ---- the operators around the attention call ----------------------------------------------
+
+
+def _readable(t: torch.Tensor) -> torch.Tensor:
+    """``t``, or a contiguous copy where its rows cannot be read in 16-byte pieces as they
+    stand (a dimension of one element has no stride to speak of)."""
+    t = t.resolve_neg()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
+            n == 1 or 0 <= s < 1 << 40 and s % 8 == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1])):
+        return t
+    return _aligned(t.contiguous())
+
+
+def _strides(t: torch.Tensor) -> list[int]:
+    """Strides of all but the last dimension (0 for dimensions of one element)."""
+    return [0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()[:-1])]
+
+
+def row_stride(cache: torch.Tensor) -> int:
+    """Elements from one row of a cache's page to the next."""
+    return cache.stride(2) if cache.shape[2] > 1 else cache.shape[3]
+
+
+def _int64s(values) -> ctypes.Array:
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def _ptr(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+ROPE_INTERLEAVED, ROPE_WEIGHT_F32, ROPE_POSITIONS_I64 = 1, 2, 4  # FA_ROPE_* of the header
+
+
+def _rope_common(cos, sin, query_weight, key_weight, positions, batch: int, interleaved: bool):
+    """(cos, sin, weights, positions) as the kernels read them, positions' strides, flags."""
+    cos, sin = _aligned(cos.contiguous()), _aligned(sin.contiguous())
+    flags = ROPE_INTERLEAVED if interleaved else 0
+    if query_weight is not None:
+        query_weight, key_weight = query_weight.contiguous(), key_weight.contiguous()
+        flags |= ROPE_WEIGHT_F32 if query_weight.dtype == torch.float32 else 0
+    pos_strides = [0, 0]
+    if positions is not None:
+        pos_strides = [0, *positions.stride()][-2:]
+        flags |= ROPE_POSITIONS_I64 if positions.dtype == torch.int64 else 0
+    return cos, sin, query_weight, key_weight, pos_strides, flags
+
+
+def qk_norm_rope(q, k, cos, sin, query_weight, key_weight, eps: float, positions,
+                 interleaved: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """Normalised and rotated q [B,Hq,N,D] and k [B,Hkv,N,D] (contiguous)."""
+    dt = _elem_dtype(q, "q")
+    B, Hq, N, D = q.shape
+    lib = _lib.load()
+    with _device_guard(q.device):
+        q, k = _readable(q), _readable(k)
+        cos, sin, wq, wk, pos_strides, flags = _rope_common(
+            cos, sin, query_weight, key_weight, positions, B, interleaved)
+        q_out = torch.empty((B, Hq, N, D), dtype=dt, device=q.device)
+        k_out = torch.empty(k.shape, dtype=dt, device=q.device)
+        strides = _int64s([*_strides(q), *_strides(k), *pos_strides])
+        _lib.check(_launch(
+            "qk_norm_rope", _entry(lib, "fa_qk_norm_rope", dt),
+            q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), cos.data_ptr(),
+            sin.data_ptr(), _ptr(positions), _ptr(wq), _ptr(wk), strides,
+            B, Hq, k.shape[1], N, D, 2 * cos.shape[1], cos.shape[0], eps, flags, _stream(q)))
+    return q_out, k_out
+
+
+def qk_norm_rope_bwd(gq, gk, q, k, cos, sin, query_weight, key_weight, eps: float, positions,
+                     interleaved: bool, weights=(True, True)):
+    """(dq, dk, dquery_weight, dkey_weight) of :func:`qk_norm_rope` from the gradients of its
+    outputs; q and k are None without weights, and a weight's gradient is None where
+    ``weights`` leaves it out."""
+    dt = _elem_dtype(gq, "gq")
+    B, Hq, N, D = gq.shape
+    Hkv = gk.shape[1]
+    lib = _lib.load()
+    norm = query_weight is not None
+    with _device_guard(gq.device):
+        gq, gk = _readable(gq), _readable(gk)
+        q, k = (_readable(q), _readable(k)) if norm else (None, None)
+        cos, sin, wq, wk, pos_strides, flags = _rope_common(
+            cos, sin, query_weight, key_weight, positions, B, interleaved)
+        dq = torch.empty(gq.shape, dtype=dt, device=gq.device)
+        dk = torch.empty(gk.shape, dtype=dt, device=gq.device)
+        dw = [torch.empty_like(w) if norm and wanted else None
+              for w, wanted in zip((wq, wk), weights)]
+        ws, ws_bytes = None, 0
+        if dw[0] is not None or dw[1] is not None:
+            ws_bytes = lib.fa_qk_norm_rope_bwd_workspace_bytes(B, Hq, Hkv, N, D)
+            if ws_bytes < 0:
+                _lib.check(ws_bytes)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=gq.device)
+        x_strides = [*_strides(q), *_strides(k)] if norm else [0] * 6
+        strides = _int64s([*_strides(gq), *_strides(gk), *x_strides, *pos_strides])
+        _lib.check(_launch(
+            "qk_norm_rope_bwd", _entry(lib, "fa_qk_norm_rope_bwd", dt),
+            gq.data_ptr(), gk.data_ptr(), _ptr(q), _ptr(k), dq.data_ptr(), dk.data_ptr(),
+            _ptr(dw[0]), _ptr(dw[1]), cos.data_ptr(), sin.data_ptr(), _ptr(positions), _ptr(wq),
+            _ptr(wk), strides, B, Hq, Hkv, N, D, 2 * cos.shape[1], cos.shape[0], eps, flags,
+            _ptr(ws), ws_bytes, _stream(gq)))
+    return dq, dk, dw[0], dw[1]
+
+
+def paged_plan(page_table, lengths, new_tokens, free_pages, free_start, page_size: int,
+               num_tokens: int):
+    """(slots, positions, starts, lengths, free_start) of a step; writes page_table."""
+    B, M = page_table.shape
+    dev = page_table.device
+    lib = _lib.load()
+    with _device_guard(dev):
+        lengths, new_tokens, free_pages = (t.contiguous() for t in (lengths, new_tokens, free_pages))
+        slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+        positions = torch.empty(num_tokens, dtype=torch.int32, device=dev)
+        starts = torch.empty(B + 1, dtype=torch.int32, device=dev)
+        lengths_out = torch.empty(B, dtype=torch.int32, device=dev)
+        free_out = torch.empty(1, dtype=torch.int32, device=dev)
+        _lib.check(_launch(
+            "paged_plan", lib.fa_paged_plan, page_table.data_ptr(), page_table.stride(0),
+            lengths.data_ptr(), new_tokens.data_ptr(), free_pages.data_ptr(), _ptr(free_start),
+            slots.data_ptr(), positions.data_ptr(), starts.data_ptr(), lengths_out.data_ptr(),
+            free_out.data_ptr(), B, M, page_size, free_pages.shape[0], num_tokens,
+            _stream(page_table)))
+    _written(page_table)
+    return slots, positions, starts, lengths_out, free_out
+
+
+def _written(*tensors) -> None:
+    """Tells autograd that a kernel wrote these tensors in place."""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
+def paged_store(key, value, key_cache, value_cache, slots) -> None:
+    """Rows of key and value [T,H,D] into their slots of the caches [pages,H,S,D]."""
+    pages, H, S, D = key_cache.shape
+    lib = _lib.load()
+    with _device_guard(key_cache.device):
+        key, value, slots = _readable(key), _readable(value), slots.contiguous()
+        strides = _int64s([*_strides(key), *_strides(value), *_cache_strides(key_cache)])
+        _lib.check(_launch(
+            "paged_store", lib.fa_paged_store, key.data_ptr(), value.data_ptr(),
+            key_cache.data_ptr(), value_cache.data_ptr(), slots.data_ptr(), strides,
+            key.shape[0], H, D, pages, S, _stream(key_cache)))
+    _written(key_cache, value_cache)
+
+
+def _cache_strides(cache: torch.Tensor) -> list[int]:
+    return [*_strides(cache)[:2], row_stride(cache)]
+
+
+def paged_fwd(q, key_cache, value_cache, page_table, lengths, scale: float) -> torch.Tensor:
+    """O [B,Hq,N,D] of the newest N tokens over the paged cache, for a positive scale."""
+    dt = _elem_dtype(q, "q")
+    B, Hq, N, D = q.shape
+    pages, Hkv, S, _ = key_cache.shape
+    M = page_table.shape[1]
+    lib = _lib.load()
+    with _device_guard(q.device):
+        q, lengths = _readable(q), lengths.contiguous()
+        if page_table.stride(1) != 1 and M > 1:
+            page_table = page_table.contiguous()
+        ws_bytes = lib.fa_paged_fwd_workspace_bytes(B, Hq, Hkv, N, D, M, S)
+        if ws_bytes < 0:
+            _lib.check(ws_bytes)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+        o = torch.empty((B, Hq, N, D), dtype=dt, device=q.device)
+        strides = _int64s([*_strides(q), *_cache_strides(key_cache), page_table.stride(0)])
+        _lib.check(_launch(
+            "paged_fwd", _entry(lib, "fa_paged_fwd", dt), q.data_ptr(), key_cache.data_ptr(),
+            value_cache.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), o.data_ptr(),
+            strides, B, Hq, Hkv, N, D, pages, M, S, scale, _ptr(ws), ws_bytes, _stream(q)))
+    return o
