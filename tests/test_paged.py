@@ -18,7 +18,7 @@ import random
 import pytest
 import torch
 
-from triton_flash_attention import (paged_attention, paged_cache_plan, paged_cache_store,
+from triton_flash_attention import (_native, paged_attention, paged_cache_plan, paged_cache_store,
                                     qk_norm_rope, scaled_dot_product_attention)
 
 HALF = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
@@ -550,6 +550,21 @@ def test_attention_kernel_refuses_what_it_cannot_serve():
         paged_attention(**a, backend="triton")
     with pytest.raises(RuntimeError, match="float16 and bfloat16"):
         paged_attention(**_attend_args("cuda", torch.float32), backend="triton")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_binding_and_op_layer(native, monkeypatch):
+    """The same calls through the C++ binding and without it."""
+    assert _native.available(), _native.status()[1]
+    if not native:
+        monkeypatch.setattr(_native, "available", lambda: False)
+    check_plan(lengths=ragged(37, 300, 1), new=ragged(37, 70, 2), S=16, start=2, device="cuda",
+               backend="triton", pad_columns=2)
+    check_store(50, 8, 128, 32, torch.float16, layout="fused", cache_layout="tokens",
+                device="cuda", backend="triton")
+    check_attend([700, 0, 33], 8, 2, 3, 96, 48, torch.bfloat16, layout="tokens", q_layout="tokens",
+                 device="cuda", backend="triton")
 
 
 # ---- a decoding loop --------------------------------------------------------------------

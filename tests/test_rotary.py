@@ -16,7 +16,7 @@ import math
 import pytest
 import torch
 
-from triton_flash_attention import qk_norm_rope
+from triton_flash_attention import _native, qk_norm_rope
 
 HALF = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
 F32 = 2.0 ** -24
@@ -341,6 +341,77 @@ def test_kernel_calls_repeat_bit_for_bit_on_other_streams_and_in_graphs():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(captured, want)), i
+
+
+def both_paths(call):
+    """call() through the C++ binding and through the Python op layer."""
+    assert _native.available(), _native.status()[1]
+    got = call()
+    with pytest.MonkeyPatch.context() as m:
+        m.setattr(_native, "available", lambda: False)
+        other = call()
+    return got, other
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("norm", [True, False])
+def test_binding_and_op_layer_agree_bit_for_bit(norm):
+    q, k, gq, gk, wq, wk = inputs(2, 8, 4, 70, 96, torch.bfloat16, 8, "tokens", "cuda")
+    cos, sin = tables(90, 64, "cuda")
+    pos = positions_of("each", 2, 70, 90).cuda()
+    leaves = [t.detach().requires_grad_() for t in (q, k)]
+    weights = {}
+    if norm:
+        leaves += [w.cuda().requires_grad_() for w in (wq, wk)]
+        weights = dict(query_weight=leaves[2], key_weight=leaves[3])
+
+    def call():
+        out = qk_norm_rope(leaves[0], leaves[1], cos, sin, positions=pos, backend="triton", **weights)
+        with torch.no_grad():
+            plain = qk_norm_rope(leaves[0], leaves[1], cos, sin, positions=pos, **weights)
+        return [*out, *plain, *torch.autograd.grad(out, leaves, (gq, gk))]
+
+    for a, b in zip(*both_paths(call)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_kernel_has_no_second_derivative():
+    q, k, gq, gk, _, _ = inputs(1, 2, 1, 8, 32, torch.float16, 9, device="cuda")
+    cos, sin = tables(8, 32, "cuda")
+    q.requires_grad_()
+
+    def call():
+        out, _ = qk_norm_rope(q, k, cos, sin, backend="triton")
+        (g,) = torch.autograd.grad(out, q, gq.requires_grad_(), create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), gq)
+        return g.detach()
+
+    a, b = both_paths(call)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_capture_beside_a_living_graph_of_the_same_leaves_is_refused():
+    q, k, gq, gk, _, _ = inputs(1, 2, 1, 8, 32, torch.float16, 9, device="cuda")
+    cos, sin = tables(8, 32, "cuda")
+    q.requires_grad_()
+    alive, _ = qk_norm_rope(q, k, cos, sin, backend="triton")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        z = gq + 0  # the graph is not empty
+        with pytest.raises(RuntimeError, match="same leaf tensors"):
+            qk_norm_rope(q, k, cos, sin, backend="triton")
+    want = torch.autograd.grad(alive, q, gq)[0]
+    del alive
+    with torch.cuda.graph(torch.cuda.CUDAGraph()) as _:
+        out, _ = qk_norm_rope(q, k, cos, sin, backend="triton")
+        torch.autograd.grad(out, q, gq)
+    del out
+    out, _ = qk_norm_rope(q, k, cos, sin, backend="triton")
+    assert torch.equal(torch.autograd.grad(out, q, gq)[0], want)
+    assert z.shape == gq.shape
 
 
 @pytest.mark.gpu

@@ -37,6 +37,8 @@
 #include <stdexcept>
 #include <string>
 
+#include "fa_native_layer.hpp"
+
 namespace {
 
 using FwdView = int (*)(const void*, const void*, const void*, void*, void*, const int64_t*,
@@ -322,4 +324,5 @@ PYBIND11_MODULE(_fa_native, m) {
   m.def("attention", &attention);
   m.def("forward", &forward_only);
   m.def("plain_scale", &plain_scale);
+  bind_layer(m);
 }

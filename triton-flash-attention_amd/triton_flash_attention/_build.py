@@ -5,7 +5,7 @@ the shared object travels with the source tree. No JIT cache is involved.
 
     python -m triton_flash_attention._build        # (re)build the library and the binding
 
-The C++ autograd binding (csrc/fa_native.cpp, ``_fa_native.so``) is host code
+The C++ binding (csrc/fa_native.cpp and fa_native_layer.cpp, ``_fa_native.so``) is host code
 only; it is compiled with g++ against PyTorch's headers (``build_native``).
 """
 
@@ -118,7 +118,7 @@ def build(output: Path = LIB_PATH, verbose: bool = False) -> Path:
     return output
 
 
-NATIVE_SOURCE = "fa_native.cpp"
+NATIVE_SOURCES = ("fa_native.cpp", "fa_native_layer.cpp")
 NATIVE_PATH = PACKAGE_DIR / "_fa_native.so"
 
 
@@ -138,7 +138,7 @@ def native_command(output: Path = NATIVE_PATH) -> list[str]:
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
         *(f"-I{p}" for p in cpp_extension.include_paths()),
         f"-I{sysconfig.get_paths()['include']}", f"-I{rocm}/include",
-        str(CSRC_DIR / NATIVE_SOURCE), "-o", str(output),
+        *(str(CSRC_DIR / s) for s in NATIVE_SOURCES), "-o", str(output),
         *(f"-L{p}" for p in libdirs), *(f"-Wl,-rpath,{p}" for p in libdirs),
         "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python",
     ]

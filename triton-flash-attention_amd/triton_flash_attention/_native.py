@@ -25,10 +25,19 @@ PATH = Path(__file__).resolve().parent / f"{NAME}.so"
 # Entry points handed to init(), in its argument order.
 ENTRY_POINTS = ("fa_fwd_view", "fa_fwd_view_bf16", "fa_bwd_view", "fa_bwd_view_bf16",
                 "fa_fwd_workspace_bytes", "fa_bwd_workspace_bytes", "fa_last_error")
+# And to init_layer() (csrc/fa_native_layer.cpp).
+LAYER_ENTRY_POINTS = ("fa_qk_norm_rope", "fa_qk_norm_rope_bf16", "fa_qk_norm_rope_bwd",
+                      "fa_qk_norm_rope_bwd_bf16", "fa_qk_norm_rope_bwd_workspace_bytes",
+                      "fa_paged_plan", "fa_paged_store", "fa_paged_fwd", "fa_paged_fwd_bf16",
+                      "fa_paged_fwd_workspace_bytes", "fa_last_error")
 
 _module = None
 _error: str | None = None
 _tried = False
+
+
+def _addresses(lib, names) -> list[int]:
+    return [ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names]
 
 
 def _load():
@@ -49,7 +58,8 @@ def _load():
         module = importlib.util.module_from_spec(spec)
         loader.exec_module(module)
         lib = _lib.load()
-        module.init(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in ENTRY_POINTS))
+        module.init(*_addresses(lib, ENTRY_POINTS))
+        module.init_layer(_addresses(lib, LAYER_ENTRY_POINTS))
     except Exception as exc:  # noqa: BLE001 - reported by status()
         _error = f"{PATH.name} failed to load: {exc}"
         return
@@ -60,6 +70,11 @@ def available() -> bool:
     if not _tried:
         _load()
     return _module is not None
+
+
+def module():
+    """The binding, or None where it is not available (the op layer then launches)."""
+    return _module if available() else None
 
 
 def status() -> tuple[bool, str]:

@@ -25,9 +25,9 @@ from typing import NamedTuple
 
 import torch
 
-from . import _ops
+from . import _native, _ops
 from .attention import _SUPPORTED_DTYPES, Backend, _forward_ad_active, _kernel_scale
-from .rotary import _check_backend, _check_tensor, _falls_back, _gpu_reason
+from .rotary import _check_backend, _check_tensor, _falls_back, _gpu_reason, _plain
 
 _PAGE_MULTIPLE = 16
 _MOST_TOKENS = (1 << 30) - 64  # that a row of the page table holds (fa_capi_layer.hip)
@@ -161,6 +161,11 @@ def paged_cache_plan(
     -1 and ``free_start`` of the result exceeds ``len(free_pages)``; tokens behind a sequence's
     M pages have slot -1 as well. Negative lengths and counts are taken as 0.
     """
+    if _plain(backend):
+        out = _native.module().paged_plan(page_table, lengths, new_tokens, free_pages, page_size,
+                                          num_tokens, free_start)
+        if out is not None:
+            return PagedPlan(*out)
     _check_backend(backend)
     _check_table(page_table, page_size)
     B, device = page_table.shape[0], page_table.device
@@ -211,6 +216,8 @@ def paged_cache_store(
     no slot names stay as they were. Gradients are not recorded: the call raises where one would
     have to be.
     """
+    if _plain(backend) and _native.module().paged_store(key, value, key_cache, value_cache, slots):
+        return
     _check_backend(backend)
     for name, t in (("key", key), ("value", value)):
         _check_tensor(name, t, 3, "(tokens, heads, head_dim)")
@@ -315,6 +322,11 @@ def paged_attention(
     splits the keys over the whole GPU whatever the lengths are. It has no backward: inputs that
     require gradients run in PyTorch under ``backend="auto"``.
     """
+    if _plain(backend) and not _forward_ad_active():
+        out = _native.module().paged_attention(query, key_cache, value_cache, page_table, lengths,
+                                               scale, enable_gqa)
+        if out is not None:
+            return out
     _check_backend(backend)
     if not isinstance(enable_gqa, bool):
         raise TypeError("enable_gqa must be a bool")

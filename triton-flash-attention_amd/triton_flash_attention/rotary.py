@@ -13,7 +13,7 @@ from numbers import Real
 
 import torch
 
-from . import _lib, _ops
+from . import _lib, _native, _ops
 from .attention import (_REASON_LIBRARY, _SUPPORTED_ARCH, _SUPPORTED_DTYPES, Backend, _device_arch,
                         _forward_ad_active, _warn_library_once)
 
@@ -21,6 +21,13 @@ from .attention import (_REASON_LIBRARY, _SUPPORTED_ARCH, _SUPPORTED_DTYPES, Bac
 def _check_backend(backend: str) -> None:
     if backend not in ("auto", "triton", "torch"):
         raise ValueError("backend must be one of: 'auto', 'triton', 'torch'")
+
+
+def _plain(backend: str) -> bool:
+    """Whether the call may go to the binding, which serves it or finds that Python has to look
+    (torch.compile cannot trace into it)."""
+    return ((backend == "auto" or backend == "triton")
+            and not torch.compiler.is_dynamo_compiling() and _native.available())
 
 
 def _check_tensor(name: str, t, ndim: int, shape: str) -> None:
@@ -201,6 +208,11 @@ def qk_norm_rope(
     multiple of 8 up to 128 and R a multiple of 16; a weight's gradient is a float32 sum in a
     fixed order.
     """
+    if _plain(backend) and not _forward_ad_active():
+        out = _native.module().qk_norm_rope(query, key, cos, sin, query_weight, key_weight, eps,
+                                            positions, interleaved)
+        if out is not None:
+            return out
     _check_backend(backend)
     _validate(query, key, cos, sin, query_weight, key_weight, eps, positions, interleaved)
     if _falls_back(backend, None if backend == "torch" else _kernel_reason(query, cos, sin)):
