@@ -225,7 +225,7 @@ int64_t paged_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t N, int64_t D
                         int64_t S) {
   const int64_t width = D <= 32 ? 32 : D <= 64 ? 64 : 128;
   const int grid = fa::paged_grid(B, Hkv, row_blocks(Hq / Hkv * N), M * S);
-  return grid == 1 ? 0 : (int64_t)grid * 2 * fa::kPagedRows * (width + 1) * 4;
+  return grid <= 1 ? 0 : (int64_t)grid * 2 * fa::kPagedRows * (width + 1) * 4;
 }
 
 int run_paged(const char* name, int dtype, const fa_half_t* q, const fa_half_t* k_cache,

@@ -101,11 +101,12 @@ struct PagedArgs {
   float c;               // scale * log2(e)
   int B, Hkv, group, N, d, M, S;
   int blocks;            // row blocks of 16 of a key/value head's group * N rows
-  int grid;              // work-groups
+  int grid;              // work-groups (paged_grid)
 };
 constexpr int kPagedRows = 16;
 constexpr int kPagedUnit = 32;  // keys
-// Work-groups and workspace bytes of a launch of these sizes.
+// Work-groups of a launch whose table rows hold `keys` keys; 0: one for each sequence,
+// key/value head and row block.
 int paged_grid(int64_t B, int64_t Hkv, int64_t blocks, int64_t keys);
 hipError_t launch_paged_fwd(const PagedArgs& a, int D, int dtype, hipStream_t stream);
 

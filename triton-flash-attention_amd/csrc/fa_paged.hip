@@ -26,9 +26,9 @@ __device__ __forceinline__ T wave_scan(T x, int lane) {
   return x;
 }
 
-// Sum over the threads before this one of a block of 256, and the block's total. `sums` holds
-// one value a wave; ends with every thread past the barrier that publishes them.
-template <class T>
+// Sum over the threads before this one of a block of W waves, and the block's total. `sums`
+// holds one value a wave; ends with every thread past the barrier that publishes them.
+template <int W = 4, class T>
 __device__ __forceinline__ T block_scan(T x, T* sums, T* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const T incl = wave_scan(x, lane);
@@ -36,7 +36,7 @@ __device__ __forceinline__ T block_scan(T x, T* sums, T* total) {
   __syncthreads();
   T before = incl - x, all = 0;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < W; ++w) {
     if (w < wave) before += sums[w];
     all += sums[w];
   }
@@ -236,9 +236,11 @@ hipError_t launch_paged_store(const StoreArgs& a, hipStream_t stream) {
 // a unit exceeds this, far below where fp16 ends.
 constexpr float kPagedSumLimit = 256.0f;
 
+constexpr int kPagedWaves = 4;  // of a work-group
+
 template <int D>
 struct PagedTile {
-  static constexpr int NW = 4;
+  static constexpr int NW = kPagedWaves;
   static constexpr int KD = D / 32, DD = D / 16;
   static constexpr int TILE = kPagedUnit * D;          // halves of a unit's K (or V) rows
   static constexpr int VI = TILE * 2 / 1024;           // 1 KiB loads of a unit's V
@@ -253,45 +255,73 @@ __device__ __forceinline__ int paged_units(const PagedArgs& a, int len) {
   return len > 0 && len <= a.M * a.S ? (len + kPagedUnit - 1) / kPagedUnit : 1;
 }
 
-// A place on the line of units: unit `unit` of triple `triple` (head-major) of sequence `b`.
-struct PagedPlace {
-  int b, triple, unit;
+// The line of units, cut into stretches of `stretch` units, one a work-group. A triple's units
+// on the line are its own, or in a launch too small to fill the grid (`padded`) its own and
+// empty ones up to a whole number of stretches, so that no work-group has two short pieces.
+struct PagedLine {
+  int total, stretch;
+  bool padded;
+  __device__ __forceinline__ int units(int own) const {
+    return padded ? (own + stretch - 1) / stretch * stretch : own;
+  }
 };
 
-// The line's length, and the place of its unit `at` (defined where at < the length). `want`
-// is computed from the length. Ends with a barrier.
-template <class Want>
-__device__ __forceinline__ int paged_find(const PagedArgs& a, int* lds, PagedPlace* place,
-                                          Want want) {
+// A place on it: unit `unit` of triple `triple` (head-major) of sequence `b`, of `len` keys.
+struct PagedPlace {
+  int b, triple, unit, len;
+};
+
+// The line, and its place at stretch `s`, which is defined where the line reaches it. For
+// blocks of W waves.
+template <int W>
+__device__ __forceinline__ PagedLine paged_find(const PagedArgs& a, int s, PagedPlace* place) {
+  __shared__ int sums[W], found[4];
+  __shared__ int64_t sums2[W];
   const int HB = a.Hkv * a.blocks;
-  const int per = (a.B + 255) / 256;
+  const int per = (a.B + 64 * W - 1) / (64 * W);
   const int b0 = threadIdx.x * per, b1 = min(a.B, b0 + per);
-  int mine = 0;
-  for (int b = b0; b < b1; ++b) mine += paged_units(a, a.lengths[b]) * HB;
-  int total;
-  const int before = block_scan(mine, lds, &total);
-  const int at = want(total);
-  if (at >= before && at < before + mine) {
-    int rest = at - before, b = b0, units = 1;
+  constexpr int S1 = kPagedWaves, S2 = 2 * kPagedWaves;  // stretches of padded lines
+  int own = 0, in1 = 0, in2 = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int u = paged_units(a, a.lengths[b]);
+    own += u * HB;
+    in1 += (u + S1 - 1) / S1 * HB;
+    in2 += (u + S2 - 1) / S2 * HB;
+  }
+  PagedLine line;
+  int64_t all12;
+  const int64_t before12 = block_scan<W>((int64_t)in2 << 32 | (uint32_t)in1, sums2, &all12);
+  int before = block_scan<W>(own, sums, &line.total), mine = own;
+  const int all1 = (int)(uint32_t)all12, all2 = (int)(all12 >> 32);
+  line.padded = all2 <= a.grid;
+  line.stretch = ((line.total + a.grid - 1) / a.grid + kPagedWaves - 1) / kPagedWaves * kPagedWaves;
+  if (line.padded) {
+    const bool one = all1 <= a.grid;
+    line.stretch = one ? S1 : S2;
+    line.total = (one ? all1 : all2) * line.stretch;
+    before = (one ? (int)(uint32_t)before12 : (int)(before12 >> 32)) * line.stretch;
+    mine = (one ? in1 : in2) * line.stretch;
+  }
+  const int64_t at = (int64_t)s * line.stretch;
+  if (at >= before && at < (int64_t)before + mine) {
+    int rest = (int)(at - before), b = b0, len = 0, units = 1;
     for (; b < b1; ++b) {
-      units = paged_units(a, a.lengths[b]);
+      len = a.lengths[b];
+      units = line.units(paged_units(a, len));
       if (rest < units * HB) break;
       rest -= units * HB;
     }
-    lds[4] = b;
-    lds[5] = rest / units;
-    lds[6] = rest % units;
+    found[0] = b;
+    found[1] = rest / units;
+    found[2] = rest % units;
+    found[3] = len;
   }
   __syncthreads();
-  place->b = uniform(lds[4]);
-  place->triple = uniform(lds[5]);
-  place->unit = uniform(lds[6]);
-  return total;
-}
-
-// Units of a work-group's stretch: a multiple of the four waves.
-__device__ __forceinline__ int paged_stretch(int total, int grid) {
-  return ((total + grid - 1) / grid + 3) / 4 * 4;
+  place->b = uniform(found[0]);
+  place->triple = uniform(found[1]);
+  place->unit = uniform(found[2]);
+  place->len = uniform(found[3]);
+  return line;
 }
 
 // A wave's units of a piece: where the half units of its next 32 units lie, one a lane
@@ -303,30 +333,36 @@ struct PagedHalves {
 
 }  // namespace
 
-template <int D, class E>
-__global__ __launch_bounds__(256, 2) void paged_fwd_kernel(PagedArgs a) {
+template <int D, class E, bool SHORT>
+__global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArgs a) {
   using T = PagedTile<D>;
   constexpr int KD = T::KD, DD = T::DD, NW = T::NW;
   constexpr int LDS_FLOATS = NW * DD * 256 + 2 * NW * kPagedRows;
   static_assert(NW * T::TILE * 2 <= LDS_FLOATS * 4, "the V tiles and the merge share it");
   __shared__ __attribute__((aligned(16))) float lds[LDS_FLOATS];
-  __shared__ int find[8];
-
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = uniform(tid >> 6);
   const int c16 = lane & 15;
   const int G = lane >> 4;
 
+  // The stretch: `left` units from the place on. In a SHORT launch a triple of its own.
   PagedPlace at;
-  int stretch = 0;
-  const int total = paged_find(a, find, &at, [&](int n) __attribute__((always_inline)) {
-    stretch = paged_stretch(n, a.grid);
-    return (int)min((int64_t)blockIdx.x * stretch, (int64_t)n);
-  });
-  const int64_t x0 = (int64_t)blockIdx.x * stretch;
-  if (x0 >= total) return;
-  int left = min(stretch, (int)(total - x0));
+  int left;
+  bool padded = true;
+  if constexpr (SHORT) {
+    at.b = blockIdx.x / (a.Hkv * a.blocks);
+    at.triple = blockIdx.x - at.b * (a.Hkv * a.blocks);
+    at.unit = 0;
+    at.len = uniform(a.lengths[at.b]);
+    left = INT32_MAX;
+  } else {
+    const PagedLine line = paged_find<NW>(a, blockIdx.x, &at);
+    const int64_t from = (int64_t)blockIdx.x * line.stretch;
+    if (from >= line.total) return;
+    left = min(line.stretch, (int)(line.total - from));
+    padded = line.padded;
+  }
   bool opening = true;  // the stretch's first piece
 
   half_t* const vt = reinterpret_cast<half_t*>(lds) + wave * T::TILE;
@@ -350,12 +386,12 @@ __global__ __launch_bounds__(256, 2) void paged_fwd_kernel(PagedArgs a) {
     t_off[dd] = row * D + 8 * swz_chunk<D>(row, col >> 3) + (col & 7);
   }
 
-  while (left > 0) {
-    const int len = uniform(a.lengths[at.b]);
+  while (true) {
+    const int len = at.len;
     const bool fits = len >= 0 && len <= a.M * a.S;
     const int keys = fits ? len : 0;
     const int units = paged_units(a, len);
-    const int u0 = at.unit, u1 = min(units, u0 + left);
+    const int u0 = at.unit, u1 = left < units - u0 ? u0 + left : units;
     const int kvh = at.triple / a.blocks, block = at.triple - kvh * a.blocks;
     const int rows = a.group * a.N;
 
@@ -552,7 +588,7 @@ __global__ __launch_bounds__(256, 2) void paged_fwd_kernel(PagedArgs a) {
       lt += wt[w] * xm[(NW + w) * kPagedRows + c16];
     }
     const float inv = lt == 0.f ? 0.f : 1.0f / lt;  // a row that saw no key is 0
-    const bool whole = u0 == 0 && u1 == units;
+    const bool whole = SHORT || (u0 == 0 && u1 == units);
     const int64_t slot = (int64_t)blockIdx.x * 2 + (opening ? 0 : 1);
     float* const part = a.part + slot * (kPagedRows * (D + 1));
     half_t* const out =
@@ -575,11 +611,13 @@ __global__ __launch_bounds__(256, 2) void paged_fwd_kernel(PagedArgs a) {
     __syncthreads();
 
     left -= u1 - u0;
+    if (padded || left <= 0) return;
     opening = false;
     at.unit = 0;
     if (++at.triple == a.Hkv * a.blocks) {
       at.triple = 0;
       ++at.b;
+      at.len = uniform(a.lengths[at.b]);
     }
   }
 }
@@ -592,19 +630,15 @@ template <int D, class E>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   constexpr int COLS = D / 4;                     // 4-column pieces of a row
   constexpr int RPP = 64 / COLS;                  // rows of a pass
-  __shared__ int find[8];
   __shared__ __attribute__((aligned(16))) float acc_s[4][64][4];
   __shared__ float m_s[4][64], l_s[4][64];
   PagedPlace at;
-  int stretch = 0;
-  const int total = paged_find(a, find, &at, [&](int n) __attribute__((always_inline)) {
-    stretch = paged_stretch(n, a.grid);
-    return (int)min(((int64_t)blockIdx.x + 1) * stretch, (int64_t)n);
-  });
+  const PagedLine line = paged_find<4>(a, blockIdx.x + 1, &at);
+  const int stretch = line.stretch;
   const int64_t border = ((int64_t)blockIdx.x + 1) * stretch;
-  if (border >= total || at.unit == 0) return;          // it cuts no triple
+  if (border >= line.total || at.unit == 0) return;     // it cuts no triple
   if (at.unit > stretch) return;                        // not the triple's first border
-  const int units = paged_units(a, uniform(a.lengths[at.b]));
+  const int units = line.units(paged_units(a, at.len));
   const int more = (units - at.unit + stretch - 1) / stretch;  // pieces after the first
   // The first piece is its stretch's only one if the triple starts with the stretch.
   const int64_t first = (int64_t)blockIdx.x * 2 + (at.unit == stretch ? 0 : 1);
@@ -676,16 +710,29 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   }
 }
 
-// Two work-groups a CU, at most one for each four units that the tables could hold.
+// Where a sequence's row of the table holds at most this many keys, a work-group takes a whole
+// triple: no line, no partials and no second launch.
+constexpr int64_t kPagedShort = 1024;
+
+// Two work-groups a CU, at most one for each four units that the tables could hold; 0: a
+// work-group for each triple.
 int paged_grid(int64_t B, int64_t Hkv, int64_t blocks, int64_t keys) {
+  if (keys <= kPagedShort) return 0;
   const int64_t units = B * Hkv * blocks * ((keys + kPagedUnit - 1) / kPagedUnit);
   return (int)std::clamp<int64_t>((units + 3) / 4, 1, 512);
 }
 
 template <int D, class E>
 hipError_t paged_start(const PagedArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL((paged_fwd_kernel<D, E>), dim3((unsigned)a.grid), dim3(256), 0, stream, a);
-  hipError_t e = hipGetLastError();
+  const dim3 block(64 * kPagedWaves);
+  if (a.grid == 0) {
+    const int64_t triples = (int64_t)a.B * a.Hkv * a.blocks;
+    if (triples > 0x7fffffff) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((paged_fwd_kernel<D, E, true>), dim3((unsigned)triples), block, 0, stream, a);
+    return hipGetLastError();
+  }
+  hipLaunchKernelGGL((paged_fwd_kernel<D, E, false>), dim3((unsigned)a.grid), block, 0, stream, a);
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.grid == 1) return e;
   constexpr int RPP = 64 / (D / 4);
   const int rows = std::min(kPagedRows, a.group * a.N);
