@@ -210,9 +210,9 @@ int check_paged(const char* name, int64_t B, int64_t Hq, int64_t Hkv, int64_t N,
   const int64_t most = (int64_t)1 << 30;
   if (B >= most || Hq >= 1 << 20 || N >= 1 << 20)
     return capi_fail(FA_ERR_TOO_LARGE, "%s: too many sequences, heads or queries", name);
-  // Units of all sequences, heads and row blocks are counted in 32 bits.
+  // Units of all sequences, heads and row blocks are counted in 32 bits, up to 24 more for each.
   const double units = (double)B * Hkv * row_blocks(Hq / Hkv * N) *
-                       ((M * S + fa::kPagedUnit - 1) / fa::kPagedUnit);
+                       ((M * S + fa::kPagedUnit - 1) / fa::kPagedUnit + 24);
   if (units >= (double)most)
     return capi_fail(FA_ERR_TOO_LARGE,
                      "%s: %lld sequences of up to %lld keys are too many for one call", name,
@@ -220,12 +220,12 @@ int check_paged(const char* name, int64_t B, int64_t Hq, int64_t Hkv, int64_t N,
   return FA_OK;
 }
 
-// Two partials a work-group: 16 rows of O and their log-sum-exps.
+// For each work-group 16 bytes, and two partials: 16 rows of O and their log-sum-exps.
 int64_t paged_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t N, int64_t D, int64_t M,
                         int64_t S) {
   const int64_t width = D <= 32 ? 32 : D <= 64 ? 64 : 128;
   const int grid = fa::paged_grid(B, Hkv, row_blocks(Hq / Hkv * N), M * S);
-  return grid <= 1 ? 0 : (int64_t)grid * 2 * fa::kPagedRows * (width + 1) * 4;
+  return grid == 0 ? 0 : (int64_t)grid * (16 + 2 * fa::kPagedRows * (width + 1) * 4);
 }
 
 int run_paged(const char* name, int dtype, const fa_half_t* q, const fa_half_t* k_cache,

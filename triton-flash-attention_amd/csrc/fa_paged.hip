@@ -240,7 +240,6 @@ constexpr int kPagedWaves = 4;  // of a work-group
 
 template <int D>
 struct PagedTile {
-  static constexpr int NW = kPagedWaves;
   static constexpr int KD = D / 32, DD = D / 16;
   static constexpr int TILE = kPagedUnit * D;          // halves of a unit's K (or V) rows
   static constexpr int VI = TILE * 2 / 1024;           // 1 KiB loads of a unit's V
@@ -255,14 +254,18 @@ __device__ __forceinline__ int paged_units(const PagedArgs& a, int len) {
   return len > 0 && len <= a.M * a.S ? (len + kPagedUnit - 1) / kPagedUnit : 1;
 }
 
-// The line of units, cut into stretches of `stretch` units, one a work-group. A triple's units
-// on the line are its own, or in a launch too small to fill the grid (`padded`) its own and
-// empty ones up to a whole number of stretches, so that no work-group has two short pieces.
+template <int D>
+constexpr int kPagedLead = 768 / D;
+
+// The line of units, cut into stretches of `stretch` units, one a work-group. A triple has its
+// own units on the line behind `lead` empty ones, which stand for what opening and closing a
+// piece takes; or, in a launch too small to fill the grid (`padded`), its own and empty ones up
+// to a whole number of stretches, so that no work-group has two short pieces.
 struct PagedLine {
-  int total, stretch;
+  int total, stretch, lead;
   bool padded;
   __device__ __forceinline__ int units(int own) const {
-    return padded ? (own + stretch - 1) / stretch * stretch : own;
+    return padded ? (own + stretch - 1) / stretch * stretch : lead + own;
   }
 };
 
@@ -273,7 +276,7 @@ struct PagedPlace {
 
 // The line, and its place at stretch `s`, which is defined where the line reaches it. For
 // blocks of W waves.
-template <int W>
+template <int D, int W>
 __device__ __forceinline__ PagedLine paged_find(const PagedArgs& a, int s, PagedPlace* place) {
   __shared__ int sums[W], found[4];
   __shared__ int64_t sums2[W];
@@ -284,7 +287,7 @@ __device__ __forceinline__ PagedLine paged_find(const PagedArgs& a, int s, Paged
   int own = 0, in1 = 0, in2 = 0;
   for (int b = b0; b < b1; ++b) {
     const int u = paged_units(a, a.lengths[b]);
-    own += u * HB;
+    own += (u + kPagedLead<D>) * HB;
     in1 += (u + S1 - 1) / S1 * HB;
     in2 += (u + S2 - 1) / S2 * HB;
   }
@@ -294,7 +297,8 @@ __device__ __forceinline__ PagedLine paged_find(const PagedArgs& a, int s, Paged
   int before = block_scan<W>(own, sums, &line.total), mine = own;
   const int all1 = (int)(uint32_t)all12, all2 = (int)(all12 >> 32);
   line.padded = all2 <= a.grid;
-  line.stretch = ((line.total + a.grid - 1) / a.grid + kPagedWaves - 1) / kPagedWaves * kPagedWaves;
+  line.lead = line.padded ? 0 : kPagedLead<D>;
+  line.stretch = (line.total + a.grid - 1) / a.grid;
   if (line.padded) {
     const bool one = all1 <= a.grid;
     line.stretch = one ? S1 : S2;
@@ -324,6 +328,18 @@ __device__ __forceinline__ PagedLine paged_find(const PagedArgs& a, int s, Paged
   return line;
 }
 
+// The triple that the end of a work-group's stretch cuts, where that is the triple's first cut:
+// `more` pieces follow the work-group's own, which is in its slot `slot`; more = 0 where there
+// is no such triple. The workspace holds one of these for each work-group, then two partials
+// for each: 16 rows of O, then their log-sum-exps.
+struct PagedCut {
+  int b, triple, more, slot;
+};
+template <int D>
+__device__ __forceinline__ float* paged_part(const PagedArgs& a, int64_t slot) {
+  return a.part + a.grid * (sizeof(PagedCut) / 4) + slot * (kPagedRows * (D + 1));
+}
+
 // A wave's units of a piece: where the half units of its next 32 units lie, one a lane
 // (lane 2 k + half for unit k).
 struct PagedHalves {
@@ -336,7 +352,7 @@ struct PagedHalves {
 template <int D, class E, bool SHORT>
 __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArgs a) {
   using T = PagedTile<D>;
-  constexpr int KD = T::KD, DD = T::DD, NW = T::NW;
+  constexpr int KD = T::KD, DD = T::DD, NW = kPagedWaves;
   constexpr int LDS_FLOATS = NW * DD * 256 + 2 * NW * kPagedRows;
   static_assert(NW * T::TILE * 2 <= LDS_FLOATS * 4, "the V tiles and the merge share it");
   __shared__ __attribute__((aligned(16))) float lds[LDS_FLOATS];
@@ -349,7 +365,9 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArg
   // The stretch: `left` units from the place on. In a SHORT launch a triple of its own.
   PagedPlace at;
   int left;
+  int lead = 0, stretch = 0;
   bool padded = true;
+  PagedCut* const cut = reinterpret_cast<PagedCut*>(a.part) + blockIdx.x;
   if constexpr (SHORT) {
     at.b = blockIdx.x / (a.Hkv * a.blocks);
     at.triple = blockIdx.x - at.b * (a.Hkv * a.blocks);
@@ -357,11 +375,14 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArg
     at.len = uniform(a.lengths[at.b]);
     left = INT32_MAX;
   } else {
-    const PagedLine line = paged_find<NW>(a, blockIdx.x, &at);
+    const PagedLine line = paged_find<D, NW>(a, blockIdx.x, &at);
     const int64_t from = (int64_t)blockIdx.x * line.stretch;
+    if (tid == 0) cut->more = 0;
     if (from >= line.total) return;
     left = min(line.stretch, (int)(line.total - from));
+    stretch = line.stretch;
     padded = line.padded;
+    lead = line.lead;
   }
   bool opening = true;  // the stretch's first piece
 
@@ -391,7 +412,10 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArg
     const bool fits = len >= 0 && len <= a.M * a.S;
     const int keys = fits ? len : 0;
     const int units = paged_units(a, len);
-    const int u0 = at.unit, u1 = left < units - u0 ? u0 + left : units;
+    const int u0 = max(at.unit - lead, 0);
+    const int line_units = lead + units;
+    const int u1 = left < line_units - at.unit ? max(at.unit + left - lead, 0) : units;
+    if (u1 <= u0) return;  // the stretch ends before the triple's first unit
     const int kvh = at.triple / a.blocks, block = at.triple - kvh * a.blocks;
     const int rows = a.group * a.N;
 
@@ -590,7 +614,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArg
     const float inv = lt == 0.f ? 0.f : 1.0f / lt;  // a row that saw no key is 0
     const bool whole = SHORT || (u0 == 0 && u1 == units);
     const int64_t slot = (int64_t)blockIdx.x * 2 + (opening ? 0 : 1);
-    float* const part = a.part + slot * (kPagedRows * (D + 1));
+    float* const part = paged_part<D>(a, slot);
     half_t* const out =
         a.o + (((int64_t)at.b * a.Hkv * a.group + kvh * a.group + h) * a.N + n) * a.d;
 #pragma unroll
@@ -610,7 +634,9 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArg
       part[kPagedRows * D + c16] = lt == 0.f ? -INFINITY : mt + log2_fast(lt);
     __syncthreads();
 
-    left -= u1 - u0;
+    left -= line_units - at.unit;
+    if (!SHORT && tid == 0 && u0 == 0 && u1 < units)  // the triple goes on in other stretches
+      *cut = {at.b, at.triple, (stretch - 1 - left) / stretch, opening ? 0 : 1};
     if (padded || left <= 0) return;
     opening = false;
     at.unit = 0;
@@ -622,122 +648,135 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArg
   }
 }
 
-// Joins the pieces of the triples that the stretches' borders cut: block w the triple that the
-// border between stretches w and w + 1 cuts, if that is its first. Piece s of a row weighs
-// exp2(lse_s) against the others'. A lane holds four columns of a row; the four waves take every
-// fourth piece and merge through LDS, in a fixed order.
+constexpr int kJoinWaves = 4;
+
+// Joins the pieces of the triples that the ends of the stretches cut: block w the triple that
+// work-group w's cut names. Piece p of a row weighs exp2(lse_p) against the others'. A lane
+// holds four columns of a row, a block as many rows as a wave has lanes for; its four waves take
+// every fourth piece and merge through LDS, in a fixed order. Most blocks have two pieces to
+// join or none, and all is latency: each wave asks for its first piece beside the cut that says
+// whether it exists.
 template <int D, class E>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
-  constexpr int COLS = D / 4;                     // 4-column pieces of a row
-  constexpr int RPP = 64 / COLS;                  // rows of a pass
-  __shared__ __attribute__((aligned(16))) float acc_s[4][64][4];
-  __shared__ float m_s[4][64], l_s[4][64];
-  PagedPlace at;
-  const PagedLine line = paged_find<4>(a, blockIdx.x + 1, &at);
-  const int stretch = line.stretch;
-  const int64_t border = ((int64_t)blockIdx.x + 1) * stretch;
-  if (border >= line.total || at.unit == 0) return;     // it cuts no triple
-  if (at.unit > stretch) return;                        // not the triple's first border
-  const int units = line.units(paged_units(a, at.len));
-  const int more = (units - at.unit + stretch - 1) / stretch;  // pieces after the first
-  // The first piece is its stretch's only one if the triple starts with the stretch.
-  const int64_t first = (int64_t)blockIdx.x * 2 + (at.unit == stretch ? 0 : 1);
-  const int kvh = at.triple / a.blocks, block = at.triple - kvh * a.blocks;
-  const int rows = min(kPagedRows, a.group * a.N - block * kPagedRows);
-  constexpr int SLOT = kPagedRows * (D + 1);
+__global__ __launch_bounds__(64 * kJoinWaves) void paged_join_kernel(PagedArgs a) {
+  constexpr int W = kJoinWaves;
+  constexpr int COLS = D / 4;       // 4-column pieces of a row
+  constexpr int RPP = 64 / COLS;    // rows of a block
+  constexpr int AHEAD = 8;          // pieces of a wave asked for at once
+  __shared__ __attribute__((aligned(16))) float acc_s[W][64][4];
+  __shared__ float m_s[W][64], l_s[W][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int col = 4 * (lane % COLS);
-  for (int r0 = blockIdx.y * RPP; r0 < rows; r0 += gridDim.y * RPP) {
-    const int row = r0 + lane / COLS;
-    float m = -INFINITY, l = 0.f;
-    float4v acc = {0.f, 0.f, 0.f, 0.f};
-    if (row < rows) {
-      for (int p0 = wave; p0 <= more; p0 += 4 * 8) {
-        float ls[8];
-        float4v v[8];
+  const int w = blockIdx.x;
+  const int row = blockIdx.y * RPP + lane / COLS, col = 4 * (lane % COLS);
+  struct Piece {
+    float lse;
+    float4v o;
+  };
+  auto load = [&](int64_t slot) __attribute__((always_inline)) {
+    const float* part = paged_part<D>(a, slot);
+    return Piece{part[kPagedRows * D + row],
+                 *reinterpret_cast<const float4v*>(part + row * D + col)};
+  };
+  // Slot 0 of the work-group `wave` behind w (of w itself also slot 1): inside the workspace,
+  // and unused unless the cut says that it was written.
+  const int64_t ahead = min(w + wave, a.grid - 1);
+  const PagedCut cut = reinterpret_cast<const PagedCut*>(a.part)[w];
+  Piece p0 = load(2 * ahead);
+  if (wave == 0) {
+    const Piece p1 = load(2 * ahead + 1);
+    if (cut.slot != 0) p0 = p1;
+  }
+  if (cut.more == 0) return;
+  const int kvh = cut.triple / a.blocks, block = cut.triple - kvh * a.blocks;
+  const int rows = min(kPagedRows, a.group * a.N - block * kPagedRows);
+  float m = -INFINITY, l = 0.f;
+  float4v acc = {0.f, 0.f, 0.f, 0.f};
+  if (wave <= cut.more) {
+    m = p0.lse;
+    l = m == -INFINITY ? 0.f : 1.f;
+    acc = p0.o;
+    for (int at = wave + W; at <= cut.more; at += W * AHEAD) {
+      Piece p[AHEAD];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int p = p0 + 4 * i;
-          ls[i] = -INFINITY;
-          v[i] = {0.f, 0.f, 0.f, 0.f};
-          if (p <= more) {
-            const int64_t slot = p == 0 ? first : ((int64_t)blockIdx.x + p) * 2;
-            const float* part = a.part + slot * SLOT;
-            ls[i] = part[kPagedRows * D + row];
-            v[i] = *reinterpret_cast<const float4v*>(part + row * D + col);
-          }
-        }
-        float mx = m;
+      for (int i = 0; i < AHEAD; ++i)
+        p[i] = at + W * i <= cut.more ? load(2 * ((int64_t)w + at + W * i))
+                                      : Piece{-INFINITY, {0.f, 0.f, 0.f, 0.f}};
+      float mx = m;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mx = __builtin_fmaxf(mx, ls[i]);
-        const float ref = exp_reference(mx);
-        const float keep = m == -INFINITY ? 0.f : exp2_fast(m - ref);
-        l *= keep;
-        acc *= keep;
+      for (int i = 0; i < AHEAD; ++i) mx = __builtin_fmaxf(mx, p[i].lse);
+      const float ref = exp_reference(mx);
+      const float keep = m == -INFINITY ? 0.f : exp2_fast(m - ref);
+      l *= keep;
+      acc *= keep;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float w = ls[i] == -INFINITY ? 0.f : exp2_fast(ls[i] - ref);
-          l += w;
-          acc += v[i] * w;
-        }
-        m = mx;
+      for (int i = 0; i < AHEAD; ++i) {
+        const float f = p[i].lse == -INFINITY ? 0.f : exp2_fast(p[i].lse - ref);
+        l += f;
+        acc += p[i].o * f;
       }
-    }
-    __syncthreads();
-    *reinterpret_cast<float4v*>(acc_s[wave][lane]) = acc;
-    m_s[wave][lane] = m;
-    l_s[wave][lane] = l;
-    __syncthreads();
-    if (wave == 0 && row < rows && col < a.d) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) mx = __builtin_fmaxf(mx, m_s[w][lane]);
-      float lt = 0.f;
-      float4v v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float mw = m_s[w][lane];
-        const float f = mw == -INFINITY ? 0.f : exp2_fast(mw - mx);
-        lt += f * l_s[w][lane];
-        v += *reinterpret_cast<const float4v*>(acc_s[w][lane]) * f;
-      }
-      v *= lt == 0.f ? 0.f : 1.0f / lt;
-      const int r = block * kPagedRows + row;
-      const int h = r / a.N, n = r - h * a.N;
-      half_t* out = a.o + (((int64_t)at.b * a.Hkv * a.group + kvh * a.group + h) * a.N + n) * a.d;
-      *reinterpret_cast<u32x2*>(out + col) = pack4<E>(v[0], v[1], v[2], v[3]);
+      m = mx;
     }
   }
+  *reinterpret_cast<float4v*>(acc_s[wave][lane]) = acc;
+  m_s[wave][lane] = m;
+  l_s[wave][lane] = l;
+  __syncthreads();
+  if (wave != 0 || row >= rows || col >= a.d) return;
+  float mx = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < W; ++i) mx = __builtin_fmaxf(mx, m_s[i][lane]);
+  float lt = 0.f;
+  float4v v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    const float f = m_s[i][lane] == -INFINITY ? 0.f : exp2_fast(m_s[i][lane] - mx);
+    lt += f * l_s[i][lane];
+    v += *reinterpret_cast<const float4v*>(acc_s[i][lane]) * f;
+  }
+  v *= lt == 0.f ? 0.f : 1.0f / lt;
+  const int r = block * kPagedRows + row;
+  const int h = r / a.N, n = r - h * a.N;
+  half_t* out = a.o + (((int64_t)cut.b * a.Hkv * a.group + kvh * a.group + h) * a.N + n) * a.d;
+  *reinterpret_cast<u32x2*>(out + col) = pack4<E>(v[0], v[1], v[2], v[3]);
 }
 
-// Where a sequence's row of the table holds at most this many keys, a work-group takes a whole
-// triple: no line, no partials and no second launch.
-constexpr int64_t kPagedShort = 1024;
+// Where a sequence's row of the table holds few keys, a work-group takes a whole triple: no
+// line, no partials and no second launch. It reads at most 61 bytes a ns, what one CU draws
+// from HBM (four units in 1.07 us at D = 128; eight waves are no faster), so the bound is where
+// that takes as long as a second launch saves: D = 128, B x Hkv 8 / 64 / 256 triples, us, this /
+// split and joined: 512 keys 8.7 / 10.7, 9.2 / 11.5, 13.5 / 20.6; 1024 keys 12.9 / 10.7, 13.6 /
+// 17.1, 22.6 / 30.1; 2048 keys 21.3 / 11.3, 22.0 / 20.4, 48.2 / 56.4 (kernels alone; the second
+// launch adds about 1.5). A longer row may hold one long sequence among short ones, whose time
+// the split would share out.
+bool paged_short(int64_t triples, int64_t keys) {
+  return keys <= 1024 || (keys <= 2048 && triples >= 256);
+}
 
 // Two work-groups a CU, at most one for each four units that the tables could hold; 0: a
 // work-group for each triple.
 int paged_grid(int64_t B, int64_t Hkv, int64_t blocks, int64_t keys) {
-  if (keys <= kPagedShort) return 0;
-  const int64_t units = B * Hkv * blocks * ((keys + kPagedUnit - 1) / kPagedUnit);
-  return (int)std::clamp<int64_t>((units + 3) / 4, 1, 512);
+  const int64_t triples = B * Hkv * blocks;
+  if (paged_short(triples, keys)) return 0;
+  const int64_t units = triples * ((keys + kPagedUnit - 1) / kPagedUnit);
+  return (int)std::min<int64_t>((units + 3) / 4, 512);
 }
 
 template <int D, class E>
 hipError_t paged_start(const PagedArgs& a, hipStream_t stream) {
-  const dim3 block(64 * kPagedWaves);
   if (a.grid == 0) {
     const int64_t triples = (int64_t)a.B * a.Hkv * a.blocks;
     if (triples > 0x7fffffff) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((paged_fwd_kernel<D, E, true>), dim3((unsigned)triples), block, 0, stream, a);
+    hipLaunchKernelGGL((paged_fwd_kernel<D, E, true>), dim3((unsigned)triples),
+                       dim3(64 * kPagedWaves), 0, stream, a);
     return hipGetLastError();
   }
-  hipLaunchKernelGGL((paged_fwd_kernel<D, E, false>), dim3((unsigned)a.grid), block, 0, stream, a);
+  hipLaunchKernelGGL((paged_fwd_kernel<D, E, false>), dim3((unsigned)a.grid), dim3(64 * kPagedWaves),
+                     0, stream, a);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.grid == 1) return e;
+  if (e != hipSuccess) return e;
   constexpr int RPP = 64 / (D / 4);
   const int rows = std::min(kPagedRows, a.group * a.N);
   const dim3 grid((unsigned)(a.grid - 1), (unsigned)((rows + RPP - 1) / RPP));
-  hipLaunchKernelGGL((paged_join_kernel<D, E>), grid, dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((paged_join_kernel<D, E>), grid, dim3(64 * kJoinWaves), 0, stream, a);
   return hipGetLastError();
 }
 

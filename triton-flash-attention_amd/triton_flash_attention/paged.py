@@ -367,7 +367,7 @@ def paged_attention(
                 t.requires_grad for t in (query, key_cache, value_cache))):
             reason = "the paged kernel has no backward"
         elif Hq >= 1 << 20 or N >= 1 << 20 or B * H * -(-(Hq // H * N) // 16) * (
-                -(-page_table.shape[1] * S // 32)) >= 1 << 30:
+                -(-page_table.shape[1] * S // 32) + 24) >= 1 << 30:
             reason = "too many sequences, heads or keys for one launch"
         else:
             reason = _cache_reason(key_cache, value_cache) or _gpu_reason(query)
