@@ -67,7 +67,7 @@ int check_rope(const char* name, const RopeSizes& z, const void* q_weight, const
                      "%s: the rotated values R must be a multiple of 16 up to the head size "
                      "%lld; got %lld", name, (long long)z.D, (long long)z.R);
   if (z.Hq >= 1 << 15 || z.Hkv >= 1 << 15 || z.B >= (int64_t)1 << 31 || z.N >= (int64_t)1 << 31 ||
-      z.B * z.N >= (int64_t)1 << 34 || z.P >= (int64_t)1 << 40)
+      z.B * z.N >= (int64_t)1 << 31 || z.P >= (int64_t)1 << 40)
     return capi_fail(FA_ERR_TOO_LARGE, "%s: too many heads, tokens or positions", name);
   if (!q_weight != !k_weight)
     return capi_fail(FA_ERR_NULL_POINTER, "%s: one of the two norm weights is missing", name);

@@ -44,6 +44,32 @@ __device__ __forceinline__ T block_scan(T x, T* sums, T* total) {
   return before;
 }
 
+// Two sums over the threads before this one of a block of 256, and the block's totals, behind
+// one barrier.
+__device__ __forceinline__ void block_scan2(int64_t x, int64_t y, int64_t (*sums)[4],
+                                            int64_t* x_before, int64_t* y_before, int64_t* x_all,
+                                            int64_t* y_all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t xi = wave_scan(x, lane), yi = wave_scan(y, lane);
+  if (lane == 63) {
+    sums[0][wave] = xi;
+    sums[1][wave] = yi;
+  }
+  __syncthreads();
+  *x_before = xi - x;
+  *y_before = yi - y;
+  *x_all = *y_all = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < wave) {
+      *x_before += sums[0][w];
+      *y_before += sums[1][w];
+    }
+    *x_all += sums[0][w];
+    *y_all += sums[1][w];
+  }
+}
+
 }  // namespace
 
 // ---- plan -------------------------------------------------------------------------------
@@ -51,25 +77,27 @@ __device__ __forceinline__ T block_scan(T x, T* sums, T* total) {
 // these need come from the list of free ones, in the order of the sequences, so two running
 // sums over the sequences place everything: of new tokens (a token's row in the step) and of
 // new pages. Every block takes kPlanTokens tokens and computes the running sums itself, 1024
-// sequences at a time in LDS, then finds each token's sequence by bisection: one launch, and
-// no block waits for another. The first token on a new page writes the page's table entry.
-// A step's plan is bound by its chain of loads (lengths, then page ids), a prompt's by writing
-// 12 bytes a token.
+// sequences at a time in LDS: one launch, and no block waits for another. A thread has OWN
+// tokens, 256 apart, whose sequences it finds by bisections side by side. The first token on a
+// new page writes the page's table entry. What bounds it is the chain of loads (lengths, then
+// page ids) behind the launch: 64 sequences with a token each 4.2 us, 509 with 520 thousand 9.4.
 constexpr int kPlanSeqs = 1024;
-constexpr int kPlanTokens = 1024;
 constexpr int kPlanMost = (1 << 30) - 1;  // largest length and number of new tokens
 
+template <int OWN>
 __global__ __launch_bounds__(256) void paged_plan_kernel(PlanArgs a) {
-  __shared__ int64_t first[kPlanSeqs];  // a sequence's first token in the step
-  __shared__ int64_t page0[kPlanSeqs];  // its first new page's place in the free list
-  __shared__ int length[kPlanSeqs];
+  // Of the group's sequences: the first token in the step, from the group's on; the first new
+  // page's place in the free list; the tokens held. Sums past 2^31 - 1 stop there, behind every
+  // token and every free page.
+  __shared__ int first[kPlanSeqs], place[kPlanSeqs], length[kPlanSeqs];
   __shared__ int64_t sums[2][4];
   const int tid = threadIdx.x;
   const bool head = blockIdx.x == 0;
-  const int64_t t0 = (int64_t)blockIdx.x * kPlanTokens;
-  const int64_t t1 = min(a.T, t0 + kPlanTokens);
+  const int64_t t0 = (int64_t)blockIdx.x * (256 * OWN);
+  const int64_t t1 = min(a.T, t0 + 256 * OWN);
   int64_t tokens = 0;                                  // before this group of sequences
   int64_t pages = a.free_start ? a.free_start[0] : 0;  // place of its first new page
+  auto capped = [](int64_t x) { return (int)max(min(x, (int64_t)INT32_MAX), (int64_t)INT32_MIN); };
   for (int b0 = 0; b0 < a.B; b0 += kPlanSeqs) {
     if (tokens >= t1 && !head) return;  // the rest belongs to later blocks
     int len[4], add[4], need[4];
@@ -81,53 +109,72 @@ __global__ __launch_bounds__(256) void paged_plan_kernel(PlanArgs a) {
       if (b < a.B) {
         len[i] = min(max(a.lengths[b], 0), kPlanMost);
         add[i] = min(max(a.new_tokens[b], 0), kPlanMost);
-        const int held = (int)(((unsigned)len[i] + a.S - 1) / a.S);
-        const int then = (int)(((unsigned)(len[i] + add[i]) + a.S - 1) / a.S);
-        need[i] = max(min(then, a.M) - held, 0);  // a row of the table holds M pages
       }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int held = (int)(((unsigned)len[i] + a.S - 1) / a.S);
+      const int then = (int)(((unsigned)(len[i] + add[i]) + a.S - 1) / a.S);
+      need[i] = max(min(then, a.M) - held, 0);  // a row of the table holds M pages
       n += add[i];
       g += need[i];
     }
-    int64_t n_all, g_all;
-    int64_t n_at = tokens + block_scan(n, sums[0], &n_all);
-    int64_t g_at = pages + block_scan(g, sums[1], &g_all);
+    int64_t n_all, g_all, n_at, g_at;
+    block_scan2(n, g, sums, &n_at, &g_at, &n_all, &g_all);
+    g_at += pages;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int b = b0 + 4 * tid + i;
-      first[4 * tid + i] = n_at;
-      page0[4 * tid + i] = g_at;
+      first[4 * tid + i] = capped(n_at);
+      place[4 * tid + i] = capped(g_at);
       length[4 * tid + i] = len[i];
       if (head && b < a.B) {
-        a.starts[b] = (int)min(n_at, (int64_t)INT32_MAX);
+        a.starts[b] = capped(tokens + n_at);
         a.lengths_out[b] = len[i] + add[i];
       }
       n_at += add[i];
       g_at += need[i];
     }
     __syncthreads();
-    const int64_t end = min(t1, tokens + n_all);
-    for (int64_t t = max(t0, tokens) + tid; t < end; t += 256) {
-      int lo = 0, hi = kPlanSeqs;  // the last sequence with first <= t holds it
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (first[mid] <= t) lo = mid;
-        else hi = mid;
+    // The thread's tokens, from the group's first on, and the last sequence with first <= t,
+    // which holds token t.
+    const int from = (int)(max(t0, tokens) - tokens) + tid;
+    const int to = (int)(min(t1, tokens + n_all) - tokens);
+    const int count = min(kPlanSeqs, a.B - b0);
+    int seq[OWN], pos[OWN], page[OWN], in_page[OWN], entry[OWN];
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) seq[i] = 0;
+    for (int step = kPlanSeqs / 2; step > 0; step >>= 1) {
+      if (step >= count) continue;
+#pragma unroll
+      for (int i = 0; i < OWN; ++i)
+        if (seq[i] + step < count && first[seq[i] + step] <= from + 256 * i) seq[i] += step;
+    }
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      const int t = from + 256 * i;
+      page[i] = entry[i] = -1;
+      if (t >= to) continue;
+      const int held_tokens = length[seq[i]];
+      pos[i] = held_tokens + (t - first[seq[i]]);
+      const int j = pos[i] / a.S, held = (int)(((unsigned)held_tokens + a.S - 1) / a.S);
+      in_page[i] = pos[i] - j * a.S;
+      if (j >= a.M) continue;
+      if (j < held) {
+        page[i] = a.table[(int64_t)(b0 + seq[i]) * a.table_stride + j];
+      } else {
+        const int64_t at = (int64_t)place[seq[i]] + (j - held);
+        if (at >= 0 && at < a.F) page[i] = a.free_pages[at];
+        if (in_page[i] == 0) entry[i] = j;  // the page's first token
       }
-      const int pos = length[lo] + (int)(t - first[lo]);
-      const int j = pos / a.S, held = (int)(((unsigned)length[lo] + a.S - 1) / a.S);
-      int page = -1;
-      if (j < a.M) {
-        int* entry = a.table + (int64_t)(b0 + lo) * a.table_stride + j;
-        if (j < held) {
-          page = *entry;
-        } else {
-          const int64_t at = page0[lo] + (j - held);
-          if (at >= 0 && at < a.F) page = a.free_pages[at];
-          if (pos == j * a.S) *entry = page;
-        }
-      }
-      a.slots[t] = page < 0 ? -1 : (int64_t)page * a.S + (pos - j * a.S);
-      a.positions[t] = pos;
+    }
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      if (from + 256 * i >= to) continue;
+      const int64_t t = tokens + from + 256 * i;
+      if (entry[i] >= 0) a.table[(int64_t)(b0 + seq[i]) * a.table_stride + entry[i]] = page[i];
+      a.slots[t] = page[i] < 0 ? -1 : (int64_t)page[i] * a.S + in_page[i];
+      a.positions[t] = pos[i];
     }
     tokens += n_all;
     pages += g_all;
@@ -138,23 +185,33 @@ __global__ __launch_bounds__(256) void paged_plan_kernel(PlanArgs a) {
     a.positions[t] = 0;
   }
   if (head && tid == 0) {
-    a.starts[a.B] = (int)min(tokens, (int64_t)INT32_MAX);
-    a.free_out[0] = (int)min(max(pages, (int64_t)0), (int64_t)INT32_MAX);
+    a.starts[a.B] = capped(tokens);
+    a.free_out[0] = max(capped(pages), 0);
   }
 }
 
-hipError_t launch_paged_plan(const PlanArgs& a, hipStream_t stream) {
-  const int64_t blocks = std::max<int64_t>(1, (a.T + kPlanTokens - 1) / kPlanTokens);
+template <int OWN>
+hipError_t paged_plan_start(const PlanArgs& a, hipStream_t stream) {
+  const int64_t blocks = std::max<int64_t>(1, (a.T + 256 * OWN - 1) / (256 * OWN));
   if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
-  hipLaunchKernelGGL(paged_plan_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(paged_plan_kernel<OWN>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
   return hipGetLastError();
+}
+
+// Two tokens a thread once the blocks of one would not run at once (520 thousand tokens: 9.4 us
+// against 11.4; four 10.3); fewer steps behind each other before (64 tokens: 4.2 against 4.5).
+hipError_t launch_paged_plan(const PlanArgs& a, hipStream_t stream) {
+  return a.T <= 256 * 1024 ? paged_plan_start<1>(a, stream) : paged_plan_start<2>(a, stream);
 }
 
 // ---- store ------------------------------------------------------------------------------
 // Row t of the keys and values to slot t's row of every head: a copy in 16-byte pieces, bound
 // by memory. W neighbouring threads share a token and walk over its 2 H chunks pieces; each
-// thread has kStoreTokens tokens in flight. Slots outside the cache are left out.
-constexpr int kStoreTokens = 4;
+// thread has kStoreTokens tokens in flight. Slots outside the cache are left out. The rows are
+// written past the caches: they are whole lines in no order, which the L2 would only hold up
+// (16381 tokens, 14334 of them stored, H8 D128: 26.2 -> 19.4 us, 6.0 TB/s; a step's 32 tokens
+// 3.6 -> 3.0 with two tokens a thread in place of four).
+constexpr int kStoreTokens = 2;
 
 template <int W>
 __global__ __launch_bounds__(256) void paged_store_kernel(StoreArgs a) {
@@ -185,7 +242,8 @@ __global__ __launch_bounds__(256) void paged_store_kernel(StoreArgs a) {
 #pragma unroll
     for (int i = 0; i < kStoreTokens; ++i)
       if (page[i] >= 0)
-        *reinterpret_cast<u32x4*>(dst + page[i] * a.ds[0] + row[i] * a.ds[2]) = v[i];
+        __builtin_nontemporal_store(
+            v[i], reinterpret_cast<u32x4*>(dst + page[i] * a.ds[0] + row[i] * a.ds[2]));
   }
 }
 

@@ -55,7 +55,8 @@ __device__ __forceinline__ u32x4 pack8(const float* f) {
 struct RopeLane {
   int c0, c1;        // first value of each chunk
   bool has0, has1;   // it exists
-  bool turns;        // the pair is rotated
+  bool turns, turns1;  // the pair, or with pairs inside a chunk each chunk, is rotated
+  int a0, a1;        // first of each four angles
   float cos[8], sin[8];
   float poison;      // 0, or NaN for a token whose position is outside the tables
 };
@@ -65,7 +66,10 @@ __device__ __forceinline__ RopeLane rope_lane(const RopeArgs& a, int p) {
   RopeLane l;
   const int turned = a.R / 16;  // pairs of chunks that are rotated
   int c0, c1;
-  if (INTER || p >= turned) {
+  if constexpr (INTER) {  // pairs within a chunk: any two chunks
+    c0 = p;
+    c1 = p + LPR;
+  } else if (p >= turned) {
     c0 = 2 * p;
     c1 = c0 + 1;
   } else {
@@ -76,14 +80,17 @@ __device__ __forceinline__ RopeLane rope_lane(const RopeArgs& a, int p) {
   l.c1 = 8 * c1;
   l.has0 = l.c0 < a.D;
   l.has1 = l.c1 < a.D;
-  l.turns = p < turned;
+  l.turns = INTER ? l.c0 < a.R : p < turned;
+  l.turns1 = INTER ? l.c1 < a.R : l.turns;
+  // the first of the two chunks' angles
+  l.a0 = INTER ? 4 * c0 : 8 * p;
+  l.a1 = INTER ? 4 * c1 : 8 * p + 4;
   return l;
 }
 
 // The angles of token (b, n). A position outside the tables reads nothing and makes the
 // token's rows NaN.
-__device__ __forceinline__ void rope_angles(const RopeArgs& a, int64_t b, int n, int p,
-                                            RopeLane& l) {
+__device__ __forceinline__ void rope_angles(const RopeArgs& a, int64_t b, int n, RopeLane& l) {
   int64_t pos = n;
   if (a.pos) {
     const int64_t i = b * a.pos_sb + n * a.pos_sn;
@@ -92,24 +99,22 @@ __device__ __forceinline__ void rope_angles(const RopeArgs& a, int64_t b, int n,
   }
   const bool ok = pos >= 0 && pos < a.P;
   l.poison = ok ? 0.f : __builtin_nanf("");
+  const int64_t at = ok ? pos * (a.R / 2) : 0;
+  float4v c0 = {1.f, 1.f, 1.f, 1.f}, c1 = c0, s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
   if (ok && l.turns) {
-    const int64_t at = pos * (a.R / 2) + 8 * p;
-    const float4v* c = reinterpret_cast<const float4v*>(a.cos + at);
-    const float4v* s = reinterpret_cast<const float4v*>(a.sin + at);
-    const float4v c0 = c[0], c1 = c[1], s0 = s[0], s1 = s[1];
+    c0 = *reinterpret_cast<const float4v*>(a.cos + at + l.a0);
+    s0 = *reinterpret_cast<const float4v*>(a.sin + at + l.a0);
+  }
+  if (ok && l.turns1) {
+    c1 = *reinterpret_cast<const float4v*>(a.cos + at + l.a1);
+    s1 = *reinterpret_cast<const float4v*>(a.sin + at + l.a1);
+  }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      l.cos[e] = c0[e];
-      l.cos[4 + e] = c1[e];
-      l.sin[e] = s0[e];
-      l.sin[4 + e] = s1[e];
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      l.cos[e] = 1.f;
-      l.sin[e] = 0.f;
-    }
+  for (int e = 0; e < 4; ++e) {
+    l.cos[e] = c0[e];
+    l.cos[4 + e] = c1[e];
+    l.sin[e] = s0[e];
+    l.sin[4 + e] = s1[e];
   }
 }
 
@@ -118,22 +123,23 @@ __device__ __forceinline__ void rope_angles(const RopeArgs& a, int64_t b, int n,
 // infinity to its partner).
 template <bool INTER, int DIR>
 __device__ __forceinline__ void rope_turn(const RopeLane& l, float* v0, float* v1) {
-  if (!l.turns) return;
   auto turn = [&](float& x, float& y, float c, float s) __attribute__((always_inline)) {
     const float t = DIR * s;
     const float nx = x * c - y * t;
     y = y * c + x * t;
     x = nx;
   };
+  if constexpr (!INTER) {
+    if (!l.turns) return;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    if constexpr (!INTER) {
-      turn(v0[e], v1[e], l.cos[e], l.sin[e]);
-    } else if (e < 4) {
-      turn(v0[2 * e], v0[2 * e + 1], l.cos[e], l.sin[e]);
-    } else {
-      turn(v1[2 * e - 8], v1[2 * e - 7], l.cos[e], l.sin[e]);
-    }
+    for (int e = 0; e < 8; ++e) turn(v0[e], v1[e], l.cos[e], l.sin[e]);
+  } else {
+    if (l.turns)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) turn(v0[2 * e], v0[2 * e + 1], l.cos[e], l.sin[e]);
+    if (l.turns1)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) turn(v1[2 * e], v1[2 * e + 1], l.cos[4 + e], l.sin[4 + e]);
   }
 }
 
@@ -176,49 +182,76 @@ __device__ __forceinline__ RopeHeads rope_heads(const RopeArgs& a, int y) {
 
 }  // namespace
 
+// A row as it comes, two 16-byte chunks a lane.
+struct RopeRow {
+  u32x4 c0, c1;
+};
+__device__ __forceinline__ RopeRow load_row(const half_t* row, const RopeLane& l) {
+  return {load_chunk(row, l.c0, l.has0), load_chunk(row, l.c1, l.has1)};
+}
+template <class E>
+__device__ __forceinline__ void store_row(half_t* row, const RopeLane& l, const float* v0,
+                                          const float* v1) {
+  if (l.has0) *reinterpret_cast<u32x4*>(row + l.c0) = pack8<E>(v0);
+  if (l.has1) *reinterpret_cast<u32x4*>(row + l.c1) = pack8<E>(v1);
+}
+
+// f(h, row[0]) for the heads [first, last), rows asked for U at a time.
+template <int U, class Load, class Use>
+__device__ __forceinline__ void rope_walk(int first, int last, Load load, Use use) {
+  int h = first;
+  for (; h + U <= last; h += U) {
+    decltype(load(0)) r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) r[u] = load(h + u);
+#pragma unroll
+    for (int u = 0; u < U; ++u) use(h + u, r[u]);
+  }
+  for (; h < last; ++h) use(h, load(h));
+}
+
 template <int LPR, class E, bool NORM, bool INTER>
 __global__ __launch_bounds__(64 * kRopeWaves) void rope_kernel(RopeArgs a) {
   constexpr int TPW = 64 / LPR;  // tokens of a wave
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int p = lane % LPR;
-  const int64_t t = ((int64_t)blockIdx.x * kRopeWaves + wave) * TPW + lane / LPR;
-  if (t >= a.T) return;  // all lanes of a row at once: the sums stay within a row
+  const uint32_t t = (blockIdx.x * kRopeWaves + wave) * TPW + lane / LPR;
+  if (t >= (uint32_t)a.T) return;  // all lanes of a row at once: the sums stay within a row
   const RopeHeads hs = rope_heads(a, blockIdx.y);
   const RopeSide& s = a.side[hs.side];
-  const int64_t b = t / a.N;
-  const int n = (int)(t - b * a.N);
+  const int64_t b = t / (uint32_t)a.N;
+  const int n = (int)(t - (uint32_t)b * (uint32_t)a.N);
   RopeLane l = rope_lane<LPR, INTER>(a, p);
-  rope_angles(a, b, n, p, l);
+  rope_angles(a, b, n, l);
   float w0[8], w1[8];
   if constexpr (NORM) rope_weights<E>(a, s.w, l, w0, w1);
-  const half_t* x = s.x + b * s.xs[0] + n * s.xs[2];
-  half_t* out = s.out + ((int64_t)b * s.H * a.N + n) * a.D;
-  for (int h = hs.first; h < hs.last; ++h) {
-    const half_t* row = x + h * s.xs[1];
-    float v0[8], v1[8];
-    unpack8<E>(load_chunk(row, l.c0, l.has0), v0);
-    unpack8<E>(load_chunk(row, l.c1, l.has1), v1);
-    if constexpr (NORM) {
-      float ss = 0.f;
+  const half_t* const x = s.x + b * s.xs[0] + n * s.xs[2];
+  half_t* const out = s.out + (b * s.H * a.N + n) * a.D;
+  rope_walk<4>(
+      hs.first, hs.last, [&](int h) __attribute__((always_inline)) { return load_row(x + h * s.xs[1], l); },
+      [&](int h, const RopeRow& row) __attribute__((always_inline)) {
+        float v0[8], v1[8];
+        unpack8<E>(row.c0, v0);
+        unpack8<E>(row.c1, v1);
+        if constexpr (NORM) {
+          float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss += v0[e] * v0[e] + v1[e] * v1[e];
-      const float r = __builtin_amdgcn_rsqf(row_sum<LPR>(ss) / (float)a.D + a.eps);
+          for (int e = 0; e < 8; ++e) ss += v0[e] * v0[e] + v1[e] * v1[e];
+          const float r = __builtin_amdgcn_rsqf(row_sum<LPR>(ss) / (float)a.D + a.eps);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v0[e] *= r * w0[e];
-        v1[e] *= r * w1[e];
-      }
-    }
-    rope_turn<INTER, 1>(l, v0, v1);
+          for (int e = 0; e < 8; ++e) {
+            v0[e] *= r * w0[e];
+            v1[e] *= r * w1[e];
+          }
+        }
+        rope_turn<INTER, 1>(l, v0, v1);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      v0[e] += l.poison;
-      v1[e] += l.poison;
-    }
-    half_t* o = out + (int64_t)h * a.N * a.D;
-    if (l.has0) *reinterpret_cast<u32x4*>(o + l.c0) = pack8<E>(v0);
-    if (l.has1) *reinterpret_cast<u32x4*>(o + l.c1) = pack8<E>(v1);
-  }
+        for (int e = 0; e < 8; ++e) {
+          v0[e] += l.poison;
+          v1[e] += l.poison;
+        }
+        store_row<E>(out + (int64_t)h * a.N * a.D, l, v0, v1);
+      });
 }
 
 // Backward. A block takes every gridDim.x-th group of tokens, so that the number of
@@ -235,53 +268,61 @@ __global__ __launch_bounds__(64 * kRopeWaves) void rope_bwd_kernel(RopeArgs a) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) d0[e] = d1[e] = 0.f;
   if constexpr (NORM) rope_weights<E>(a, s.w, l, w0, w1);
-  const int64_t step = (int64_t)gridDim.x * kRopeWaves * TPW;
-  for (int64_t t = ((int64_t)blockIdx.x * kRopeWaves + wave) * TPW + lane / LPR; t < a.T;
+  const uint32_t step = gridDim.x * kRopeWaves * TPW;
+  for (uint32_t t = (blockIdx.x * kRopeWaves + wave) * TPW + lane / LPR; t < (uint32_t)a.T;
        t += step) {
-    const int64_t b = t / a.N;
-    const int n = (int)(t - b * a.N);
-    rope_angles(a, b, n, p, l);
-    const half_t* g = s.g + b * s.gs[0] + n * s.gs[2];
-    const half_t* x = NORM ? s.x + b * s.xs[0] + n * s.xs[2] : nullptr;
-    half_t* out = s.out + ((int64_t)b * s.H * a.N + n) * a.D;
-    for (int h = hs.first; h < hs.last; ++h) {
-      float u0[8], u1[8], x0[8], x1[8];
-      unpack8<E>(load_chunk(g + h * s.gs[1], l.c0, l.has0), u0);
-      unpack8<E>(load_chunk(g + h * s.gs[1], l.c1, l.has1), u1);
-      if constexpr (NORM) {
-        unpack8<E>(load_chunk(x + h * s.xs[1], l.c0, l.has0), x0);
-        unpack8<E>(load_chunk(x + h * s.xs[1], l.c1, l.has1), x1);
-      }
-      rope_turn<INTER, -1>(l, u0, u1);
-      if constexpr (NORM) {
-        float ss = 0.f, tx = 0.f;  // sums of x^2 and of t x
+    const int64_t b = t / (uint32_t)a.N;
+    const int n = (int)(t - (uint32_t)b * (uint32_t)a.N);
+    rope_angles(a, b, n, l);
+    const half_t* const g = s.g + b * s.gs[0] + n * s.gs[2];
+    const half_t* const x = NORM ? s.x + b * s.xs[0] + n * s.xs[2] : nullptr;
+    half_t* const out = s.out + (b * s.H * a.N + n) * a.D;
+    struct Rows {
+      RopeRow g, x;
+    };
+    rope_walk<2>(
+        hs.first, hs.last,
+        [&](int h) __attribute__((always_inline)) {
+          Rows r;
+          r.g = load_row(g + h * s.gs[1], l);
+          if constexpr (NORM) r.x = load_row(x + h * s.xs[1], l);
+          return r;
+        },
+        [&](int h, const Rows& row) __attribute__((always_inline)) {
+          float u0[8], u1[8];
+          unpack8<E>(row.g.c0, u0);
+          unpack8<E>(row.g.c1, u1);
+          rope_turn<INTER, -1>(l, u0, u1);
+          if constexpr (NORM) {
+            float x0[8], x1[8];
+            unpack8<E>(row.x.c0, x0);
+            unpack8<E>(row.x.c1, x1);
+            float ss = 0.f, tx = 0.f;  // sums of x^2 and of t x
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          ss += x0[e] * x0[e] + x1[e] * x1[e];
-          tx += u0[e] * w0[e] * x0[e] + u1[e] * w1[e] * x1[e];
-        }
-        const float inv_d = 1.f / (float)a.D;
-        const float r = __builtin_amdgcn_rsqf(row_sum<LPR>(ss) * inv_d + a.eps) + l.poison;
-        const float m = row_sum<LPR>(tx) * r * inv_d;  // mean of t x r
+            for (int e = 0; e < 8; ++e) {
+              ss += x0[e] * x0[e] + x1[e] * x1[e];
+              tx += u0[e] * w0[e] * x0[e] + u1[e] * w1[e] * x1[e];
+            }
+            const float inv_d = 1.f / (float)a.D;
+            const float r = __builtin_amdgcn_rsqf(row_sum<LPR>(ss) * inv_d + a.eps) + l.poison;
+            const float m = row_sum<LPR>(tx) * r * inv_d;  // mean of t x r
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float n0 = x0[e] * r, n1 = x1[e] * r;
-          d0[e] += u0[e] * n0;
-          d1[e] += u1[e] * n1;
-          u0[e] = r * (u0[e] * w0[e] - n0 * m);
-          u1[e] = r * (u1[e] * w1[e] - n1 * m);
-        }
-      } else {
+            for (int e = 0; e < 8; ++e) {
+              const float n0 = x0[e] * r, n1 = x1[e] * r;
+              d0[e] += u0[e] * n0;
+              d1[e] += u1[e] * n1;
+              u0[e] = r * (u0[e] * w0[e] - n0 * m);
+              u1[e] = r * (u1[e] * w1[e] - n1 * m);
+            }
+          } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          u0[e] += l.poison;
-          u1[e] += l.poison;
-        }
-      }
-      half_t* o = out + (int64_t)h * a.N * a.D;
-      if (l.has0) *reinterpret_cast<u32x4*>(o + l.c0) = pack8<E>(u0);
-      if (l.has1) *reinterpret_cast<u32x4*>(o + l.c1) = pack8<E>(u1);
-    }
+            for (int e = 0; e < 8; ++e) {
+              u0[e] += l.poison;
+              u1[e] += l.poison;
+            }
+          }
+          store_row<E>(out + (int64_t)h * a.N * a.D, l, u0, u1);
+        });
   }
   if constexpr (NORM) {
     if (s.part == nullptr) return;
@@ -329,23 +370,27 @@ struct RopeReduceArgs {
   int w32;
 };
 
-// dw = the sum of the blocks' partial sums: 16 columns of one tensor a block, 16 threads a
-// column that each add every 16th row.
+// dw = the sum of the blocks' partial sums: 16 columns of one tensor a block, 64 threads a
+// column that each add every 64th row.
+constexpr int kReduceGroups = 64;
+
 template <class E>
-__global__ __launch_bounds__(256) void rope_reduce_kernel(RopeReduceArgs a) {
-  __shared__ float sums[16][17];
+__global__ __launch_bounds__(16 * kReduceGroups) void rope_reduce_kernel(RopeReduceArgs a) {
+  __shared__ float sums[kReduceGroups][17];
   const int side = blockIdx.y, c = threadIdx.x & 15, g = threadIdx.x >> 4;
   const int col = blockIdx.x * 16 + c;
   if (a.dw[side] == nullptr) return;
   float v = 0.f;
-  if (col < a.D)
-    for (int r = g; r < a.rows[side]; r += 16) v += a.part[side][(int64_t)r * a.D + col];
+  if (col < a.D) {
+#pragma unroll 8
+    for (int r = g; r < a.rows[side]; r += kReduceGroups) v += a.part[side][(int64_t)r * a.D + col];
+  }
   sums[g][c] = v;
   __syncthreads();
   if (g != 0 || col >= a.D) return;
   v = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v += sums[i][c];
+  for (int i = 0; i < kReduceGroups; ++i) v += sums[i][c];
   if (a.w32) static_cast<float*>(a.dw[side])[col] = v;
   else static_cast<half_t*>(a.dw[side])[col] = to_elem<E>(v);
 }
@@ -353,6 +398,9 @@ __global__ __launch_bounds__(256) void rope_reduce_kernel(RopeReduceArgs a) {
 namespace {
 
 int rope_lanes(int D) { return D > 64 ? 8 : D > 32 ? 4 : 2; }
+
+constexpr int64_t kRopeBlocks = 384;
+constexpr int64_t kRopeBwdBlocks = 512;
 
 // A launch: `heads` heads of one tensor a chunk, chunks[0] of the queries and chunks[1] of the
 // keys along the grid's second axis, `grid` blocks along its first.
@@ -367,12 +415,12 @@ RopePlan rope_plan(int64_t T, int D, int Hq, int Hkv, bool bwd) {
   const int64_t tokens = kRopeWaves * 64 / rope_lanes(D);
   const int64_t tiles = (T + tokens - 1) / tokens;
   RopePlan p;
-  // As few heads a chunk as fill the chip (about 2048 blocks).
-  p.heads = (int)std::clamp<int64_t>(tiles * (Hq + Hkv) / 2048, 1, 16);
+  // As few heads a chunk as fill the chip (about kRopeBlocks blocks).
+  p.heads = (int)std::clamp<int64_t>(tiles * (Hq + Hkv) / kRopeBlocks, 1, 16);
   p.chunks[0] = (Hq + p.heads - 1) / p.heads;
   p.chunks[1] = (Hkv + p.heads - 1) / p.heads;
   p.grid = tiles;
-  if (bwd) p.grid = std::min(tiles, std::max<int64_t>(1, 512 / (p.chunks[0] + p.chunks[1])));
+  if (bwd) p.grid = std::min(tiles, std::max<int64_t>(1, kRopeBwdBlocks / (p.chunks[0] + p.chunks[1])));
   return p;
 }
 
@@ -440,8 +488,8 @@ hipError_t launch_rope_bwd(const RopeArgs& args, int dtype, bool norm, bool inte
   r.D = a.D;
   r.w32 = a.w32;
   const dim3 grid((unsigned)((a.D + 15) / 16), 2);
-  if (dtype == kBF16) hipLaunchKernelGGL((rope_reduce_kernel<BF16>), grid, dim3(256), 0, stream, r);
-  else hipLaunchKernelGGL((rope_reduce_kernel<F16>), grid, dim3(256), 0, stream, r);
+  if (dtype == kBF16) hipLaunchKernelGGL((rope_reduce_kernel<BF16>), grid, dim3(16 * kReduceGroups), 0, stream, r);
+  else hipLaunchKernelGGL((rope_reduce_kernel<F16>), grid, dim3(16 * kReduceGroups), 0, stream, r);
   return hipGetLastError();
 }
 

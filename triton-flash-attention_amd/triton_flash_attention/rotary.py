@@ -115,7 +115,7 @@ def _validate(query, key, cos, sin, query_weight, key_weight, eps, positions, in
             raise ValueError("positions must be int32 or int64 on the query's device")
 
 
-def _kernel_reason(query, cos, sin) -> str | None:
+def _kernel_reason(query, key, cos, sin) -> str | None:
     if query.device.type != "cuda":
         return _gpu_reason(query)
     if query.dtype not in _SUPPORTED_DTYPES:
@@ -124,7 +124,7 @@ def _kernel_reason(query, cos, sin) -> str | None:
         return "head_dim must be a multiple of 8 of at most 128"
     if cos.shape[1] % 8:
         return "the number of rotated values must be a multiple of 16"
-    if max(query.shape[1], query.shape[0] * query.shape[2] >> 20) >= 1 << 14:
+    if max(query.shape[1], key.shape[1]) >= 1 << 15 or query.shape[0] * query.shape[2] >= 1 << 31:
         return "too many heads or tokens for one launch"
     if _forward_ad_active() or (torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad)):
         return "the kernel has no derivative in cos and sin and no forward-mode derivative"
@@ -215,7 +215,7 @@ def qk_norm_rope(
             return out
     _check_backend(backend)
     _validate(query, key, cos, sin, query_weight, key_weight, eps, positions, interleaved)
-    if _falls_back(backend, None if backend == "torch" else _kernel_reason(query, cos, sin)):
+    if _falls_back(backend, None if backend == "torch" else _kernel_reason(query, key, cos, sin)):
         return tuple(_torch_rope(x, w, cos, sin, eps, positions, interleaved).contiguous()
                      for x, w in ((query, query_weight), (key, key_weight)))
     weights = () if query_weight is None else (query_weight, key_weight)
