@@ -236,6 +236,9 @@ def test_store_kernel_copies_keys_it_cannot_read():
         assert torch.equal(c[1, :, 15], t[1]) and torch.equal(c[0, :, 5], t[2])
 
 
+_SAME = torch.zeros(4, 2, 16, 32).half()
+
+
 def _store_args(device="cpu", dtype=torch.float16):
     z = dict(dtype=dtype, device=device)
     return dict(key=torch.zeros(3, 2, 32, **z), value=torch.zeros(3, 2, 32, **z),
@@ -259,6 +262,7 @@ def _store_args(device="cpu", dtype=torch.float16):
     (dict(slots=[0, 1, 2]), TypeError, "slots"),
     (dict(key=torch.zeros(3, 2, 32).half().requires_grad_()), RuntimeError, "no gradients"),
     (dict(key_cache=torch.zeros(1, 2, 16, 32).half().expand(4, 2, 16, 32)), ValueError, "expanded"),
+    (dict(key_cache=_SAME, value_cache=_SAME), ValueError, "different tensors"),
     (dict(backend="triton"), RuntimeError, "CUDA tensor"),
 ])
 def test_store_refusals(change, error, message):
@@ -272,9 +276,9 @@ def test_store_kernel_refuses_caches_it_cannot_address():
     with pytest.raises(RuntimeError, match="same strides"):
         paged_cache_store(**{**a, "key_cache": torch.zeros(4, 16, 2, 32, device="cuda").half()
                              .transpose(1, 2)}, backend="triton")
-    odd = torch.zeros(4, 2, 16, 33, device="cuda").half()[..., 1:]
+    odd, odd2 = (torch.zeros(4, 2, 16, 33, device="cuda").half()[..., 1:] for _ in range(2))
     with pytest.raises(RuntimeError, match="16-byte aligned"):
-        paged_cache_store(**{**a, "key_cache": odd, "value_cache": odd}, backend="triton")
+        paged_cache_store(**{**a, "key_cache": odd, "value_cache": odd2}, backend="triton")
     b = _store_args("cuda", torch.float32)
     with pytest.raises(RuntimeError, match="float16 and bfloat16"):
         paged_cache_store(**b, backend="triton")
@@ -468,6 +472,39 @@ def test_attention_kernel_over_work_groups(case, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("case", [
+    # tables wide enough for the launch that splits, filled a little or a lot
+    ([40], 4, 1, 1, 64, 16, 80),              # lines with room for every head: one round
+    ([40, 300, 7, 0, 1], 8, 2, 1, 128, 16, 80),
+    ([2000, 3, 2000], 8, 8, 1, 64, 16, 130),  # two rounds
+    ([0, 0, 0], 4, 2, 1, 32, 16, 100),
+    (ragged(600, 30, 12), 2, 2, 1, 32, 16, 70),    # several sequences a thread
+    (ragged(1100, 9, 13), 4, 4, 1, 64, 16, 70),    # many short pieces a work-group
+    (ragged(24, 1100, 14), 16, 4, 3, 128, 16, 90),
+    ([17] * 40 + [5000] + [17] * 40, 8, 2, 1, 64, 16, 320),
+    ([1500] * 64, 4, 4, 1, 32, 16, 100),      # 256 heads, at most 2048 keys: one launch
+])
+def test_attention_kernel_in_wide_tables(case):
+    *shape, M = case
+    check_attend(*shape, torch.float16, M=M, device="cuda", backend="triton")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(16))
+def test_attention_kernel_random(seed):
+    rng = random.Random(seed)
+    Hkv = rng.choice([1, 2, 3, 5])
+    S, B = rng.choice([16, 32, 48, 80]), rng.choice([1, 2, 7, 33, 90])
+    hi = rng.choice([60, 700, 3000]) if B < 90 else 300
+    lengths = ragged(B, hi, seed)
+    check_attend(lengths, Hkv * rng.choice([1, 2, 4, 6]), Hkv, rng.choice([1, 1, 2, 3]),
+                 rng.choice([8, 32, 48, 64, 104, 128]), S, rng.choice([torch.float16, torch.bfloat16]),
+                 layout=rng.choice(["heads", "tokens"]), q_layout=rng.choice(["heads", "tokens"]),
+                 M=max(cdiv(hi, S), rng.choice([1, cdiv(1100, S), cdiv(9000, S)])), seed=seed,
+                 device="cuda", backend="triton")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1.7, 1e-40])
 def test_attention_kernel_scales(scale):
     check_attend([400, 7, 0], 4, 2, 2, 64, 16, torch.float16, scale=scale, device="cuda",
@@ -658,6 +695,91 @@ def test_decoding_loop_kernels(dtype):
 @pytest.mark.gpu
 def test_decoding_loop_captured_and_replayed():
     decode("cuda", "triton", torch.bfloat16, 12, graph=True)
+
+
+def test_torch_forms_compile():
+    """The PyTorch forms trace as one graph."""
+    a = _attend_args(dtype=torch.float32)
+
+    def f(q, t, n):
+        o = paged_attention(q, a["key_cache"], a["value_cache"], t, n, enable_gqa=True)
+        return o + paged_cache_plan(t, n, n, n, page_size=16, num_tokens=4).slots.sum()
+
+    args = (a["query"], a["page_table"], a["lengths"])
+    torch._dynamo.reset()
+    torch.testing.assert_close(torch.compile(f, fullgraph=True, backend="eager")(*args), f(*args))
+
+
+@pytest.mark.gpu
+def test_kernels_under_torch_compile():
+    """Calls that the kernels serve run beside the compiled graph, with the same results."""
+    a = _attend_args("cuda")
+    a["key_cache"].normal_()
+    a["value_cache"].normal_()
+    a["query"].normal_()
+    a["lengths"].fill_(20)
+    cos = torch.randn(4, 16, device="cuda")
+
+    def f(q):
+        q, k = qk_norm_rope(q + 1, q - 1, cos, cos)
+        return paged_attention(q * 2, a["key_cache"], a["value_cache"], a["page_table"],
+                               a["lengths"], enable_gqa=True) + k
+
+    with torch.no_grad():
+        torch._dynamo.reset()
+        assert torch.equal(torch.compile(f, backend="eager")(a["query"]), f(a["query"]))
+
+
+@pytest.mark.gpu
+def test_kernels_from_two_threads_on_two_streams():
+    """Calls at once, each with tensors and a workspace of its own."""
+    import threading
+
+    failures = []
+
+    def work(seed):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for i in range(4):
+                    check_attend([2500, 40, 1200], 8, 2, 1, 64, 16, torch.float16,
+                                 seed=10 * seed + i, device="cuda", backend="triton")
+                    check_plan(ragged(70, 300, seed), ragged(70, 9, i), 16, device="cuda",
+                               backend="triton")
+                stream.synchronize()
+        except BaseException as e:  # noqa: BLE001 - raised below
+            failures.append(e)
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures[0]
+
+
+@pytest.mark.gpu
+def test_two_captured_steps_replayed_in_turn():
+    """Two graphs of attention calls that share torch's pool: each keeps its own partials."""
+    cases = [make_paged([3000, 17], 2, 16, 64, torch.float16, device="cuda", seed=s) for s in (1, 2)]
+    gen = torch.Generator().manual_seed(4)
+    q = torch.randn(2, 8, 1, 64, generator=gen).half().cuda()
+    pool = torch.cuda.graph_pool_handle()
+    graphs, outs, wants = [], [], []
+    for views, table, lens, dense in cases:
+        paged_attention(q, *views, table, lens, enable_gqa=True, backend="triton")
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            outs.append(paged_attention(q, *views, table, lens, enable_gqa=True, backend="triton"))
+        graphs.append(g)
+    for i in range(3):
+        q.copy_(torch.randn(2, 8, 1, 64, generator=gen).half())
+        wants = [paged_attention(q, *v, t, n, enable_gqa=True, backend="triton")
+                 for v, t, n, _ in cases]
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, wants)), i
 
 
 @pytest.mark.gpu

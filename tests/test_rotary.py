@@ -404,11 +404,11 @@ def test_capture_beside_a_living_graph_of_the_same_leaves_is_refused():
         with pytest.raises(RuntimeError, match="same leaf tensors"):
             qk_norm_rope(q, k, cos, sin, backend="triton")
     want = torch.autograd.grad(alive, q, gq)[0]
-    del alive
-    with torch.cuda.graph(torch.cuda.CUDAGraph()) as _:
+    del alive, _
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
         out, _ = qk_norm_rope(q, k, cos, sin, backend="triton")
         torch.autograd.grad(out, q, gq)
-    del out
+    del out, _
     out, _ = qk_norm_rope(q, k, cos, sin, backend="triton")
     assert torch.equal(torch.autograd.grad(out, q, gq)[0], want)
     assert z.shape == gq.shape

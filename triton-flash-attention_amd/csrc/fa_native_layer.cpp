@@ -230,7 +230,8 @@ class QkNormRope : public torch::autograd::Function<QkNormRope> {
       row_strides(q, s + 6);
       row_strides(k, s + 9);
       for (int i = 0; i < 2; ++i)
-        if (ctx->needs_input_grad(2 + i)) dw[i] = at::empty_like(r.qw);
+        if (ctx->needs_input_grad(2 + i))
+          dw[i] = at::empty(r.qw.sizes(), r.qw.options().requires_grad(false));
     }
     r.position_strides(s + 12);
     const auto like = gq.options().requires_grad(false);
@@ -415,7 +416,7 @@ bool native_store(py::handle key, py::handle value, py::handle key_cache, py::ha
                    *vc = plain(value_cache), *s = plain(slots);
   if (!k || !v || !kc || !vc || !s || !plain_caches(*kc, *vc) || !served(kc->device())) return false;
   const at::Device device = kc->device();
-  if (k->scalar_type() != kc->scalar_type() || v->scalar_type() != kc->scalar_type() ||
+  if (kc->data_ptr() == vc->data_ptr() || k->scalar_type() != kc->scalar_type() || v->scalar_type() != kc->scalar_type() ||
       k->device() != device || v->device() != device || s->device() != device || k->dim() != 3 ||
       v->sizes() != k->sizes() || k->size(1) != kc->size(1) || k->size(2) != kc->size(3) ||
       s->scalar_type() != at::kLong || s->dim() != 1 || s->size(0) != k->size(0) ||

@@ -208,9 +208,10 @@ hipError_t launch_paged_plan(const PlanArgs& a, hipStream_t stream) {
 // Row t of the keys and values to slot t's row of every head: a copy in 16-byte pieces, bound
 // by memory. W neighbouring threads share a token and walk over its 2 H chunks pieces; each
 // thread has kStoreTokens tokens in flight. Slots outside the cache are left out. The rows are
-// written past the caches: they are whole lines in no order, which the L2 would only hold up
-// (16381 tokens, 14334 of them stored, H8 D128: 26.2 -> 19.4 us, 6.0 TB/s; a step's 32 tokens
-// 3.6 -> 3.0 with two tokens a thread in place of four).
+// written past the caches: a prompt's attention reads its own keys and values, and until the
+// next step reads the cache, the other layers' have passed through (16381 tokens, 14334 of them
+// stored, H8 D128: 26.2 -> 19.4 us, 6.0 TB/s; 16384 tokens and at once a step's attention over
+// these alone 48.0 -> 51.2). A step's 32 tokens: 3.0 us, with four tokens a thread 3.6.
 constexpr int kStoreTokens = 2;
 
 template <int W>

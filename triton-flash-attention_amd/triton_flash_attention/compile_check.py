@@ -29,7 +29,7 @@ from . import _build
 SUPPORTED_ARCHS = ("gfx950",)
 
 # Kernel instances the default tiling table (kDefault in csrc/fa_capi.hip) and
-# its shape rules select, as demangled name prefixes, for D = 32, 64, 128, both
+# its shape rules select, and the kernels of the operators around the attention call, as demangled name prefixes, for D = 32, 64, 128, both
 # mask modes and both element types (at D = 128 the forward takes the 4-wave
 # pipelined kernel, the 8-wave one where its rounds are whole, the two-key-group
 # one for launches of about one work-group per CU, and the classic one for short
@@ -85,6 +85,17 @@ def _defaults() -> tuple[str, ...]:
         names += [f"fa::{k}_kernel<{d}, {e}>" for k in ("fwd_decode", "preprocess")
                   for d in (32, 64, 128)]
         names.append(f"fa::split_reduce_kernel<{e}>")
+    # The operators around the attention call.
+    flags = [f"{n}, {i}" for n in ("false", "true") for i in ("false", "true")]
+    for e in ("fa::F16", "fa::BF16"):
+        names += [f"fa::{k}_kernel<{lanes}, {e}, {f}>" for k in ("rope", "rope_bwd")
+                  for lanes in (2, 4, 8) for f in flags]
+        names += [f"fa::paged_fwd_kernel<{d}, {e}, {s}>" for d in (32, 64, 128)
+                  for s in ("false", "true")]
+        names += [f"fa::paged_join_kernel<{d}, {e}>" for d in (32, 64, 128)]
+        names.append(f"fa::rope_reduce_kernel<{e}>")
+    names += ["fa::paged_plan_kernel<1>", "fa::paged_plan_kernel<2>"]
+    names += [f"fa::paged_store_kernel<{w}>" for w in (32, 64, 128, 256)]
     names += [f"fa::{k}_kernel<128, false, 4, 32, {e}>" for k in ("dq", "dkdv")
               for e in ("fa::F16", "fa::BF16")]
     return tuple(names)

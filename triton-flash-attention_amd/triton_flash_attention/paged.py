@@ -213,8 +213,8 @@ def paged_cache_store(
     [B, Hkv, N, D] tensor); ``slots`` [T] (int64) as :func:`paged_cache_plan` returns them:
     slot s is row ``s % page_size`` of page ``s // page_size``. Negative slots and slots behind
     the last page are left out; the others must differ from each other. Rows of the cache that
-    no slot names stay as they were. Gradients are not recorded: the call raises where one would
-    have to be.
+    no slot names stay as they were. key and value must not share memory with the cache.
+    Gradients are not recorded: the call raises where one would have to be.
     """
     if _plain(backend) and _native.module().paged_store(key, value, key_cache, value_cache, slots):
         return
@@ -243,6 +243,8 @@ def paged_cache_store(
     if any(s == 0 and n > 1 for t in (key_cache, value_cache)
            for s, n in zip(t.stride(), t.shape)):
         raise ValueError("the caches must not be expanded tensors")
+    if not torch.compiler.is_dynamo_compiling() and key_cache.data_ptr() == value_cache.data_ptr():
+        raise ValueError("key_cache and value_cache must be different tensors")
     reason = None
     if backend != "torch":
         reason = (_gpu_reason(key_cache) if key_cache.device.type != "cuda"
@@ -356,12 +358,11 @@ def paged_attention(
         raise ValueError(
             "the number of query heads must be divisible by the number of key/value heads")
     softmax_scale = float(scale) if scale is not None else D ** -0.5
-    served = _kernel_scale(softmax_scale)
-    reason = None
+    reason = served = None
     if backend != "torch":
         if query.device.type != "cuda":
             reason = _gpu_reason(query)
-        elif served is None:
+        elif (served := _kernel_scale(softmax_scale)) is None:
             reason = f"scale {softmax_scale!r} overflows the gfx950 kernel's float32 arithmetic"
         elif _forward_ad_active() or (torch.is_grad_enabled() and any(
                 t.requires_grad for t in (query, key_cache, value_cache))):

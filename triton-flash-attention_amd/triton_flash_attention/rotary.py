@@ -201,7 +201,8 @@ def qk_norm_rope(
     values are rotated in pairs by its token's R / 2 angles: the values i and i + R / 2, or with
     ``interleaved`` 2 i and 2 i + 1. ``cos`` and ``sin`` [P, R / 2] hold the angles' cosines and
     sines in float32 for P positions; ``positions`` [N] or [B, N] (int32 or int64) names each
-    token's row, by default 0 .. N - 1. A token whose position is not in [0, P) gets NaN.
+    token's row, by default 0 .. N - 1. A token whose position is not in [0, P) gets NaN, in its
+    gradients too.
 
     Returns contiguous (query, key), computed in float32 and rounded once, differentiable in
     query, key and the weights. The gfx950 kernels serve float16 and bfloat16 with head_dim a
