@@ -196,7 +196,10 @@ int check_cache(const char* name, const int64_t* s, int64_t pages, int64_t D) {
   return FA_OK;
 }
 
-int64_t row_blocks(int64_t rows) { return (rows + fa::kPagedRows - 1) / fa::kPagedRows; }
+int64_t row_blocks(int64_t rows) {
+  const int64_t block = fa::paged_rows(rows);
+  return (rows + block - 1) / block;
+}
 
 int check_paged(const char* name, int64_t B, int64_t Hq, int64_t Hkv, int64_t N, int64_t D,
                 int64_t M, int64_t S) {
@@ -220,12 +223,13 @@ int check_paged(const char* name, int64_t B, int64_t Hq, int64_t Hkv, int64_t N,
   return FA_OK;
 }
 
-// For each work-group 16 bytes, and two partials: 16 rows of O and their log-sum-exps.
+// For each work-group 16 bytes, and two partials: a row block of O and its log-sum-exps.
 int64_t paged_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t N, int64_t D, int64_t M,
                         int64_t S) {
   const int64_t width = D <= 32 ? 32 : D <= 64 ? 64 : 128;
-  const int grid = fa::paged_grid(B, Hkv, row_blocks(Hq / Hkv * N), M * S);
-  return grid == 0 ? 0 : (int64_t)grid * (16 + 2 * fa::kPagedRows * (width + 1) * 4);
+  const int64_t rows = Hq / Hkv * N;
+  const int grid = fa::paged_grid(B, Hkv, row_blocks(rows), M * S);
+  return grid == 0 ? 0 : (int64_t)grid * (16 + 2 * fa::paged_rows(rows) * (width + 1) * 4);
 }
 
 int run_paged(const char* name, int dtype, const fa_half_t* q, const fa_half_t* k_cache,
@@ -273,6 +277,7 @@ int run_paged(const char* name, int dtype, const fa_half_t* q, const fa_half_t* 
   a.d = (int)D;
   a.M = (int)M;
   a.S = (int)S;
+  a.rows = fa::paged_rows(Hq / Hkv * N);
   a.blocks = (int)row_blocks(Hq / Hkv * N);
   a.grid = fa::paged_grid(B, Hkv, a.blocks, M * S);
   return fa::capi_launch_result(

@@ -100,11 +100,13 @@ struct PagedArgs {
   int64_t pages;
   float c;               // scale * log2(e)
   int B, Hkv, group, N, d, M, S;
-  int blocks;            // row blocks of 16 of a key/value head's group * N rows
+  int rows;              // of a row block: 16 or 32 (paged_rows)
+  int blocks;            // row blocks of a key/value head's group * N rows
   int grid;              // work-groups (paged_grid)
 };
-constexpr int kPagedRows = 16;
 constexpr int kPagedUnit = 32;  // keys
+// Rows of the blocks that `rows` rows are worked on in.
+inline int paged_rows(int64_t rows) { return rows <= 16 ? 16 : 32; }
 // Work-groups of a launch whose table rows hold `keys` keys; 0: one for each sequence,
 // key/value head and row block.
 int paged_grid(int64_t B, int64_t Hkv, int64_t blocks, int64_t keys);

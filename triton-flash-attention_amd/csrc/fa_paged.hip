@@ -266,7 +266,7 @@ hipError_t launch_paged_store(const StoreArgs& a, hipStream_t stream) {
 
 // ---- attention --------------------------------------------------------------------------
 // o = softmax(scale q K^T) V of the group * N query rows that read one key/value head, in
-// blocks of 16 rows (one MFMA block): query n of a sequence of len keys sees keys
+// blocks of 16 rows (one MFMA block) or, where there are more, of 32: query n of a sequence of len keys sees keys
 // j <= len - N + n. K and V are read once a row block and next to nothing is computed, so
 // what bounds the kernel is the bytes in flight.
 //
@@ -390,13 +390,13 @@ __device__ __forceinline__ PagedLine paged_find(const PagedArgs& a, int s, Paged
 // The triple that the end of a work-group's stretch cuts, where that is the triple's first cut:
 // `more` pieces follow the work-group's own, which is in its slot `slot`; more = 0 where there
 // is no such triple. The workspace holds one of these for each work-group, then two partials
-// for each: 16 rows of O, then their log-sum-exps.
+// for each: a row block's rows of O, then their log-sum-exps.
 struct PagedCut {
   int b, triple, more, slot;
 };
 template <int D>
 __device__ __forceinline__ float* paged_part(const PagedArgs& a, int64_t slot) {
-  return a.part + a.grid * (sizeof(PagedCut) / 4) + slot * (kPagedRows * (D + 1));
+  return a.part + a.grid * (sizeof(PagedCut) / 4) + slot * (a.rows * (D + 1));
 }
 
 // A wave's units of a piece: where the half units of its next 32 units lie, one a lane
@@ -406,13 +406,24 @@ struct PagedHalves {
   int rows;         // rows that exist
 };
 
+// A row of a triple: query n of the group's head h, if it exists; and its row of the output.
+struct PagedRow {
+  bool ok;
+  int h, n;
+};
+__device__ __forceinline__ int64_t paged_out_row(const PagedArgs& a, int b, int kvh,
+                                                 const PagedRow& r) {
+  return ((int64_t)(b * (int64_t)a.Hkv + kvh) * a.group + r.h) * a.N + r.n;
+}
+
 }  // namespace
 
-template <int D, class E, bool SHORT>
+template <int D, class E, int RB, bool SHORT>
 __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArgs a) {
   using T = PagedTile<D>;
   constexpr int KD = T::KD, DD = T::DD, NW = kPagedWaves;
-  constexpr int LDS_FLOATS = NW * DD * 256 + 2 * NW * kPagedRows;
+  constexpr int ROWS = 16 * RB;
+  constexpr int LDS_FLOATS = NW * RB * DD * 256 + 2 * NW * ROWS;
   static_assert(NW * T::TILE * 2 <= LDS_FLOATS * 4, "the V tiles and the merge share it");
   __shared__ __attribute__((aligned(16))) float lds[LDS_FLOATS];
   const int tid = threadIdx.x;
@@ -478,23 +489,26 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArg
     const int kvh = at.triple / a.blocks, block = at.triple - kvh * a.blocks;
     const int rows = a.group * a.N;
 
-    // The lane's row.
-    const int r = block * kPagedRows + c16;
-    const bool row_ok = r < rows;
-    const int h = r / a.N, n = r - h * a.N;
-    // It sees the keys below this. Rows that do not exist score 0 everywhere: masked, they
-    // would move the reference max in every unit.
-    const int see = row_ok ? keys - a.N + n + 1 : INT32_MAX;
-    const int all_see = keys - a.N + 1;               // every row does
-    half8 qf[KD];
-    {
-      const half_t* q = a.q + at.b * a.qs[0] + (int64_t)(kvh * a.group + h) * a.qs[1] + n * a.qs[2];
+    // The lane's rows. Each sees the keys below see[]; rows that do not exist score 0
+    // everywhere: masked, they would move the reference max in every unit.
+    auto row_of = [&](int rb) __attribute__((always_inline)) {
+      const int r = block * ROWS + 16 * rb + c16;
+      return PagedRow{r < rows, r / a.N, r % a.N};
+    };
+    const int all_see = keys - a.N + 1;  // every row sees the keys below this
+    int see[RB];
+    half8 qf[RB][KD];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const PagedRow r = row_of(rb);
+      see[rb] = r.ok ? all_see + r.n : INT32_MAX;
+      const half_t* q = a.q + at.b * a.qs[0] + (int64_t)(kvh * a.group + r.h) * a.qs[1] + r.n * a.qs[2];
 #pragma unroll
       for (int kd = 0; kd < KD; ++kd) {
         u32x4 v = {0u, 0u, 0u, 0u};
         const int col = 32 * kd + 8 * G;
-        if (row_ok && col < a.d) v = *reinterpret_cast<const u32x4*>(q + col);
-        qf[kd] = __builtin_bit_cast(half8, v);
+        if (r.ok && col < a.d) v = *reinterpret_cast<const u32x4*>(q + col);
+        qf[rb][kd] = __builtin_bit_cast(half8, v);
       }
     }
 
@@ -566,10 +580,15 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArg
       }
     };
 
-    float4v o[DD];
+    float4v o[RB][DD];
+    float m[RB], l[RB];
 #pragma unroll
-    for (int dd = 0; dd < DD; ++dd) o[dd] = {0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
+    for (int rb = 0; rb < RB; ++rb) {
+#pragma unroll
+      for (int dd = 0; dd < DD; ++dd) o[rb][dd] = {0.f, 0.f, 0.f, 0.f};
+      m[rb] = -INFINITY;
+      l[rb] = 0.f;
+    }
     const float c = a.c;
 
     turn_to(0);
@@ -577,56 +596,61 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArg
     load_v();
     for (int i = 0; i < mine; ++i) {
       const int ka = (u0 + wave + NW * i) * kPagedUnit;
-      float4v s[2];
+      float4v s[RB][2];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        s[kb] = {0.f, 0.f, 0.f, 0.f};
+      for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-        for (int kd = 0; kd < KD; ++kd)
-          s[kb] = mma16<E>(__builtin_bit_cast(half8, kx[kb][kd]), qf[kd], s[kb]);
-      }
+        for (int kb = 0; kb < 2; ++kb) {
+          s[rb][kb] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kd = 0; kd < KD; ++kd)
+            s[rb][kb] = mma16<E>(__builtin_bit_cast(half8, kx[kb][kd]), qf[rb][kd], s[rb][kb]);
+        }
       turn_to(i + 1);  // past the last unit: no rows
       load_k();
 #pragma unroll
       for (int j = 0; j < T::VI; ++j) *reinterpret_cast<u32x4*>(vt + v_at[j]) = vx[j];
       load_v();
-      if (ka + kPagedUnit > all_see) {
+      half8 pa[RB];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+      for (int rb = 0; rb < RB; ++rb) {
+        if (ka + kPagedUnit > all_see) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (ka + 16 * kb + 4 * G + j >= see) s[kb][j] = -INFINITY;
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (ka + 16 * kb + 4 * G + j >= see[rb]) s[rb][kb][j] = -INFINITY;
+        }
+        auto probs = [&](float ref) __attribute__((always_inline)) {
+          float sum = 0.f;
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float p = exp2_fast(fmaf(s[rb][kb][j], c, -ref));
+              sum += p;
+              pa[rb][4 * kb + j] = to_elem<E>(p);
+            }
+          return sum;
+        };
+        float l_u = probs(m[rb]);
+        if (__builtin_amdgcn_ballot_w64(!(l_u <= kPagedSumLimit)) != 0) {
+          float mt = s[rb][0][0];
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mt = __builtin_fmaxf(mt, s[rb][kb][j]);
+          const float m_new = __builtin_fmaxf(m[rb], quarters_max(mt) * c);
+          const float ref = exp_reference(m_new);
+          const float alpha = exp2_fast(m[rb] - ref);
+          l[rb] *= alpha;
+#pragma unroll
+          for (int dd = 0; dd < DD; ++dd) o[rb][dd] *= alpha;
+          m[rb] = m_new;
+          l_u = probs(ref);
+        }
+        l[rb] += l_u;
       }
-      half8 pa;
-      auto probs = [&](float ref) __attribute__((always_inline)) {
-        float sum = 0.f;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float p = exp2_fast(fmaf(s[kb][j], c, -ref));
-            sum += p;
-            pa[4 * kb + j] = to_elem<E>(p);
-          }
-        return sum;
-      };
-      float l_u = probs(m);
-      if (__builtin_amdgcn_ballot_w64(!(l_u <= kPagedSumLimit)) != 0) {
-        float mt = s[0][0];
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) mt = __builtin_fmaxf(mt, s[kb][j]);
-        const float m_new = __builtin_fmaxf(m, quarters_max(mt) * c);
-        const float ref = exp_reference(m_new);
-        const float alpha = exp2_fast(m - ref);
-        l *= alpha;
-#pragma unroll
-        for (int dd = 0; dd < DD; ++dd) o[dd] *= alpha;
-        m = m_new;
-        l_u = probs(ref);
-      }
-      l += l_u;
 #pragma unroll
       for (int dd = 0; dd < DD; ++dd) {
         const half4 lo = __builtin_bit_cast(
@@ -639,58 +663,66 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArg
           va[e] = lo[e];
           va[4 + e] = hi[e];
         }
-        o[dd] = mma16<E>(va, pa, o[dd]);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) o[rb][dd] = mma16<E>(va, pa[rb], o[rb][dd]);
       }
     }
 
     // Merge of the waves' results: O, and per row m and l.
     __syncthreads();
-    float* const xo = lds;                    // [wave][dd][lane][4]
-    float* const xm = lds + NW * DD * 256;    // [wave][row], m then l
-    float lw = quarters_sum(l);
-    if (bad) {  // NaN, whatever the other waves and pieces hold
-      lw = __builtin_nanf("");
-      m = m == -INFINITY ? 0.f : m;
-    }
+    float* const xo = lds;                        // [wave][row block][dd][lane][4]
+    float* const xm = lds + NW * RB * DD * 256;   // [wave][row], m then l
 #pragma unroll
-    for (int dd = 0; dd < DD; ++dd)
-      *reinterpret_cast<float4v*>(xo + ((wave * DD + dd) * 64 + lane) * 4) = o[dd];
-    if (G == 0) {
-      xm[wave * kPagedRows + c16] = m;
-      xm[(NW + wave) * kPagedRows + c16] = lw;
+    for (int rb = 0; rb < RB; ++rb) {
+      float lw = quarters_sum(l[rb]), mw = m[rb];
+      if (bad) {  // NaN, whatever the other waves and pieces hold
+        lw = __builtin_nanf("");
+        mw = mw == -INFINITY ? 0.f : mw;
+      }
+#pragma unroll
+      for (int dd = 0; dd < DD; ++dd)
+        *reinterpret_cast<float4v*>(xo + (((wave * RB + rb) * DD + dd) * 64 + lane) * 4) = o[rb][dd];
+      if (G == 0) {
+        xm[wave * ROWS + 16 * rb + c16] = mw;
+        xm[(NW + wave) * ROWS + 16 * rb + c16] = lw;
+      }
     }
     __syncthreads();
-    float mt = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) mt = __builtin_fmaxf(mt, xm[w * kPagedRows + c16]);
-    float wt[NW], lt = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float mw = xm[w * kPagedRows + c16];
-      wt[w] = mw == -INFINITY ? 0.f : exp2_fast(mw - mt);  // a wave that saw no key weighs 0
-      lt += wt[w] * xm[(NW + w) * kPagedRows + c16];
-    }
-    const float inv = lt == 0.f ? 0.f : 1.0f / lt;  // a row that saw no key is 0
     const bool whole = SHORT || (u0 == 0 && u1 == units);
-    const int64_t slot = (int64_t)blockIdx.x * 2 + (opening ? 0 : 1);
-    float* const part = paged_part<D>(a, slot);
-    half_t* const out =
-        a.o + (((int64_t)at.b * a.Hkv * a.group + kvh * a.group + h) * a.N + n) * a.d;
+    float* const part = paged_part<D>(a, (int64_t)blockIdx.x * 2 + (opening ? 0 : 1));
 #pragma unroll
-    for (int dd = wave; dd < DD; dd += NW) {
-      float4v v = {0.f, 0.f, 0.f, 0.f};
+    for (int rb = 0; rb < RB; ++rb) {
+      const int x = 16 * rb + c16;
+      float mt = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < NW; ++w)
-        v += *reinterpret_cast<const float4v*>(xo + ((w * DD + dd) * 64 + lane) * 4) * wt[w];
-      v *= inv;
-      const int col = 16 * dd + 4 * G;
-      if (!row_ok) continue;
-      if (!whole) *reinterpret_cast<float4v*>(part + c16 * D + col) = v;
-      else if (col < a.d)
-        *reinterpret_cast<u32x2*>(out + col) = pack4<E>(v[0], v[1], v[2], v[3]);
+      for (int w = 0; w < NW; ++w) mt = __builtin_fmaxf(mt, xm[w * ROWS + x]);
+      float wt[NW], lt = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float mw = xm[w * ROWS + x];
+        wt[w] = mw == -INFINITY ? 0.f : exp2_fast(mw - mt);  // a wave that saw no key weighs 0
+        lt += wt[w] * xm[(NW + w) * ROWS + x];
+      }
+      const float inv = lt == 0.f ? 0.f : 1.0f / lt;  // a row that saw no key is 0
+      const PagedRow r = row_of(rb);
+      half_t* const out = a.o + paged_out_row(a, at.b, kvh, r) * a.d;
+#pragma unroll
+      for (int dd = wave; dd < DD; dd += NW) {
+        float4v v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < NW; ++w)
+          v += *reinterpret_cast<const float4v*>(xo + (((w * RB + rb) * DD + dd) * 64 + lane) * 4) *
+               wt[w];
+        v *= inv;
+        const int col = 16 * dd + 4 * G;
+        if (!r.ok) continue;
+        if (!whole) *reinterpret_cast<float4v*>(part + x * D + col) = v;
+        else if (col < a.d)
+          *reinterpret_cast<u32x2*>(out + col) = pack4<E>(v[0], v[1], v[2], v[3]);
+      }
+      if (!whole && wave == 0 && G == 0 && r.ok)
+        part[ROWS * D + x] = lt == 0.f ? -INFINITY : mt + log2_fast(lt);
     }
-    if (!whole && wave == 0 && G == 0 && row_ok)
-      part[kPagedRows * D + c16] = lt == 0.f ? -INFINITY : mt + log2_fast(lt);
     __syncthreads();
 
     left -= line_units - at.unit;
@@ -707,58 +739,71 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArg
   }
 }
 
+// Joins the pieces of the triples that the ends of the stretches cut: block (w, y) rows of the
+// triple that work-group w's cut names. Piece p of a row weighs exp2(lse_p) against the others'.
+// A lane holds four columns of a row, a wave RPP rows; of a block's four waves `groups` take
+// different rows, and the 4 / groups waves that share theirs take every (4 / groups)-th piece
+// and merge through LDS, in a fixed order. Most blocks have two pieces to join or none, and all
+// is latency: each wave asks for its first piece beside the cut that says whether it exists.
 constexpr int kJoinWaves = 4;
+template <int D>
+constexpr int kJoinRows = 64 / (D / 4);  // of a wave
 
-// Joins the pieces of the triples that the ends of the stretches cut: block w the triple that
-// work-group w's cut names. Piece p of a row weighs exp2(lse_p) against the others'. A lane
-// holds four columns of a row, a block as many rows as a wave has lanes for; its four waves take
-// every fourth piece and merge through LDS, in a fixed order. Most blocks have two pieces to
-// join or none, and all is latency: each wave asks for its first piece beside the cut that says
-// whether it exists.
+inline __host__ __device__ int join_groups(int rows, int wave_rows) {
+  return rows <= wave_rows ? 1 : rows <= 2 * wave_rows ? 2 : 4;
+}
+
 template <int D, class E>
 __global__ __launch_bounds__(64 * kJoinWaves) void paged_join_kernel(PagedArgs a) {
   constexpr int W = kJoinWaves;
-  constexpr int COLS = D / 4;       // 4-column pieces of a row
-  constexpr int RPP = 64 / COLS;    // rows of a block
-  constexpr int AHEAD = 8;          // pieces of a wave asked for at once
+  constexpr int COLS = D / 4;           // 4-column pieces of a row
+  constexpr int RPP = kJoinRows<D>;
+  constexpr int AHEAD = 8;              // pieces of a wave asked for at once
   __shared__ __attribute__((aligned(16))) float acc_s[W][64][4];
   __shared__ float m_s[W][64], l_s[W][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int w = blockIdx.x;
-  const int row = blockIdx.y * RPP + lane / COLS, col = 4 * (lane % COLS);
+  const int groups = join_groups(min(a.rows, a.group * a.N), RPP);
+  const int group = wave % groups, part0 = wave / groups, step = W / groups;
+  const int row = (blockIdx.y * groups + group) * RPP + lane / COLS, col = 4 * (lane % COLS);
   struct Piece {
     float lse;
     float4v o;
   };
+  const bool held = row < a.rows;  // the partials hold such a row
   auto load = [&](int64_t slot) __attribute__((always_inline)) {
-    const float* part = paged_part<D>(a, slot);
-    return Piece{part[kPagedRows * D + row],
-                 *reinterpret_cast<const float4v*>(part + row * D + col)};
+    Piece p = {-INFINITY, {0.f, 0.f, 0.f, 0.f}};
+    if (held) {
+      const float* part = paged_part<D>(a, slot);
+      p.lse = part[a.rows * D + row];
+      p.o = *reinterpret_cast<const float4v*>(part + row * D + col);
+    }
+    return p;
   };
-  // Slot 0 of the work-group `wave` behind w (of w itself also slot 1): inside the workspace,
+  // Slot 0 of the work-group part0 behind w (of w itself also slot 1): inside the workspace,
   // and unused unless the cut says that it was written.
-  const int64_t ahead = min(w + wave, a.grid - 1);
+  const int64_t ahead = min(w + part0, a.grid - 1);
   const PagedCut cut = reinterpret_cast<const PagedCut*>(a.part)[w];
   Piece p0 = load(2 * ahead);
-  if (wave == 0) {
+  if (part0 == 0) {
     const Piece p1 = load(2 * ahead + 1);
     if (cut.slot != 0) p0 = p1;
   }
   if (cut.more == 0) return;
   const int kvh = cut.triple / a.blocks, block = cut.triple - kvh * a.blocks;
-  const int rows = min(kPagedRows, a.group * a.N - block * kPagedRows);
+  const int rows = min(a.rows, a.group * a.N - block * a.rows);
   float m = -INFINITY, l = 0.f;
   float4v acc = {0.f, 0.f, 0.f, 0.f};
-  if (wave <= cut.more) {
+  if (part0 <= cut.more) {
     m = p0.lse;
     l = m == -INFINITY ? 0.f : 1.f;
     acc = p0.o;
-    for (int at = wave + W; at <= cut.more; at += W * AHEAD) {
+    for (int at = part0 + step; at <= cut.more; at += step * AHEAD) {
       Piece p[AHEAD];
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i)
-        p[i] = at + W * i <= cut.more ? load(2 * ((int64_t)w + at + W * i))
-                                      : Piece{-INFINITY, {0.f, 0.f, 0.f, 0.f}};
+        p[i] = at + step * i <= cut.more ? load(2 * ((int64_t)w + at + step * i))
+                                         : Piece{-INFINITY, {0.f, 0.f, 0.f, 0.f}};
       float mx = m;
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) mx = __builtin_fmaxf(mx, p[i].lse);
@@ -779,22 +824,19 @@ __global__ __launch_bounds__(64 * kJoinWaves) void paged_join_kernel(PagedArgs a
   m_s[wave][lane] = m;
   l_s[wave][lane] = l;
   __syncthreads();
-  if (wave != 0 || row >= rows || col >= a.d) return;
+  if (part0 != 0 || row >= rows || col >= a.d) return;
   float mx = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < W; ++i) mx = __builtin_fmaxf(mx, m_s[i][lane]);
+  for (int i = group; i < W; i += groups) mx = __builtin_fmaxf(mx, m_s[i][lane]);
   float lt = 0.f;
   float4v v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < W; ++i) {
+  for (int i = group; i < W; i += groups) {
     const float f = m_s[i][lane] == -INFINITY ? 0.f : exp2_fast(m_s[i][lane] - mx);
     lt += f * l_s[i][lane];
     v += *reinterpret_cast<const float4v*>(acc_s[i][lane]) * f;
   }
   v *= lt == 0.f ? 0.f : 1.0f / lt;
-  const int r = block * kPagedRows + row;
-  const int h = r / a.N, n = r - h * a.N;
-  half_t* out = a.o + (((int64_t)cut.b * a.Hkv * a.group + kvh * a.group + h) * a.N + n) * a.d;
+  const int r = block * a.rows + row;
+  half_t* out = a.o + paged_out_row(a, cut.b, kvh, {true, r / a.N, r % a.N}) * a.d;
   *reinterpret_cast<u32x2*>(out + col) = pack4<E>(v[0], v[1], v[2], v[3]);
 }
 
@@ -819,24 +861,29 @@ int paged_grid(int64_t B, int64_t Hkv, int64_t blocks, int64_t keys) {
   return (int)std::min<int64_t>((units + 3) / 4, 512);
 }
 
-template <int D, class E>
+template <int D, class E, int RB>
 hipError_t paged_start(const PagedArgs& a, hipStream_t stream) {
   if (a.grid == 0) {
     const int64_t triples = (int64_t)a.B * a.Hkv * a.blocks;
     if (triples > 0x7fffffff) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((paged_fwd_kernel<D, E, true>), dim3((unsigned)triples),
+    hipLaunchKernelGGL((paged_fwd_kernel<D, E, RB, true>), dim3((unsigned)triples),
                        dim3(64 * kPagedWaves), 0, stream, a);
     return hipGetLastError();
   }
-  hipLaunchKernelGGL((paged_fwd_kernel<D, E, false>), dim3((unsigned)a.grid), dim3(64 * kPagedWaves),
-                     0, stream, a);
+  hipLaunchKernelGGL((paged_fwd_kernel<D, E, RB, false>), dim3((unsigned)a.grid),
+                     dim3(64 * kPagedWaves), 0, stream, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  constexpr int RPP = 64 / (D / 4);
-  const int rows = std::min(kPagedRows, a.group * a.N);
-  const dim3 grid((unsigned)(a.grid - 1), (unsigned)((rows + RPP - 1) / RPP));
+  const int rows = std::min(a.rows, a.group * a.N);
+  const int block_rows = kJoinRows<D> * join_groups(rows, kJoinRows<D>);
+  const dim3 grid((unsigned)(a.grid - 1), (unsigned)((rows + block_rows - 1) / block_rows));
   hipLaunchKernelGGL((paged_join_kernel<D, E>), grid, dim3(64 * kJoinWaves), 0, stream, a);
   return hipGetLastError();
+}
+
+template <int D, class E>
+hipError_t paged_start(const PagedArgs& a, hipStream_t stream) {
+  return a.rows == 16 ? paged_start<D, E, 1>(a, stream) : paged_start<D, E, 2>(a, stream);
 }
 
 hipError_t launch_paged_fwd(const PagedArgs& a, int D, int dtype, hipStream_t stream) {

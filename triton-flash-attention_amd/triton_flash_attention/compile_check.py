@@ -90,8 +90,8 @@ def _defaults() -> tuple[str, ...]:
     for e in ("fa::F16", "fa::BF16"):
         names += [f"fa::{k}_kernel<{lanes}, {e}, {f}>" for k in ("rope", "rope_bwd")
                   for lanes in (2, 4, 8) for f in flags]
-        names += [f"fa::paged_fwd_kernel<{d}, {e}, {s}>" for d in (32, 64, 128)
-                  for s in ("false", "true")]
+        names += [f"fa::paged_fwd_kernel<{d}, {e}, {r}, {s}>" for d in (32, 64, 128)
+                  for r in (1, 2) for s in ("false", "true")]
         names += [f"fa::paged_join_kernel<{d}, {e}>" for d in (32, 64, 128)]
         names.append(f"fa::rope_reduce_kernel<{e}>")
     names += ["fa::paged_plan_kernel<1>", "fa::paged_plan_kernel<2>"]
