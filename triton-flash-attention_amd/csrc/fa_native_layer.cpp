@@ -351,6 +351,15 @@ bool plain_table(const at::Tensor& t, I64 S) {
          t.size(0) < I64{1} << 24;
 }
 
+// n values of a one-dimensional tensor from `from` on, as a tensor of its own on its memory.
+at::Tensor piece_of(const at::Tensor& t, I64 from, I64 n) {
+  at::Tensor p = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(t.storage()), t.key_set(),
+                                                          t.dtype());
+  p.unsafeGetTensorImpl()->set_storage_offset(from);
+  p.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return p;
+}
+
 py::object native_plan(py::handle table, py::handle lengths, py::handle new_tokens,
                        py::handle free_pages, py::handle page_size, py::handle num_tokens,
                        py::handle free_start) {
@@ -378,9 +387,11 @@ py::object native_plan(py::handle table, py::handle lengths, py::handle new_toke
   at::AutoDispatchBelowAutograd below;
   const auto i32 = t->options(), i64 = i32.dtype(at::kLong);
   const at::Tensor lc = l->contiguous(), nc = n->contiguous(), fc = f->contiguous();
-  at::Tensor slots = at::empty({T}, i64), positions = at::empty({T}, i32);
-  at::Tensor starts = at::empty({B + 1}, i32), held = at::empty({B}, i32);
-  at::Tensor free_out = at::empty({1}, i32);
+  // One allocation for the four int32 results (a step's plan waits for the host otherwise).
+  const at::Tensor small = at::empty({T + 2 * B + 2}, i32);
+  at::Tensor slots = at::empty({T}, i64), positions = piece_of(small, 0, T);
+  at::Tensor starts = piece_of(small, T, B + 1), held = piece_of(small, T + B + 1, B);
+  at::Tensor free_out = piece_of(small, T + 2 * B + 1, 1);
   check(g.plan(t->data_ptr(), t->stride(0), lc.data_ptr(), nc.data_ptr(), fc.data_ptr(),
                pointer(start), slots.data_ptr(), positions.data_ptr(), starts.data_ptr(),
                held.data_ptr(), free_out.data_ptr(), B, M, S, fc.size(0), T, stream_of(*t)));
