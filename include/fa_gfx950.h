@@ -434,6 +434,7 @@ int fa_qk_norm_rope_bwd_bf16(const fa_half_t* gq, const fa_half_t* gk, const fa_
  *   starts [B + 1]        a sequence's first token, and their number
  *   lengths_out [B]       lengths + new_tokens
  *   free_start_out [1]    the place behind the last page taken
+ * T is below 2^30.
  * Tokens past T get neither a slot nor a page table entry. When the free pages run out, the
  * entries of the missing ones are -1 and so are their tokens' slots (free_start_out counts them:
  * it is above F); tokens behind a sequence's M pages have slot -1. The outputs must not overlap

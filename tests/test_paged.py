@@ -532,6 +532,24 @@ def test_attention_kernel_bad_rows(dtype):
 
 
 @pytest.mark.gpu
+def test_kernels_take_any_stride_of_one_element_dimensions():
+    """One page, one head: the strides of such dimensions say nothing."""
+    gen = torch.Generator().manual_seed(5)
+    kc = torch.randn(16, 64, generator=gen).half().cuda().as_strided((1, 1, 16, 64), (3, 5, 64, 1))
+    vc = torch.randn(16, 64, generator=gen).half().cuda().as_strided((1, 1, 16, 64), (7, 0, 64, 1))
+    key, value = (torch.randn(2, 1, 64, generator=gen).half().cuda() for _ in range(2))
+    paged_cache_store(key, value, kc, vc, torch.tensor([3, 0]).cuda(), backend="triton")
+    assert torch.equal(kc[0, 0, 3], key[0, 0]) and torch.equal(vc[0, 0, 0], value[1, 0])
+    q = torch.randn(1, 4, 1, 64, generator=gen).half().cuda()
+    o = paged_attention(q, kc, vc, torch.zeros(1, 1, dtype=torch.int32).cuda(),
+                        torch.tensor([11], dtype=torch.int32).cuda(), enable_gqa=True,
+                        backend="triton")
+    dense = [[t[0, :, :11].transpose(0, 1).double().cpu() for t in (kc, vc)]]
+    want, bound = attention_reference(q, dense, 0.125, torch.float16)
+    assert ((o.double().cpu() - want).abs() <= HALF[torch.float16] * want.abs() * 1.01 + bound).all()
+
+
+@pytest.mark.gpu
 def test_attention_kernel_bad_page_of_a_long_sequence():
     """One bad page among many work-groups' pieces."""
     views, table, lens, _ = make_paged([5000, 64], 1, 16, 64, torch.float16, device="cuda", fill=0.0)

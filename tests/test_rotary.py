@@ -343,6 +343,19 @@ def test_kernel_calls_repeat_bit_for_bit_on_other_streams_and_in_graphs():
         assert all(torch.equal(a, b) for a, b in zip(captured, want)), i
 
 
+@pytest.mark.gpu
+def test_kernel_reads_tables_as_views_of_complex_numbers():
+    """cos and sin as parts of one complex tensor, conjugated: lazily negated and strided."""
+    turns = torch.polar(torch.ones(9, 16), torch.randn(9, 16, generator=torch.Generator()
+                                                       .manual_seed(3))).cuda().conj()
+    q = torch.randn(1, 2, 9, 32, generator=torch.Generator().manual_seed(4)).half().cuda()
+    for sin in (turns.imag, torch._neg_view(-turns.imag.clone())):
+        assert sin.is_neg()
+        got, other = both_paths(lambda: qk_norm_rope(q, q, turns.real, sin, backend="triton")[0])
+        want = qk_norm_rope(q, q, turns.real.clone(), sin.resolve_neg().clone(), backend="triton")[0]
+        assert torch.equal(got, want) and torch.equal(other, want)
+
+
 def both_paths(call):
     """call() through the C++ binding and through the Python op layer."""
     assert _native.available(), _native.status()[1]

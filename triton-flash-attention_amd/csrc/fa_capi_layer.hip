@@ -339,7 +339,7 @@ int fa_paged_plan(int32_t* page_table, int64_t table_stride, const int32_t* leng
   if (const int rc = check_pages(name, S, M)) return rc;
   if (B < 0 || F < 0 || T < 0)
     return capi_fail(FA_ERR_BAD_SHAPE, "%s: B, F and T must not be negative", name);
-  if (B >= (int64_t)1 << 30 || F >= (int64_t)1 << 31 || T >= (int64_t)1 << 31)
+  if (B >= (int64_t)1 << 30 || F >= (int64_t)1 << 31 || T >= (int64_t)1 << 30)
     return capi_fail(FA_ERR_TOO_LARGE, "%s: too many sequences, free pages or tokens", name);
   if (const int rc = check_pointers(name, {starts, free_start_out})) return rc;
   if (B > 0)

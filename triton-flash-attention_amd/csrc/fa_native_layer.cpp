@@ -116,10 +116,10 @@ bool readable(const at::Tensor& t) {
 }
 
 at::Tensor aligned(const at::Tensor& t) {
-  const at::Tensor c = t.contiguous();
+  const at::Tensor c = t.resolve_neg().contiguous();
   return address16(c) ? c : c.clone(at::MemoryFormat::Contiguous);
 }
-at::Tensor operand(const at::Tensor& t) { return readable(t) ? t : aligned(t.resolve_neg()); }
+at::Tensor operand(const at::Tensor& t) { return readable(t) ? t : aligned(t); }
 
 I64 stride_of(const at::Tensor& t, int i) { return t.size(i) == 1 ? 0 : t.stride(i); }
 
@@ -155,8 +155,8 @@ struct RopeTables {
       : cos(aligned(c)), sin(aligned(s)), positions(pos), eps((float)e),
         flags(interleaved ? kInterleaved : 0) {
     if (q_weight.defined()) {
-      qw = q_weight.contiguous();
-      kw = k_weight.contiguous();
+      qw = q_weight.resolve_neg().contiguous();
+      kw = k_weight.resolve_neg().contiguous();
       if (qw.scalar_type() == at::kFloat) flags |= kWeightF32;
     }
     if (pos.defined() && pos.scalar_type() == at::kLong) flags |= kPositionsI64;
@@ -260,8 +260,9 @@ class QkNormRope : public torch::autograd::Function<QkNormRope> {
 };
 
 // A leaf keeps the stream that its gradient is accumulated on while any graph that uses it is
-// alive. A backward that is being captured would draw that stream into the capture, which
-// fails in ways that can end the process, so such a call is refused before it starts.
+// alive. Where that is the default stream, a backward that is being captured would draw it into
+// the capture, which it cannot take part in: that fails in ways that can end the process, so such
+// a call is refused before it starts.
 void refuse_mixed_capture(std::initializer_list<const at::Tensor*> leaves) {
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
   for (const at::Tensor* t : leaves) {
@@ -269,10 +270,11 @@ void refuse_mixed_capture(std::initializer_list<const at::Tensor*> leaves) {
     const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
     if (!node) continue;
     const auto stream = node->stream();
-    if (stream && *stream != c10::hip::getCurrentHIPStream(t->device().index()).unwrap())
+    // (by id: autograd's streams pass for CUDA ones)
+    if (stream && stream->id() == c10::hip::getDefaultHIPStream(t->device().index()).id())
       throw std::runtime_error(
           "qk_norm_rope is being captured into a graph while a result of an earlier call with the "
-          "same leaf tensors is alive on another stream: drop it first, or detach it");
+          "same leaf tensors is alive on the default stream: drop it first, or detach it");
   }
 }
 
@@ -367,7 +369,7 @@ py::object native_plan(py::handle table, py::handle lengths, py::handle new_toke
   const at::Tensor *t = plain(table), *l = plain(lengths), *n = plain(new_tokens),
                    *f = plain(free_pages);
   const I64 S = whole(page_size), T = whole(num_tokens);
-  if (!t || !l || !n || !f || T < 0 || T >= I64{1} << 31 || !plain_table(*t, S) ||
+  if (!t || !l || !n || !f || T < 0 || T >= I64{1} << 30 || !plain_table(*t, S) ||
       !served(t->device()))
     return py::none();
   const at::Device device = t->device();

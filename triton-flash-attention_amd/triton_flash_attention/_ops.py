@@ -379,9 +379,9 @@ def _strides(t: torch.Tensor) -> list[int]:
     return [0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()[:-1])]
 
 
-def row_stride(cache: torch.Tensor) -> int:
-    """Elements from one row of a cache's page to the next."""
-    return cache.stride(2) if cache.shape[2] > 1 else cache.shape[3]
+def cache_strides(cache: torch.Tensor) -> list[int]:
+    """Page, head and row stride of a cache [pages, H, S, D]."""
+    return _strides(cache)
 
 
 def _int64s(values) -> ctypes.Array:
@@ -397,10 +397,10 @@ ROPE_INTERLEAVED, ROPE_WEIGHT_F32, ROPE_POSITIONS_I64 = 1, 2, 4  # FA_ROPE_* of 
 
 def _rope_common(cos, sin, query_weight, key_weight, positions, batch: int, interleaved: bool):
     """(cos, sin, weights, positions) as the kernels read them, positions' strides, flags."""
-    cos, sin = _aligned(cos.contiguous()), _aligned(sin.contiguous())
+    cos, sin = (_aligned(t.resolve_neg().contiguous()) for t in (cos, sin))
     flags = ROPE_INTERLEAVED if interleaved else 0
     if query_weight is not None:
-        query_weight, key_weight = query_weight.contiguous(), key_weight.contiguous()
+        query_weight, key_weight = (t.resolve_neg().contiguous() for t in (query_weight, key_weight))
         flags |= ROPE_WEIGHT_F32 if query_weight.dtype == torch.float32 else 0
     pos_strides = [0, 0]
     if positions is not None:
@@ -502,16 +502,12 @@ def paged_store(key, value, key_cache, value_cache, slots) -> None:
     lib = _lib.load()
     with _device_guard(key_cache.device):
         key, value, slots = _readable(key), _readable(value), slots.contiguous()
-        strides = _int64s([*_strides(key), *_strides(value), *_cache_strides(key_cache)])
+        strides = _int64s([*_strides(key), *_strides(value), *cache_strides(key_cache)])
         _lib.check(_launch(
             "paged_store", lib.fa_paged_store, key.data_ptr(), value.data_ptr(),
             key_cache.data_ptr(), value_cache.data_ptr(), slots.data_ptr(), strides,
             key.shape[0], H, D, pages, S, _stream(key_cache)))
     _written(key_cache, value_cache)
-
-
-def _cache_strides(cache: torch.Tensor) -> list[int]:
-    return [*_strides(cache)[:2], row_stride(cache)]
 
 
 def paged_fwd(q, key_cache, value_cache, page_table, lengths, scale: float) -> torch.Tensor:
@@ -530,7 +526,7 @@ def paged_fwd(q, key_cache, value_cache, page_table, lengths, scale: float) -> t
             _lib.check(ws_bytes)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
         o = torch.empty((B, Hq, N, D), dtype=dt, device=q.device)
-        strides = _int64s([*_strides(q), *_cache_strides(key_cache), page_table.stride(0)])
+        strides = _int64s([*_strides(q), *cache_strides(key_cache), page_table.stride(0)])
         _lib.check(_launch(
             "paged_fwd", _entry(lib, "fa_paged_fwd", dt), q.data_ptr(), key_cache.data_ptr(),
             value_cache.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), o.data_ptr(),

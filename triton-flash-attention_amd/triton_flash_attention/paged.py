@@ -83,13 +83,14 @@ def _cache_reason(key_cache, value_cache) -> str | None:
         return "the kernel currently supports float16 and bfloat16"
     if key_cache.shape[3] > 128 or key_cache.shape[3] % 8:
         return "head_dim must be a multiple of 8 of at most 128"
-    if key_cache.stride() != value_cache.stride():
+    strides = _ops.cache_strides(key_cache)
+    if strides != _ops.cache_strides(value_cache):
         return "key_cache and value_cache must have the same strides"
-    if key_cache.stride(3) != 1 or any(s % 8 for s in key_cache.stride()[:3]) or any(
-            t.data_ptr() % 16 for t in (key_cache, value_cache)):
+    if any(t.stride(3) != 1 or t.data_ptr() % 16 or t.is_neg() for t in (key_cache, value_cache)) or (
+            any(s % 8 for s in strides)):
         return "the caches' rows must be contiguous, 16-byte aligned and a multiple of 8 apart"
-    if not key_cache.shape[3] <= _ops.row_stride(key_cache) < 1 << 25 or max(
-            key_cache.stride()) >= 1 << 40 or key_cache.shape[0] >= 1 << 31:
+    if not key_cache.shape[3] <= strides[2] < 1 << 25 or max(strides) >= 1 << 40 or (
+            key_cache.shape[0] >= 1 << 31):
         return "the caches' strides are outside the kernel's addressing"
     return None
 
@@ -179,8 +180,8 @@ def paged_cache_plan(
         if free_start.numel() != 1 or free_start.dtype != torch.int32 or free_start.device != device:
             raise ValueError(f"free_start must be one int32 value on {device}")
     if isinstance(num_tokens, bool) or not isinstance(num_tokens, int) or not (
-            0 <= num_tokens < 1 << 31):
-        raise ValueError(f"num_tokens must be an int from 0 to 2^31 - 1; got {num_tokens!r}")
+            0 <= num_tokens < 1 << 30):
+        raise ValueError(f"num_tokens must be an int from 0 to 2^30 - 1; got {num_tokens!r}")
     if B > 1 and page_table.stride(0) < page_table.shape[1]:
         raise ValueError("the rows of page_table must not overlap")
     reason = None
@@ -294,6 +295,11 @@ def _torch_paged(query, key_cache, value_cache, page_table, lengths, scale):
     return torch.stack(out).to(query.dtype)
 
 
+def _row_blocks(rows: int) -> int:
+    """Passes over a key/value head's keys that its query rows take (fa_layer.hpp paged_rows)."""
+    return 1 if rows <= 32 else -(-rows // 32)
+
+
 def paged_attention(
     query: torch.Tensor,
     key_cache: torch.Tensor,
@@ -320,7 +326,7 @@ def paged_attention(
     rows too.
 
     The gfx950 kernel serves float16 and bfloat16 with head_dim a multiple of 8 up to 128. It
-    reads the cache once for each 16 of the Hq / Hkv * N rows that share a key/value head, and
+    reads the cache once for each 32 of the Hq / Hkv * N rows that share a key/value head, and
     splits the keys over the whole GPU whatever the lengths are. It has no backward: inputs that
     require gradients run in PyTorch under ``backend="auto"``.
     """
@@ -367,7 +373,7 @@ def paged_attention(
         elif _forward_ad_active() or (torch.is_grad_enabled() and any(
                 t.requires_grad for t in (query, key_cache, value_cache))):
             reason = "the paged kernel has no backward"
-        elif Hq >= 1 << 20 or N >= 1 << 20 or B * H * -(-(Hq // H * N) // 16) * (
+        elif Hq >= 1 << 20 or N >= 1 << 20 or B * H * _row_blocks(Hq // H * N) * (
                 -(-page_table.shape[1] * S // 32) + 24) >= 1 << 30:
             reason = "too many sequences, heads or keys for one launch"
         else:
