@@ -25,9 +25,9 @@ from typing import NamedTuple
 
 import torch
 
-from . import _native, _ops
+from . import _ops
 from .attention import _SUPPORTED_DTYPES, Backend, _forward_ad_active, _kernel_scale
-from .rotary import _check_backend, _check_tensor, _falls_back, _gpu_reason, _plain
+from .rotary import _binding, _check_backend, _check_tensor, _falls_back, _gpu_reason
 
 _PAGE_MULTIPLE = 16
 _MOST_TOKENS = (1 << 30) - 64  # that a row of the page table holds (fa_capi_layer.hip)
@@ -162,9 +162,10 @@ def paged_cache_plan(
     -1 and ``free_start`` of the result exceeds ``len(free_pages)``; tokens behind a sequence's
     M pages have slot -1 as well. Negative lengths and counts are taken as 0.
     """
-    if _plain(backend):
-        out = _native.module().paged_plan(page_table, lengths, new_tokens, free_pages, page_size,
-                                          num_tokens, free_start)
+    native = _binding(backend)
+    if native is not None:
+        out = native.paged_plan(page_table, lengths, new_tokens, free_pages, page_size, num_tokens,
+                                free_start)
         if out is not None:
             return PagedPlan(*out)
     _check_backend(backend)
@@ -217,7 +218,8 @@ def paged_cache_store(
     no slot names stay as they were. key and value must not share memory with the cache.
     Gradients are not recorded: the call raises where one would have to be.
     """
-    if _plain(backend) and _native.module().paged_store(key, value, key_cache, value_cache, slots):
+    native = _binding(backend)
+    if native is not None and native.paged_store(key, value, key_cache, value_cache, slots):
         return
     _check_backend(backend)
     for name, t in (("key", key), ("value", value)):
@@ -330,9 +332,10 @@ def paged_attention(
     splits the keys over the whole GPU whatever the lengths are. It has no backward: inputs that
     require gradients run in PyTorch under ``backend="auto"``.
     """
-    if _plain(backend) and not _forward_ad_active():
-        out = _native.module().paged_attention(query, key_cache, value_cache, page_table, lengths,
-                                               scale, enable_gqa)
+    native = _binding(backend)
+    if native is not None and not _forward_ad_active():
+        out = native.paged_attention(query, key_cache, value_cache, page_table, lengths, scale,
+                                     enable_gqa)
         if out is not None:
             return out
     _check_backend(backend)

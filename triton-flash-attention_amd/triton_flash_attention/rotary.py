@@ -23,11 +23,12 @@ def _check_backend(backend: str) -> None:
         raise ValueError("backend must be one of: 'auto', 'triton', 'torch'")
 
 
-def _plain(backend: str) -> bool:
-    """Whether the call may go to the binding, which serves it or finds that Python has to look
-    (torch.compile cannot trace into it)."""
-    return ((backend == "auto" or backend == "triton")
-            and not torch.compiler.is_dynamo_compiling() and _native.available())
+def _binding(backend: str):
+    """The C++ binding, which serves the call or finds that Python has to look; None where the
+    call does not go there (torch.compile cannot trace into it)."""
+    if (backend == "auto" or backend == "triton") and not torch.compiler.is_dynamo_compiling():
+        return _native.module()
+    return None
 
 
 def _check_tensor(name: str, t, ndim: int, shape: str) -> None:
@@ -209,9 +210,10 @@ def qk_norm_rope(
     multiple of 8 up to 128 and R a multiple of 16; a weight's gradient is a float32 sum in a
     fixed order.
     """
-    if _plain(backend) and not _forward_ad_active():
-        out = _native.module().qk_norm_rope(query, key, cos, sin, query_weight, key_weight, eps,
-                                            positions, interleaved)
+    native = _binding(backend)
+    if native is not None and not _forward_ad_active():
+        out = native.qk_norm_rope(query, key, cos, sin, query_weight, key_weight, eps, positions,
+                                  interleaved)
         if out is not None:
             return out
     _check_backend(backend)
