@@ -130,6 +130,7 @@ def test_plan_kernel(case):
     dict(lengths=ragged(7, 4000, 7), new=ragged(7, 9000, 8), S=128),
     dict(lengths=[0] * 3000 + [7], new=[0] * 3000 + [2500], S=16),
     dict(lengths=[100000], new=[70001], S=64),
+    dict(lengths=ragged(1500, 500, 9), new=ragged(1500, 700, 10), S=16),  # 300 thousand tokens
 ])
 def test_plan_kernel_over_groups_and_blocks(case):
     check_plan(**case, device="cuda", backend="triton")
@@ -487,6 +488,39 @@ def test_attention_kernel_over_work_groups(case, dtype):
 def test_attention_kernel_in_wide_tables(case):
     *shape, M = case
     check_attend(*shape, torch.float16, M=M, device="cuda", backend="triton")
+
+
+@pytest.mark.gpu
+def test_plan_kernel_reads_strided_lengths():
+    lengths, new = (torch.tensor(v, dtype=torch.int32, device="cuda").view(4, 2)[:, 0]
+                    for v in ([3, 9, 20, 9, 0, 9, 33, 9], [1, 7, 2, 7, 5, 7, 0, 7]))
+    free = torch.arange(20, dtype=torch.int32, device="cuda")[::2]
+    tables = [torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4).t().contiguous()
+              .repeat(1, 2) for _ in range(2)]
+    start = torch.tensor(2, dtype=torch.int32, device="cuda")
+    plans = [paged_cache_plan(t, lengths, new, free, page_size=16, num_tokens=9, free_start=start,
+                              backend=b) for t, b in zip(tables, ("triton", "torch"))]
+    assert torch.equal(*tables)
+    assert all(torch.equal(a, b) for a, b in zip(*plans))
+
+
+@pytest.mark.gpu
+def test_attention_kernel_reads_a_transposed_table():
+    views, table, lens, dense = make_paged([100, 37], 2, 16, 32, torch.float16, device="cuda")
+    q = torch.randn(2, 4, 1, 32).half().cuda()
+    want = paged_attention(q, *views, table, lens, enable_gqa=True, backend="triton")
+    odd = table.t().contiguous().t()
+    assert odd.stride(1) != 1
+    strided = torch.stack([lens, lens * 0], 1)[:, 0]
+    got = paged_attention(q, *views, odd, strided, enable_gqa=True, backend="triton")
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_attention_kernel_many_units_a_wave():
+    """Stretches of hundreds of units: each wave takes new pages many times."""
+    lengths = [32768 - 1777 * b for b in range(16)]
+    check_attend(lengths, 16, 16, 1, 8, 128, torch.float16, device="cuda", backend="triton")
 
 
 @pytest.mark.gpu

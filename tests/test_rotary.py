@@ -291,6 +291,40 @@ def test_kernel_reads_expanded_and_odd_inputs():
 
 
 @pytest.mark.gpu
+def test_kernel_past_32_bits():
+    """Queries of more than 2^32 bytes and 2^31 values, as views of the projection's layout."""
+    N, H, D = 460_000, 40, 128
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.empty(1, N, H, D, dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+    q = q.transpose(1, 2)
+    assert q.numel() > 1 << 31
+    k = q[:, :1]
+    cos, sin = tables(4096, D, "cuda")
+    pos = torch.arange(N, device="cuda") % 4096
+    oq, ok = qk_norm_rope(q, k, cos, sin, positions=pos, backend="triton")
+    for h, n in ((0, 0), (39, N - 5), (20, 233_000)):
+        part = q[:, h:h + 1, n:n + 5].cpu()
+        ref = reference(part, None, cos.cpu(), sin.cpu(), 1e-6, pos[n:n + 5].cpu(), False)
+        close("query", oq[:, h:h + 1, n:n + 5], *ref, torch.bfloat16)
+    assert torch.equal(ok, oq[:, :1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_kernel_norms_of_small_and_large_rows(dtype):
+    """Rows whose squares reach both ends of float32's range, and a row of zeros, as PyTorch."""
+    scale = [0.0, 6e-8, 1e-4, 1.0, 6e4] if dtype == torch.float16 else [0.0, 1e-18, 1e-4, 1e4, 1e18]
+    q = torch.randn(1, 1, 5, 64, generator=torch.Generator().manual_seed(2))
+    q = (q.clamp(-1, 1) * torch.tensor(scale)[:, None]).to(dtype).cuda()
+    w = torch.ones(64, dtype=dtype, device="cuda")
+    cos, sin = tables(5, 64, "cuda")
+    for eps in (0.0, 1e-6):
+        got, want = (qk_norm_rope(q, q, cos, sin, query_weight=w, key_weight=w, eps=eps,
+                                  backend=b)[0] for b in ("triton", "torch"))
+        torch.testing.assert_close(got, want, rtol=2 * HALF[dtype] * 2, atol=1e-6, equal_nan=True)
+
+
+@pytest.mark.gpu
 def test_kernel_gradients_of_a_part():
     """Weights without gradients, one input alone, an output that is not used."""
     q, k, gq, gk, wq, wk = inputs(1, 4, 2, 33, 64, torch.float16, 4, device="cuda")

@@ -240,7 +240,7 @@ __global__ __launch_bounds__(64 * kRopeWaves) void rope_kernel(RopeArgs a) {
           float ss = 0.f;
 #pragma unroll
           for (int e = 0; e < 8; ++e) ss += v0[e] * v0[e] + v1[e] * v1[e];
-          const float r = __builtin_amdgcn_rsqf(row_sum<LPR>(ss) / (float)a.D + a.eps);
+          const float r = rsqrtf(row_sum<LPR>(ss) / (float)a.D + a.eps);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             v0[e] *= r * w0[e];
@@ -307,7 +307,7 @@ __global__ __launch_bounds__(64 * kRopeWaves) void rope_bwd_kernel(RopeArgs a) {
               tx += u0[e] * w0[e] * x0[e] + u1[e] * w1[e] * x1[e];
             }
             const float inv_d = 1.f / (float)a.D;
-            const float r = __builtin_amdgcn_rsqf(row_sum<LPR>(ss) * inv_d + a.eps) + l.poison;
+            const float r = rsqrtf(row_sum<LPR>(ss) * inv_d + a.eps) + l.poison;
             const float m = row_sum<LPR>(tx) * r * inv_d;  // mean of t x r
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
