@@ -26,22 +26,42 @@ __device__ __forceinline__ T wave_scan(T x, int lane) {
   return x;
 }
 
-// Sum over the threads before this one of a block of W waves, and the block's total. `sums`
-// holds one value a wave; ends with every thread past the barrier that publishes them.
-template <int W = 4, class T>
-__device__ __forceinline__ T block_scan(T x, T* sums, T* total) {
+// The same of an int, by DPP: no trip through the LDS unit.
+__device__ __forceinline__ int wave_scan(int x) {
+#define FA_SCAN_STEP(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xF, false)
+  FA_SCAN_STEP(0x111, 0xF);  // row_shr 1, 2, 4, 8: within 16 lanes
+  FA_SCAN_STEP(0x112, 0xF);
+  FA_SCAN_STEP(0x114, 0xF);
+  FA_SCAN_STEP(0x118, 0xF);
+  FA_SCAN_STEP(0x142, 0xA);  // row_bcast 15 to rows 1 and 3, then 31 to rows 2 and 3
+  FA_SCAN_STEP(0x143, 0xC);
+#undef FA_SCAN_STEP
+  return x;
+}
+
+// Sums over the threads before this one of a block of W waves (before[i] of x[i]) and the
+// block's totals (all[i]), behind one barrier.
+template <int W, int K>
+__device__ __forceinline__ void block_scan(const int (&x)[K], int (*sums)[K], int (&before)[K],
+                                           int (&all)[K]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const T incl = wave_scan(x, lane);
-  if (lane == 63) sums[wave] = incl;
-  __syncthreads();
-  T before = incl - x, all = 0;
+  int incl[K];
 #pragma unroll
-  for (int w = 0; w < W; ++w) {
-    if (w < wave) before += sums[w];
-    all += sums[w];
+  for (int i = 0; i < K; ++i) incl[i] = wave_scan(x[i]);
+  if (lane == 63)
+#pragma unroll
+    for (int i = 0; i < K; ++i) sums[wave][i] = incl[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    before[i] = incl[i] - x[i];
+    all[i] = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (w < wave) before[i] += sums[w][i];
+      all[i] += sums[w][i];
+    }
   }
-  *total = all;
-  return before;
 }
 
 // Two sums over the threads before this one of a block of 256, and the block's totals, behind
@@ -346,33 +366,36 @@ struct PagedPlace {
 // blocks of W waves.
 template <int D, int W>
 __device__ __forceinline__ PagedLine paged_find(const PagedArgs& a, int s, PagedPlace* place) {
-  __shared__ int sums[W], found[4];
-  __shared__ int64_t sums2[W];
+  __shared__ int sums[W][3], found[4];
   const int HB = a.Hkv * a.blocks;
   const int per = (a.B + 64 * W - 1) / (64 * W);
   const int b0 = threadIdx.x * per, b1 = min(a.B, b0 + per);
   constexpr int S1 = kPagedWaves, S2 = 2 * kPagedWaves;  // stretches of padded lines
-  int own = 0, in1 = 0, in2 = 0;
+  // Of the thread's sequences: units on a line that is not padded, stretches on the padded ones.
+  int own[3] = {0, 0, 0}, first[3], all[3];
   for (int b = b0; b < b1; ++b) {
     const int u = paged_units(a, a.lengths[b]);
-    own += (u + kPagedLead<D>) * HB;
-    in1 += (u + S1 - 1) / S1 * HB;
-    in2 += (u + S2 - 1) / S2 * HB;
+    own[0] += (u + kPagedLead<D>) * HB;
+    own[1] += (u + S1 - 1) / S1 * HB;
+    own[2] += (u + S2 - 1) / S2 * HB;
   }
+  block_scan<W>(own, sums, first, all);
   PagedLine line;
-  int64_t all12;
-  const int64_t before12 = block_scan<W>((int64_t)in2 << 32 | (uint32_t)in1, sums2, &all12);
-  int before = block_scan<W>(own, sums, &line.total), mine = own;
-  const int all1 = (int)(uint32_t)all12, all2 = (int)(all12 >> 32);
-  line.padded = all2 <= a.grid;
-  line.lead = line.padded ? 0 : kPagedLead<D>;
-  line.stretch = (line.total + a.grid - 1) / a.grid;
+  line.padded = all[2] <= a.grid;
+  int before, mine;
   if (line.padded) {
-    const bool one = all1 <= a.grid;
-    line.stretch = one ? S1 : S2;
-    line.total = (one ? all1 : all2) * line.stretch;
-    before = (one ? (int)(uint32_t)before12 : (int)(before12 >> 32)) * line.stretch;
-    mine = (one ? in1 : in2) * line.stretch;
+    const int i = all[1] <= a.grid ? 1 : 2;
+    line.lead = 0;
+    line.stretch = i == 1 ? S1 : S2;
+    line.total = (i == 1 ? all[1] : all[2]) * line.stretch;
+    before = (i == 1 ? first[1] : first[2]) * line.stretch;
+    mine = (i == 1 ? own[1] : own[2]) * line.stretch;
+  } else {
+    line.lead = kPagedLead<D>;
+    line.total = all[0];
+    line.stretch = (line.total + a.grid - 1) / a.grid;
+    before = first[0];
+    mine = own[0];
   }
   const int64_t at = (int64_t)s * line.stretch;
   if (at >= before && at < (int64_t)before + mine) {
@@ -407,13 +430,6 @@ template <int D>
 __device__ __forceinline__ float* paged_part(const PagedArgs& a, int64_t slot) {
   return a.part + a.grid * (sizeof(PagedCut) / 4) + slot * (a.rows * (D + 1));
 }
-
-// A wave's units of a piece: where the half units of its next 32 units lie, one a lane
-// (lane 2 k + half for unit k).
-struct PagedHalves {
-  uint32_t lo, hi;  // byte offset of the half's first row from its head's rows in page 0
-  int rows;         // rows that exist
-};
 
 // A row of a triple: query n of the group's head h, if it exists; and its row of the output.
 struct PagedRow {
@@ -526,56 +542,43 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArg
     const half_t* const k_head = a.k + kvh * a.ks[1];
     const half_t* const v_head = a.v + kvh * a.ks[1];
     bool bad = !fits;
-    // The page of half unit lane & 1 of unit i0 + lane / 2, and from it where that half lies.
+    // The page of half unit lane & 1 of unit i0 + lane / 2, and its first row there.
     auto half_key = [&](int i0) __attribute__((always_inline)) {
-      const int i = i0 + (lane >> 1);
-      return i < mine ? (u0 + wave + NW * i) * kPagedUnit + 16 * (lane & 1) : keys;
+      return (u0 + wave + NW * (i0 + (lane >> 1))) * kPagedUnit + 16 * (lane & 1);
     };
     auto half_page = [&](int i0) __attribute__((always_inline)) {
       const int key = half_key(i0);
-      return key < keys ? a.table[at.b * a.table_stride + key / a.S] : 0;
+      return i0 + (lane >> 1) < mine && key < keys
+                 ? a.table[at.b * a.table_stride + key / a.S] : 0;
     };
-    auto halves = [&](int i0, int page) __attribute__((always_inline)) {
-      const int key = half_key(i0);
-      PagedHalves p = {0u, 0u, 0};
-      if (key >= keys) return p;
-      if (page < 0 || page >= a.pages) {
-        p.rows = -1;  // no such page
-        return p;
-      }
-      const int64_t off = (page * a.ks[0] + key % a.S * a.ks[2]) * 2;
-      p.lo = (uint32_t)off;
-      p.hi = (uint32_t)(off >> 32);
-      p.rows = min(16, keys - key);
-      return p;
-    };
-    PagedHalves now = halves(0, half_page(0));
+    int page = half_page(0), row = half_key(0) % a.S;  // of the units from i & ~31 on
     int next_page = half_page(32);
 
     u32x4 kx[2][KD], vx[T::VI];
     int64_t off[2];
     uint32_t bytes[2];
-    // Where unit i lies; its K and its V on their way to the registers.
+    // Where unit i lies; its K and its V on their way to the registers. Past the wave's last
+    // unit, and in pages that do not exist, no rows.
     auto turn_to = [&](int i) __attribute__((always_inline)) {
       if ((i & 31) == 0 && i > 0) {
-        now = halves(i, next_page);
+        page = next_page;
+        row = half_key(i) % a.S;
         next_page = half_page(i + 32);
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int from = 2 * (i & 31) + e;
-        const uint32_t lo = __builtin_amdgcn_readlane(now.lo, from);
-        const uint32_t hi = __builtin_amdgcn_readlane(now.hi, from);
-        const int n_rows = __builtin_amdgcn_readlane(now.rows, from);
-        off[e] = (int64_t)((uint64_t)hi << 32 | lo);
-        bytes[e] = n_rows > 0 ? (uint32_t)((n_rows - 1) * row_bytes + a.d * 2) : 0u;
-        bad |= n_rows < 0;
+        const int there = keys - ((u0 + wave + NW * i) * kPagedUnit + 16 * e);
+        const int pg = __builtin_amdgcn_readlane(page, 2 * (i & 31) + e);
+        const bool any = i < mine && there > 0, known = pg >= 0 && pg < a.pages;
+        bad |= any && !known;
+        off[e] = pg * a.ks[0] + __builtin_amdgcn_readlane(row, 2 * (i & 31) + e) * a.ks[2];
+        bytes[e] = any && known ? (uint32_t)((min(there, 16) - 1) * row_bytes + a.d * 2) : 0u;
       }
     };
     auto load_k = [&]() __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const rsrc_t r_k = make_rsrc(reinterpret_cast<const char*>(k_head) + off[e], bytes[e]);
+        const rsrc_t r_k = make_rsrc(k_head + off[e], bytes[e]);
 #pragma unroll
         for (int kd = 0; kd < KD; ++kd) kx[e][kd] = buf_load_b128(r_k, k_off[kd]);
       }
@@ -584,7 +587,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArg
 #pragma unroll
       for (int j = 0; j < T::VI; ++j) {
         const int e = j * T::VROWS / 16;
-        const rsrc_t r_v = make_rsrc(reinterpret_cast<const char*>(v_head) + off[e], bytes[e]);
+        const rsrc_t r_v = make_rsrc(v_head + off[e], bytes[e]);
         vx[j] = buf_load_b128(r_v, v_off[j]);
       }
     };
