@@ -5,7 +5,7 @@ the GPU, and a decoding loop that runs them together with qk_norm_rope.
 Tolerance of an attention output, element by element, with A = sum_j p_j |v_j| (p the exact
 probabilities), u half a step of the type (``finfo.eps / 2``): the probabilities are rounded to
 the type for the product with V, u A (fp16 below 2^-14: 2^-25 each, of a row whose largest is
-at least 1: 2^-25 sum_j |v_j|), the output once, u |o|. In float32 the scores are sums of at
+at least 2^7: 2^-32 sum_j |v_j|), the output once, u |o|. In float32 the scores are sums of at
 most 128 products, off by (128 + 8) 2^-24 of scale sum |q| |k|, exp2 and its argument by a few
 2^-24 of |s|: a relative error of e^d - 1 in numerator and denominator, 4 d A with d the sum of
 the two; the sums over n keys add n 2^-24 A at most."""
@@ -335,7 +335,7 @@ def attention_reference(q, dense, scale, dtype):
             size = (kk.abs() @ qi.abs()).squeeze(-1).amax(-1) * abs(scale)
             d = (136 * size + 8 * s.abs().amax(-1)) * F32
             bound[b, :, i] = (A * (HALF[dtype] + seen * F32 + 4 * d[:, None])
-                              + (2.0 ** -25 * vv.abs().sum(1) if dtype == torch.float16 else 0))
+                              + (2.0 ** -32 * vv.abs().sum(1) if dtype == torch.float16 else 0))
     return o, bound
 
 
@@ -550,6 +550,31 @@ def test_attention_kernel_large_scores():
     """Scores in the thousands: one key takes all the weight, wherever it lies."""
     check_attend([777, 2000], 8, 2, 1, 64, 16, torch.bfloat16, spread=30.0, device="cuda",
                  backend="triton")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize(("B", "n"), [(1, 896), (512, 32768)])
+def test_attention_kernel_counts_the_many_small_weights_of_long_rows(B, n, dtype):
+    """Every wave's first unit holds the largest score, 18 above all others: 2^-26 of its weight
+    each, and the only ones with a value. All sequences share the pages."""
+    S, D = 16, 32
+    k, v = (torch.zeros(2, 1, S, D, dtype=dtype, device="cuda") for _ in range(2))
+    k[1, 0, 0, 0], v[:] = 18.0, 1.0
+    v[1, 0, 0] = 0.0
+    table = torch.zeros(1, n // S, dtype=torch.int32, device="cuda")
+    table[0, :8:2] = 1
+    q = torch.zeros(B, 1, 1, D, dtype=dtype, device="cuda")
+    q[..., 0] = 1.0
+    o = paged_attention(q, k, v, table.expand(B, -1),
+                        torch.full((B,), n, dtype=torch.int32, device="cuda"), scale=1.0,
+                        backend="triton").double().cpu()
+    peaks, small = 4, (n - 4) * math.exp(-18.0)
+    want = small / (peaks + small)
+    d = (136 + 8) * 18 * F32
+    bound = want * (2 * HALF[dtype] + n * F32 + 4 * d) + (
+        n / peaks * 2.0 ** -32 + 2.0 ** -25 if dtype == torch.float16 else 0)
+    assert float((o - want).abs().max()) <= bound
 
 
 @pytest.mark.gpu

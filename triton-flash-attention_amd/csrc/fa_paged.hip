@@ -7,6 +7,7 @@
 // slots and positions hold is on the GPU and is checked here, entry by entry, before an address
 // is made of it.
 #include <algorithm>
+#include <type_traits>
 
 #include "fa_common.hpp"
 #include "fa_layer.hpp"
@@ -316,9 +317,15 @@ hipError_t launch_paged_store(const StoreArgs& a, hipStream_t stream) {
 //   O^T block dd: lane holds row c16, d = 16 dd + 4 G + j.
 // Row r of the triple is query r % N of the group's head r / N.
 
-// A row's probabilities are taken against a reference max that moves only when their sum over
-// a unit exceeds this, far below where fp16 ends.
-constexpr float kPagedSumLimit = 256.0f;
+// A row's probabilities are taken against a reference that moves only when their sum over a
+// lane's eight keys of a unit exceeds a limit. fp16 ends at 2^16 and rounds to zero below 2^-25:
+// there the reference is 2^7 below the max, so that the many small ones of a long row (2^-26 of
+// the largest, a million times) still count. bf16 has room at both ends, but values up to
+// 2^128, whose sums have none: there it is the max.
+template <class E>
+constexpr float kPagedShift = std::is_same_v<E, F16> ? 7.f : 0.f;
+template <class E>
+constexpr float kPagedSumLimit = std::is_same_v<E, F16> ? 32768.f : 256.f;
 
 constexpr int kPagedWaves = 4;  // of a work-group
 
@@ -646,13 +653,13 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArg
           return sum;
         };
         float l_u = probs(m[rb]);
-        if (__builtin_amdgcn_ballot_w64(!(l_u <= kPagedSumLimit)) != 0) {
+        if (__builtin_amdgcn_ballot_w64(!(l_u <= kPagedSumLimit<E>)) != 0) {
           float mt = s[rb][0][0];
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int j = 0; j < 4; ++j) mt = __builtin_fmaxf(mt, s[rb][kb][j]);
-          const float m_new = __builtin_fmaxf(m[rb], quarters_max(mt) * c);
+          const float m_new = __builtin_fmaxf(m[rb], quarters_max(mt) * c - kPagedShift<E>);
           const float ref = exp_reference(m_new);
           const float alpha = exp2_fast(m[rb] - ref);
           l[rb] *= alpha;
