@@ -440,23 +440,24 @@ def test_kernel_has_no_second_derivative():
 
 
 @pytest.mark.gpu
-def test_capture_beside_a_living_graph_of_the_same_leaves_is_refused():
+@pytest.mark.parametrize("eps", [1e-6, 0])  # an int goes through the Python Function
+def test_capture_beside_a_living_graph_of_the_same_leaves_is_refused(eps):
     q, k, gq, gk, _, _ = inputs(1, 2, 1, 8, 32, torch.float16, 9, device="cuda")
     cos, sin = tables(8, 32, "cuda")
     q.requires_grad_()
-    alive, _ = qk_norm_rope(q, k, cos, sin, backend="triton")
+    alive, _ = qk_norm_rope(q, k, cos, sin, eps=eps, backend="triton")
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         z = gq + 0  # the graph is not empty
         with pytest.raises(RuntimeError, match="same leaf tensors"):
-            qk_norm_rope(q, k, cos, sin, backend="triton")
+            qk_norm_rope(q, k, cos, sin, eps=eps, backend="triton")
     want = torch.autograd.grad(alive, q, gq)[0]
     del alive, _
     with torch.cuda.graph(torch.cuda.CUDAGraph()):
-        out, _ = qk_norm_rope(q, k, cos, sin, backend="triton")
+        out, _ = qk_norm_rope(q, k, cos, sin, eps=eps, backend="triton")
         torch.autograd.grad(out, q, gq)
     del out, _
-    out, _ = qk_norm_rope(q, k, cos, sin, backend="triton")
+    out, _ = qk_norm_rope(q, k, cos, sin, eps=eps, backend="triton")
     assert torch.equal(torch.autograd.grad(out, q, gq)[0], want)
     assert z.shape == gq.shape
 

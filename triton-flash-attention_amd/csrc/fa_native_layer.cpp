@@ -263,15 +263,16 @@ class QkNormRope : public torch::autograd::Function<QkNormRope> {
 // alive. Where that is the default stream, a backward that is being captured would draw it into
 // the capture, which it cannot take part in: that fails in ways that can end the process, so such
 // a call is refused before it starts.
-void refuse_mixed_capture(std::initializer_list<const at::Tensor*> leaves) {
+template <class Tensors>
+void refuse_mixed_capture(const Tensors& leaves) {
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-  for (const at::Tensor* t : leaves) {
-    if (!wants_grad(*t) || !t->is_leaf()) continue;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+  for (const at::Tensor& t : leaves) {
+    if (!wants_grad(t) || !t.is_cuda() || !t.is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
     if (!node) continue;
     const auto stream = node->stream();
     // (by id: autograd's streams pass for CUDA ones)
-    if (stream && stream->id() == c10::hip::getDefaultHIPStream(t->device().index()).id())
+    if (stream && stream->id() == c10::hip::getDefaultHIPStream(t.device().index()).id())
       throw std::runtime_error(
           "qk_norm_rope is being captured into a graph while a result of an earlier call with the "
           "same leaf tensors is alive on the default stream: drop it first, or detach it");
@@ -325,7 +326,7 @@ py::object native_rope(py::handle query, py::handle key, py::handle cos, py::han
   c10::DeviceGuard guard(device);
   if (at::GradMode::is_enabled() &&
       (wants_grad(*q) || wants_grad(*k) || wants_grad(qw) || wants_grad(kw))) {
-    refuse_mixed_capture({q, k, &qw, &kw});
+    refuse_mixed_capture(std::array<at::Tensor, 4>{*q, *k, qw, kw});
     const auto out = QkNormRope::apply(*q, *k, maybe(qw), maybe(kw), *c, *s, maybe(pos), ep, inter);
     return py::make_tuple(out[0], out[1]);
   }
@@ -516,6 +517,7 @@ void init_layer(const std::vector<I64>& addresses) {
 void bind_layer(py::module_& m) {
   m.def("init_layer", &init_layer);
   m.def("qk_norm_rope", &native_rope);
+  m.def("refuse_mixed_capture", &refuse_mixed_capture<std::vector<at::Tensor>>);
   m.def("paged_plan", &native_plan);
   m.def("paged_store", &native_store);
   m.def("paged_attention", &native_paged);

@@ -223,6 +223,8 @@ def qk_norm_rope(
                      for x, w in ((query, query_weight), (key, key_weight)))
     weights = () if query_weight is None else (query_weight, key_weight)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (query, key, *weights)):
+        if native is not None:
+            native.refuse_mixed_capture([query, key, *weights])
         return _QkNormRope.apply(query, key, query_weight, key_weight, cos, sin, positions,
                                  float(eps), interleaved)
     return _ops.qk_norm_rope(query, key, cos, sin, query_weight, key_weight, float(eps), positions,
