@@ -865,7 +865,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void paged_join_kernel(PagedArgs a
 // that takes as long as a second launch saves: D = 128, B x Hkv 8 / 64 / 256 triples, us, this /
 // split and joined: 512 keys 8.9 / 11.3, 9.3 / 13.2, 13.6 / 20.2; 1024 keys 13.5 / 10.4, 13.8 /
 // 16.3, 25.8 / 34.3; 2048 keys 21.1 / 11.0, 21.9 / 20.1, 47.7 / 57.3 (kernels alone; the second
-// launch adds about 1.5, and 2 on the host). A longer row may hold one long sequence among short
+// launch adds about 1.5). A longer row may hold one long sequence among short
 // ones, whose time the split would share out.
 bool paged_short(int64_t triples, int64_t keys) {
   return keys <= 1024 || (keys <= 2048 && triples >= 256);
