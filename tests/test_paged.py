@@ -491,6 +491,20 @@ def test_attention_kernel_in_wide_tables(case):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("case", [
+    # heads that share a line, token by token: consecutive stretches an XCD
+    (ragged(24, 1500, 15), 8, 4, 1, 32, 16, 100),
+    ([9000, 1, 130], 4, 2, 5, 24, 16, 600),
+    (ragged(40, 900, 16), 3, 3, 1, 56, 32, 70),
+    ([1200, 5], 2, 2, 1, 8, 16, 80),          # fewer work-groups than the chip holds
+])
+def test_attention_kernel_of_heads_that_share_lines(case):
+    *shape, M = case
+    o = check_attend(*shape, torch.float16, M=M, layout="tokens", device="cuda", backend="triton")
+    assert torch.equal(o, check_attend(*shape, torch.float16, M=M, device="cuda", backend="triton"))
+
+
+@pytest.mark.gpu
 def test_plan_kernel_reads_strided_lengths():
     lengths, new = (torch.tensor(v, dtype=torch.int32, device="cuda").view(4, 2)[:, 0]
                     for v in ([3, 9, 20, 9, 0, 9, 33, 9], [1, 7, 2, 7, 5, 7, 0, 7]))
