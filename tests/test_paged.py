@@ -136,6 +136,44 @@ def test_plan_kernel_over_groups_and_blocks(case):
     check_plan(**case, device="cuda", backend="triton")
 
 
+def check_plan_of_counts_past_32_bits(big, T, device, backend):
+    """``big`` counts of 2^30 - 1 in the first 1024 sequences, then many of one token: the
+    step's T tokens all belong to sequence 0, and only their pages are written."""
+    S, M, B, most = 16, 4, 2100, (1 << 30) - 1
+    i32 = dict(dtype=torch.int32, device=device)
+    new = torch.ones(B, **i32)
+    new[:1024] = 0
+    new[:big] = most
+    free = torch.arange(10, 10 + 4 * B, **i32)
+    table = torch.full((B, M), -9, **i32)
+    plan = paged_cache_plan(table, torch.zeros(B, **i32), new, free, page_size=S, num_tokens=T,
+                            backend=backend)
+    entries = torch.full((B, M), -9, dtype=torch.int32)
+    entries[0, :cdiv(T, S)] = torch.arange(10, 10 + cdiv(T, S))
+    assert torch.equal(table.cpu(), entries)
+    t = torch.arange(T)
+    assert torch.equal(plan.slots.cpu(), 10 * S + t) and torch.equal(plan.positions.cpu(), t.int())
+    total = [0]
+    for n in new.tolist():
+        total.append(min(total[-1] + n, 1 << 62))
+    assert plan.starts.tolist() == [min(n, (1 << 31) - 1) for n in total]
+    assert torch.equal(plan.lengths, new) and plan.free_start.tolist() == [M * big + B - 1024]
+
+
+COUNTS_PAST_32_BITS = [(2, 64), (3, 64), (4, 0), (4, 50), (4, 64), (5, 64), (8, 64), (12, 64)]
+
+
+@pytest.mark.parametrize(("big", "T"), COUNTS_PAST_32_BITS)
+def test_plan_torch_form_of_counts_past_32_bits(big, T):
+    check_plan_of_counts_past_32_bits(big, T, "cpu", "torch")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize(("big", "T"), COUNTS_PAST_32_BITS)
+def test_plan_kernel_of_counts_past_32_bits(big, T):
+    check_plan_of_counts_past_32_bits(big, T, "cuda", "triton")
+
+
 def _plan_args():
     i = torch.int32
     return dict(page_table=torch.zeros(2, 4, dtype=i), lengths=torch.zeros(2, dtype=i),

@@ -160,7 +160,8 @@ __global__ __launch_bounds__(256) void paged_plan_kernel(PlanArgs a) {
     // The thread's tokens, from the group's first on, and the last sequence with first <= t,
     // which holds token t.
     const int from = (int)(max(t0, tokens) - tokens) + tid;
-    const int to = (int)(min(t1, tokens + n_all) - tokens);
+    // (none in block 0's later groups, whose distance from its tokens may pass 32 bits)
+    const int to = (int)(max(min(t1, tokens + n_all), tokens) - tokens);
     const int count = min(kPlanSeqs, a.B - b0);
     int seq[OWN], pos[OWN], page[OWN], in_page[OWN], entry[OWN];
 #pragma unroll
