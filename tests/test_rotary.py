@@ -180,6 +180,61 @@ def test_positions_outside_the_tables_are_nan():
             assert o[:, :, 1].isnan().all() and not o[:, :, 0::2].isnan().any()
 
 
+def check_gradients_of_bad_positions(norm, interleaved, each, device, backend, dtype):
+    """Tokens outside the tables have NaN for their gradients, and so have the weights; the other
+    tokens' gradients are those of a call without them."""
+    B, N, D, R = 2, 5, 48, 32
+    q, k, gq, gk, wq, wk = inputs(B, 4, 2, N, D, dtype, 7, device=device)
+    cos, sin = tables(6, R, device)
+    if each:
+        pos = torch.tensor([[0, 1, 2, 3, 6], [-1, 5, 4, 1 << 30, 0]], device=device)
+    else:
+        pos = torch.tensor([3, -7, 5, 6, 0], device=device)
+    bad = ((pos < 0) | (pos >= 6)).expand(B, N)
+
+    def grads(positions):
+        leaves = [t.detach().requires_grad_() for t in (q, k)]
+        weights = {}
+        if norm:
+            leaves += [w.to(device).requires_grad_() for w in (wq, wk)]
+            weights = dict(query_weight=leaves[2], key_weight=leaves[3])
+        out = qk_norm_rope(leaves[0], leaves[1], cos, sin, positions=positions,
+                           interleaved=interleaved, backend=backend, **weights)
+        return torch.autograd.grad(out, leaves, (gq, gk))
+
+    got, want = grads(pos), grads(torch.where((pos < 0) | (pos >= 6), 0, pos))
+    for g, w in zip(got[:2], want):
+        rows = bad[:, None, :, None].expand_as(g)
+        assert g[rows].isnan().all() and torch.equal(g[~rows], w[~rows])
+    assert all(g.isnan().all() for g in got[2:]) and not any(w.isnan().any() for w in want)
+
+
+BAD_POSITIONS = [(n, i, e) for n in (True, False) for i in (True, False) for e in (True, False)]
+
+
+@pytest.mark.parametrize(("norm", "interleaved", "each"), BAD_POSITIONS)
+def test_gradients_of_positions_outside_the_tables(norm, interleaved, each):
+    for dtype in (torch.float32, torch.float64, torch.bfloat16):
+        check_gradients_of_bad_positions(norm, interleaved, each, "cpu", "torch", dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize(("norm", "interleaved", "each"), BAD_POSITIONS)
+def test_kernel_gradients_of_positions_outside_the_tables(norm, interleaved, each):
+    for dtype in (torch.float16, torch.bfloat16):
+        check_gradients_of_bad_positions(norm, interleaved, each, "cuda", "triton", dtype)
+
+
+def test_tables_take_no_gradient_from_positions_outside_them():
+    q = torch.randn(1, 2, 3, 16)
+    leaves = [t.requires_grad_() for t in tables(4, 8)]
+    out = qk_norm_rope(q, q, *leaves, positions=torch.tensor([1, 4, 3]))
+    got = torch.autograd.grad(sum(o.sum() for o in out), leaves)
+    out = qk_norm_rope(q[:, :, ::2], q[:, :, ::2], *leaves, positions=torch.tensor([1, 3]))
+    want = torch.autograd.grad(sum(o.sum() for o in out), leaves)
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
 def _valid():
     cos, sin = tables(8, 16)
     return dict(query=torch.randn(1, 2, 4, 32), key=torch.randn(1, 1, 4, 32), cos=cos, sin=sin)

@@ -136,18 +136,20 @@ def _torch_rope(x, w, cos, sin, eps, positions, interleaved):
     """The formulas in PyTorch, in float32 (float64 for a float64 input)."""
     wide = torch.float64 if x.dtype == torch.float64 else torch.float32
     y = x.to(wide)
-    if w is not None:
-        y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + eps) * w.to(wide)
     if positions is None:
         c, s = cos[:x.shape[2]], sin[:x.shape[2]]
     else:
         known = (positions >= 0) & (positions < cos.shape[0])
         at = torch.where(known, positions, 0).long()
-        # [N, R/2] or [B, 1, N, R/2]; a token outside the tables is NaN
-        c, s = cos[at], sin[at]
-        y = torch.where((known if known.ndim == 1 else known[:, None])[..., None], y, math.nan)
+        # [N, R/2] or [B, 1, N, R/2]; a token outside the tables is NaN, and by the product so
+        # are its gradients (the tables' are not: where keeps them apart)
+        known = known[..., None]
+        c, s = (torch.where(known, t[at], math.nan) for t in (cos, sin))
         if positions.ndim == 2:
-            c, s = c[:, None], s[:, None]
+            known, c, s = known[:, None], c[:, None], s[:, None]
+        y = y * torch.where(known, 1.0, math.nan).to(wide)
+    if w is not None:
+        y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + eps) * w.to(wide)
     c, s, half = c.to(wide), s.to(wide), cos.shape[1]
     turned, rest = y[..., :2 * half], y[..., 2 * half:]
     if interleaved:
