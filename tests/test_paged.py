@@ -629,6 +629,46 @@ def test_attention_kernel_counts_the_many_small_weights_of_long_rows(B, n, dtype
     assert float((o - want).abs().max()) <= bound
 
 
+def large_values(kind, lengths, M, dtype, device, backend):
+    """Values of up to 2^127, whose sums have no room in float32, under scores that are random,
+    all equal, or grow with the key: the output is no larger than the largest value."""
+    S, D, Hq, Hkv, N = 16, 32, 4, 2, 2
+    views, table, lens, dense = make_paged(lengths, Hkv, S, D, dtype, M=M, seed=6)
+    views[1].abs_().mul_(2.0 ** 124)  # exact
+    for b, (k, v) in enumerate(dense):
+        v.abs_().mul_(2.0 ** 124)
+        at = torch.arange(lengths[b])
+        if kind == "equal":
+            k.zero_()
+        elif kind == "grow":  # by steps of 4: a weight of e^4 against the keys before
+            k.zero_()[:, :, 0] = (at // 40 * 4.0).clamp(max=120.0)[:, None]
+        views[0][table[b].long()[at // S], :, at % S] = k.to(dtype)
+    q = torch.randn(len(lengths), Hq, N, D, generator=torch.Generator().manual_seed(7)).to(dtype)
+    if kind == "grow":
+        q[..., 0] = 1.0
+    views = [v.to(device) for v in views]
+    o = paged_attention(q.to(device), *views, table.to(device), lens.to(device), scale=1.0,
+                        enable_gqa=True, backend=backend)
+    want, bound = attention_reference(q, dense, 1.0, dtype)
+    limit = HALF[dtype] * want.abs() * 1.01 + bound * 1.01
+    assert bool(((o.double().cpu() - want).abs() <= limit).all())
+
+
+LARGE_VALUES = [(kind, *c) for kind in ("random", "equal", "grow")
+                for c in (([300, 1, 33], None), ([9000, 40, 1200], 600))]
+
+
+@pytest.mark.parametrize(("kind", "lengths", "M"), LARGE_VALUES)
+def test_attention_torch_form_large_values(kind, lengths, M):
+    large_values(kind, lengths, M, torch.bfloat16, "cpu", "torch")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize(("kind", "lengths", "M"), LARGE_VALUES)
+def test_attention_kernel_large_values(kind, lengths, M):
+    large_values(kind, lengths, M, torch.bfloat16, "cuda", "triton")
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("fill", [math.inf, -math.inf, 65504.0])
 def test_attention_kernel_never_sees_what_lies_behind_the_length(fill):

@@ -318,15 +318,22 @@ hipError_t launch_paged_store(const StoreArgs& a, hipStream_t stream) {
 //   O^T block dd: lane holds row c16, d = 16 dd + 4 G + j.
 // Row r of the triple is query r % N of the group's head r / N.
 
-// A row's probabilities are taken against a reference that moves only when their sum over a
-// lane's eight keys of a unit exceeds a limit. fp16 ends at 2^16 and rounds to zero below 2^-25:
-// there the reference is 2^7 below the max, so that the many small ones of a long row (2^-26 of
-// the largest, a million times) still count. bf16 has room at both ends, but values up to
-// 2^128, whose sums have none: there it is the max.
+// A row's probabilities are taken against a reference that moves only when they outgrow a limit.
+// fp16 ends at 2^16 and rounds to zero below 2^-25: there the reference is 2^7 below the max, so
+// that the many small ones of a long row (2^-26 of the largest, a million times) still count, and
+// moves when a lane's eight of a unit sum to more than the type holds. bf16 has room at both ends,
+// but values up to 2^128, whose sums in float32 have none: there all probabilities so far are held
+// to a sum of 2^-5 a lane, 2^-3 a wave, 1/2 with the four waves, so that no sum of values passes
+// the largest of them. The reference moves to 2^16 above the max, or above the sum where many keys
+// alike have filled it (8 thousand keys a wave, then once in 2^11 times as many); a weight below
+// 2^-110 of the largest is zero. It costs nothing (32 sequences of 17 to 8192 keys 106.3 us with
+// sums that are not held).
 template <class E>
-constexpr float kPagedShift = std::is_same_v<E, F16> ? 7.f : 0.f;
+constexpr bool kPagedWide = std::is_same_v<E, BF16>;
 template <class E>
-constexpr float kPagedSumLimit = std::is_same_v<E, F16> ? 32768.f : 256.f;
+constexpr float kPagedShift = kPagedWide<E> ? -16.f : 7.f;
+template <class E>
+constexpr float kPagedSumLimit = kPagedWide<E> ? 0.03125f : 32768.f;
 
 constexpr int kPagedWaves = 4;  // of a work-group
 
@@ -660,14 +667,18 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArg
             }
           return sum;
         };
+        // The probabilities' sum, and what the limit holds: this unit's, or all so far.
         float l_u = probs(m[rb]);
-        if (__builtin_amdgcn_ballot_w64(!(l_u <= kPagedSumLimit<E>)) != 0) {
+        const float held = kPagedWide<E> ? l[rb] + l_u : l_u;
+        if (__builtin_amdgcn_ballot_w64(!(held <= kPagedSumLimit<E>)) != 0) {
           float mt = s[rb][0][0];
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int j = 0; j < 4; ++j) mt = __builtin_fmaxf(mt, s[rb][kb][j]);
-          const float m_new = __builtin_fmaxf(m[rb], quarters_max(mt) * c - kPagedShift<E>);
+          float m_new = __builtin_fmaxf(m[rb], quarters_max(mt) * c - kPagedShift<E>);
+          if constexpr (kPagedWide<E>)
+            m_new = __builtin_fmaxf(m_new, m[rb] + log2_fast(quarters_max(l[rb])) - kPagedShift<E>);
           const float ref = exp_reference(m_new);
           const float alpha = exp2_fast(m[rb] - ref);
           l[rb] *= alpha;
@@ -775,6 +786,9 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArg
 constexpr int kJoinWaves = 4;
 template <int D>
 constexpr int kJoinRows = 64 / (D / 4);  // of a wave
+// The weight of a row's largest piece: those of 512 pieces, the most there are, sum to 1/2, so
+// that sums of values near 2^128 stay in float32.
+constexpr float kJoinWeight = 0x1p-10f;
 
 inline __host__ __device__ int join_groups(int rows, int wave_rows) {
   return rows <= wave_rows ? 1 : rows <= 2 * wave_rows ? 2 : 4;
@@ -823,8 +837,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void paged_join_kernel(PagedArgs a
   float4v acc = {0.f, 0.f, 0.f, 0.f};
   if (part0 <= cut.more) {
     m = p0.lse;
-    l = m == -INFINITY ? 0.f : 1.f;
-    acc = p0.o;
+    l = m == -INFINITY ? 0.f : kJoinWeight;
+    acc = p0.o * kJoinWeight;
     for (int at = part0 + step; at <= cut.more; at += step * AHEAD) {
       Piece p[AHEAD];
 #pragma unroll
@@ -840,7 +854,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void paged_join_kernel(PagedArgs a
       acc *= keep;
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
-        const float f = p[i].lse == -INFINITY ? 0.f : exp2_fast(p[i].lse - ref);
+        const float f = p[i].lse == -INFINITY ? 0.f : exp2_fast(p[i].lse - ref) * kJoinWeight;
         l += f;
         acc += p[i].o * f;
       }
