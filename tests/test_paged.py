@@ -275,6 +275,25 @@ def test_store_kernel_copies_keys_it_cannot_read():
         assert torch.equal(c[1, :, 15], t[1]) and torch.equal(c[0, :, 5], t[2])
 
 
+@pytest.mark.gpu
+def test_store_kernel_of_more_tokens_than_a_grid_holds():
+    """2^24 blocks of two tokens and some: rows 16 bytes apart of one buffer, a few with slots."""
+    T, H, D, S = (1 << 25) + 5, 8, 128, 16
+    base = torch.empty(8 * T + 9 * 1024, dtype=torch.float16, device="cuda").normal_()
+    key, value = (t.as_strided((T, H, D), (8, 1024, 1)) for t in (base, base[1024:]))
+    edge = (1 << 25) - 2
+    chosen = torch.tensor([0, 1, 77, edge - 1, edge, edge + 1, 1 << 25, T - 2, T - 1], device="cuda")
+    slots = torch.full((T,), -1, dtype=torch.int64, device="cuda")
+    slots[chosen] = torch.arange(9, device="cuda") * 5
+    caches = [torch.zeros(3, H, S, D, dtype=torch.float16, device="cuda") for _ in range(2)]
+    paged_cache_store(key, value, *caches, slots, backend="triton")
+    for c, t in zip(caches, (key, value)):
+        rows = c.transpose(1, 2).reshape(3 * S, H, D)
+        assert torch.equal(rows[:45:5], t[chosen])
+        rows[:45:5] = 0
+        assert not rows.any()
+
+
 _SAME = torch.zeros(4, 2, 16, 32).half()
 
 

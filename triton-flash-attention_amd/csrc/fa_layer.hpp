@@ -15,6 +15,9 @@ int capi_fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3
 // FA_OK, or the hipError_t of a launch of the entry point `name` with its message.
 int capi_launch_result(hipError_t e, const char* name);
 
+// Blocks of 256 threads along a grid's first axis: HIP takes fewer than 2^32 threads there.
+constexpr int64_t kMostBlocks = 0xffffffff / 256;
+
 // ---- norm and rotation of queries and keys ----------------------------------------------
 
 // One of the two tensors, [B, H, N, D] with strides in elements (multiples of 8).

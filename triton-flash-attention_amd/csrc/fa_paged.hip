@@ -270,20 +270,26 @@ __global__ __launch_bounds__(256) void paged_store_kernel(StoreArgs a) {
   }
 }
 
-hipError_t launch_paged_store(const StoreArgs& a, hipStream_t stream) {
-  const int pieces = 2 * a.H * a.chunks;
+hipError_t launch_paged_store(const StoreArgs& args, hipStream_t stream) {
+  const int pieces = 2 * args.H * args.chunks;
   const int W = pieces > 128 ? 256 : pieces > 64 ? 128 : pieces > 32 ? 64 : 32;
-  const int64_t tokens = 256 / W * kStoreTokens;
-  const int64_t blocks = (a.T + tokens - 1) / tokens;
-  if (blocks <= 0 || blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
-  const dim3 grid((unsigned)blocks), block(256);
-  switch (W) {
-    case 256: hipLaunchKernelGGL(paged_store_kernel<256>, grid, block, 0, stream, a); break;
-    case 128: hipLaunchKernelGGL(paged_store_kernel<128>, grid, block, 0, stream, a); break;
-    case 64: hipLaunchKernelGGL(paged_store_kernel<64>, grid, block, 0, stream, a); break;
-    default: hipLaunchKernelGGL(paged_store_kernel<32>, grid, block, 0, stream, a); break;
+  const int64_t tokens = 256 / W * kStoreTokens, most = kMostBlocks * tokens;
+  for (int64_t t = 0; t < args.T; t += most) {  // tokens past one grid's blocks: another launch
+    StoreArgs a = args;
+    a.T = std::min(most, args.T - t);
+    a.slots += t;
+    for (int i = 0; i < 2; ++i) a.src[i] += t * a.ss[i][0];
+    const dim3 grid((unsigned)((a.T + tokens - 1) / tokens)), block(256);
+    switch (W) {
+      case 256: hipLaunchKernelGGL(paged_store_kernel<256>, grid, block, 0, stream, a); break;
+      case 128: hipLaunchKernelGGL(paged_store_kernel<128>, grid, block, 0, stream, a); break;
+      case 64: hipLaunchKernelGGL(paged_store_kernel<64>, grid, block, 0, stream, a); break;
+      default: hipLaunchKernelGGL(paged_store_kernel<32>, grid, block, 0, stream, a); break;
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
   }
-  return hipGetLastError();
+  return hipSuccess;
 }
 
 // ---- attention --------------------------------------------------------------------------
