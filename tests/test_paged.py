@@ -765,6 +765,29 @@ def test_attention_kernel_over_a_cache_past_32_bits():
 
 
 @pytest.mark.gpu
+def test_attention_kernel_of_more_heads_than_a_grid_holds():
+    """2^24 heads of 2^21 sequences and some, short tables: all read one page. Against calls of
+    the sequences' parts."""
+    B, H, S, D = (1 << 21) + 9, 8, 16, 8
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    kc, vc = (torch.randn(2, H, S, D, dtype=torch.float16, device="cuda", generator=gen)
+              for _ in range(2))
+    q = torch.empty(B, H, 1, D, dtype=torch.float16, device="cuda").normal_(generator=gen)
+    lens = torch.randint(0, S + 1, (B,), dtype=torch.int32, device="cuda", generator=gen)
+    table = torch.ones(1, 1, dtype=torch.int32, device="cuda").expand(B, 1)
+    o = paged_attention(q, kc, vc, table, lens, backend="triton")
+    for a in range(0, B, 1 << 18):
+        part = slice(a, min(a + (1 << 18), B))
+        want = paged_attention(q[part], kc, vc, table[part], lens[part], backend="triton")
+        assert torch.equal(o[part], want), a
+    want, bound = attention_reference(
+        q[-5:], [[t[1].transpose(0, 1)[:n].double().cpu() for t in (kc, vc)]
+                 for n in lens[-5:].tolist()], D ** -0.5, torch.float16)
+    assert ((o[-5:].double().cpu() - want).abs() <= HALF[torch.float16] * want.abs() * 1.01
+            + bound * 1.01 + 2.0 ** -24).all()
+
+
+@pytest.mark.gpu
 def test_attention_kernel_refuses_what_it_cannot_serve():
     a = _attend_args("cuda")
     a["query"].requires_grad_()

@@ -895,8 +895,9 @@ __global__ __launch_bounds__(64 * kJoinWaves) void paged_join_kernel(PagedArgs a
 // 16.3, 25.8 / 34.3; 2048 keys 21.1 / 11.0, 21.9 / 20.1, 47.7 / 57.3 (kernels alone; the second
 // launch adds about 1.5). A longer row may hold one long sequence among short
 // ones, whose time the split would share out.
+// More triples than a grid has blocks take the split launch, whose work-groups walk over them.
 bool paged_short(int64_t triples, int64_t keys) {
-  return keys <= 1024 || (keys <= 2048 && triples >= 256);
+  return triples <= kMostBlocks && (keys <= 1024 || (keys <= 2048 && triples >= 256));
 }
 
 // Two work-groups a CU, at most one for each four units that the tables could hold; 0: a
@@ -912,7 +913,6 @@ template <int D, class E, int RB>
 hipError_t paged_start(const PagedArgs& a, hipStream_t stream) {
   if (a.grid == 0) {
     const int64_t triples = (int64_t)a.B * a.Hkv * a.blocks;
-    if (triples > 0x7fffffff) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL((paged_fwd_kernel<D, E, RB, true>), dim3((unsigned)triples),
                        dim3(64 * kPagedWaves), 0, stream, a);
     return hipGetLastError();
