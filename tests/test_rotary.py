@@ -365,6 +365,29 @@ def test_kernel_past_32_bits():
 
 
 @pytest.mark.gpu
+def test_kernel_of_more_tokens_than_a_grid_holds():
+    """2^24 blocks of 32 tokens and some: rows 16 bytes apart of one buffer, 77 GB a result."""
+    N, D = (1 << 29) + 77, 72
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 180 << 30:
+        pytest.skip("needs 180 GB of free GPU memory")
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    base = torch.empty(8 * N + D, dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+    q = base.as_strided((1, 1, N, D), (0, 0, 8, 1))
+    cos, sin = tables(64, 64, "cuda")
+    pos = (torch.arange(N, dtype=torch.int32, device="cuda") % 64)
+    oq, ok = qk_norm_rope(q, q, cos, sin, positions=pos, backend="triton")
+    edge = (1 << 29) - 32
+    for n in (0, 12345, edge - 40, edge, 1 << 29, N - 40):
+        part = slice(n, n + 40)
+        ref = reference(q[:, :, part].cpu(), None, cos.cpu(), sin.cpu(), 1e-6, pos[part].cpu(), False)
+        for o in (oq, ok):
+            close("query", o[:, :, part], *ref, torch.bfloat16)
+    del oq, ok, o, base, q, pos
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_kernel_norms_of_small_and_large_rows(dtype):
     """Rows whose squares reach both ends of float32's range, and a row of zeros, as PyTorch."""

@@ -43,13 +43,14 @@ struct RopeArgs {
   int64_t P;             // rows of cos and sin
   int N, D, R;
   int heads;             // heads of a chunk, filled in by the launcher
+  uint32_t first;        // forward: the launch's first token, filled in by the launcher
   int pos64, w32;        // positions are int64; weights are fp32
   float eps;
 };
 
 // Bytes of the backward's partial weight gradients (fp32, [blocks, D]).
 int64_t rope_workspace_bytes(int64_t T, int D, int Hq, int Hkv);
-hipError_t launch_rope(const RopeArgs& a, int dtype, bool norm, bool interleaved,
+hipError_t launch_rope(const RopeArgs& args, int dtype, bool norm, bool interleaved,
                        hipStream_t stream);
 // dw: the two weight gradients, in the weights' type (null to leave one out); part: the
 // workspace (unused without weight gradients).

@@ -218,7 +218,7 @@ __global__ __launch_bounds__(64 * kRopeWaves) void rope_kernel(RopeArgs a) {
   constexpr int TPW = 64 / LPR;  // tokens of a wave
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int p = lane % LPR;
-  const uint32_t t = (blockIdx.x * kRopeWaves + wave) * TPW + lane / LPR;
+  const uint32_t t = a.first + (blockIdx.x * kRopeWaves + wave) * TPW + lane / LPR;
   if (t >= (uint32_t)a.T) return;  // all lanes of a row at once: the sums stay within a row
   const RopeHeads hs = rope_heads(a, blockIdx.y);
   const RopeSide& s = a.side[hs.side];
@@ -401,6 +401,7 @@ __global__ __launch_bounds__(16 * kReduceGroups) void rope_reduce_kernel(RopeRed
 namespace {
 
 int rope_lanes(int D) { return D > 64 ? 8 : D > 32 ? 4 : 2; }
+int rope_tokens(int D) { return kRopeWaves * 64 / rope_lanes(D); }  // of a block
 
 // Blocks that fill the chip. With more each loads its tokens' angles for fewer heads (forward
 // of the case above: 384 to 512 blocks 17.2 us, 1024 19.3, 2048 21.1; its backward, which walks
@@ -418,7 +419,7 @@ struct RopePlan {
 };
 
 RopePlan rope_plan(int64_t T, int D, int Hq, int Hkv, bool bwd) {
-  const int64_t tokens = kRopeWaves * 64 / rope_lanes(D);
+  const int64_t tokens = rope_tokens(D);
   const int64_t tiles = (T + tokens - 1) / tokens;
   RopePlan p;
   // As few heads a chunk as fill the chip (about kRopeBlocks blocks).
@@ -449,7 +450,7 @@ hipError_t rope_start(const RopeArgs& a, const RopePlan& p, bool bwd, bool norm,
 
 hipError_t rope_start(RopeArgs a, const RopePlan& p, bool bwd, int dtype, bool norm, bool inter,
                       hipStream_t stream) {
-  if (p.grid <= 0 || p.grid > 0x7fffffff || p.chunks[0] + p.chunks[1] > 65535)
+  if (p.grid <= 0 || p.grid > kMostBlocks || p.chunks[0] + p.chunks[1] > 65535)
     return hipErrorInvalidConfiguration;
   a.heads = p.heads;
   for (int i = 0; i < 2; ++i) a.side[i].chunks = (int)p.chunks[i];
@@ -470,10 +471,18 @@ int64_t rope_workspace_bytes(int64_t T, int D, int Hq, int Hkv) {
   return rope_plan(T, D, Hq, Hkv, true).parts() * D * 4;
 }
 
-hipError_t launch_rope(const RopeArgs& a, int dtype, bool norm, bool interleaved,
+hipError_t launch_rope(const RopeArgs& args, int dtype, bool norm, bool interleaved,
                        hipStream_t stream) {
-  const RopePlan p = rope_plan(a.T, a.D, a.side[0].H, a.side[1].H, false);
-  return rope_start(a, p, false, dtype, norm, interleaved, stream);
+  RopeArgs a = args;
+  const RopePlan all = rope_plan(a.T, a.D, a.side[0].H, a.side[1].H, false);
+  for (int64_t b = 0; b < all.grid; b += kMostBlocks) {  // past one grid's blocks: another launch
+    RopePlan p = all;
+    p.grid = std::min(kMostBlocks, all.grid - b);
+    a.first = (uint32_t)(b * rope_tokens(a.D));
+    const hipError_t e = rope_start(a, p, false, dtype, norm, interleaved, stream);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_rope_bwd(const RopeArgs& args, int dtype, bool norm, bool interleaved,
