@@ -385,8 +385,9 @@ int64_t fa_fwd_noalloc_max_workspace_bytes(void);
  * float32 [P, R / 2], contiguous; R a multiple of 16 up to D. positions [B, N]: the row of cos
  * and sin of each token, or NULL for 0 .. N - 1; a token whose position is not in [0, P) has
  * NaN for its rows. Weights [D]: of the element type or float32. `strides` holds the batch,
- * head and row stride of q, those of k, and the batch and token stride of positions. Arithmetic
- * in float32, rounded once. */
+ * head and row stride of q, those of k, and the batch and token stride of positions, which are
+ * not negative; positions and weights are aligned to their type. Arithmetic in float32, rounded
+ * once. */
 int fa_qk_norm_rope(const fa_half_t* q, const fa_half_t* k, fa_half_t* q_out, fa_half_t* k_out,
                     const float* cos, const float* sin, const void* positions,
                     const void* q_weight, const void* k_weight, const int64_t* strides,

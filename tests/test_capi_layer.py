@@ -95,6 +95,31 @@ def test_rope_bwd_rejects(lib):
     rejected(lib.fa_qk_norm_rope_bwd_workspace_bytes(0, 4, 2, 8, 64), "FA_ERR_BAD_SHAPE", "positive")
 
 
+@pytest.mark.parametrize(("change", "code", "message"), [
+    (dict(positions=P + 2), "FA_ERR_MISALIGNED", "4-byte"),
+    (dict(positions=P + 4, flags=4), "FA_ERR_MISALIGNED", "8-byte"),
+    (dict(q_weight=P + 1), "FA_ERR_MISALIGNED", "2-byte"),
+    (dict(k_weight=P + 1), "FA_ERR_MISALIGNED", "2-byte"),
+    (dict(k_weight=P + 2, flags=2), "FA_ERR_MISALIGNED", "4-byte"),
+    (dict(strides=(2048, 512, 64, 1024, 512, 64, -8, 1)), "FA_ERR_BAD_STRIDE", "the positions"),
+    (dict(strides=(2048, 512, 64, 1024, 512, 64, 8, -1)), "FA_ERR_BAD_STRIDE", "the positions"),
+])
+def test_rope_rejects_odd_positions_and_weights(lib, change, code, message):
+    for name in ("fa_qk_norm_rope", "fa_qk_norm_rope_bf16"):
+        rejected(rope(lib, name, **change), code, message)
+    change = {{"q_weight": "qw", "k_weight": "kw"}.get(n, n): v for n, v in change.items()}
+    if "strides" in change:
+        change.update(positions=P, strides=(2048, 512, 64, 1024, 512, 64) * 2 + change["strides"][6:])
+    rejected(rope_bwd(lib, **change), code, message)
+
+
+@pytest.mark.parametrize(("change", "message"), [
+    (dict(dqw=P + 1), "2-byte"), (dict(dkw=P + 1), "2-byte"), (dict(dkw=P + 2, flags=2), "4-byte"),
+])
+def test_rope_bwd_rejects_odd_weight_gradients(lib, change, message):
+    rejected(rope_bwd(lib, **change), "FA_ERR_MISALIGNED", message)
+
+
 def plan(lib, **change):
     a = dict(table=P, table_stride=4, lengths=P, new=P, free=P, start=None, slots=P, positions=P,
              starts=P, lengths_out=P, free_out=P, B=2, M=4, S=16, F=8, T=8)

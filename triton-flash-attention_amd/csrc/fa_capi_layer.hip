@@ -79,6 +79,22 @@ int check_rope(const char* name, const RopeSizes& z, const void* q_weight, const
   return FA_OK;
 }
 
+// The positions, the weights and (backward) their gradients, which are read and written value by
+// value.
+int check_rope_values(const char* name, int flags, const void* positions,
+                      const int64_t* position_strides,
+                      std::initializer_list<const void*> weights) {
+  const int value = flags & FA_ROPE_WEIGHT_F32 ? 4 : 2;
+  if (const int rc = check_aligned(name, value, weights)) return rc;
+  if (!positions) return FA_OK;
+  if (const int rc = check_aligned(name, flags & FA_ROPE_POSITIONS_I64 ? 8 : 4, {positions})) return rc;
+  for (int i = 0; i < 2; ++i)
+    if (position_strides[i] < 0)
+      return capi_fail(FA_ERR_BAD_STRIDE, "%s: a negative stride of the positions: %lld", name,
+                       (long long)position_strides[i]);
+  return FA_OK;
+}
+
 fa::RopeArgs rope_args(const RopeSizes& z, const float* cos, const float* sin,
                        const void* positions, const int64_t* position_strides,
                        const void* q_weight, const void* k_weight) {
@@ -115,6 +131,8 @@ int run_rope(const char* name, int dtype, const fa_half_t* q, const fa_half_t* k
   if (const int rc = check_aligned(name, 16, {q, k, q_out, k_out, cos, sin})) return rc;
   if (const int rc = check_strides(name, "the query", strides, 3)) return rc;
   if (const int rc = check_strides(name, "the key", strides + 3, 3)) return rc;
+  if (const int rc = check_rope_values(name, z.flags, positions, strides + 6, {q_weight, k_weight}))
+    return rc;
   fa::RopeArgs a = rope_args(z, cos, sin, positions, strides + 6, q_weight, k_weight);
   a.side[0].x = elems(q);
   a.side[1].x = elems(k);
@@ -144,6 +162,9 @@ int run_rope_bwd(const char* name, int dtype, const fa_half_t* gq, const fa_half
   const char* what[4] = {"the query's gradient", "the key's gradient", "the query", "the key"};
   for (int i = 0; i < (norm ? 4 : 2); ++i)
     if (const int rc = check_strides(name, what[i], strides + 3 * i, 3)) return rc;
+  if (const int rc = check_rope_values(name, z.flags, positions, strides + 12,
+                                       {q_weight, k_weight, dq_weight, dk_weight}))
+    return rc;
   if (norm && (dq_weight || dk_weight)) {
     const int64_t need = fa::rope_workspace_bytes(z.B * z.N, (int)z.D, (int)z.Hq, (int)z.Hkv);
     if (!workspace) return capi_fail(FA_ERR_NULL_POINTER, "%s: null pointer", name);
