@@ -171,6 +171,16 @@ def test_gradients_against_differences():
                                     positions=pos, interleaved=inter), (q, k, wq, wk))
 
 
+def test_eps_of_any_real_type():
+    from fractions import Fraction
+
+    q, w = torch.randn(1, 2, 3, 16), torch.ones(16)
+    args = (q, q, *tables(3, 8))
+    want = qk_norm_rope(*args, query_weight=w, key_weight=w, eps=0.5)[0]
+    assert torch.equal(qk_norm_rope(*args, query_weight=w, key_weight=w, eps=Fraction(1, 2))[0], want)
+    assert not qk_norm_rope(*args, query_weight=w, key_weight=w, eps=10 ** 40)[0].any()
+
+
 def test_positions_outside_the_tables_are_nan():
     q, k = torch.randn(1, 2, 3, 16), torch.randn(1, 1, 3, 16)
     cos, sin = tables(4, 8)
@@ -553,3 +563,20 @@ def test_kernel_refuses_what_it_cannot_serve():
         qk_norm_rope(q[..., :20], q[..., :20], cos[:, :8], sin[:, :8], backend="triton")
     with pytest.raises(RuntimeError, match="derivative in cos"):
         qk_norm_rope(q, q, cos.requires_grad_(), sin, backend="triton")
+
+
+@pytest.mark.gpu
+def test_eps_outside_float32():
+    """PyTorch serves it (the norm's root is infinite); the kernel says why it does not."""
+    q = torch.randn(1, 2, 4, 32, device="cuda").half()
+    w = torch.ones(32, device="cuda")
+    args = (q, q, *tables(4, 16, "cuda"))
+    for eps in (1e39, 10 ** 40):
+        weights = dict(query_weight=w, key_weight=w, eps=eps)
+        got, want = (qk_norm_rope(*args, backend=b, **weights)[0] for b in ("auto", "torch"))
+        assert torch.equal(got, want) and not want.any()
+        with pytest.raises(RuntimeError, match="outside float32"):
+            qk_norm_rope(*args, backend="triton", **weights)
+    weights["eps"] = 3e38
+    got, want = (qk_norm_rope(*args, backend=b, **weights)[0] for b in ("triton", "torch"))
+    assert torch.equal(got, want)

@@ -116,7 +116,7 @@ def _validate(query, key, cos, sin, query_weight, key_weight, eps, positions, in
             raise ValueError("positions must be int32 or int64 on the query's device")
 
 
-def _kernel_reason(query, key, cos, sin) -> str | None:
+def _kernel_reason(query, key, cos, sin, eps) -> str | None:
     if query.device.type != "cuda":
         return _gpu_reason(query)
     if query.dtype not in _SUPPORTED_DTYPES:
@@ -127,6 +127,8 @@ def _kernel_reason(query, key, cos, sin) -> str | None:
         return "the number of rotated values must be a multiple of 16"
     if max(query.shape[1], key.shape[1]) >= 1 << 15 or query.shape[0] * query.shape[2] >= 1 << 31:
         return "too many heads or tokens for one launch"
+    if eps > torch.finfo(torch.float32).max:
+        return f"eps {eps!r} is outside float32"
     if _forward_ad_active() or (torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad)):
         return "the kernel has no derivative in cos and sin and no forward-mode derivative"
     return _gpu_reason(query)
@@ -220,7 +222,9 @@ def qk_norm_rope(
             return out
     _check_backend(backend)
     _validate(query, key, cos, sin, query_weight, key_weight, eps, positions, interleaved)
-    if _falls_back(backend, None if backend == "torch" else _kernel_reason(query, key, cos, sin)):
+    eps = float(eps)
+    if _falls_back(backend, None if backend == "torch" else _kernel_reason(
+            query, key, cos, sin, eps)):
         return tuple(_torch_rope(x, w, cos, sin, eps, positions, interleaved).contiguous()
                      for x, w in ((query, query_weight), (key, key_weight)))
     weights = () if query_weight is None else (query_weight, key_weight)
@@ -228,6 +232,6 @@ def qk_norm_rope(
         if native is not None:
             native.refuse_mixed_capture([query, key, *weights])
         return _QkNormRope.apply(query, key, query_weight, key_weight, cos, sin, positions,
-                                 float(eps), interleaved)
-    return _ops.qk_norm_rope(query, key, cos, sin, query_weight, key_weight, float(eps), positions,
+                                 eps, interleaved)
+    return _ops.qk_norm_rope(query, key, cos, sin, query_weight, key_weight, eps, positions,
                              interleaved)
