@@ -2669,3 +2669,16 @@ def test_head_sizes_up_to_96_leave_the_last_columns_out(n, n_kv, d, causal):
                 _lib.set_tiling(kernel, 128, causal, -1)
         for name, a, b in zip(("o", "dq", "dk", "dv"), got, want):
             assert torch.equal(a, b[..., :d]), (name, fwd)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+def test_launches_of_more_threads_than_a_grid_holds_are_refused(causal):
+    """2^25 heads and some, a work-group each: the grid would wrap around and leave most of the
+    output unwritten."""
+    q = torch.ones((1 << 22) + 1, 8, 1, 32, dtype=torch.float16, device=DEV)
+    with pytest.raises(RuntimeError, match="launch: "):
+        scaled_dot_product_attention(q, q, q, is_causal=causal, backend="triton")
+    part = q[: 1 << 19]
+    out = scaled_dot_product_attention(part, part, part, is_causal=causal, backend="triton")
+    assert torch.equal(out, part)

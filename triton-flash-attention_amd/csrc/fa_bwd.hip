@@ -71,7 +71,7 @@ hipError_t launch_preprocess_e(const half_t* o, const half_t* dO, const Layout& 
                                hipStream_t stream) {
   const int64_t threads = rows * (D / 8);
   const int64_t blocks = (threads + 255) / 256;
-  if (blocks <= 0 || blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+  if (!grid_fits(blocks, 256)) return hipErrorInvalidConfiguration;
   const auto launch = [&](auto* kernel) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, o, dO, dol, delta, rows,
                        (int)H, (int)N, cols);
@@ -144,7 +144,7 @@ hipError_t launch_split_sum(const float* part, half_t* out, int64_t rows, int D,
                             int nsplit, int dtype, hipStream_t stream) {
   const int64_t elems4 = rows * D / 4;
   const int64_t blocks = (elems4 + 255) / 256;
-  if (head_dim_index(D) < 0 || nsplit < 2 || blocks <= 0 || blocks > 0x7fffffff)
+  if (head_dim_index(D) < 0 || nsplit < 2 || !grid_fits(blocks, 256))
     return hipErrorInvalidValue;
   hipLaunchKernelGGL((dtype == kBF16 ? split_sum_kernel<BF16> : split_sum_kernel<F16>),
                      dim3((unsigned)blocks), dim3(256), 0, stream, part, out, elems4, log2_of(D),
@@ -156,7 +156,7 @@ hipError_t launch_split_reduce(const float* part, half_t* dk, half_t* dv, int64_
                                int d, int nsplit, int dtype, hipStream_t stream) {
   const int64_t plane4 = rows * D / 4;
   const int64_t blocks = (2 * plane4 + 255) / 256;
-  if (head_dim_index(D) < 0 || blocks <= 0 || blocks > 0x7fffffff) return hipErrorInvalidValue;
+  if (head_dim_index(D) < 0 || !grid_fits(blocks, 256)) return hipErrorInvalidValue;
   hipLaunchKernelGGL((dtype == kBF16 ? split_reduce_kernel<BF16> : split_reduce_kernel<F16>),
                      dim3((unsigned)blocks), dim3(256), 0, stream, part, dk, dv, plane4,
                      log2_of(D), d, nsplit);
@@ -474,7 +474,7 @@ hipError_t dkdv_launch(const BwdArgs& a, hipStream_t stream) {
   b.num_tiles = (a.Nkv + T::BKV - 1) / T::BKV;
   if (b.nsplit < 1 || (b.nsplit > 1 && b.part == nullptr)) return hipErrorInvalidValue;
   const int64_t blocks = (int64_t)b.num_tiles * a.BHkv * b.nsplit;
-  if (blocks <= 0 || blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+  if (!grid_fits(blocks, T::NT)) return hipErrorInvalidConfiguration;
   hipLaunchKernelGGL((dkdv_kernel<D, CAUSAL, NW, QT, E>), dim3((unsigned)blocks), dim3(T::NT), 0,
                      stream, b);
   return hipGetLastError();
@@ -505,7 +505,7 @@ hipError_t dkdv_pipe_launch(const BwdArgs& a, hipStream_t stream) {
   b.num_tiles = (a.Nkv + T::BKV - 1) / T::BKV;
   if (b.nsplit < 1 || (b.nsplit > 1 && b.part == nullptr)) return hipErrorInvalidValue;
   const int64_t blocks = (int64_t)b.num_tiles * a.BHkv * b.nsplit;
-  if (blocks <= 0 || blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+  if (!grid_fits(blocks, T::NT)) return hipErrorInvalidConfiguration;
   auto kernel = &dkdv_pipe_kernel<D, CAUSAL, NW, E>;
   if constexpr (D == 128)
     if (a.d <= kUsed96) kernel = &dkdv_pipe_used96_kernel<CAUSAL, NW, E>;
@@ -727,7 +727,7 @@ hipError_t dq_launch(const BwdArgs& a, hipStream_t stream) {
       (int64_t)b.nsplit * b.split_keys < visible_kv<CAUSAL>(a))
     return hipErrorInvalidValue;
   const int64_t blocks = (int64_t)b.num_tiles * a.BH * b.nsplit;
-  if (blocks <= 0 || blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+  if (!grid_fits(blocks, T::NT)) return hipErrorInvalidConfiguration;
   hipLaunchKernelGGL((dq_kernel<D, CAUSAL, NW, KT, E>), dim3((unsigned)blocks), dim3(T::NT), 0,
                      stream, b);
   return hipGetLastError();
@@ -762,7 +762,7 @@ hipError_t dq_pipe_launch(const BwdArgs& a, hipStream_t stream) {
       (int64_t)b.nsplit * b.split_keys < visible_kv<CAUSAL>(a))
     return hipErrorInvalidValue;
   const int64_t blocks = (int64_t)b.num_tiles * a.BH * b.nsplit;
-  if (blocks <= 0 || blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+  if (!grid_fits(blocks, T::NT)) return hipErrorInvalidConfiguration;
   const bool tail = !dq_tail_free(b, CAUSAL);
   auto kernel = tail ? &dq_pipe_kernel<D, CAUSAL, NW, E, true> : &dq_pipe_kernel<D, CAUSAL, NW, E, false>;
   if constexpr (D == 128)
@@ -802,7 +802,7 @@ hipError_t dkdv_pipe16_launch(const BwdArgs& a, hipStream_t stream) {
   b.num_tiles = (a.Nkv + T::BKV - 1) / T::BKV;
   if (b.nsplit < 1 || (b.nsplit > 1 && b.part == nullptr)) return hipErrorInvalidValue;
   const int64_t blocks = (int64_t)b.num_tiles * a.BHkv * b.nsplit;
-  if (blocks <= 0 || blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+  if (!grid_fits(blocks, T::NT)) return hipErrorInvalidConfiguration;
   hipLaunchKernelGGL((dkdv_pipe16_kernel<D, CAUSAL, NW, E>), dim3((unsigned)blocks), dim3(T::NT),
                      0, stream, b);
   return hipGetLastError();
@@ -827,7 +827,7 @@ hipError_t dq_pipe16_launch(const BwdArgs& a, hipStream_t stream) {
       (int64_t)b.nsplit * b.split_keys < visible_kv<CAUSAL>(a))
     return hipErrorInvalidValue;
   const int64_t blocks = (int64_t)b.num_tiles * a.BH * b.nsplit;
-  if (blocks <= 0 || blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+  if (!grid_fits(blocks, T::NT)) return hipErrorInvalidConfiguration;
   if (dq_tail_free(b, CAUSAL))
     hipLaunchKernelGGL((dq_pipe16_kernel<D, CAUSAL, NW, E, false>), dim3((unsigned)blocks),
                        dim3(T::NT), 0, stream, b);

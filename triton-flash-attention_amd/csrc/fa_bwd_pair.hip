@@ -70,7 +70,7 @@ hipError_t bwd_pair_launch(const BwdArgs& dkdv, const BwdArgs& dq, hipStream_t s
     return hipErrorInvalidValue;
   const int64_t nk = (int64_t)ad.num_tiles * ad.BHkv * ad.nsplit;
   const int64_t nq = (int64_t)aq.num_tiles * aq.BH;
-  if (nk <= 0 || nq <= 0 || nk + nq > 0x7fffffff) return hipErrorInvalidConfiguration;
+  if (nk <= 0 || nq <= 0 || !grid_fits(nk + nq, TK::NT)) return hipErrorInvalidConfiguration;
   if (dq_tail_free(aq, CAUSAL))
     hipLaunchKernelGGL((bwd_pair_kernel<D, CAUSAL, NW, E, false>), dim3((unsigned)(nk + nq)),
                        dim3(TK::NT), 0, stream, ad, aq, (unsigned)nk, (unsigned)nq);

@@ -1328,7 +1328,7 @@ hipError_t fwd_pipe_jobs_launch(const FwdArgs& a, hipStream_t stream) {
         return hipErrorInvalidValue;
     }
     const int64_t blocks = (int64_t)jb->ngroups * jb->nbin;
-    if (blocks <= 0 || blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+    if (!grid_fits(blocks, T::NT)) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL((fwd_pipe_jobs_kernel<D, NW, E>), dim3((unsigned)blocks), dim3(T::NT), 0,
                        stream, b, *jb);
     return hipGetLastError();
@@ -1346,7 +1346,7 @@ hipError_t fwd_pipe_launch(const FwdArgs& a, hipStream_t stream) {
       (int64_t)b.nsplit * b.split_keys < visible_kv<CAUSAL>(a))
     return hipErrorInvalidValue;
   const int64_t blocks = (int64_t)b.num_tiles * (a.BH / b.pack) * b.nsplit;
-  if (blocks <= 0 || blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+  if (!grid_fits(blocks, T::NT)) return hipErrorInvalidConfiguration;
   auto kernel = &fwd_pipe_kernel<D, CAUSAL, NW, UPS, E, KG>;
   if constexpr (D == 128)
     if (a.d <= kUsed96) kernel = &fwd_pipe_used96_kernel<CAUSAL, NW, E, KG>;
@@ -1381,7 +1381,7 @@ hipError_t fwd_pipe16_launch(const FwdArgs& a, hipStream_t stream) {
       (int64_t)b.nsplit * b.split_keys < visible_kv<CAUSAL>(a))
     return hipErrorInvalidValue;
   const int64_t blocks = (int64_t)b.num_tiles * (a.BH / b.pack) * b.nsplit;
-  if (blocks <= 0 || blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+  if (!grid_fits(blocks, T::NT)) return hipErrorInvalidConfiguration;
   hipLaunchKernelGGL((fwd_pipe16_kernel<D, CAUSAL, E, QB>), dim3((unsigned)blocks), dim3(T::NT),
                      0, stream, b);
   return hipGetLastError();
@@ -1439,7 +1439,7 @@ hipError_t fwd_launch(const FwdArgs& a, hipStream_t stream) {
       b.split_keys % 128 != 0 || (int64_t)b.nsplit * b.split_keys < visible_kv<CAUSAL>(a))
     return hipErrorInvalidValue;
   const int64_t blocks = (int64_t)b.num_tiles * (a.BH / b.pack) * b.nsplit;
-  if (blocks <= 0 || blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+  if (!grid_fits(blocks, T::NT)) return hipErrorInvalidConfiguration;
   hipLaunchKernelGGL((fwd_kernel<D, CAUSAL, NW, BN, E>), dim3((unsigned)blocks), dim3(T::NT), 0,
                      stream, b);
   return hipGetLastError();
@@ -1498,7 +1498,7 @@ template <int D, class E>
 hipError_t fwd_combine_launch(const float* part, half_t* o, float* lse, int64_t rows, int cols,
                               int nsplit, hipStream_t stream) {
   const int64_t blocks = (rows * (D / 4) + 255) / 256;
-  if (nsplit < 2 || nsplit > kMaxFwdSplitKv || blocks <= 0 || blocks > 0x7fffffff)
+  if (nsplit < 2 || nsplit > kMaxFwdSplitKv || !grid_fits(blocks, 256))
     return hipErrorInvalidValue;
   hipLaunchKernelGGL((fwd_combine_kernel<D, E>), dim3((unsigned)blocks), dim3(256), 0, stream,
                      part, o, lse, rows, cols, nsplit);

@@ -259,7 +259,7 @@ hipError_t fwd_decode_launch(const FwdArgs& a, hipStream_t stream) {
       (int64_t)a.nsplit * a.split_keys < a.Nkv)
     return hipErrorInvalidValue;
   const int64_t blocks = (int64_t)(a.BH / a.group) * a.nsplit;
-  if (blocks <= 0 || blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+  if (!grid_fits(blocks, 256)) return hipErrorInvalidConfiguration;
   hipLaunchKernelGGL((fwd_decode_kernel<D, E>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
   return hipGetLastError();
 }

@@ -255,6 +255,12 @@ constexpr int kUsed96 = 96;
 hipError_t launch_fwd_combine(const float* part, half_t* o, float* lse, int64_t rows, int D,
                               int cols, int nsplit, int dtype, hipStream_t stream);
 
+// Whether a grid holds so many blocks of so many threads: HIP has fewer than 2^32 threads along
+// an axis, and larger grids wrap around without an error.
+inline bool grid_fits(int64_t blocks, int threads) {
+  return blocks > 0 && blocks <= 0xffffffff / threads;
+}
+
 inline int log2_of(int x) {
   int s = 0;
   while ((1 << s) < x) ++s;
