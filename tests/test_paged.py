@@ -908,6 +908,52 @@ def test_decoding_loop_captured_and_replayed():
     decode("cuda", "triton", torch.bfloat16, 12, graph=True)
 
 
+def run_module_example(device, dtype):
+    """The step of the module's docstring as it stands, on prompts of several lengths."""
+    from triton_flash_attention import paged
+
+    code = "\n".join(line[4:] for line in paged.__doc__.splitlines() if line.startswith("    "))
+    assert code.startswith("plan = paged_cache_plan(")
+    B, Hq, Hkv, D, n, T, S = 3, 4, 2, 64, 2, 44, 16
+    gen = torch.Generator().manual_seed(12)
+    i32, z = dict(dtype=torch.int32, device=device), dict(dtype=dtype, device=device)
+    new = [5, 2, 33]
+    angle = torch.rand(64, D // 2, generator=gen)
+    q, k, v = (torch.randn(1, h, T, D, generator=gen).to(**z) for h in (Hq, Hkv, Hkv))
+    names = dict(
+        torch=torch, n=n, T=T, table=torch.full((B, 4), -1, **i32), lengths=torch.zeros(B, **i32),
+        new_tokens=torch.tensor(new, **i32), free_pages=torch.arange(7, -1, -1, **i32), q=q, k=k, v=v,
+        cos=angle.cos().to(device), sin=angle.sin().to(device),
+        key_cache=torch.zeros(8, Hkv, S, D, **z), value_cache=torch.zeros(8, Hkv, S, D, **z),
+        paged_cache_plan=paged_cache_plan, paged_cache_store=paged_cache_store,
+        paged_attention=paged_attention, qk_norm_rope=qk_norm_rope)
+    exec(code, names)
+    keys, values, dense, ends = names["k"][0], v[0], [], [5, 7, 40]
+    for end, c in zip(ends, new):
+        dense.append([t[:, end - c:end].transpose(0, 1).double().cpu() for t in (keys, values)])
+    assert names["q"].shape == (B, Hq, n, D)
+    want, bound = attention_reference(names["q"], dense, D ** -0.5, dtype)
+    off = (names["out"].double().cpu() - want).abs()
+    assert (off <= HALF[dtype] * want.abs() * 1.01 + bound * 1.01 + 2.0 ** -24).all()
+    # the rotated queries of the newest tokens
+    place = torch.tensor([c - n + j for c in new for j in range(n)])
+    row = torch.tensor([e - n + j for e in ends for j in range(n)])
+    x = q[0][:, row.to(device)].double().cpu()
+    c, s, h = angle.cos()[place].double(), angle.sin()[place].double(), D // 2
+    x = torch.cat((x[..., :h] * c - x[..., h:] * s, x[..., h:] * c + x[..., :h] * s), -1)
+    got = names["q"].transpose(0, 1).flatten(1, 2).double().cpu()
+    assert torch.allclose(got, x, rtol=0, atol=8 * HALF[dtype])
+
+
+def test_module_example():
+    run_module_example("cpu", torch.float32)
+
+
+@pytest.mark.gpu
+def test_module_example_on_the_kernels():
+    run_module_example("cuda", torch.float16)
+
+
 def test_torch_forms_compile():
     """The PyTorch forms trace as one graph."""
     a = _attend_args(dtype=torch.float32)

@@ -4,13 +4,19 @@ the cache (csrc/fa_paged.hip).
 
 The cache is two tensors [pages, Hkv, page_size, D] that the program allocates once; a page
 holds ``page_size`` tokens (a multiple of 16) of one sequence, and row b of the page table
-[B, M] names the pages of sequence b in order. Lengths, tables and slots stay on the GPU: no
-call here reads them on the host, so a decoding step can be captured into a graph. What they
-hold is checked on the GPU.
+[B, M] names the pages of sequence b in order. Lengths, tables and slots stay on the GPU: the
+kernels' calls read none of them on the host, so a decoding step can be captured into a graph
+(the PyTorch forms of the plan and the store do read them). What they hold is checked on the GPU.
+
+A step of T tokens, q [1, Hq, T, D], k and v [1, Hkv, T, D], of which each sequence's newest n
+are attended (``starts`` says where a sequence's tokens end; when decoding, T = B and n = 1):
 
     plan = paged_cache_plan(table, lengths, new_tokens, free_pages, page_size=16, num_tokens=T)
-    q, k = qk_norm_rope(q, k, cos, sin, positions=plan.positions, ...)
-    paged_cache_store(k, v, key_cache, value_cache, plan.slots)
+    q, k = qk_norm_rope(q, k, cos, sin, positions=plan.positions)
+    paged_cache_store(k[0].transpose(0, 1), v[0].transpose(0, 1), key_cache, value_cache,
+                      plan.slots)
+    newest = plan.starts[1:, None] - n + torch.arange(n, device=q.device)
+    q = q[0][:, newest].transpose(0, 1)  # [B, Hq, n, D]
     out = paged_attention(q, key_cache, value_cache, table, plan.lengths, enable_gqa=True)
 
 No counterpart in the reference, which attends over dense [B, H, N, D] tensors. Names, checks
@@ -328,9 +334,12 @@ def paged_attention(
     rows too.
 
     The gfx950 kernel serves float16 and bfloat16 with head_dim a multiple of 8 up to 128. It
-    reads the cache once for each 32 of the Hq / Hkv * N rows that share a key/value head, and
-    splits the keys over the whole GPU whatever the lengths are. It has no backward: inputs that
-    require gradients run in PyTorch under ``backend="auto"``.
+    reads the cache once for each 32 of the Hq / Hkv * N rows that share a key/value head, so it
+    is made for one token or a few, not for a prompt's. Where a row of the table holds more than
+    1024 keys (2048 where B * Hkv is 256 or more) the keys are split over the whole GPU whatever
+    the lengths are; in a narrower table one work-group takes each of B * Hkv heads, which is
+    faster for short sequences. It has no backward: inputs that require gradients run in PyTorch
+    under ``backend="auto"``.
     """
     native = _binding(backend)
     if native is not None and not _forward_ad_active():
