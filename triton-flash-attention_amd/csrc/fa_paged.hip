@@ -305,8 +305,13 @@ hipError_t launch_paged_store(const StoreArgs& args, hipStream_t stream) {
 // reads no length on the host, so it can be captured). A stretch covers whole triples, which
 // are written as they end, and at most one piece at each end of a triple that it shares with
 // its neighbours: those go to the workspace as a normalised partial O and a base-2 log-sum-exp,
-// and paged_join_kernel joins them. Sequences of any mix of lengths load the chip evenly (32 of
-// 17 to 8192 keys, 554 MB: 101 us, where 32 of 4096, 537 MB, take 96).
+// and paged_join_kernel joins them. Sequences of any mix of lengths load the chip evenly (Hkv8
+// D128, pages that hold head by head: 32 of 17 to 8192 keys, 554 MB, 101 us, where 32 of 4096,
+// 537 MB, take 96).
+//
+// Each row block walks over the keys for itself, also over those that a long chunk's early queries
+// do not see: rows past 32 a head are served, far below the matrix unit's rate (4 sequences of 4000
+// keys, 64 queries, Hq16 Hkv2 D128 bf16: 40 us).
 //
 // Within a stretch a work-group's four waves take every fourth unit, each on its own, and
 // merge through LDS at the end of a piece. K and V of the next unit are on their way to a
@@ -334,6 +339,10 @@ hipError_t launch_paged_store(const StoreArgs& args, hipStream_t stream) {
 // alike have filled it (8 thousand keys a wave, then once in 2^11 times as many); a weight below
 // 2^-110 of the largest is zero. It costs nothing (32 sequences of 17 to 8192 keys 106.3 us with
 // sums that are not held).
+// The probabilities are rounded to the type for the product with V, as in the dense forward; their
+// sums are of the unrounded ones, in float32. Against 64 bits that makes 2.9e-4 (fp16) and 2.2e-3
+// (bf16) rel-L2 of what one rounding of the output alone would leave at 2.1e-4 and 1.6e-3; the
+// alternative is two products, of a high and a low part.
 template <class E>
 constexpr bool kPagedWide = std::is_same_v<E, BF16>;
 template <class E>
@@ -480,8 +489,8 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_fwd_kernel(PagedArg
 
   // The work-group's stretch. Where the rows of neighbouring heads share 128-byte lines, an XCD
   // takes consecutive stretches, so that its L2 holds a line for both (39 sequences of 1710 to
-  // 3420 keys, Hkv8 D32, token by token: 38.9 -> 32.0 us); elsewhere those are better spread
-  // (32 sequences of 4096 keys, Hkv8 D128: 99.3 against 103.7; one head after another the same).
+  // 3420 keys, Hkv8 D32, pages that hold token by token: 38.9 -> 32.0 us); elsewhere those are
+  // better spread (32 sequences of 4096 keys, Hkv8 D128, token by token: 99.3 against 103.7).
   const bool lines_shared = D <= 64 && !SHORT && a.Hkv > 1 && a.ks[1] < 64 && a.grid % 8 == 0;
   const int s_at = lines_shared ? (int)(blockIdx.x % 8) * (a.grid / 8) + (int)(blockIdx.x / 8)
                                 : (int)blockIdx.x;
@@ -889,12 +898,17 @@ __global__ __launch_bounds__(64 * kJoinWaves) void paged_join_kernel(PagedArgs a
 
 // Where a sequence's row of the table holds few keys, a work-group takes a whole triple: no
 // line, no partials and no second launch. It reads at most 61 bytes a ns, what one CU draws
-// from HBM (four units in 1.07 us at D = 128; eight waves are no faster), so the bound is where
-// that takes as long as a second launch saves: D = 128, B x Hkv 8 / 64 / 256 triples, us, this /
-// split and joined: 512 keys 8.9 / 11.3, 9.3 / 13.2, 13.6 / 20.2; 1024 keys 13.5 / 10.4, 13.8 /
-// 16.3, 25.8 / 34.3; 2048 keys 21.1 / 11.0, 21.9 / 20.1, 47.7 / 57.3 (kernels alone; the second
-// launch adds about 1.5). A longer row may hold one long sequence among short
-// ones, whose time the split would share out.
+// from HBM (four units in 1.07 us at D = 128; eight waves are no faster), so the bound is about
+// where that takes as long as a second launch saves: D = 128, B x Hkv 8 / 64 / 256 triples, us,
+// this / split and joined (kernels alone; the second launch adds about 1.5):
+//   512 keys   8.9 / 11.3   9.3 / 13.2  13.6 / 20.2
+//   1024 keys 13.5 / 10.4  13.8 / 16.3  25.8 / 34.3
+//   2048 keys 21.1 / 11.0  21.9 / 20.1  47.7 / 57.3
+// At 1024 keys the bound favours the 64 triples and more of a batch: 8 triples would end 1.6 us
+// earlier split. A longer row may hold one long sequence among short ones, whose time the split
+// shares out. The lengths are on the GPU, so the table's width decides: sequences that are short
+// for their table take the split, 257 keys in a table of 8192 (8, 64, 256 triples) 7.7 + 3.6,
+// 8.4 + 3.5 and 13.7 + 4.0 us, against 6.9, 7.2 and 9.7 in a table of 272.
 // More triples than a grid has blocks take the split launch, whose work-groups walk over them.
 bool paged_short(int64_t triples, int64_t keys) {
   return triples <= kMostBlocks && (keys <= 1024 || (keys <= 2048 && triples >= 256));

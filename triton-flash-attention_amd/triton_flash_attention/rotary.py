@@ -213,6 +213,11 @@ def qk_norm_rope(
     query, key and the weights. The gfx950 kernels serve float16 and bfloat16 with head_dim a
     multiple of 8 up to 128 and R a multiple of 16; a weight's gradient is a float32 sum in a
     fixed order.
+
+    A call that records gradients raises while it is captured into a graph if a result of an
+    earlier call with the same leaf tensors is alive on the default stream, since a backward
+    captured with it would draw that stream into the capture: drop or detach the result first,
+    and capture a forward alone under ``torch.no_grad()``.
     """
     native = _binding(backend)
     if native is not None and not _forward_ad_active():
