@@ -29,7 +29,8 @@ from . import _build
 SUPPORTED_ARCHS = ("gfx950",)
 
 # Kernel instances the default tiling table (kDefault in csrc/fa_capi.hip) and
-# its shape rules select, and the kernels of the operators around the attention call, as demangled name prefixes, for D = 32, 64, 128, both
+# its shape rules select, and the kernels of the operators around the attention
+# call, as demangled name prefixes, for D = 32, 64, 128, both
 # mask modes and both element types (at D = 128 the forward takes the 4-wave
 # pipelined kernel, the 8-wave one where its rounds are whole, the two-key-group
 # one for launches of about one work-group per CU, and the classic one for short
