@@ -222,8 +222,8 @@ int64_t row_blocks(int64_t rows) {
   return (rows + block - 1) / block;
 }
 
-int check_paged(const char* name, int64_t B, int64_t Hq, int64_t Hkv, int64_t N, int64_t D,
-                int64_t M, int64_t S) {
+int check_attention(const char* name, int64_t B, int64_t Hq, int64_t Hkv, int64_t N, int64_t D,
+                    int64_t M, int64_t S) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || N <= 0 || Hq % Hkv)
     return capi_fail(FA_ERR_BAD_SHAPE,
                      "%s: B, Hq, Hkv and N must be positive and Hq divisible by Hkv (got %lld, "
@@ -234,6 +234,13 @@ int check_paged(const char* name, int64_t B, int64_t Hq, int64_t Hkv, int64_t N,
   const int64_t most = (int64_t)1 << 30;
   if (B >= most || Hq >= 1 << 20 || N >= 1 << 20)
     return capi_fail(FA_ERR_TOO_LARGE, "%s: too many sequences, heads or queries", name);
+  return FA_OK;
+}
+
+int check_paged(const char* name, int64_t B, int64_t Hq, int64_t Hkv, int64_t N, int64_t D,
+                int64_t M, int64_t S) {
+  if (const int rc = check_attention(name, B, Hq, Hkv, N, D, M, S)) return rc;
+  const int64_t most = (int64_t)1 << 30;
   // Units of all sequences, heads and row blocks are counted in 32 bits, up to 24 more for each.
   const double units = (double)B * Hkv * row_blocks(Hq / Hkv * N) *
                        ((M * S + fa::kPagedUnit - 1) / fa::kPagedUnit + 24);
@@ -241,6 +248,15 @@ int check_paged(const char* name, int64_t B, int64_t Hq, int64_t Hkv, int64_t N,
     return capi_fail(FA_ERR_TOO_LARGE,
                      "%s: %lld sequences of up to %lld keys are too many for one call", name,
                      (long long)B, (long long)(M * S));
+  return FA_OK;
+}
+
+int check_scale(const char* name, float scale) {
+  const float c = scale * fa::kLog2e;
+  if (!isfinite(scale) || !isfinite(c) || !(c >= FLT_MIN))
+    return capi_fail(FA_ERR_BAD_SCALE,
+                     "%s: scale must be finite and > 0 with scale * log2(e) a normal float32 (got "
+                     "%g)", name, (double)scale);
   return FA_OK;
 }
 
@@ -267,10 +283,7 @@ int run_paged(const char* name, int dtype, const fa_half_t* q, const fa_half_t* 
   if (const int rc = check_cache(name, strides + 3, pages, D)) return rc;
   if (strides[6] < 0) return capi_fail(FA_ERR_BAD_STRIDE, "%s: a negative page table stride", name);
   const float c = scale * fa::kLog2e;
-  if (!isfinite(scale) || !isfinite(c) || !(c >= FLT_MIN))
-    return capi_fail(FA_ERR_BAD_SCALE,
-                     "%s: scale must be finite and > 0 with scale * log2(e) a normal float32 (got "
-                     "%g)", name, (double)scale);
+  if (const int rc = check_scale(name, scale)) return rc;
   const int64_t need = paged_workspace(B, Hq, Hkv, N, D, M, S);
   if (need > 0 && !workspace) return capi_fail(FA_ERR_NULL_POINTER, "%s: null pointer", name);
   if (workspace_bytes < need)
@@ -304,6 +317,82 @@ int run_paged(const char* name, int dtype, const fa_half_t* q, const fa_half_t* 
   return fa::capi_launch_result(
       fa::launch_paged_fwd(a, D <= 32 ? 32 : D <= 64 ? 64 : 128, dtype,
                            static_cast<hipStream_t>(stream)), name);
+}
+
+int check_prefix(const char* name, int64_t B, int64_t G, int64_t Hq, int64_t Hkv, int64_t N,
+                 int64_t D, int64_t M, int64_t S) {
+  if (const int rc = check_attention(name, B, Hq, Hkv, N, D, M, S)) return rc;
+  if (G < 0) return capi_fail(FA_ERR_BAD_SHAPE, "%s: G must not be negative", name);
+  const int64_t R = Hq / Hkv * N;
+  // Rows that read a head and units of the line are counted in 32 bits; two rows or more of the
+  // output are a block of the join, whose grid's threads are too.
+  if (G >= (int64_t)1 << 30 || R >= (int64_t)1 << 25 || B * Hkv * R > 2 * fa::kMostBlocks ||
+      fa::prefix_sizes(B, G, Hkv, R, D, M * S).units >= (double)((int64_t)1 << 30))
+    return capi_fail(FA_ERR_TOO_LARGE,
+                     "%s: %lld sequences of up to %lld keys in %lld groups are too many for one call",
+                     name, (long long)B, (long long)(M * S), (long long)G);
+  return FA_OK;
+}
+
+int run_prefix(const char* name, int dtype, const fa_half_t* q, const fa_half_t* k_cache,
+               const fa_half_t* v_cache, const int32_t* page_table, const int32_t* lengths,
+               const int32_t* group_starts, const int32_t* prefix_lengths, fa_half_t* o,
+               const int64_t* strides, int64_t B, int64_t G, int64_t Hq, int64_t Hkv, int64_t N,
+               int64_t D, int64_t pages, int64_t M, int64_t S, float scale, void* workspace,
+               int64_t workspace_bytes, void* stream) {
+  if (const int rc = check_pointers(name, {q, k_cache, v_cache, page_table, lengths, group_starts, o,
+                                           strides, workspace}))
+    return rc;
+  if (const int rc = check_prefix(name, B, G, Hq, Hkv, N, D, M, S)) return rc;
+  if (G > 0)
+    if (const int rc = check_pointers(name, {prefix_lengths})) return rc;
+  if (const int rc = check_aligned(name, 16, {q, k_cache, v_cache, o, workspace})) return rc;
+  if (const int rc = check_aligned(name, 4, {page_table, lengths, group_starts, prefix_lengths}))
+    return rc;
+  if (const int rc = check_strides(name, "the query", strides, 3)) return rc;
+  if (const int rc = check_cache(name, strides + 3, pages, D)) return rc;
+  if (strides[6] < 0) return capi_fail(FA_ERR_BAD_STRIDE, "%s: a negative page table stride", name);
+  const float c = scale * fa::kLog2e;
+  if (const int rc = check_scale(name, scale)) return rc;
+  const int64_t R = Hq / Hkv * N;
+  const fa::PrefixSizes z = fa::prefix_sizes(B, G, Hkv, R, D, M * S);
+  if (workspace_bytes < z.bytes)
+    return capi_fail(FA_ERR_BAD_SHAPE, "%s: workspace of %lld bytes is smaller than the %lld needed",
+                     name, (long long)workspace_bytes, (long long)z.bytes);
+  fa::PrefixArgs a;
+  a.q = elems(q);
+  a.k = elems(k_cache);
+  a.v = elems(v_cache);
+  a.table = page_table;
+  a.lengths = lengths;
+  a.starts = group_starts;
+  a.prefix = prefix_lengths;
+  a.o = elems(o);
+  a.ws = static_cast<int*>(workspace);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + z.head_bytes);
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = strides[i];
+    a.ks[i] = strides[3 + i];
+  }
+  a.table_stride = strides[6];
+  a.pages = pages;
+  a.pslots = z.pslots;
+  a.c = c;
+  a.B = (int)B;
+  a.G = (int)G;
+  a.Hkv = (int)Hkv;
+  a.group = (int)(Hq / Hkv);
+  a.N = (int)N;
+  a.d = (int)D;
+  a.M = (int)M;
+  a.S = (int)S;
+  a.R = (int)R;
+  a.blocks = z.blocks;
+  a.prows = z.prows;
+  a.srows = z.srows;
+  a.grid = z.grid;
+  return fa::capi_launch_result(fa::launch_prefix_fwd(a, dtype, static_cast<hipStream_t>(stream)),
+                                name);
 }
 
 }  // namespace
@@ -450,6 +539,30 @@ int fa_paged_fwd_bf16(FA_PAGED_PARAMS) {
   return run_paged("fa_paged_fwd_bf16", fa::kBF16, q, k_cache, v_cache, page_table, lengths, o,
                    strides, B, Hq, Hkv, N, D, pages, M, S, scale, workspace, workspace_bytes,
                    stream);
+}
+
+int64_t fa_paged_prefix_fwd_workspace_bytes(int64_t B, int64_t G, int64_t Hq, int64_t Hkv, int64_t N,
+                                            int64_t D, int64_t M, int64_t S) {
+  if (const int rc = check_prefix("fa_paged_prefix_fwd_workspace_bytes", B, G, Hq, Hkv, N, D, M, S))
+    return rc;
+  return fa::prefix_sizes(B, G, Hkv, Hq / Hkv * N, D, M * S).bytes;
+}
+
+#define FA_PREFIX_PARAMS                                                                           \
+  const fa_half_t *q, const fa_half_t *k_cache, const fa_half_t *v_cache,                          \
+      const int32_t *page_table, const int32_t *lengths, const int32_t *group_starts,              \
+      const int32_t *prefix_lengths, fa_half_t *o, const int64_t *strides, int64_t B, int64_t G,    \
+      int64_t Hq, int64_t Hkv, int64_t N, int64_t D, int64_t pages, int64_t M, int64_t S,           \
+      float scale, void *workspace, int64_t workspace_bytes, void *stream
+int fa_paged_prefix_fwd(FA_PREFIX_PARAMS) {
+  return run_prefix("fa_paged_prefix_fwd", fa::kF16, q, k_cache, v_cache, page_table, lengths,
+                    group_starts, prefix_lengths, o, strides, B, G, Hq, Hkv, N, D, pages, M, S,
+                    scale, workspace, workspace_bytes, stream);
+}
+int fa_paged_prefix_fwd_bf16(FA_PREFIX_PARAMS) {
+  return run_prefix("fa_paged_prefix_fwd_bf16", fa::kBF16, q, k_cache, v_cache, page_table, lengths,
+                    group_starts, prefix_lengths, o, strides, B, G, Hq, Hkv, N, D, pages, M, S,
+                    scale, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -18,6 +18,46 @@ int capi_launch_result(hipError_t e, const char* name);
 // Blocks of 256 threads along a grid's first axis: HIP takes fewer than 2^32 threads there.
 constexpr int64_t kMostBlocks = 0xffffffff / 256;
 
+// ---- sums over a block's threads --------------------------------------------------------
+
+// Inclusive sum over the lanes of a wave, up to this one, by DPP: no trip through the LDS unit.
+__device__ __forceinline__ int wave_scan(int x) {
+#define FA_SCAN_STEP(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xF, false)
+  FA_SCAN_STEP(0x111, 0xF);  // row_shr 1, 2, 4, 8: within 16 lanes
+  FA_SCAN_STEP(0x112, 0xF);
+  FA_SCAN_STEP(0x114, 0xF);
+  FA_SCAN_STEP(0x118, 0xF);
+  FA_SCAN_STEP(0x142, 0xA);  // row_bcast 15 to rows 1 and 3, then 31 to rows 2 and 3
+  FA_SCAN_STEP(0x143, 0xC);
+#undef FA_SCAN_STEP
+  return x;
+}
+
+// Sums over the threads before this one of a block of W waves (before[i] of x[i]) and the
+// block's totals (all[i]), behind one barrier.
+template <int W, int K>
+__device__ __forceinline__ void block_scan(const int (&x)[K], int (*sums)[K], int (&before)[K],
+                                           int (&all)[K]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int incl[K];
+#pragma unroll
+  for (int i = 0; i < K; ++i) incl[i] = wave_scan(x[i]);
+  if (lane == 63)
+#pragma unroll
+    for (int i = 0; i < K; ++i) sums[wave][i] = incl[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    before[i] = incl[i] - x[i];
+    all[i] = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (w < wave) before[i] += sums[w][i];
+      all[i] += sums[w][i];
+    }
+  }
+}
+
 // ---- norm and rotation of queries and keys ----------------------------------------------
 
 // One of the two tensors, [B, H, N, D] with strides in elements (multiples of 8).
@@ -115,5 +155,53 @@ inline int paged_rows(int64_t rows) { return rows <= 16 ? 16 : 32; }
 // key/value head and row block.
 int paged_grid(int64_t B, int64_t Hkv, int64_t blocks, int64_t keys);
 hipError_t launch_paged_fwd(const PagedArgs& a, int D, int dtype, hipStream_t stream);
+
+// ---- the same where groups of sequences share a prefix (prefix_fwd_kernel) ----------------
+
+struct PrefixArgs {
+  const half_t* q;       // [B, Hq, N, d], strides qs
+  const half_t* k;       // [pages, Hkv, S, d], strides ks; v the same
+  const half_t* v;
+  const int* table;      // [B, M], rows table_stride apart
+  const int* lengths;    // [B]
+  const int* starts;     // [G + 1], the groups' first sequences and the end of the last
+  const int* prefix;     // [G], keys of the groups' prefixes
+  half_t* o;             // contiguous [B, Hq, N, d]
+  int* ws;               // two ints, then from int 16 on the join's PrefixSeq [B], PrefixGroup [G]
+  float* part;           // partials: pslots slots of prows rows, then those of srows rows
+  int64_t qs[3];         // batch, head and row stride, elements
+  int64_t ks[3];         // page, head and row stride
+  int64_t table_stride;
+  int64_t pages;
+  int64_t pslots;
+  float c;               // scale * log2(e)
+  int B, G, Hkv, group, N, d, M, S;
+  int R;                 // rows of a sequence that read a key/value head: group * N
+  int blocks;            // tiles of them
+  int prows, srows;      // rows of a prefix's and of a sequence's own slot
+  int grid;              // work-groups
+};
+// Where sequence b's own units, and group g's, lie on the line of units.
+struct PrefixSeq {
+  int own_base, own_units, group, member;
+};
+struct PrefixGroup {
+  int base, units, first, tiles;
+};
+constexpr int kPrefixTile = 128;   // query rows of a tile
+constexpr int kPrefixLead = 6;     // empty units in front of a triple on the line
+constexpr int kPrefixStretch = 4;  // least units of a work-group
+inline __host__ __device__ int prefix_tiles(int64_t sequences, int64_t R) {
+  return (int)((sequences * R + kPrefixTile - 1) / kPrefixTile);
+}
+// What a launch takes: its workspace, the slots of prefixes and the work-groups; `units` bounds
+// the line.
+struct PrefixSizes {
+  int64_t bytes, head_bytes, pslots;
+  double units;
+  int blocks, prows, srows, grid;
+};
+PrefixSizes prefix_sizes(int64_t B, int64_t G, int64_t Hkv, int64_t R, int64_t D, int64_t keys);
+hipError_t launch_prefix_fwd(const PrefixArgs& a, int dtype, hipStream_t stream);
 
 }  // namespace fa

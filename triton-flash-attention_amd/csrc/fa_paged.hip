@@ -27,44 +27,6 @@ __device__ __forceinline__ T wave_scan(T x, int lane) {
   return x;
 }
 
-// The same of an int, by DPP: no trip through the LDS unit.
-__device__ __forceinline__ int wave_scan(int x) {
-#define FA_SCAN_STEP(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xF, false)
-  FA_SCAN_STEP(0x111, 0xF);  // row_shr 1, 2, 4, 8: within 16 lanes
-  FA_SCAN_STEP(0x112, 0xF);
-  FA_SCAN_STEP(0x114, 0xF);
-  FA_SCAN_STEP(0x118, 0xF);
-  FA_SCAN_STEP(0x142, 0xA);  // row_bcast 15 to rows 1 and 3, then 31 to rows 2 and 3
-  FA_SCAN_STEP(0x143, 0xC);
-#undef FA_SCAN_STEP
-  return x;
-}
-
-// Sums over the threads before this one of a block of W waves (before[i] of x[i]) and the
-// block's totals (all[i]), behind one barrier.
-template <int W, int K>
-__device__ __forceinline__ void block_scan(const int (&x)[K], int (*sums)[K], int (&before)[K],
-                                           int (&all)[K]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int incl[K];
-#pragma unroll
-  for (int i = 0; i < K; ++i) incl[i] = wave_scan(x[i]);
-  if (lane == 63)
-#pragma unroll
-    for (int i = 0; i < K; ++i) sums[wave][i] = incl[i];
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < K; ++i) {
-    before[i] = incl[i] - x[i];
-    all[i] = 0;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      if (w < wave) before[i] += sums[w][i];
-      all[i] += sums[w][i];
-    }
-  }
-}
-
 // Two sums over the threads before this one of a block of 256, and the block's totals, behind
 // one barrier.
 __device__ __forceinline__ void block_scan2(int64_t x, int64_t y, int64_t (*sums)[4],

@@ -15,6 +15,7 @@ from .paged import PagedPlan as PagedPlan
 from .paged import paged_attention as paged_attention
 from .paged import paged_cache_plan as paged_cache_plan
 from .paged import paged_cache_store as paged_cache_store
+from .prefix import paged_prefix_attention as paged_prefix_attention
 from .rotary import qk_norm_rope as qk_norm_rope
 
 __version__ = "0.2.0+gfx950"

@@ -14,7 +14,7 @@ from pathlib import Path
 
 from ._build import LIB_PATH
 
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 FA_OK = 0
 FA_ERR_NULL_POINTER = -1
@@ -110,7 +110,9 @@ SIGNATURES["fa_paged_plan"] = (_INT, (_P, _I64) + (_P,) * 9 + (_I64,) * 5 + (_P,
 SIGNATURES["fa_paged_store"] = (_INT, (_P,) * 6 + (_I64,) * 5 + (_P,))
 SIGNATURES["fa_paged_fwd_workspace_bytes"] = (_I64, (_I64,) * 7)
 SIGNATURES["fa_paged_fwd"] = (_INT, (_P,) * 7 + (_I64,) * 8 + (_F32, _P, _I64, _P))
-for _name in ("fa_qk_norm_rope", "fa_qk_norm_rope_bwd", "fa_paged_fwd"):
+SIGNATURES["fa_paged_prefix_fwd_workspace_bytes"] = (_I64, (_I64,) * 8)
+SIGNATURES["fa_paged_prefix_fwd"] = (_INT, (_P,) * 9 + (_I64,) * 9 + (_F32, _P, _I64, _P))
+for _name in ("fa_qk_norm_rope", "fa_qk_norm_rope_bwd", "fa_paged_fwd", "fa_paged_prefix_fwd"):
     SIGNATURES[_name + "_bf16"] = SIGNATURES[_name]
 del _name
 

@@ -532,3 +532,31 @@ def paged_fwd(q, key_cache, value_cache, page_table, lengths, scale: float) -> t
             value_cache.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), o.data_ptr(),
             strides, B, Hq, Hkv, N, D, pages, M, S, scale, _ptr(ws), ws_bytes, _stream(q)))
     return o
+
+
+def paged_prefix_fwd(q, key_cache, value_cache, page_table, lengths, group_starts, prefix_lengths,
+                     scale: float) -> torch.Tensor:
+    """O [B,Hq,N,D] of the newest N tokens over the paged cache whose groups share prefixes."""
+    dt = _elem_dtype(q, "q")
+    B, Hq, N, D = q.shape
+    pages, Hkv, S, _ = key_cache.shape
+    M, G = page_table.shape[1], prefix_lengths.shape[0]
+    lib = _lib.load()
+    with _device_guard(q.device):
+        q = _readable(q)
+        lengths, group_starts, prefix_lengths = (
+            t.contiguous() for t in (lengths, group_starts, prefix_lengths))
+        if page_table.stride(1) != 1 and M > 1:
+            page_table = page_table.contiguous()
+        ws_bytes = lib.fa_paged_prefix_fwd_workspace_bytes(B, G, Hq, Hkv, N, D, M, S)
+        if ws_bytes < 0:
+            _lib.check(ws_bytes)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+        o = torch.empty((B, Hq, N, D), dtype=dt, device=q.device)
+        strides = _int64s([*_strides(q), *cache_strides(key_cache), page_table.stride(0)])
+        _lib.check(_launch(
+            "paged_prefix_fwd", _entry(lib, "fa_paged_prefix_fwd", dt), q.data_ptr(),
+            key_cache.data_ptr(), value_cache.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
+            group_starts.data_ptr(), prefix_lengths.data_ptr(), o.data_ptr(), strides, B, G, Hq, Hkv,
+            N, D, pages, M, S, scale, ws.data_ptr(), ws_bytes, _stream(q)))
+    return o

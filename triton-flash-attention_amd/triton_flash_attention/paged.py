@@ -303,6 +303,65 @@ def _torch_paged(query, key_cache, value_cache, page_table, lengths, scale):
     return torch.stack(out).to(query.dtype)
 
 
+def _check_attention(query, key_cache, value_cache, page_table, lengths, scale, enable_gqa) -> None:
+    if not isinstance(enable_gqa, bool):
+        raise TypeError("enable_gqa must be a bool")
+    if scale is not None and (not isinstance(scale, Real) or not math.isfinite(float(scale))):
+        raise ValueError("scale must be a finite real number or None")
+    _check_tensor("query", query, 4, "(batch, heads, sequence, head_dim)")
+    if 0 in query.shape:
+        raise ValueError("query dimensions must all be greater than zero")
+    _check_caches(key_cache, value_cache)
+    B, Hq, N, D = query.shape
+    H, S = key_cache.shape[1:3]
+    _check_table(page_table, S)
+    if query.device != key_cache.device or page_table.device != query.device:
+        raise ValueError("query, the caches, page_table and lengths must be on the same device")
+    if query.dtype != key_cache.dtype:
+        raise ValueError("query and the caches must have the same dtype")
+    if key_cache.shape[3] != D:
+        raise ValueError("query and cache head dimensions must match")
+    if page_table.shape[0] != B:
+        raise ValueError("page_table must have a row for each sequence of query")
+    _check_ints("lengths", lengths, (B,), query.device)
+    if Hq != H and not enable_gqa:
+        raise ValueError(
+            "query has a different number of heads from key/value; pass "
+            "enable_gqa=True to use grouped-query attention")
+    if Hq % H:
+        raise ValueError(
+            "the number of query heads must be divisible by the number of key/value heads")
+
+
+def _attention_reason(backend, query, key_cache, value_cache, softmax_scale, too_many):
+    """(why no kernel serves the attention call or None, how its scale is served)."""
+    if backend == "torch":
+        return None, None
+    served = None
+    if query.device.type != "cuda":
+        reason = _gpu_reason(query)
+    elif (served := _kernel_scale(softmax_scale)) is None:
+        reason = f"scale {softmax_scale!r} overflows the gfx950 kernel's float32 arithmetic"
+    elif _forward_ad_active() or (torch.is_grad_enabled() and any(
+            t.requires_grad for t in (query, key_cache, value_cache))):
+        reason = "the paged kernel has no backward"
+    elif too_many:
+        reason = "too many sequences, heads or keys for one launch"
+    else:
+        reason = _cache_reason(key_cache, value_cache) or _gpu_reason(query)
+    return reason, served
+
+
+def _scaled_query(query, served):
+    """The query and the positive scale that the kernels take for it."""
+    kernel_scale, mode = served
+    if mode == "negate":  # (-q).k |scale|
+        query = -query
+    elif mode == "zero":
+        query = torch.zeros_like(query)
+    return query, kernel_scale
+
+
 def _row_blocks(rows: int) -> int:
     """Passes over a key/value head's keys that its query rows take (fa_layer.hpp paged_rows)."""
     return 1 if rows <= 32 else -(-rows // 32)
@@ -348,53 +407,14 @@ def paged_attention(
         if out is not None:
             return out
     _check_backend(backend)
-    if not isinstance(enable_gqa, bool):
-        raise TypeError("enable_gqa must be a bool")
-    if scale is not None and (not isinstance(scale, Real) or not math.isfinite(float(scale))):
-        raise ValueError("scale must be a finite real number or None")
-    _check_tensor("query", query, 4, "(batch, heads, sequence, head_dim)")
-    if 0 in query.shape:
-        raise ValueError("query dimensions must all be greater than zero")
-    _check_caches(key_cache, value_cache)
+    _check_attention(query, key_cache, value_cache, page_table, lengths, scale, enable_gqa)
     B, Hq, N, D = query.shape
     H, S = key_cache.shape[1:3]
-    _check_table(page_table, S)
-    if query.device != key_cache.device or page_table.device != query.device:
-        raise ValueError("query, the caches, page_table and lengths must be on the same device")
-    if query.dtype != key_cache.dtype:
-        raise ValueError("query and the caches must have the same dtype")
-    if key_cache.shape[3] != D:
-        raise ValueError("query and cache head dimensions must match")
-    if page_table.shape[0] != B:
-        raise ValueError("page_table must have a row for each sequence of query")
-    _check_ints("lengths", lengths, (B,), query.device)
-    if Hq != H and not enable_gqa:
-        raise ValueError(
-            "query has a different number of heads from key/value; pass "
-            "enable_gqa=True to use grouped-query attention")
-    if Hq % H:
-        raise ValueError(
-            "the number of query heads must be divisible by the number of key/value heads")
     softmax_scale = float(scale) if scale is not None else D ** -0.5
-    reason = served = None
-    if backend != "torch":
-        if query.device.type != "cuda":
-            reason = _gpu_reason(query)
-        elif (served := _kernel_scale(softmax_scale)) is None:
-            reason = f"scale {softmax_scale!r} overflows the gfx950 kernel's float32 arithmetic"
-        elif _forward_ad_active() or (torch.is_grad_enabled() and any(
-                t.requires_grad for t in (query, key_cache, value_cache))):
-            reason = "the paged kernel has no backward"
-        elif Hq >= 1 << 20 or N >= 1 << 20 or B * H * _row_blocks(Hq // H * N) * (
-                -(-page_table.shape[1] * S // 32) + 24) >= 1 << 30:
-            reason = "too many sequences, heads or keys for one launch"
-        else:
-            reason = _cache_reason(key_cache, value_cache) or _gpu_reason(query)
+    too_many = Hq >= 1 << 20 or N >= 1 << 20 or B * H * _row_blocks(Hq // H * N) * (
+        -(-page_table.shape[1] * S // 32) + 24) >= 1 << 30
+    reason, served = _attention_reason(backend, query, key_cache, value_cache, softmax_scale, too_many)
     if _falls_back(backend, reason):
         return _torch_paged(query, key_cache, value_cache, page_table, lengths, softmax_scale)
-    kernel_scale, mode = served
-    if mode == "negate":  # (-q).k |scale|
-        query = -query
-    elif mode == "zero":
-        query = torch.zeros_like(query)
+    query, kernel_scale = _scaled_query(query, served)
     return _ops.paged_fwd(query, key_cache, value_cache, page_table, lengths, kernel_scale)
