@@ -499,6 +499,52 @@ int fa_paged_prefix_fwd_bf16(const fa_half_t* q, const fa_half_t* k_cache, const
                              int64_t Hkv, int64_t N, int64_t D, int64_t pages, int64_t M, int64_t S,
                              float scale, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Pages that sequences share. A page may be held by several entries of the page table (and by the
+ * program itself); page_shares[pages] counts its holders beyond the first, so 0 for the pages that
+ * fa_paged_plan hands out. A begun page (the last one of a sequence that does not fill it) is held
+ * by one row. free_pages[F] from place free_start[0] (NULL: 0; taken into [0, F]) on are the free
+ * pages.
+ *
+ * fa_paged_fork: row b of page_table [B, M] becomes the old row parents[b], or is given up where
+ * that is not in [0, B). Its entries for the tokens it holds are written, no others. Whole pages
+ * are shared. A begun page goes on with one child of its row (the row itself if it is one, else the
+ * first); each other child b takes the next free page targets[b], and the first tokens[b] rows of
+ * page sources[b] have to be copied to it (fa_paged_copy); sources and targets are -1 and tokens 0
+ * where nothing is to be copied. Where the free pages run out, targets and entries are -1. Pages
+ * that nobody holds any more return to the list, in ascending order in front of the free ones that
+ * are left; free_start_out is the place of the first. lengths_out [B] are the new rows' lengths.
+ * Negative lengths count as 0; entries that are not in [0, pages) hold nothing and are handed on.
+ * Writes page_table, page_shares and free_pages in place; the other outputs must not overlap the
+ * inputs. The result does not depend on the order of the atomics. */
+int64_t fa_paged_fork_workspace_bytes(int64_t B, int64_t M, int64_t pages);
+int fa_paged_fork(int32_t* page_table, int64_t table_stride, const int32_t* lengths,
+                  const int32_t* parents, int32_t* free_pages, const int32_t* free_start,
+                  int32_t* page_shares, int32_t* lengths_out, int32_t* sources, int32_t* targets,
+                  int32_t* tokens, int32_t* free_start_out, int64_t B, int64_t M, int64_t S,
+                  int64_t F, int64_t pages, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Rows 0 to tokens[i] - 1 (all S where tokens is NULL) of page sources[i] of both caches into page
+ * targets[i], for i < n. Pairs of which a page is not in [0, pages) are left out; the other targets
+ * must differ from each other and from all sources. 16-bit elements of any type. `strides`: page,
+ * head and row stride of the caches. */
+int fa_paged_copy(fa_half_t* k_cache, fa_half_t* v_cache, const int32_t* sources,
+                  const int32_t* targets, const int32_t* tokens, const int64_t* strides, int64_t n,
+                  int64_t H, int64_t D, int64_t pages, int64_t S, void* stream);
+
+/* Held pages, those that free_pages does not name from free_start on, move to the front: of `used`
+ * held ones (used_out [1]) the k-th from place `used` on, sources[k], to the k-th free one in front
+ * of it, targets[k]; both [F] and -1 behind the last move. The pages themselves are copied by
+ * fa_paged_copy. table_out [B, M], shares_out [pages] and free_pages_out [F] are the renumbered
+ * table (every entry that names a moved page), counts (0 for free pages) and list (the entries in
+ * front of free_start as they were, then used, used + 1, ... and -1). The outputs must not overlap
+ * the inputs. */
+int64_t fa_paged_compact_workspace_bytes(int64_t pages);
+int fa_paged_compact(const int32_t* page_table, int64_t table_stride, const int32_t* free_pages,
+                     const int32_t* free_start, const int32_t* page_shares, int32_t* table_out,
+                     int32_t* free_pages_out, int32_t* shares_out, int32_t* sources,
+                     int32_t* targets, int32_t* used_out, int64_t B, int64_t M, int64_t F,
+                     int64_t pages, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Thread-local description of the last failure on the calling thread
  * ("" if none). The pointer stays valid until the next call on the thread. */
 const char* fa_last_error(void);

@@ -1,5 +1,6 @@
 // fa_capi_layer.hip — extern "C" entry points of the operators around the attention call
-// (declared in include/fa_gfx950.h; kernels in fa_rope.hip and fa_paged.hip). As in
+// (declared in include/fa_gfx950.h; kernels in fa_rope.hip, fa_paged.hip, fa_prefix.hip and
+// fa_pages.hip). As in
 // fa_capi.hip every argument is checked before any HIP call.
 #include <float.h>
 #include <math.h>
@@ -319,6 +320,25 @@ int run_paged(const char* name, int dtype, const fa_half_t* q, const fa_half_t* 
                            static_cast<hipStream_t>(stream)), name);
 }
 
+int check_workspace(const char* name, int64_t bytes, int64_t need) {
+  if (bytes < need)
+    return capi_fail(FA_ERR_BAD_SHAPE, "%s: workspace of %lld bytes is smaller than the %lld needed",
+                     name, (long long)bytes, (long long)need);
+  return FA_OK;
+}
+
+// A page table, a list of pages and the cache's pages, as the calls on pages number them.
+int check_rows(const char* name, int64_t B, int64_t M, int64_t F, int64_t pages) {
+  if (B < 0 || F < 0 || M <= 0 || pages <= 0)
+    return capi_fail(FA_ERR_BAD_SHAPE,
+                     "%s: M and pages must be positive, B and F must not be negative", name);
+  const int64_t most = (int64_t)1 << 30;
+  // (a launch has up to 16 blocks of 1024 threads for a row)
+  if (B >= 1 << 17 || M >= most || F >= most || pages >= most || B * M >= (int64_t)1 << 40)
+    return capi_fail(FA_ERR_TOO_LARGE, "%s: too many sequences or pages", name);
+  return FA_OK;
+}
+
 int check_prefix(const char* name, int64_t B, int64_t G, int64_t Hq, int64_t Hkv, int64_t N,
                  int64_t D, int64_t M, int64_t S) {
   if (const int rc = check_attention(name, B, Hq, Hkv, N, D, M, S)) return rc;
@@ -356,9 +376,7 @@ int run_prefix(const char* name, int dtype, const fa_half_t* q, const fa_half_t*
   if (const int rc = check_scale(name, scale)) return rc;
   const int64_t R = Hq / Hkv * N;
   const fa::PrefixSizes z = fa::prefix_sizes(B, G, Hkv, R, D, M * S);
-  if (workspace_bytes < z.bytes)
-    return capi_fail(FA_ERR_BAD_SHAPE, "%s: workspace of %lld bytes is smaller than the %lld needed",
-                     name, (long long)workspace_bytes, (long long)z.bytes);
+  if (const int rc = check_workspace(name, workspace_bytes, z.bytes)) return rc;
   fa::PrefixArgs a;
   a.q = elems(q);
   a.k = elems(k_cache);
@@ -539,6 +557,135 @@ int fa_paged_fwd_bf16(FA_PAGED_PARAMS) {
   return run_paged("fa_paged_fwd_bf16", fa::kBF16, q, k_cache, v_cache, page_table, lengths, o,
                    strides, B, Hq, Hkv, N, D, pages, M, S, scale, workspace, workspace_bytes,
                    stream);
+}
+
+int64_t fa_paged_fork_workspace_bytes(int64_t B, int64_t M, int64_t pages) {
+  if (const int rc = check_rows("fa_paged_fork_workspace_bytes", B, M, 0, pages)) return rc;
+  return fa::fork_workspace_bytes(B, M, pages);
+}
+
+int fa_paged_fork(int32_t* page_table, int64_t table_stride, const int32_t* lengths,
+                  const int32_t* parents, int32_t* free_pages, const int32_t* free_start,
+                  int32_t* page_shares, int32_t* lengths_out, int32_t* sources, int32_t* targets,
+                  int32_t* tokens, int32_t* free_start_out, int64_t B, int64_t M, int64_t S,
+                  int64_t F, int64_t pages, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* name = "fa_paged_fork";
+  if (const int rc = check_pages(name, S, M)) return rc;
+  if (const int rc = check_rows(name, B, M, F, pages)) return rc;
+  if (const int rc = check_pointers(name, {page_shares, free_start_out, workspace})) return rc;
+  if (B > 0)
+    if (const int rc = check_pointers(name, {page_table, lengths, parents, lengths_out, sources,
+                                             targets, tokens}))
+      return rc;
+  if (F > 0)
+    if (const int rc = check_pointers(name, {free_pages})) return rc;
+  if (const int rc = check_aligned(name, 4, {page_table, lengths, parents, free_pages, free_start,
+                                             page_shares, lengths_out, sources, targets, tokens,
+                                             free_start_out, workspace}))
+    return rc;
+  if (table_stride < 0 || (B > 1 && table_stride < M))
+    return capi_fail(FA_ERR_BAD_STRIDE, "%s: rows of the page table must not overlap", name);
+  if (const int rc = check_workspace(name, workspace_bytes, fa::fork_workspace_bytes(B, M, pages)))
+    return rc;
+  fa::ForkArgs a;
+  memset(&a, 0, sizeof(a));
+  a.table = page_table;
+  a.lengths = lengths;
+  a.parents = parents;
+  a.free_pages = free_pages;
+  a.free_start = free_start;
+  a.shares = page_shares;
+  a.lengths_out = lengths_out;
+  a.sources = sources;
+  a.targets = targets;
+  a.tokens = tokens;
+  a.free_out = free_start_out;
+  a.table_stride = table_stride;
+  a.B = (int)B;
+  a.M = (int)M;
+  a.F = (int)F;
+  a.S = (int)S;
+  a.pages = (int)pages;
+  return fa::capi_launch_result(fa::launch_fork(a, workspace, static_cast<hipStream_t>(stream)), name);
+}
+
+int fa_paged_copy(fa_half_t* k_cache, fa_half_t* v_cache, const int32_t* sources,
+                  const int32_t* targets, const int32_t* tokens, const int64_t* strides, int64_t n,
+                  int64_t H, int64_t D, int64_t pages, int64_t S, void* stream) {
+  const char* name = "fa_paged_copy";
+  if (n == 0) return FA_OK;
+  if (const int rc = check_pointers(name, {k_cache, v_cache, sources, targets, strides})) return rc;
+  if (n < 0 || H <= 0) return capi_fail(FA_ERR_BAD_SHAPE, "%s: n and H must be positive", name);
+  if (n >= (int64_t)1 << 31 || H >= 1 << 20)
+    return capi_fail(FA_ERR_TOO_LARGE, "%s: too many pages or heads", name);
+  if (const int rc = check_head_size(name, D)) return rc;
+  if (const int rc = check_pages(name, S, 1)) return rc;
+  if (H * S * (D / 8) >= (int64_t)1 << 30)
+    return capi_fail(FA_ERR_TOO_LARGE, "%s: pages of %lld tokens and %lld heads are too large", name,
+                     (long long)S, (long long)H);
+  if (const int rc = check_aligned(name, 16, {k_cache, v_cache})) return rc;
+  if (const int rc = check_aligned(name, 4, {sources, targets, tokens})) return rc;
+  if (const int rc = check_cache(name, strides, pages, D)) return rc;
+  fa::CopyArgs a;
+  memset(&a, 0, sizeof(a));
+  a.k = elems(k_cache);
+  a.v = elems(v_cache);
+  a.sources = sources;
+  a.targets = targets;
+  a.tokens = tokens;
+  for (int i = 0; i < 3; ++i) a.ks[i] = strides[i];
+  a.n = n;
+  a.pages = pages;
+  a.H = (int)H;
+  a.S = (int)S;
+  a.chunks = (int)(D / 8);
+  return fa::capi_launch_result(fa::launch_page_copy(a, static_cast<hipStream_t>(stream)), name);
+}
+
+int64_t fa_paged_compact_workspace_bytes(int64_t pages) {
+  if (const int rc = check_rows("fa_paged_compact_workspace_bytes", 0, 1, 0, pages)) return rc;
+  return fa::compact_workspace_bytes(pages);
+}
+
+int fa_paged_compact(const int32_t* page_table, int64_t table_stride, const int32_t* free_pages,
+                     const int32_t* free_start, const int32_t* page_shares, int32_t* table_out,
+                     int32_t* free_pages_out, int32_t* shares_out, int32_t* sources,
+                     int32_t* targets, int32_t* used_out, int64_t B, int64_t M, int64_t F,
+                     int64_t pages, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* name = "fa_paged_compact";
+  if (const int rc = check_rows(name, B, M, F, pages)) return rc;
+  if (const int rc = check_pointers(name, {page_shares, shares_out, used_out, workspace})) return rc;
+  if (B > 0)
+    if (const int rc = check_pointers(name, {page_table, table_out})) return rc;
+  if (F > 0)
+    if (const int rc = check_pointers(name, {free_pages, free_pages_out, sources, targets})) return rc;
+  if (const int rc = check_aligned(name, 4, {page_table, free_pages, free_start, page_shares,
+                                             table_out, free_pages_out, shares_out, sources, targets,
+                                             used_out, workspace}))
+    return rc;
+  if (table_stride < 0)
+    return capi_fail(FA_ERR_BAD_STRIDE, "%s: a negative page table stride", name);
+  if (const int rc = check_workspace(name, workspace_bytes, fa::compact_workspace_bytes(pages)))
+    return rc;
+  fa::CompactArgs a;
+  memset(&a, 0, sizeof(a));
+  a.table = page_table;
+  a.free_pages = free_pages;
+  a.free_start = free_start;
+  a.shares = page_shares;
+  a.table_out = table_out;
+  a.free_pages_out = free_pages_out;
+  a.shares_out = shares_out;
+  a.sources = sources;
+  a.targets = targets;
+  a.used = used_out;
+  a.table_stride = table_stride;
+  a.B = (int)B;
+  a.M = (int)M;
+  a.F = (int)F;
+  a.pages = (int)pages;
+  return fa::capi_launch_result(fa::launch_compact(a, workspace, static_cast<hipStream_t>(stream)),
+                                name);
 }
 
 int64_t fa_paged_prefix_fwd_workspace_bytes(int64_t B, int64_t G, int64_t Hq, int64_t Hkv, int64_t N,

@@ -156,7 +156,71 @@ inline int paged_rows(int64_t rows) { return rows <= 16 ? 16 : 32; }
 int paged_grid(int64_t B, int64_t Hkv, int64_t blocks, int64_t keys);
 hipError_t launch_paged_fwd(const PagedArgs& a, int D, int dtype, hipStream_t stream);
 
-// ---- the same where groups of sequences share a prefix (prefix_fwd_kernel) ----------------
+// ---- pages that sequences share -----------------------------------------------------------
+
+// Row b of the page table becomes row parents[b] (fork_count_kernel).
+struct ForkArgs {
+  int* table;             // [B, M], rows table_stride apart
+  const int* lengths;     // [B]
+  const int* parents;     // [B]
+  int* free_pages;        // [F]
+  const int* free_start;  // null for 0
+  int* shares;            // [pages], entries that hold a page beyond the first
+  int* lengths_out;       // [B]; the copies that the rows need, -1 and 0 where they need none:
+  int* sources;
+  int* targets;
+  int* tokens;
+  int* free_out;          // [1]
+  int64_t table_stride;
+  int B, M, F, S, pages;
+  // the workspace, and blocks a row, filled in by the launcher
+  int* keeper;            // [B], the child that goes on in the row's begun page
+  unsigned* bits;         // pages whose count fell below zero
+  int* rows;              // [B, M], the new rows
+  int parts;
+};
+int64_t fork_workspace_bytes(int64_t B, int64_t M, int64_t pages);
+hipError_t launch_fork(const ForkArgs& a, void* workspace, hipStream_t stream);
+
+// Pages of the caches [pages, H, S, D] into others (page_copy_kernel), strides in elements.
+struct CopyArgs {
+  half_t* k;
+  half_t* v;
+  const int* sources;  // [n]
+  const int* targets;
+  const int* tokens;   // rows that are copied, null for all
+  int64_t ks[3];       // page, head and row stride of both
+  int64_t n, pages;
+  int H, S, chunks;    // chunks: 16-byte pieces of a row
+  // filled in by the launcher: blocks a pair, whether rows lie closer than heads, and without gaps
+  unsigned blocks;
+  int rows_inside, together;
+};
+hipError_t launch_page_copy(const CopyArgs& a, hipStream_t stream);
+
+// Held pages move to the front of the cache (compact_rank_kernel).
+struct CompactArgs {
+  const int* table;       // [B, M], rows table_stride apart
+  const int* free_pages;  // [F]
+  const int* free_start;  // null for 0
+  const int* shares;      // [pages]
+  int* table_out;         // contiguous [B, M]
+  int* free_pages_out;    // [F]
+  int* shares_out;        // [pages]
+  int* sources;           // [F], the moves, -1 behind the last
+  int* targets;
+  int* used;              // [1], held pages
+  int64_t table_stride;
+  int B, M, F, pages;
+  // the workspace, filled in by the launcher
+  int* counts;            // [1], moves
+  unsigned* bits;         // free pages
+  int* place;             // [pages], a moved page's place among the moves
+};
+int64_t compact_workspace_bytes(int64_t pages);
+hipError_t launch_compact(const CompactArgs& a, void* workspace, hipStream_t stream);
+
+// ---- attention where groups of sequences share a prefix (prefix_fwd_kernel) ----------------
 
 struct PrefixArgs {
   const half_t* q;       // [B, Hq, N, d], strides qs

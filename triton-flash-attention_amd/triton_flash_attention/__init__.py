@@ -2,7 +2,8 @@
 
 The reference package's import surface (triton_flash_attention/__init__.py:3-15), and the
 operators that a decoder runs around the attention call: the norm and rotation of queries and
-keys (:mod:`.rotary`) and the paged key/value cache of a serving program (:mod:`.paged`).
+keys (:mod:`.rotary`), the paged key/value cache of a serving program (:mod:`.paged`), the pages
+that its sequences share (:mod:`.pages`) and the attention over shared prefixes (:mod:`.prefix`).
 """
 
 from .attention import (
@@ -15,6 +16,11 @@ from .paged import PagedPlan as PagedPlan
 from .paged import paged_attention as paged_attention
 from .paged import paged_cache_plan as paged_cache_plan
 from .paged import paged_cache_store as paged_cache_store
+from .pages import PagedCompaction as PagedCompaction
+from .pages import PagedFork as PagedFork
+from .pages import paged_cache_compact as paged_cache_compact
+from .pages import paged_cache_copy as paged_cache_copy
+from .pages import paged_cache_fork as paged_cache_fork
 from .prefix import paged_prefix_attention as paged_prefix_attention
 from .rotary import qk_norm_rope as qk_norm_rope
 

@@ -24,7 +24,7 @@ LIB_NAME = "libfa_gfx950.so"
 LIB_PATH = PACKAGE_DIR / LIB_NAME
 
 SOURCES = ("fa_fwd.hip", "fa_fwd_decode.hip", "fa_bwd.hip", "fa_bwd_pair.hip", "fa_rope.hip",
-           "fa_paged.hip", "fa_prefix.hip", "fa_capi.hip", "fa_capi_layer.hip")
+           "fa_paged.hip", "fa_prefix.hip", "fa_pages.hip", "fa_capi.hip", "fa_capi_layer.hip")
 HEADERS = ("fa_common.hpp", "fa_kernels.hpp", "fa_bwd_pipe.hpp", "fa_layer.hpp")
 
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 in generated code.

@@ -112,6 +112,11 @@ SIGNATURES["fa_paged_fwd_workspace_bytes"] = (_I64, (_I64,) * 7)
 SIGNATURES["fa_paged_fwd"] = (_INT, (_P,) * 7 + (_I64,) * 8 + (_F32, _P, _I64, _P))
 SIGNATURES["fa_paged_prefix_fwd_workspace_bytes"] = (_I64, (_I64,) * 8)
 SIGNATURES["fa_paged_prefix_fwd"] = (_INT, (_P,) * 9 + (_I64,) * 9 + (_F32, _P, _I64, _P))
+SIGNATURES["fa_paged_fork_workspace_bytes"] = (_I64, (_I64,) * 3)
+SIGNATURES["fa_paged_fork"] = (_INT, (_P, _I64) + (_P,) * 10 + (_I64,) * 5 + (_P, _I64, _P))
+SIGNATURES["fa_paged_copy"] = (_INT, (_P,) * 6 + (_I64,) * 5 + (_P,))
+SIGNATURES["fa_paged_compact_workspace_bytes"] = (_I64, (_I64,))
+SIGNATURES["fa_paged_compact"] = (_INT, (_P, _I64) + (_P,) * 9 + (_I64,) * 4 + (_P, _I64, _P))
 for _name in ("fa_qk_norm_rope", "fa_qk_norm_rope_bwd", "fa_paged_fwd", "fa_paged_prefix_fwd"):
     SIGNATURES[_name + "_bf16"] = SIGNATURES[_name]
 del _name

@@ -560,3 +560,61 @@ def paged_prefix_fwd(q, key_cache, value_cache, page_table, lengths, group_start
             group_starts.data_ptr(), prefix_lengths.data_ptr(), o.data_ptr(), strides, B, G, Hq, Hkv,
             N, D, pages, M, S, scale, ws.data_ptr(), ws_bytes, _stream(q)))
     return o
+
+
+def _workspace(n: int, device) -> torch.Tensor:
+    if n < 0:
+        _lib.check(n)
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def paged_fork(page_table, lengths, parents, free_pages, page_shares, free_start, page_size: int):
+    """(lengths, sources, targets, tokens, free_start) of the new rows; writes page_table,
+    free_pages and page_shares."""
+    B, M = page_table.shape
+    pages, dev = page_shares.shape[0], page_table.device
+    lib = _lib.load()
+    with _device_guard(dev):
+        lengths, parents = lengths.contiguous(), parents.contiguous()
+        out = [torch.empty(n, dtype=torch.int32, device=dev) for n in (B, B, B, B, 1)]
+        ws = _workspace(lib.fa_paged_fork_workspace_bytes(B, M, pages), dev)
+        _lib.check(_launch(
+            "paged_fork", lib.fa_paged_fork, page_table.data_ptr(), page_table.stride(0),
+            lengths.data_ptr(), parents.data_ptr(), free_pages.data_ptr(), _ptr(free_start),
+            page_shares.data_ptr(), *(t.data_ptr() for t in out), B, M, page_size,
+            free_pages.shape[0], pages, ws.data_ptr(), ws.shape[0], _stream(page_table)))
+    _written(page_table, free_pages, page_shares)
+    return out
+
+
+def paged_copy(key_cache, value_cache, sources, targets, tokens) -> None:
+    """Pages ``sources`` of the caches [pages,H,S,D] into pages ``targets``."""
+    pages, H, S, D = key_cache.shape
+    lib = _lib.load()
+    with _device_guard(key_cache.device):
+        sources, targets = sources.contiguous(), targets.contiguous()
+        tokens = None if tokens is None else tokens.contiguous()
+        _lib.check(_launch(
+            "paged_copy", lib.fa_paged_copy, key_cache.data_ptr(), value_cache.data_ptr(),
+            sources.data_ptr(), targets.data_ptr(), _ptr(tokens), _int64s(cache_strides(key_cache)),
+            sources.shape[0], H, D, pages, S, _stream(key_cache)))
+    _written(key_cache, value_cache)
+
+
+def paged_compact(page_table, free_pages, page_shares, free_start):
+    """(page_table, free_pages, page_shares, sources, targets, used) of the compacted cache."""
+    B, M = page_table.shape
+    F, pages, dev = free_pages.shape[0], page_shares.shape[0], page_table.device
+    lib = _lib.load()
+    with _device_guard(dev):
+        if page_table.stride(1) != 1 and M > 1:
+            page_table = page_table.contiguous()
+        free_pages, page_shares = free_pages.contiguous(), page_shares.contiguous()
+        out = [torch.empty(n, dtype=torch.int32, device=dev) for n in ((B, M), F, pages, F, F, 1)]
+        ws = _workspace(lib.fa_paged_compact_workspace_bytes(pages), dev)
+        _lib.check(_launch(
+            "paged_compact", lib.fa_paged_compact, page_table.data_ptr(), page_table.stride(0),
+            free_pages.data_ptr(), _ptr(free_start), page_shares.data_ptr(),
+            *(t.data_ptr() for t in out), B, M, F, pages, ws.data_ptr(), ws.shape[0],
+            _stream(page_table)))
+    return out
