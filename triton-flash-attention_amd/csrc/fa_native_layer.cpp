@@ -1,12 +1,12 @@
 // fa_native_layer.cpp — C++ binding of the operators around the attention call (fa_rope.hip,
-// fa_paged.hip), part of the _fa_native module (host code only).
+// fa_paged.hip, fa_prefix.hip, fa_pages.hip), part of the _fa_native module (host code only).
 //
 // Their kernels take 3 to 30 us in a decoding step or a layer's training step; the Python op
 // layer's checks, allocations and ctypes call take 13 to 20 us beside them, and a Python
 // autograd Function another 100 us for its backward. Each function here serves a plain call:
 // it makes every check of the public function that the call has to pass, well inside its
 // bounds, and launches; for any other call it returns None, and Python then checks it one
-// rule at a time to word its error or choose its path (rotary.py, paged.py).
+// rule at a time to word its error or choose its path (rotary.py, paged.py, prefix.py, pages.py).
 #include <torch/extension.h>
 
 #include <ATen/core/grad_mode.h>
@@ -44,6 +44,16 @@ using Store = int (*)(CPtr, CPtr, Ptr, Ptr, CPtr, const I64*, I64, I64, I64, I64
 using PagedBytes = I64 (*)(I64, I64, I64, I64, I64, I64, I64);
 using Paged = int (*)(CPtr, CPtr, CPtr, CPtr, CPtr, Ptr, const I64*, I64, I64, I64, I64, I64, I64,
                       I64, I64, float, Ptr, I64, Ptr);
+using PrefixBytes = I64 (*)(I64, I64, I64, I64, I64, I64, I64, I64);
+using Prefix = int (*)(CPtr, CPtr, CPtr, CPtr, CPtr, CPtr, CPtr, Ptr, const I64*, I64, I64, I64, I64,
+                       I64, I64, I64, I64, I64, float, Ptr, I64, Ptr);
+using ForkBytes = I64 (*)(I64, I64, I64);
+using Fork = int (*)(Ptr, I64, CPtr, CPtr, Ptr, CPtr, Ptr, Ptr, Ptr, Ptr, Ptr, Ptr, I64, I64, I64, I64,
+                     I64, Ptr, I64, Ptr);
+using Copy = int (*)(Ptr, Ptr, CPtr, CPtr, CPtr, const I64*, I64, I64, I64, I64, I64, Ptr);
+using CompactBytes = I64 (*)(I64);
+using Compact = int (*)(CPtr, I64, CPtr, CPtr, CPtr, Ptr, Ptr, Ptr, Ptr, Ptr, Ptr, I64, I64, I64, I64,
+                        Ptr, I64, Ptr);
 using LastError = const char* (*)();
 
 // Entry points; index 0 = fp16, 1 = bf16.
@@ -55,6 +65,13 @@ struct Entries {
   Store store;
   Paged paged[2];
   PagedBytes paged_bytes;
+  Prefix prefix[2];
+  PrefixBytes prefix_bytes;
+  Fork fork;
+  ForkBytes fork_bytes;
+  Copy copy;
+  Compact compact;
+  CompactBytes compact_bytes;
   LastError last_error;
 };
 Entries g = {};
@@ -451,51 +468,207 @@ bool native_store(py::handle key, py::handle value, py::handle key_cache, py::ha
   return true;
 }
 
+// An attention call over the cache whose arguments pass every check; q == null for any doubt.
+struct PagedCall {
+  const at::Tensor *q = nullptr, *kc, *vc, *t, *l;
+  I64 B, Hq, H, N, D, pages, M, S;
+  float scale;
+
+  PagedCall(py::handle query, py::handle key_cache, py::handle value_cache, py::handle table,
+            py::handle lengths, py::handle sc, py::handle enable_gqa) {
+    const at::Tensor* x = plain(query);
+    kc = plain(key_cache), vc = plain(value_cache), t = plain(table), l = plain(lengths);
+    if (!x || !kc || !vc || !t || !l || !PyBool_Check(enable_gqa.ptr()) || !plain_caches(*kc, *vc) ||
+        !plain_table(*t, kc->size(2)) || !served(x->device()))
+      return;
+    const at::Device device = x->device();
+    constexpr I64 kMany = I64{1} << 16;
+    if (x->scalar_type() != kc->scalar_type() || kc->device() != device || t->device() != device ||
+        x->dim() != 4 || !all_positive(*x, kMany) || x->size(3) != kc->size(3) ||
+        t->size(0) != x->size(0) || !is_int32(*l, device, 1) || l->size(0) != x->size(0))
+      return;
+    B = x->size(0), Hq = x->size(1), N = x->size(2), D = x->size(3);
+    pages = kc->size(0), H = kc->size(1), S = kc->size(2), M = t->size(1);
+    if (Hq % H || (Hq != H && enable_gqa.ptr() != Py_True)) return;
+    if (at::GradMode::is_enabled() && (wants_grad(*x) || wants_grad(*kc) || wants_grad(*vc))) return;
+    double s = 0.0;
+    if (sc.is_none()) s = std::pow(static_cast<double>(D), -0.5);
+    else if (PyFloat_CheckExact(sc.ptr())) s = PyFloat_AS_DOUBLE(sc.ptr());
+    if (!(s >= 1e-30 && s <= 1e30)) return;
+    scale = (float)s;
+    q = x;
+  }
+  void strides(const at::Tensor& query, I64* st) const {
+    row_strides(query, st);
+    cache_strides(*kc, st + 3);
+    st[6] = t->stride(0);
+  }
+  at::Tensor output(const at::Tensor& query) const {
+    return at::empty({B, Hq, N, D}, query.options().requires_grad(false));
+  }
+};
+
 py::object native_paged(py::handle query, py::handle key_cache, py::handle value_cache,
                         py::handle table, py::handle lengths, py::handle scale,
                         py::handle enable_gqa) {
   if (!g_ready) return py::none();
-  const at::Tensor *q = plain(query), *kc = plain(key_cache), *vc = plain(value_cache),
-                   *t = plain(table), *l = plain(lengths);
-  if (!q || !kc || !vc || !t || !l || !PyBool_Check(enable_gqa.ptr()) || !plain_caches(*kc, *vc) ||
-      !plain_table(*t, kc->size(2)) || !served(q->device()))
+  const PagedCall c(query, key_cache, value_cache, table, lengths, scale, enable_gqa);
+  if (!c.q) return py::none();
+  const I64 n = g.paged_bytes(c.B, c.Hq, c.H, c.N, c.D, c.M, c.S);
+  if (n < 0) return py::none();
+  c10::DeviceGuard guard(c.q->device());
+  at::AutoDispatchBelowAutograd below;
+  const at::Tensor qr = operand(*c.q), lc = c.l->contiguous();
+  const at::Tensor ws = bytes(n, qr);
+  at::Tensor o = c.output(qr);
+  I64 st[7];
+  c.strides(qr, st);
+  check(g.paged[elem_index(qr)](qr.data_ptr(), c.kc->data_ptr(), c.vc->data_ptr(), c.t->data_ptr(),
+                                lc.data_ptr(), o.data_ptr(), st, c.B, c.Hq, c.H, c.N, c.D, c.pages,
+                                c.M, c.S, c.scale, pointer(ws), n, stream_of(qr)));
+  return py::cast(o);
+}
+
+py::object native_prefix(py::handle query, py::handle key_cache, py::handle value_cache,
+                         py::handle table, py::handle lengths, py::handle group_starts,
+                         py::handle prefix_lengths, py::handle scale, py::handle enable_gqa) {
+  if (!g_ready) return py::none();
+  const PagedCall c(query, key_cache, value_cache, table, lengths, scale, enable_gqa);
+  const at::Tensor *s = plain(group_starts), *p = plain(prefix_lengths);
+  if (!c.q || !s || !p) return py::none();
+  const at::Device device = c.q->device();
+  if (!is_int32(*s, device, 1) || !is_int32(*p, device, 1) || s->size(0) != p->size(0) + 1)
     return py::none();
-  const at::Device device = q->device();
-  constexpr I64 kMany = I64{1} << 16;
-  if (q->scalar_type() != kc->scalar_type() || kc->device() != device || t->device() != device ||
-      q->dim() != 4 || !all_positive(*q, kMany) || q->size(3) != kc->size(3) ||
-      t->size(0) != q->size(0) || !is_int32(*l, device, 1) || l->size(0) != q->size(0))
-    return py::none();
-  const I64 B = q->size(0), Hq = q->size(1), N = q->size(2), D = q->size(3);
-  const I64 pages = kc->size(0), H = kc->size(1), S = kc->size(2), M = t->size(1);
-  if (Hq % H || (Hq != H && enable_gqa.ptr() != Py_True)) return py::none();
-  if (at::GradMode::is_enabled() && (wants_grad(*q) || wants_grad(*kc) || wants_grad(*vc)))
-    return py::none();
-  double sc = 0.0;
-  if (scale.is_none()) sc = std::pow(static_cast<double>(D), -0.5);
-  else if (PyFloat_CheckExact(scale.ptr())) sc = PyFloat_AS_DOUBLE(scale.ptr());
-  if (!(sc >= 1e-30 && sc <= 1e30)) return py::none();
-  const I64 n = g.paged_bytes(B, Hq, H, N, D, M, S);
+  const I64 G = p->size(0), n = g.prefix_bytes(c.B, G, c.Hq, c.H, c.N, c.D, c.M, c.S);
   if (n < 0) return py::none();
   c10::DeviceGuard guard(device);
   at::AutoDispatchBelowAutograd below;
-  const at::Tensor qr = operand(*q), lc = l->contiguous();
+  const at::Tensor qr = operand(*c.q), lc = c.l->contiguous(), sc = s->contiguous(),
+                   pc = p->contiguous();
   const at::Tensor ws = bytes(n, qr);
-  at::Tensor o = at::empty({B, Hq, N, D}, qr.options().requires_grad(false));
+  at::Tensor o = c.output(qr);
   I64 st[7];
-  row_strides(qr, st);
-  cache_strides(*kc, st + 3);
-  st[6] = t->stride(0);
-  check(g.paged[elem_index(*q)](qr.data_ptr(), kc->data_ptr(), vc->data_ptr(), t->data_ptr(),
-                                lc.data_ptr(), o.data_ptr(), st, B, Hq, H, N, D, pages, M, S,
-                                (float)sc, pointer(ws), n, stream_of(*q)));
+  c.strides(qr, st);
+  check(g.prefix[elem_index(qr)](qr.data_ptr(), c.kc->data_ptr(), c.vc->data_ptr(), c.t->data_ptr(),
+                                 lc.data_ptr(), sc.data_ptr(), pc.data_ptr(), o.data_ptr(), st, c.B, G,
+                                 c.Hq, c.H, c.N, c.D, c.pages, c.M, c.S, c.scale, pointer(ws), n,
+                                 stream_of(qr)));
   return py::cast(o);
+}
+
+// ---- pages that sequences share ---------------------------------------------------------
+
+constexpr I64 kMostPages = I64{1} << 30;
+
+// A list of int32 on the device, and the place in it that may be left out; false for any doubt.
+bool plain_list(const at::Tensor* t, const at::Device& device, I64 least) {
+  return t && is_int32(*t, device, 1) && t->size(0) >= least && t->size(0) < kMostPages;
+}
+bool plain_start(py::handle h, const at::Device& device, at::Tensor* start) {
+  if (h.is_none()) return true;
+  const at::Tensor* p = plain(h);
+  if (!p || p->scalar_type() != at::kInt || p->device() != device || p->numel() != 1) return false;
+  *start = *p;
+  return true;
+}
+
+py::object native_fork(py::handle table, py::handle lengths, py::handle parents,
+                       py::handle free_pages, py::handle page_shares, py::handle page_size,
+                       py::handle free_start) {
+  if (!g_ready) return py::none();
+  const at::Tensor *t = plain(table), *l = plain(lengths), *p = plain(parents),
+                   *f = plain(free_pages), *s = plain(page_shares);
+  const I64 S = whole(page_size);
+  if (!t || !l || !p || !plain_table(*t, S) || !served(t->device())) return py::none();
+  const at::Device device = t->device();
+  const I64 B = t->size(0), M = t->size(1);
+  at::Tensor start;
+  if (!is_int32(*l, device, 1) || !is_int32(*p, device, 1) || l->size(0) != B || p->size(0) != B ||
+      B >= 1 << 17 || !plain_list(f, device, 0) || !plain_list(s, device, 1) || !f->is_contiguous() ||
+      !s->is_contiguous() || (B > 1 && t->stride(0) < M) || !plain_start(free_start, device, &start))
+    return py::none();
+  c10::DeviceGuard guard(device);
+  at::AutoDispatchBelowAutograd below;
+  const at::Tensor lc = l->contiguous(), pc = p->contiguous();
+  // One allocation for the five results.
+  const at::Tensor small = at::empty({4 * B + 1}, t->options());
+  at::Tensor out[5];
+  for (int i = 0; i < 5; ++i) out[i] = piece_of(small, i * B, i < 4 ? B : 1);
+  const I64 n = g.fork_bytes(B, M, s->size(0));
+  const at::Tensor ws = bytes(n, *t);
+  check(g.fork(t->data_ptr(), t->stride(0), lc.data_ptr(), pc.data_ptr(), f->data_ptr(),
+               pointer(start), s->data_ptr(), out[0].data_ptr(), out[1].data_ptr(),
+               out[2].data_ptr(), out[3].data_ptr(), out[4].data_ptr(), B, M, S, f->size(0),
+               s->size(0), pointer(ws), n, stream_of(*t)));
+  written(*t);
+  written(*f);
+  written(*s);
+  return py::make_tuple(out[0], out[1], out[2], out[3], out[4]);
+}
+
+// True where the copy was made.
+bool native_copy(py::handle key_cache, py::handle value_cache, py::handle sources,
+                 py::handle targets, py::handle tokens) {
+  if (!g_ready) return false;
+  const at::Tensor *kc = plain(key_cache), *vc = plain(value_cache), *a = plain(sources),
+                   *b = plain(targets);
+  if (!kc || !vc || !plain_caches(*kc, *vc) || !served(kc->device())) return false;
+  const at::Device device = kc->device();
+  if (kc->data_ptr() == vc->data_ptr() || !plain_list(a, device, 1) || !plain_list(b, device, 1) ||
+      b->size(0) != a->size(0) || kc->size(1) >= 1 << 20 ||
+      kc->size(1) * kc->size(2) >= (I64{1} << 33) / kc->size(3))
+    return false;
+  const at::Tensor* k = nullptr;
+  if (!tokens.is_none()) {
+    k = plain(tokens);
+    if (!plain_list(k, device, 1) || k->size(0) != a->size(0)) return false;
+  }
+  if (at::GradMode::is_enabled() && (wants_grad(*kc) || wants_grad(*vc))) return false;
+  c10::DeviceGuard guard(device);
+  at::AutoDispatchBelowAutograd below;
+  const at::Tensor ac = a->contiguous(), bc = b->contiguous();
+  const at::Tensor tc = k ? k->contiguous() : at::Tensor();
+  I64 st[3];
+  cache_strides(*kc, st);
+  check(g.copy(kc->data_ptr(), vc->data_ptr(), ac.data_ptr(), bc.data_ptr(), pointer(tc), st,
+               ac.size(0), kc->size(1), kc->size(3), kc->size(0), kc->size(2), stream_of(*kc)));
+  written(*kc);
+  written(*vc);
+  return true;
+}
+
+py::object native_compact(py::handle table, py::handle free_pages, py::handle page_shares,
+                          py::handle free_start) {
+  if (!g_ready) return py::none();
+  const at::Tensor *t = plain(table), *f = plain(free_pages), *s = plain(page_shares);
+  if (!t || !plain_table(*t, 16) || !served(t->device())) return py::none();
+  const at::Device device = t->device();
+  const I64 B = t->size(0), M = t->size(1);
+  at::Tensor start;
+  if (B >= 1 << 17 || !plain_list(f, device, 0) || !plain_list(s, device, 1) ||
+      !plain_start(free_start, device, &start))
+    return py::none();
+  c10::DeviceGuard guard(device);
+  at::AutoDispatchBelowAutograd below;
+  const at::Tensor fc = f->contiguous(), sc = s->contiguous();
+  const I64 F = fc.size(0), P = sc.size(0);
+  const at::Tensor small = at::empty({3 * F + P + 1}, t->options());
+  at::Tensor table_out = at::empty({B, M}, t->options()), free_out = piece_of(small, 0, F);
+  at::Tensor sources = piece_of(small, F, F), targets = piece_of(small, 2 * F, F);
+  at::Tensor shares_out = piece_of(small, 3 * F, P), used = piece_of(small, 3 * F + P, 1);
+  const I64 n = g.compact_bytes(P);
+  const at::Tensor ws = bytes(n, *t);
+  check(g.compact(t->data_ptr(), t->stride(0), fc.data_ptr(), pointer(start), sc.data_ptr(),
+                  table_out.data_ptr(), free_out.data_ptr(), shares_out.data_ptr(),
+                  sources.data_ptr(), targets.data_ptr(), used.data_ptr(), B, M, F, P, pointer(ws), n,
+                  stream_of(*t)));
+  return py::make_tuple(table_out, free_out, shares_out, sources, targets, used);
 }
 
 // Takes the entry points' addresses, in the order of Entries.
 void init_layer(const std::vector<I64>& addresses) {
-  if (addresses.size() != 11)
-    throw std::invalid_argument("gfx950 layer operators: 11 entry points are needed");
+  if (addresses.size() != 19)
+    throw std::invalid_argument("gfx950 layer operators: 19 entry points are needed");
   for (const I64 a : addresses)
     if (a == 0) throw std::invalid_argument("gfx950 layer operators: a null entry point was passed");
   auto at = [&](int i) { return reinterpret_cast<Ptr>(static_cast<uintptr_t>(addresses[i])); };
@@ -508,7 +681,14 @@ void init_layer(const std::vector<I64>& addresses) {
   g.plan = reinterpret_cast<Plan>(at(5));
   g.store = reinterpret_cast<Store>(at(6));
   g.paged_bytes = reinterpret_cast<PagedBytes>(at(9));
-  g.last_error = reinterpret_cast<LastError>(at(10));
+  for (int i = 0; i < 2; ++i) g.prefix[i] = reinterpret_cast<Prefix>(at(10 + i));
+  g.prefix_bytes = reinterpret_cast<PrefixBytes>(at(12));
+  g.fork = reinterpret_cast<Fork>(at(13));
+  g.fork_bytes = reinterpret_cast<ForkBytes>(at(14));
+  g.copy = reinterpret_cast<Copy>(at(15));
+  g.compact = reinterpret_cast<Compact>(at(16));
+  g.compact_bytes = reinterpret_cast<CompactBytes>(at(17));
+  g.last_error = reinterpret_cast<LastError>(at(18));
   g_ready = true;
 }
 
@@ -521,4 +701,8 @@ void bind_layer(py::module_& m) {
   m.def("paged_plan", &native_plan);
   m.def("paged_store", &native_store);
   m.def("paged_attention", &native_paged);
+  m.def("paged_prefix_attention", &native_prefix);
+  m.def("paged_fork", &native_fork);
+  m.def("paged_copy", &native_copy);
+  m.def("paged_compact", &native_compact);
 }

@@ -29,7 +29,10 @@ ENTRY_POINTS = ("fa_fwd_view", "fa_fwd_view_bf16", "fa_bwd_view", "fa_bwd_view_b
 LAYER_ENTRY_POINTS = ("fa_qk_norm_rope", "fa_qk_norm_rope_bf16", "fa_qk_norm_rope_bwd",
                       "fa_qk_norm_rope_bwd_bf16", "fa_qk_norm_rope_bwd_workspace_bytes",
                       "fa_paged_plan", "fa_paged_store", "fa_paged_fwd", "fa_paged_fwd_bf16",
-                      "fa_paged_fwd_workspace_bytes", "fa_last_error")
+                      "fa_paged_fwd_workspace_bytes", "fa_paged_prefix_fwd",
+                      "fa_paged_prefix_fwd_bf16", "fa_paged_prefix_fwd_workspace_bytes",
+                      "fa_paged_fork", "fa_paged_fork_workspace_bytes", "fa_paged_copy",
+                      "fa_paged_compact", "fa_paged_compact_workspace_bytes", "fa_last_error")
 
 _module = None
 _error: str | None = None

@@ -161,7 +161,7 @@ def paged_cache_fork(
     the holders: where it does not, pages may return too early or never.
     """
     native = _binding(backend)
-    if native is not None and hasattr(native, "paged_fork"):
+    if native is not None:
         out = native.paged_fork(page_table, lengths, parents, free_pages, page_shares, page_size,
                                 free_start)
         if out is not None:
@@ -214,7 +214,7 @@ def paged_cache_copy(
     to be.
     """
     native = _binding(backend)
-    if native is not None and hasattr(native, "paged_copy") and native.paged_copy(
+    if native is not None and native.paged_copy(
             key_cache, value_cache, sources, targets, tokens):
         return
     _check_backend(backend)
@@ -302,7 +302,7 @@ def paged_cache_compact(
     in stay as they are, and a program that holds pages outside the table finds them in ``sources``.
     """
     native = _binding(backend)
-    if native is not None and hasattr(native, "paged_compact"):
+    if native is not None:
         out = native.paged_compact(page_table, free_pages, page_shares, free_start)
         if out is not None:
             return PagedCompaction(*out)

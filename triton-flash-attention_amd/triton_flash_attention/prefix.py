@@ -106,7 +106,7 @@ def paged_prefix_attention(
     ``paged_attention`` is faster. They have no backward.
     """
     native = _binding(backend)
-    if native is not None and not _forward_ad_active() and hasattr(native, "paged_prefix_attention"):
+    if native is not None and not _forward_ad_active():
         out = native.paged_prefix_attention(query, key_cache, value_cache, page_table, lengths,
                                             group_starts, prefix_lengths, scale, enable_gqa)
         if out is not None:
