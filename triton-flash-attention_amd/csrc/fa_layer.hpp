@@ -231,7 +231,7 @@ struct PrefixArgs {
   const int* starts;     // [G + 1], the groups' first sequences and the end of the last
   const int* prefix;     // [G], keys of the groups' prefixes
   half_t* o;             // contiguous [B, Hq, N, d]
-  int* ws;               // two ints, then from int 16 on the join's PrefixSeq [B], PrefixGroup [G]
+  int* ws;               // four ints, then from int 16 on the join's PrefixSeq [B], PrefixGroup [G]
   float* part;           // partials: pslots slots of prows rows, then those of srows rows
   int64_t qs[3];         // batch, head and row stride, elements
   int64_t ks[3];         // page, head and row stride
@@ -245,16 +245,20 @@ struct PrefixArgs {
   int prows, srows;      // rows of a prefix's and of a sequence's own slot
   int grid;              // work-groups
 };
-// Where sequence b's own units, and group g's, lie on the line of units.
+// Where a sequence's own units lie on the line of units, and its group and its place in it.
 struct PrefixSeq {
   int own_base, own_units, group, member;
 };
+// Where a group's units lie on the line and which of the line's triples is its first, or which of the
+// long prefixes' pieces, `cuts` a triple.
 struct PrefixGroup {
-  int base, units, first, tiles;
+  int base, units, first, tiles, cuts, pad[3];
 };
 constexpr int kPrefixTile = 128;   // query rows of a tile
 constexpr int kPrefixLead = 6;     // empty units in front of a triple on the line
 constexpr int kPrefixStretch = 4;  // least units of a work-group
+constexpr int kOwnRows = 32;       // most rows of a sequence whose own keys are a wave's work,
+constexpr int kOwnLead = 1;        // and the empty units in front of them
 inline __host__ __device__ int prefix_tiles(int64_t sequences, int64_t R) {
   return (int)((sequences * R + kPrefixTile - 1) / kPrefixTile);
 }

@@ -9,6 +9,7 @@
 // in a group of one, whose sequence reads them as its own): keys j < P of all its sequences lie in
 // the pages of the first one, keys j >= P in each one's own.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "fa_common.hpp"
@@ -17,15 +18,26 @@
 namespace fa {
 
 // The work is a list of triples: (group, key/value head, tile of 128 query rows) over the keys of
-// the group's prefix, then (sequence, key/value head, tile) over a sequence's own keys. A tile's
+// the group's prefix, and (sequence, key/value head, tile) over a sequence's own keys. A tile's
 // rows are those that read the key/value head: the group's heads and the N tokens of one sequence
-// after the other. Units of 32 keys of all triples lie on one line, each triple's behind `lead`
-// empty ones that stand for opening and closing a piece; every work-group takes an equal stretch of
-// it, found from the lengths on the GPU. It writes what it has of a triple as one piece, normalised
-// partial O and base-2 log-sum-exp of each row, into a slot of its own: stretch s + triple t, which
-// no two pieces share since from one piece to the next on the line either s or t grows by one.
+// after the other. A work-group writes what it has of a triple as one piece, normalised partial O
+// and base-2 log-sum-exp of each row, into a slot of its own.
+//
+// Prefixes meet many rows: a work-group's four waves share each unit of 32 keys (prefix_piece). A
+// sequence's own keys meet few, at most 32 in decoding, and come in many short triples: there each
+// wave works on a triple of its own, so that eight are open on a CU (own_piece); with more rows a
+// head they go the prefixes' way (WAVES false).
+//
+// Units of all triples lie on a line, each triple's behind `lead` empty ones that stand for opening
+// and closing a piece; the line is cut into equal stretches, one a work-group or a wave, found from
+// the lengths on the GPU, as in fa_paged.hip. Stretch s has its piece of the line's triple t in
+// slot s + t, which no two pieces share since from one piece to the next either s or t grows by one.
+//
+// A prefix that is long against a stretch is not on the line: each of its triples is cut into k
+// equal pieces, so that no work-group opens two, and the tiles of one range of keys go to
+// neighbouring work-groups of one XCD, whose L2 then reads the keys once for all of them.
 constexpr int kPrefixWaves = 4;
-constexpr int kPrefixStarts = 2048;       // of the groups' starts that are kept in LDS
+constexpr int kPrefixKeptGroups = 1024, kPrefixKeptSeqs = 2048;  // whose values are kept in LDS
 
 template <int D>
 struct PrefixRing {
@@ -66,154 +78,299 @@ __device__ __forceinline__ int prefix_keys(const PrefixArgs& a, int g, int b, in
 __device__ __forceinline__ int key_units(int first, int end) {
   return end > first ? (end - (first & ~15) + 31) / 32 : 0;
 }
-__device__ __forceinline__ int on_line(int units) { return units > 0 ? units + kPrefixLead : 0; }
+__device__ __forceinline__ int on_line(int units, int lead) { return units > 0 ? units + lead : 0; }
 
-// Where the search for sequence b among the groups ends: the last g with starts[g] <= b, or -1.
-__device__ __forceinline__ int group_of(const int* starts, int G, int b) {
-  int g = -1;
-  for (int step = 1 << (31 - __builtin_clz(G + 1)); step > 0; step >>= 1)
-    if (g + step <= G && starts[g + step] <= b) g += step;
-  return g;
-}
-
-// A place on the line: unit `unit` (lead included) of triple `sub` (head-major) of group `at` or,
-// behind the prefixes, of sequence `at`; `first` is the index of that group's first triple.
+// A place: unit `unit` (lead included) of triple `sub` (head-major) of group or sequence `at`, and
+// what its keys are.
 struct PrefixPlace {
-  int own;  // 0: a prefix, 1: a sequence's own keys
-  int at, sub, unit, first;
+  int kind;    // 0: a group's prefix on the line, 1: a sequence's own keys, 2: a piece of a long prefix
+  int at, sub, unit;
+  int first;   // kind 0: the line's triple index of the group's first triple
+  int b0, n;   // first sequence and number of sequences of the rows
+  int k_first, k_end;
+  int g, g_end;  // kind 1: the sequence's group, and the first sequence behind it
 };
 struct PrefixLine {
-  int total, stretch;
-  bool bad;  // the groups' starts do not ascend within [0, B]
+  int stretch, left;  // a work-group's; left: 0 where it has nothing to do
+  int s;              // its stretch, or its place among the pieces of long prefixes
+  int pieces;         // of long prefixes
+  bool own;           // it, or its waves, take sequences' own keys
+  bool bad;           // the groups' starts do not ascend within [0, B]
 };
 
-// What the kernels know of sequence b's rows: written by work-group 0 for the join.
+// What the join needs, written by block 0: the stretch, a wave's stretch, whether the starts are bad,
+// and the long prefixes' pieces; then every sequence's and every
+// group's places.
 __device__ __forceinline__ PrefixSeq* prefix_seqs(const PrefixArgs& a) {
   return reinterpret_cast<PrefixSeq*>(a.ws + 16);
 }
+__device__ __forceinline__ PrefixGroup* prefix_groups(const PrefixArgs& a) {
+  return reinterpret_cast<PrefixGroup*>(prefix_seqs(a) + a.B);
+}
 
-// The line, and its place at stretch `s`, defined where the line reaches it. `lds`: the
-// work-group's memory, free before and after.
-__device__ __forceinline__ PrefixLine prefix_find(const PrefixArgs& a, int s, int* lds,
-                                                  PrefixPlace* place) {
+// Pieces that a triple of `units` units is cut into where a work-group takes L; 0: it is on the line.
+__device__ __forceinline__ int prefix_cuts(int units, int L, bool cut) {
+  const int each = L - kPrefixLead;
+  return cut && each >= kPrefixLead && units >= 2 * each ? (units + each - 1) / each : 0;
+}
+
+// A wave's stretch of the sequences' own keys, where a work-group's is L.
+__device__ __forceinline__ int own_stretch(int L) { return max((L + kPrefixWaves - 1) / kPrefixWaves, 2); }
+
+// The work-group's place, or the wave's. `lds`: the work-group's memory, free before and after.
+template <bool WAVES>
+__device__ __forceinline__ PrefixLine prefix_find(const PrefixArgs& a, int* lds, PrefixPlace* place) {
   constexpr int W = kPrefixWaves, T = 64 * W;
-  int* const found = lds;                                  // [8]
-  int(*const sums)[3] = reinterpret_cast<int(*)[3]>(lds + 8);  // [W]
-  int* const kept = lds + 32;                              // the starts
+  int(*const found)[12] = reinterpret_cast<int(*)[12]>(lds);    // [W]
+  int* const wrongs = lds + 48;                                // [W]
+  int(*const sums)[4] = reinterpret_cast<int(*)[4]>(lds + 52);  // [2 W], used in turn
+  int* const kept_starts = lds + 96;
+  int* const kept_prefix = kept_starts + kPrefixKeptGroups;
+  int* const kept_lengths = kept_prefix + kPrefixKeptGroups;
   const int tid = threadIdx.x;
   bool wrong = false;
   for (int g = tid; g <= a.G; g += T) {
     const int x = a.starts[g];
     wrong |= x < 0 || x > a.B || (g > 0 && a.starts[g - 1] > x);
-    if (g < kPrefixStarts) kept[g] = x;
+    if (a.G < kPrefixKeptGroups) {
+      kept_starts[g] = x;
+      if (g < a.G) kept_prefix[g] = a.prefix[g];
+    }
   }
-  // (the flags of the waves, beside found[]: __syncthreads_or would take LDS of its own)
-  if ((tid & 63) == 0) lds[24 + (tid >> 6)] = 0;
-  if (wrong) lds[24 + (tid >> 6)] = 1;
+  if (a.B <= kPrefixKeptSeqs)
+    for (int b = tid; b < a.B; b += T) kept_lengths[b] = a.lengths[b];
+  if ((tid & 63) == 0) wrongs[tid >> 6] = 0;
+  if (wrong) wrongs[tid >> 6] = 1;
   __syncthreads();
   PrefixLine line;
-  line.bad = (lds[24] | lds[25] | lds[26] | lds[27]) != 0;
+  line.bad = uniform(wrongs[0] | wrongs[1] | wrongs[2] | wrongs[3]) != 0;
   const int G = line.bad ? 0 : a.G;
-  const int* const starts = a.G < kPrefixStarts ? kept : a.starts;
-
-  // The thread's groups and sequences: their parts of the line, and the groups' triples.
-  const int per_g = (G + T - 1) / T, g0 = tid * per_g, g1 = min(G, g0 + per_g);
-  const int per_b = (a.B + T - 1) / T, b0 = tid * per_b, b1 = min(a.B, b0 + per_b);
-  auto group_triples = [&](int g) __attribute__((always_inline)) {
-    return prefix_tiles(starts[g + 1] - starts[g], a.R) * a.Hkv;
+  auto start = [&](int g) __attribute__((always_inline)) {
+    return a.G < kPrefixKeptGroups ? kept_starts[g] : a.starts[g];
   };
-  auto group_units = [&](int g) __attribute__((always_inline)) {
-    return key_units(0, prefix_keys(a, g, starts[g], starts[g + 1]));
+  auto length = [&](int b) __attribute__((always_inline)) {
+    return fitting(a, a.B <= kPrefixKeptSeqs ? kept_lengths[b] : a.lengths[b]);
   };
-  auto group_at = [&](int b) __attribute__((always_inline)) {
-    const int g = G > 0 ? group_of(starts, G, b) : -1;
-    return g < G ? g : -1;  // behind the last group there is none
-  };
+  // Prefix keys of group g, and its triples.
   auto front_of = [&](int g) __attribute__((always_inline)) {
-    return g < 0 ? 0 : prefix_keys(a, g, starts[g], starts[g + 1]);
+    const int b = start(g), e = start(g + 1);
+    if (e - b < 2) return 0;
+    const int keys = a.G < kPrefixKeptGroups ? kept_prefix[g] : a.prefix[g];
+    return min(max(keys, 0), length(b));
   };
-  auto own_units = [&](int b, int front) __attribute__((always_inline)) {
-    return key_units(front, fitting(a, a.lengths[b]));
+  auto triples_of = [&](int g) __attribute__((always_inline)) {
+    return prefix_tiles(start(g + 1) - start(g), a.R) * a.Hkv;
   };
-  int own[3] = {0, 0, 0}, first[3], all[3];
-  for (int g = g0; g < g1; ++g) {
-    const int u = group_units(g), t = u > 0 ? group_triples(g) : 0;
-    own[0] += on_line(u) * t;
-    own[1] += t;
-  }
-  const int HB = a.Hkv * a.blocks;
-  for (int b = b0; b < b1; ++b) own[2] += on_line(own_units(b, front_of(group_at(b)))) * HB;
-  block_scan<W>(own, sums, first, all);
-  line.total = all[0] + all[2];
-  line.stretch = max((line.total + a.grid - 1) / a.grid, kPrefixStretch);
-  first[2] += all[0];
+  // The last group that begins at sequence b or before, -1 or G for a sequence outside all.
+  auto group_at = [&](int b) __attribute__((always_inline)) {
+    int g = -1;
+    for (int step = 1 << (31 - __builtin_clz(G + 1)); step > 0; step >>= 1)
+      if (g + step <= G && start(g + step) <= b) g += step;
+    return g;
+  };
+  auto front_at = [&](int g) __attribute__((always_inline)) { return g >= 0 && g < G ? front_of(g) : 0; };
 
-  const int64_t at = (int64_t)s * line.stretch;
-  if (at >= first[0] && at < (int64_t)first[0] + own[0]) {
-    int rest = (int)(at - first[0]), t = first[1];
+  // The thread's groups and sequences, and their parts of the work.
+  const int per_g = (G + T - 1) / T, g0 = min(G, tid * per_g), g1 = min(G, g0 + per_g);
+  const int per_b = (a.B + T - 1) / T, b0 = min(a.B, tid * per_b), b1 = min(a.B, b0 + per_b);
+  const int HB = a.Hkv * a.blocks, lead = WAVES ? kOwnLead : kPrefixLead;
+  int own = 0;
+  for (int b = b0; b < b1; ++b)
+    own += on_line(key_units(G > 0 ? front_at(group_at(b)) : 0, length(b)), lead) * HB;
+  // Sums: long prefixes' pieces; units and triples of the others; units of sequences' own keys.
+  int x[4], before[4], all[4];
+  bool cut = true;
+  int L = 0;
+  for (int round = 0;; ++round) {
+    x[0] = x[1] = x[2] = 0;
+    x[3] = own;
     for (int g = g0; g < g1; ++g) {
-      const int u = group_units(g), n = u > 0 ? group_triples(g) : 0;
-      const int len = on_line(u);
-      if (rest < len * n) {
-        found[0] = 0;
-        found[1] = g;
-        found[2] = rest / len;
-        found[3] = rest % len;
-        found[4] = t;
-        break;
+      const int u = key_units(0, front_of(g)), t = u > 0 ? triples_of(g) : 0;
+      const int k = prefix_cuts(u, L, cut);
+      if (k > 0) {
+        x[0] += t * k;
+      } else {
+        x[1] += on_line(u, kPrefixLead) * t;
+        x[2] += t;
       }
-      rest -= len * n;
-      t += n;
+    }
+    block_scan<W>(x, sums + W * (round & 1), before, all);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) all[i] = uniform(all[i]);
+    if (round == 0) {  // all of it (L = 0 cuts nothing)
+      L = max((all[1] + all[3] + a.grid - 1) / a.grid, kPrefixStretch);
+      if (all[1] == 0) break;
+      continue;
+    }
+    // Work-groups that it takes: a longer stretch, until the grid holds them.
+    const int each = WAVES ? W * own_stretch(L) : L;
+    const int need = (all[0] + 7) / 8 * 8 + (WAVES ? (all[1] + L - 1) / L + (all[3] + each - 1) / each
+                                                   : (all[1] + all[3] + L - 1) / L);
+    if (need <= a.grid) break;
+    if (round < 10) {
+      L += max(max(1, L / 32), (int)((int64_t)L * (need - a.grid) / a.grid));
+    } else {
+      cut = false;
+      L *= 2;
     }
   }
-  if (at >= first[2] && at < (int64_t)first[2] + own[2]) {
-    int rest = (int)(at - first[2]);
-    for (int b = b0; b < b1; ++b) {
-      const int len = on_line(own_units(b, front_of(group_at(b))));
-      if (rest < len * HB) {
-        found[0] = 1;
-        found[1] = b;
-        found[2] = rest / len;
-        found[3] = rest % len;
-        found[4] = 0;
+  line.stretch = L;
+  line.pieces = all[0];
+
+  // Block i takes pieces of long prefixes first, an XCD consecutive ones, then a stretch of the
+  // others, then sequences' own keys.
+  const int xcd = blockIdx.x % 8, i = blockIdx.x / 8, each = (all[0] + 7) / 8;
+  const bool piece = i < each;
+  line.s = piece ? xcd * each + i : (i - each) * 8 + xcd;
+  const int stretches = WAVES ? (all[1] + L - 1) / L : 0;
+  line.own = !piece && WAVES && line.s >= stretches;
+  int mine = L, end = WAVES ? all[1] : all[1] + all[3];  // of the line
+  if (line.own) {
+    line.s = (line.s - stretches) * W + (tid >> 6);
+    mine = own_stretch(L);
+    end = all[3];
+  }
+  int64_t from = (int64_t)line.s * mine;
+  line.left = piece ? (line.s < all[0] ? 1 : 0) : from < end ? (int)min((int64_t)mine, end - from) : 0;
+  if (piece) {
+    if (line.s >= before[0] && line.s < before[0] + x[0]) {
+      int at = line.s - before[0];
+      for (int g = g0; g < g1; ++g) {
+        const int keys = front_of(g), u = key_units(0, keys), k = prefix_cuts(u, L, true);
+        const int n = k > 0 ? triples_of(g) * k : 0;
+        if (at >= n) {
+          at -= n;
+          continue;
+        }
+        // piece p of head kvh, tile t: place (kvh k + p) tiles + t
+        const int tiles = triples_of(g) / a.Hkv, t = at % tiles, p = at / tiles % k;
+        int* const f = found[0];
+        f[0] = 2;
+        f[1] = g;
+        f[2] = at / tiles / k * tiles + t;
+        f[3] = 0;
+        f[4] = 0;
+        f[5] = start(g);
+        f[6] = start(g + 1) - start(g);
+        f[7] = 32 * (int)((int64_t)u * p / k);
+        f[8] = min(keys, 32 * (int)((int64_t)u * (p + 1) / k));
         break;
       }
-      rest -= len * HB;
     }
+  } else {
+    if (!line.own && from >= before[1] && from < (int64_t)before[1] + x[1]) {
+      int at = (int)(from - before[1]), t = before[2];
+      for (int g = g0; g < g1; ++g) {
+        const int keys = front_of(g), u = key_units(0, keys);
+        const int n = u > 0 && prefix_cuts(u, L, cut) == 0 ? triples_of(g) : 0;
+        const int len = on_line(u, kPrefixLead);
+        if (at < len * n) {
+          int* const f = found[0];
+          f[0] = 0;
+          f[1] = g;
+          f[2] = at / len;
+          f[3] = at % len;
+          f[4] = t;
+          f[5] = start(g);
+          f[6] = start(g + 1) - start(g);
+          f[7] = 0;
+          f[8] = keys;
+          break;
+        }
+        at -= len * n;
+        t += n;
+      }
+    }
+    // The waves' places, or the work-group's.
+    if (line.own || !WAVES)
+      for (int w = 0; w < (WAVES ? W : 1); ++w) {
+        if (WAVES) from = (int64_t)((line.s & ~(W - 1)) + w) * mine;
+        else from = (int64_t)line.s * mine - all[1];
+        if (from < before[3] || from >= (int64_t)before[3] + own) continue;
+        int at = (int)(from - before[3]);
+        for (int b = b0; b < b1; ++b) {
+          const int g = G > 0 ? group_at(b) : -1, keys = front_at(g), stop = length(b);
+          const int len = on_line(key_units(keys, stop), lead);
+          if (at < len * HB) {
+            int* const f = found[w];
+            f[0] = 1;
+            f[1] = b;
+            f[2] = at / len;
+            f[3] = at % len;
+            f[4] = 0;
+            f[5] = b;
+            f[6] = 1;
+            f[7] = keys;
+            f[8] = stop;
+            f[9] = g;
+            f[10] = g < 0 ? (G > 0 ? start(0) : a.B) : g < G ? start(g + 1) : a.B;
+            break;
+          }
+          at -= len * HB;
+        }
+      }
   }
-  if (s == 0) {
-    // The join's part: where each sequence's and each group's units lie.
+  if (blockIdx.x == 0) {
     if (tid == 0) {
-      a.ws[0] = line.stretch;
-      a.ws[1] = line.bad;
+      a.ws[0] = L;
+      a.ws[1] = WAVES ? own_stretch(L) : L;
+      a.ws[2] = line.bad;
+      a.ws[3] = all[0];
     }
-    int base = first[2];
+    int base = (WAVES ? 0 : all[1]) + before[3];
     for (int b = b0; b < b1; ++b) {
-      const int g = group_at(b), front = front_of(g), u = own_units(b, front);
-      PrefixSeq* const q = prefix_seqs(a) + b;
-      q->own_base = base;
-      q->own_units = u;
-      q->group = g;
-      q->member = g < 0 ? 0 : b - starts[g];
-      base += on_line(u) * HB;
+      const int g = G > 0 ? group_at(b) : -1, u = key_units(front_at(g), length(b));
+      const bool in = g >= 0 && g < G;
+      prefix_seqs(a)[b] = {base, u, in ? g : -1, in ? b - start(g) : 0};
+      base += on_line(u, lead) * HB;
     }
-    PrefixGroup* const gs = reinterpret_cast<PrefixGroup*>(prefix_seqs(a) + a.B);
-    int pre = first[0], t = first[1];
+    int pieces = before[0], t = before[2];
+    base = before[1];
     for (int g = g0; g < g1; ++g) {
-      const int u = group_units(g), n = u > 0 ? group_triples(g) : 0;
-      gs[g] = {pre, u, t, group_triples(g) / a.Hkv};
-      pre += on_line(u) * n;
-      t += n;
+      const int u = key_units(0, front_of(g)), n = triples_of(g), k = prefix_cuts(u, L, cut);
+      prefix_groups(a)[g] = {k > 0 ? pieces : base, u, t, n / a.Hkv, k, 0, 0, 0};
+      if (k > 0) {
+        pieces += n * k;
+      } else if (u > 0) {
+        base += on_line(u, kPrefixLead) * n;
+        t += n;
+      }
     }
   }
   __syncthreads();
-  place->own = uniform(found[0]);
-  place->at = uniform(found[1]);
-  place->sub = uniform(found[2]);
-  place->unit = uniform(found[3]);
-  place->first = uniform(found[4]);
+  const int* const f = found[line.own ? tid >> 6 : 0];
+  place->kind = uniform(f[0]);
+  place->at = uniform(f[1]);
+  place->sub = uniform(f[2]);
+  place->unit = uniform(f[3]);
+  place->first = uniform(f[4]);
+  place->b0 = uniform(f[5]);
+  place->n = uniform(f[6]);
+  place->k_first = uniform(f[7]);
+  place->k_end = uniform(f[8]);
+  place->g = uniform(f[9]);
+  place->g_end = uniform(f[10]);
+  line.s = uniform(line.s);
+  line.left = uniform(line.left);
   __syncthreads();
   return line;
+}
+
+// Turns to the next sequence that has keys of its own; false behind the last.
+__device__ __forceinline__ bool next_sequence(const PrefixArgs& a, PrefixPlace& at) {
+  do {
+    ++at.at;
+    while (at.at >= at.g_end && at.at < a.B) {  // in the next group, or behind the last
+      const int begin = at.g_end;
+      ++at.g;
+      at.g_end = at.g < a.G ? uniform(a.starts[at.g + 1]) : a.B;
+      at.k_first = at.g < a.G ? uniform(prefix_keys(a, at.g, begin, at.g_end)) : 0;
+    }
+    if (at.at >= a.B) return false;
+    at.k_end = uniform(fitting(a, a.lengths[at.at]));
+  } while (key_units(at.k_first, at.k_end) == 0);
+  at.b0 = at.at;
+  return true;
 }
 
 // Slots of pieces: a prefix's hold a.prows rows, a sequence's own keys' a.srows.
@@ -301,8 +458,8 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const PrefixJo
   all_see = uniform(min(all_see, job.k_hi));
 
   const int row_bytes = (int)a.ks[2] * 2;
-  const half_t* const k_head = a.k + job.kvh * a.ks[1];
-  const half_t* const v_head = a.v + job.kvh * a.ks[1];
+  const char* const k_head = reinterpret_cast<const char*>(a.k + job.kvh * a.ks[1]);
+  const char* const v_head = reinterpret_cast<const char*>(a.v + job.kvh * a.ks[1]);
   const int units = (job.k_hi - job.k_lo + T::KT - 1) / T::KT;
 
   // The wave's share of a unit: its 1 KiB pieces, all in half `e` of the unit.
@@ -318,38 +475,36 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const PrefixJo
     dma.voff[i] = 8 * c < a.d ? (uint32_t)((row & 15) * row_bytes + 16 * c) : kOutOfRange;
   }
 
-  // Pages of the half units from unit i & ~31 on, one a lane, and the next 32 units'.
+  // Where the half units from unit iu & ~31 on lie, one a lane: the byte offset of the first of
+  // their rows that exist, and the bytes from it to the end of the last; and the next 32 units'
+  // pages (clamped to the last key's, so that the load needs no branch and none waits for it).
   int bad_key = INT32_MAX;  // first key of the first page that does not exist
   auto half_key = [&](int i) __attribute__((always_inline)) { return job.k_lo + 32 * i + 16 * lane; };
   auto fetch = [&](int i) __attribute__((always_inline)) {
-    const int key = half_key(i);
-    return key < job.k_hi ? job.table[key / a.S] : 0;
-  };
-  auto known = [&](int page, int i) __attribute__((always_inline)) {
-    const bool ok = page >= 0 && page < a.pages;
-    if (!ok) bad_key = min(bad_key, half_key(i));
-    return ok ? page : -1;
+    return job.table[min(half_key(i), job.k_hi - 1) / a.S];
   };
   int next_page = fetch(0);
-  int page = 0, in_page = 0;
+  int64_t off = 0;
+  uint32_t rows_bytes = 0;
   int iu = 0;  // next unit to ask for
   const uint32_t lds0 = lds_addr(lds);
   auto issue = [&](int slot) __attribute__((always_inline)) {
     if ((iu & 31) == 0) {
-      page = known(next_page, iu);
-      in_page = half_key(iu) % a.S;
+      const int key = half_key(iu), skip = max(job.k_first - key, 0);
+      const int there = min(job.k_hi - key, 16) - skip;
+      const bool ok = next_page >= 0 && next_page < a.pages;
+      if (there > 0 && !ok) bad_key = min(bad_key, key);
+      off = 2 * (next_page * a.ks[0] + (key % a.S + skip) * a.ks[2]);
+      rows_bytes = ok && there > 0 ? (uint32_t)((there - 1) * row_bytes + a.d * 2) : 0u;
       next_page = fetch(iu + 32);
     }
-    const int key = job.k_lo + T::KT * iu + 16 * e;
     const int at = 2 * (iu & 31) + e;
-    const int pg = __builtin_amdgcn_readlane(page, at);
-    const int skip = max(job.k_first - key, 0);  // rows in front of the first key
-    const int there = min(job.k_hi - key, 16) - skip;
-    const int64_t off = pg * a.ks[0] + (__builtin_amdgcn_readlane(in_page, at) + skip) * a.ks[2];
-    const uint32_t bytes = there > 0 && pg >= 0 ? (uint32_t)((there - 1) * row_bytes + a.d * 2) : 0u;
-    issue_kv_unit<T::TILE * 2>(dma, make_rsrc_words(k_head + off, bytes),
-                               make_rsrc_words(v_head + off, bytes), -skip,
-                               lds0 + (uint32_t)slot * (T::STAGE * 2u) + (uint32_t)piece0 * 1024u);
+    const int skip = iu == 0 ? max(job.k_first - job.k_lo - 16 * e, 0) : 0;
+    const uint64_t o = (uint32_t)__builtin_amdgcn_readlane((int)off, at) |
+                       (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(off >> 32), at) << 32;
+    const uint32_t n = __builtin_amdgcn_readlane(rows_bytes, at);
+    issue_kv_unit<T::TILE * 2>(dma, make_rsrc_words(k_head + o, n), make_rsrc_words(v_head + o, n),
+                               -skip, lds0 + (uint32_t)slot * (T::STAGE * 2u) + (uint32_t)piece0 * 1024u);
     ++iu;
   };
 
@@ -584,72 +739,291 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const PrefixJo
   __syncthreads();
 }
 
+// A wave's piece of a sequence's own keys [k_lo, k_hi), of which k_first is the first (k_lo is that
+// rounded down to 16), against the R <= 32 rows of head kvh, as in paged_fwd_kernel: K rows come in
+// the layout of the MFMA operand, V rows go through a tile in LDS (`vt`) for the transposing reads,
+// both asked for a unit ahead.
 template <int D, class E>
+__device__ __forceinline__ void own_piece(const PrefixArgs& a, int b, int kvh, int k_lo, int k_first,
+                                          int k_hi, int len, float* slot, half_t* vt) {
+  constexpr int KD = D / 32, DD = D / 16, RB = 2;
+  constexpr int VI = 32 * D * 2 / 1024, VROWS = 512 / D;  // 1 KiB loads of a unit's V, rows of one
+  const int lane = threadIdx.x & 63, c16 = lane & 15, G = lane >> 4;
+  const int row_bytes = (int)a.ks[2] * 2;
+  uint32_t k_off[KD], v_off[VI];
+  int v_at[VI], t_off[DD];
+#pragma unroll
+  for (int kd = 0; kd < KD; ++kd) {
+    const int col = 32 * kd + 8 * G;
+    k_off[kd] = col < a.d ? (uint32_t)(c16 * row_bytes + col * 2) : kOutOfRange;
+  }
+#pragma unroll
+  for (int i = 0; i < VI; ++i) {
+    const int row = i * VROWS + lane / (D / 8), chunk = lane % (D / 8);
+    v_off[i] = 8 * chunk < a.d ? (uint32_t)((row & 15) * row_bytes + chunk * 16) : kOutOfRange;
+    v_at[i] = swz_offset<D>(row, chunk);
+  }
+#pragma unroll
+  for (int dd = 0; dd < DD; ++dd) {
+    const int row = 4 * G + (c16 >> 2), col = 16 * dd + 4 * (c16 & 3);
+    t_off[dd] = row * D + 8 * swz_chunk<D>(row, col >> 3) + (col & 7);
+  }
+
+  const int units = (k_hi - k_lo + 31) / 32;
+  const int* const table = a.table + b * a.table_stride;
+  auto half_key = [&](int i) __attribute__((always_inline)) { return k_lo + 32 * i + 16 * lane; };
+  auto fetch = [&](int i) __attribute__((always_inline)) {
+    return table[min(half_key(i), k_hi - 1) / a.S];
+  };
+  int next_page = fetch(0);
+
+  // The lane's rows. Each sees the keys below see[]; rows that do not exist score 0 everywhere.
+  const int all_see = len - a.N + 1;
+  int see[RB];
+  half8 qf[RB][KD];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const int r = 16 * rb + c16, h = r / a.N, n = r - h * a.N;
+    see[rb] = r < a.R ? min(all_see + n, k_hi) : INT32_MAX;
+    const half_t* q = a.q + b * a.qs[0] + (int64_t)(kvh * a.group + h) * a.qs[1] + n * a.qs[2];
+#pragma unroll
+    for (int kd = 0; kd < KD; ++kd) {
+      u32x4 v = {0u, 0u, 0u, 0u};
+      const int col = 32 * kd + 8 * G;
+      if (r < a.R && col < a.d) v = *reinterpret_cast<const u32x4*>(q + col);
+      qf[rb][kd] = __builtin_bit_cast(half8, v);
+    }
+  }
+
+  const char* const k_head = reinterpret_cast<const char*>(a.k + kvh * a.ks[1]);
+  const char* const v_head = reinterpret_cast<const char*>(a.v + kvh * a.ks[1]);
+  bool bad = false;
+  int64_t off = 0;  // where the half units from i & ~31 on lie, one a lane, as in prefix_piece
+  uint32_t bytes = 0;
+  u32x4 kx[2][KD], vx[VI];
+  uint64_t at[2];
+  uint32_t n[2], back[2];
+  auto turn_to = [&](int i) __attribute__((always_inline)) {
+    if ((i & 31) == 0) {
+      const int key = half_key(i), skip = max(k_first - key, 0);
+      const int there = min(k_hi - key, 16) - skip;
+      const bool ok = next_page >= 0 && next_page < a.pages;
+      bad |= there > 0 && !ok;
+      off = 2 * (next_page * a.ks[0] + (key % a.S + skip) * a.ks[2]);
+      bytes = ok && there > 0 ? (uint32_t)((there - 1) * row_bytes + a.d * 2) : 0u;
+      next_page = fetch(i + 32);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int l = 2 * (i & 31) + e;
+      at[e] = (uint32_t)__builtin_amdgcn_readlane((int)off, l) |
+              (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(off >> 32), l) << 32;
+      n[e] = __builtin_amdgcn_readlane(bytes, l);
+      back[e] = i == 0 ? (uint32_t)(max(k_first - k_lo - 16 * e, 0) * row_bytes) : 0u;
+    }
+  };
+  auto load_k = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const rsrc_t r = make_rsrc(k_head + at[e], n[e]);
+#pragma unroll
+      for (int kd = 0; kd < KD; ++kd) kx[e][kd] = buf_load_b128(r, k_off[kd] - back[e]);
+    }
+  };
+  auto load_v = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < VI; ++j) {
+      const int e = j * VROWS / 16;
+      vx[j] = buf_load_b128(make_rsrc(v_head + at[e], n[e]), v_off[j] - back[e]);
+    }
+  };
+
+  float4v o[RB][DD];
+  float m[RB], l[RB];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+#pragma unroll
+    for (int dd = 0; dd < DD; ++dd) o[rb][dd] = {0.f, 0.f, 0.f, 0.f};
+    m[rb] = -INFINITY;
+    l[rb] = 0.f;
+  }
+  const float c = a.c;
+  turn_to(0);
+  load_k();
+  load_v();
+  for (int i = 0; i < units; ++i) {
+    const int ka = k_lo + 32 * i;
+    float4v s[RB][2];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        s[rb][kb] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kd = 0; kd < KD; ++kd)
+          s[rb][kb] = mma16<E>(__builtin_bit_cast(half8, kx[kb][kd]), qf[rb][kd], s[rb][kb]);
+      }
+    turn_to(i + 1);  // past the last unit: no rows
+    load_k();
+#pragma unroll
+    for (int j = 0; j < VI; ++j) *reinterpret_cast<u32x4*>(vt + v_at[j]) = vx[j];
+    load_v();
+    half8 pa[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      if (ka + 32 > min(all_see, k_hi) || ka < k_first) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int key = ka + 16 * kb + 4 * G + j;
+            if (key >= see[rb] || key < k_first) s[rb][kb][j] = -INFINITY;
+          }
+      }
+      auto probs = [&](float ref) __attribute__((always_inline)) {
+        float sum = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float p = exp2_fast(fmaf(s[rb][kb][j], c, -ref));
+            sum += p;
+            pa[rb][4 * kb + j] = to_elem<E>(p);
+          }
+        return sum;
+      };
+      float l_u = probs(m[rb]);
+      const float held = kPrefixWide<E> ? l[rb] + l_u : l_u;
+      if (__builtin_amdgcn_ballot_w64(!(held <= 0.5f * kPrefixSumLimit<E>)) != 0) {
+        float mt = s[rb][0][0];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mt = __builtin_fmaxf(mt, s[rb][kb][j]);
+        float m_new = __builtin_fmaxf(m[rb], quarters_max(mt) * c - kPrefixShift<E>);
+        if constexpr (kPrefixWide<E>)
+          m_new = __builtin_fmaxf(m_new, m[rb] + log2_fast(quarters_max(l[rb])) - kPrefixShift<E>);
+        const float ref = exp_reference(m_new);
+        const float alpha = exp2_fast(m[rb] - ref);
+        l[rb] *= alpha;
+#pragma unroll
+        for (int dd = 0; dd < DD; ++dd) o[rb][dd] *= alpha;
+        m[rb] = m_new;
+        l_u = probs(ref);
+      }
+      l[rb] += l_u;
+    }
+#pragma unroll
+    for (int dd = 0; dd < DD; ++dd) {
+      const half4 lo = __builtin_bit_cast(
+          half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(vt + t_off[dd])));
+      const half4 hi = __builtin_bit_cast(
+          half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(vt + t_off[dd] + 16 * D)));
+      half8 va;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        va[e] = lo[e];
+        va[4 + e] = hi[e];
+      }
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) o[rb][dd] = mma16<E>(va, pa[rb], o[rb][dd]);
+    }
+  }
+
+  bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const int r = 16 * rb + c16;
+    float lt = quarters_sum(l[rb]);
+    if (bad) lt = __builtin_nanf("");
+    if (r >= a.R) continue;
+    const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+#pragma unroll
+    for (int dd = 0; dd < DD; ++dd)
+      *reinterpret_cast<float4v*>(slot + (int64_t)r * D + 16 * dd + 4 * G) = o[rb][dd] * inv;
+    if (G == 0) slot[(int64_t)a.srows * D + r] = lt == 0.f ? -INFINITY : m[rb] + log2_fast(lt);
+  }
+}
+
+template <int D, class E, bool WAVES>
 __global__ __launch_bounds__(64 * kPrefixWaves, PrefixRing<D>::WGS) void prefix_fwd_kernel(PrefixArgs a) {
   __shared__ __attribute__((aligned(1024))) half_t lds[PrefixRing<D>::HALVES];
-  static_assert(sizeof(lds) >= (32 + kPrefixStarts) * 4, "the line is found in the ring's memory");
-  const int s = blockIdx.x;
+  static_assert(sizeof(lds) >= (96 + 2 * kPrefixKeptGroups + kPrefixKeptSeqs) * 4,
+                "places are found in the ring's memory");
   PrefixPlace at;
-  const PrefixLine line = prefix_find(a, s, reinterpret_cast<int*>(lds), &at);
-  const int64_t from = (int64_t)s * line.stretch;
-  if (from >= line.total) return;
-  int left = min(line.stretch, (int)(line.total - from));
-  const int G = line.bad ? 0 : a.G;
+  const PrefixLine line = prefix_find<WAVES>(a, reinterpret_cast<int*>(lds), &at);
+  int left = line.left;
+  if (left <= 0) return;
   const int HB = a.Hkv * a.blocks;
-  PrefixJob job;
-  int units = 0, subs = 0, tiles = 1, k0 = 0, k_first = 0, k_end = 0;
-  bool turned = true;  // to another group or sequence
-  while (true) {
-    if (turned) {
-      if (at.own == 0 && at.at >= G) at = {1, 0, 0, 0, 0};
-      if (at.own == 0) {
-        job.b0 = uniform(a.starts[at.at]);
-        const int end = uniform(a.starts[at.at + 1]);
-        k_first = 0;
-        k_end = uniform(prefix_keys(a, at.at, job.b0, end));
-        tiles = prefix_tiles(end - job.b0, a.R);
-        job.rows = (end - job.b0) * a.R;
-        job.slot_rows = a.prows;
-      } else {
-        job.b0 = at.at;
-        const int g = G > 0 ? uniform(group_of(a.starts, G, at.at)) : -1;
-        k_first = g < 0 || g >= G ? 0 : uniform(prefix_keys(a, g, a.starts[g], a.starts[g + 1]));
-        k_end = uniform(fitting(a, a.lengths[at.at]));
-        tiles = a.blocks;
-        job.rows = a.R;
-        job.slot_rows = a.srows;
-      }
-      job.table = a.table + job.b0 * a.table_stride;
-      units = key_units(k_first, k_end);
-      subs = units > 0 ? tiles * a.Hkv : 0;
-      k0 = k_first & ~15;
-      turned = false;
-    }
-    if (at.sub >= subs) {
-      at.first += subs;
-      ++at.at;
+  if (WAVES && line.own) {
+    half_t* const vt = lds + uniform(threadIdx.x >> 6) * (32 * D);
+    while (true) {
+      const int k0 = at.k_first & ~15, units = key_units(at.k_first, at.k_end);
+      const int len = units + kOwnLead;
+      const int u0 = max(at.unit - kOwnLead, 0);
+      const int u1 = left < len - at.unit ? max(at.unit + left - kOwnLead, 0) : units;
+      if (u1 > u0)
+        own_piece<D, E>(a, at.at, at.sub, k0 + 32 * u0, max(at.k_first, k0 + 32 * u0),
+                        min(at.k_end, k0 + 32 * u1), at.k_end,
+                        own_slot(a, D, (int64_t)line.s + (int64_t)at.at * HB + at.sub), vt);
+      left -= len - at.unit;
+      if (left <= 0) return;
+      at.unit = 0;
+      if (++at.sub < HB) continue;
       at.sub = 0;
-      turned = true;
-      continue;
+      if (!next_sequence(a, at)) return;
     }
-    // The part of the triple's units that is the work-group's.
+  }
+  while (true) {
+    // The triple's part that is the work-group's.
+    PrefixJob job;
+    const int tiles = at.kind == 1 ? a.blocks : prefix_tiles(at.n, a.R);
+    job.kvh = at.sub / tiles;
+    job.row0 = (at.sub - job.kvh * tiles) * kPrefixTile;
+    job.b0 = at.b0;
+    job.rows = at.n * a.R;
+    job.table = a.table + at.b0 * a.table_stride;
+    job.slot_rows = at.kind == 1 ? a.srows : a.prows;
+    const bool piece = at.kind == 2;
+    const int k0 = at.k_first & ~15, units = key_units(at.k_first, at.k_end);
     const int len = units + kPrefixLead;
-    const int u0 = max(at.unit - kPrefixLead, 0);
-    const int u1 = left < len - at.unit ? max(at.unit + left - kPrefixLead, 0) : units;
+    const int u0 = piece ? 0 : max(at.unit - kPrefixLead, 0);
+    const int u1 = piece || left >= len - at.unit ? units : max(at.unit + left - kPrefixLead, 0);
     if (u1 > u0) {
-      job.kvh = at.sub / tiles;
-      job.row0 = (at.sub - job.kvh * tiles) * kPrefixTile;
       job.k_lo = k0 + 32 * u0;
-      job.k_first = max(k_first, job.k_lo);
-      job.k_hi = min(k_end, k0 + 32 * u1);
-      job.slot = at.own == 0 ? prefix_slot(a, D, (int64_t)s + at.first + at.sub)
-                             : own_slot(a, D, (int64_t)s + (int64_t)at.at * HB + at.sub);
+      job.k_first = max(at.k_first, job.k_lo);
+      job.k_hi = min(at.k_end, k0 + 32 * u1);
+      job.slot = piece          ? prefix_slot(a, D, line.s)
+                 : at.kind == 0 ? prefix_slot(a, D, (int64_t)line.pieces + line.s + at.first + at.sub)
+                                : own_slot(a, D, (int64_t)line.s + (int64_t)at.at * HB + at.sub);
       prefix_piece<D, E>(a, job, lds);
     }
+    if (piece) return;
     left -= len - at.unit;
     if (left <= 0) return;
+    // The next triple on the line, of this group or sequence or the next that has any there.
     at.unit = 0;
-    ++at.sub;
+    if (++at.sub < tiles * a.Hkv) continue;
+    at.sub = 0;
+    if (at.kind == 0) {
+      at.first += tiles * a.Hkv;
+      int units = 0;
+      while (units == 0 && ++at.at < a.G) {
+        at.b0 = uniform(a.starts[at.at]);
+        const int end = uniform(a.starts[at.at + 1]);
+        at.n = end - at.b0;
+        at.k_end = uniform(prefix_keys(a, at.at, at.b0, end));
+        units = key_units(0, at.k_end);
+        if (prefix_cuts(units, line.stretch, line.pieces > 0) > 0) units = 0;
+      }
+      if (units > 0) continue;
+      if (WAVES) return;
+      at.kind = at.n = 1;  // the line goes on with the sequences' own keys
+      at.at = at.g = -1;
+      at.g_end = line.bad || a.G == 0 ? a.B : uniform(a.starts[0]);
+      at.k_first = 0;
+    }
+    if (!next_sequence(a, at)) return;
   }
 }
 
@@ -675,26 +1049,40 @@ __global__ __launch_bounds__(64 * kPrefixWaves) void prefix_join_kernel(PrefixAr
   const int64_t rr = real ? row : 0;
   const int b = (int)(rr / seq_rows), in_seq = (int)(rr - b * seq_rows);
   const int kvh = in_seq / a.R, r = in_seq - kvh * a.R;
-  const int stretch = a.ws[0];
-  const bool bad = a.ws[1] != 0;
+  const int stretch = a.ws[0], own_stretch = a.ws[1], cut = a.ws[3];
+  const bool bad = a.ws[2] != 0;
   const int len = a.lengths[b];
   const PrefixSeq q = prefix_seqs(a)[b];
-  PrefixGroup grp = {0, 0, 0, 0};
-  if (q.group >= 0) grp = reinterpret_cast<const PrefixGroup*>(prefix_seqs(a) + a.B)[q.group];
+  PrefixGroup grp = {0, 0, 0, 1, 0, 0, 0, 0};
+  if (q.group >= 0) grp = prefix_groups(a)[q.group];
 
-  // The stretches s0 .. s1 that hold the units of triple `sub`, whose line begins at `base`.
-  auto range = [&](int base, int units, int sub, int* s0, int* s1) __attribute__((always_inline)) {
-    const int64_t at = base + (int64_t)sub * on_line(units) + kPrefixLead;
-    *s0 = (int)(at / stretch);
-    *s1 = units > 0 ? (int)((at + units - 1) / stretch) : *s0 - 1;
+  // Pieces of a triple on the line whose part of it begins at `base`: the first one's stretch, and
+  // how many there are.
+  auto range = [](int64_t base, int units, int lead, int stretch, int* n) __attribute__((always_inline)) {
+    const int64_t at = base + lead;
+    const int s0 = (int)(at / stretch);
+    *n = units > 0 ? (int)((at + units - 1) / stretch) - s0 + 1 : 0;
+    return s0;
   };
-  int p0, p1, q0, q1;
   const int64_t gr = (int64_t)q.member * a.R + r;
-  const int psub = kvh * grp.tiles + (int)(gr / kPrefixTile);
-  range(grp.base, grp.units, psub, &p0, &p1);
+  const int tile = (int)(gr / kPrefixTile), psub = kvh * grp.tiles + tile;
+  int np, no, step = 1;
+  int64_t pslot;
+  if (grp.cuts > 0) {
+    np = grp.cuts;
+    step = grp.tiles;
+    pslot = (int64_t)grp.base + (int64_t)kvh * grp.cuts * grp.tiles + tile;
+  } else {
+    pslot = range(grp.base + (int64_t)psub * on_line(grp.units, kPrefixLead), grp.units, kPrefixLead,
+                  stretch, &np);
+    pslot += (int64_t)cut + grp.first + psub;
+  }
   const int osub = kvh * a.blocks + r / kPrefixTile;
-  range(q.own_base, q.own_units, osub, &q0, &q1);
-  const int np = p1 - p0 + 1, count = real ? np + (q1 - q0 + 1) : 0;
+  const int lead = a.R <= kOwnRows ? kOwnLead : kPrefixLead;
+  int64_t oslot = range(q.own_base + (int64_t)osub * on_line(q.own_units, lead), q.own_units, lead,
+                        own_stretch, &no);
+  oslot += (int64_t)b * a.Hkv * a.blocks + osub;
+  const int count = real ? np + no : 0;
   struct Piece {
     float lse;
     float4v o;
@@ -703,8 +1091,8 @@ __global__ __launch_bounds__(64 * kPrefixWaves) void prefix_join_kernel(PrefixAr
     Piece p = {-INFINITY, {0.f, 0.f, 0.f, 0.f}};
     if (i < count) {
       const bool pre = i < np;
-      const float* slot = pre ? prefix_slot(a, D, (int64_t)p0 + i + grp.first + psub)
-                              : own_slot(a, D, (int64_t)q0 + (i - np) + (int64_t)b * a.Hkv * a.blocks + osub);
+      const float* slot = pre ? prefix_slot(a, D, pslot + (int64_t)i * step)
+                              : own_slot(a, D, oslot + (i - np));
       const int at = pre ? (int)(gr % kPrefixTile) : r % kPrefixTile;
       p.lse = slot[(int64_t)(pre ? a.prows : a.srows) * D + at];
       p.o = *reinterpret_cast<const float4v*>(slot + (int64_t)at * D + col);
@@ -769,18 +1157,22 @@ PrefixSizes prefix_sizes(int64_t B, int64_t G, int64_t Hkv, int64_t R, int64_t D
   const double each = (double)((keys + 31) / 32 + 1 + kPrefixLead);
   z.units = each * ((double)triples + (double)own);
   const int64_t most = 256 * (prefix_width(D) == 128 ? 2 : 3);
-  z.grid = (int)std::max(1.0, std::min((double)most, z.units / kPrefixStretch));
+  // Work-groups that the chip holds at once, at most one for each four units that the tables could
+  // hold; as many on each XCD.
+  z.grid = (int)std::min((double)most, std::ceil(z.units / kPrefixStretch));
+  z.grid = (z.grid + 7) / 8 * 8;
   z.pslots = triples > 0 ? z.grid + triples : 0;
   z.head_bytes = (64 + B * (int64_t)sizeof(PrefixSeq) + G * (int64_t)sizeof(PrefixGroup) + 63) / 64 * 64;
-  const int64_t rows = z.pslots * z.prows + (z.grid + own) * z.srows;
+  const int64_t rows = z.pslots * z.prows + (kPrefixWaves * z.grid + own) * z.srows;
   z.bytes = z.head_bytes + rows * (prefix_width(D) + 4) * 4;
   return z;
 }
 
 template <int D, class E>
 hipError_t prefix_start(const PrefixArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL((prefix_fwd_kernel<D, E>), dim3((unsigned)a.grid), dim3(64 * kPrefixWaves), 0,
-                     stream, a);
+  const dim3 grid((unsigned)a.grid), block(64 * kPrefixWaves);
+  if (a.R <= kOwnRows) hipLaunchKernelGGL((prefix_fwd_kernel<D, E, true>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((prefix_fwd_kernel<D, E, false>), grid, block, 0, stream, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   constexpr int RPP = 64 / (D / 4);
