@@ -409,6 +409,7 @@ int run_prefix(const char* name, int dtype, const fa_half_t* q, const fa_half_t*
   a.prows = z.prows;
   a.srows = z.srows;
   a.grid = z.grid;
+  a.most_pieces = z.most_pieces;
   return fa::capi_launch_result(fa::launch_prefix_fwd(a, dtype, static_cast<hipStream_t>(stream)),
                                 name);
 }
@@ -661,8 +662,9 @@ int fa_paged_compact(const int32_t* page_table, int64_t table_stride, const int3
     if (const int rc = check_pointers(name, {free_pages, free_pages_out, sources, targets})) return rc;
   if (const int rc = check_aligned(name, 4, {page_table, free_pages, free_start, page_shares,
                                              table_out, free_pages_out, shares_out, sources, targets,
-                                             used_out, workspace}))
+                                             used_out}))
     return rc;
+  if (const int rc = check_aligned(name, 16, {workspace})) return rc;
   if (table_stride < 0)
     return capi_fail(FA_ERR_BAD_STRIDE, "%s: a negative page table stride", name);
   if (const int rc = check_workspace(name, workspace_bytes, fa::compact_workspace_bytes(pages)))

@@ -244,6 +244,7 @@ struct PrefixArgs {
   int blocks;            // tiles of them
   int prows, srows;      // rows of a prefix's and of a sequence's own slot
   int grid;              // work-groups
+  int most_pieces;       // of long prefixes
 };
 // Where a sequence's own units lie on the line of units, and its group and its place in it.
 struct PrefixSeq {
@@ -267,7 +268,7 @@ inline __host__ __device__ int prefix_tiles(int64_t sequences, int64_t R) {
 struct PrefixSizes {
   int64_t bytes, head_bytes, pslots;
   double units;
-  int blocks, prows, srows, grid;
+  int blocks, prows, srows, grid, most_pieces;
 };
 PrefixSizes prefix_sizes(int64_t B, int64_t G, int64_t Hkv, int64_t R, int64_t D, int64_t keys);
 hipError_t launch_prefix_fwd(const PrefixArgs& a, int dtype, hipStream_t stream);

@@ -50,10 +50,11 @@ __device__ __forceinline__ void block_sum_min(int& sum, int& low, int (*scratch)
 // each other child takes a page from the free list to copy it to. A page whose count falls below
 // zero is held by nobody and returns to the list.
 //
-// Three launches, since a row is read by blocks that write others: fork_count_kernel counts and
+// Two launches and more, since a row is read by blocks that write others: fork_count_kernel counts and
 // puts the new rows aside, fork_finish_kernel writes them; in between lies the order of all atomics.
-// Counts do not depend on it. The released pages are marked in a bitmap and return in ascending
-// order, so that the result does not either. What bounds it is the chain behind each launch.
+// Counts do not depend on it. The released pages return in ascending order, so that the result does
+// not either: one block looks through the counts for them or, in a large cache, through a bitmap
+// that is marked beside the counts. What bounds it is the chain behind each launch.
 
 // A row's pages, and the tokens of the last one if it has begun (0: it is full).
 __device__ __forceinline__ int fork_held(const ForkArgs& a, int len, int* begun) {
@@ -86,7 +87,8 @@ __global__ __launch_bounds__(256) void fork_count_kernel(ForkArgs a) {
     if (n == 1) continue;
     const int p = row[j];
     if (!fork_page(a, p)) continue;
-    if (atomicAdd(a.shares + p, n - 1) + n - 1 < 0) atomicOr(a.bits + (p >> 5), 1u << (p & 31));
+    const bool gone = atomicAdd(a.shares + p, n - 1) + n - 1 < 0;
+    if (gone && a.bits) atomicOr(a.bits + (p >> 5), 1u << (p & 31));
   }
   const int par = a.parents[b];
   if (par < 0 || par >= a.B || par == b) return;
@@ -104,10 +106,71 @@ __device__ __forceinline__ bool fork_copies(const ForkArgs& a, int b, int* last,
   return *begun > 0 && a.keeper[par] != b && fork_page(a, a.rows[(int64_t)b * a.M + *last]);
 }
 
+// The pages that nobody holds any more go back to the list, whose first `copies` pages from `start` on
+// are taken. A block of 1024 threads finds them: in a small cache in the counts, from which it makes a
+// bitmap in LDS with the released pages in front of each of its words; in a large one each thread
+// looks through a run of the call's bitmap of candidates.
+constexpr int kForkPages = 1 << 13;  // of a small cache
+struct ForkFound {
+  unsigned bits[kForkPages / 32];
+  int fronts[kForkPages / 32], sums[16][1];
+};
+__device__ __forceinline__ void fork_release(const ForkArgs& a, int start, int copies, ForkFound& f) {
+  constexpr int W = 16, T = 64 * W, WORDS = kForkPages / 32;
+  static_assert(WORDS <= T, "a word a thread");
+  const int tid = threadIdx.x;
+  int n[1] = {0}, before[1], released[1];
+  if (!a.bits) {
+#pragma unroll
+    for (int i = 0; i < kForkPages / T; ++i) {
+      const int p = T * i + tid;
+      const uint64_t m = __builtin_amdgcn_ballot_w64(p < a.pages && a.shares[p] < 0);
+      if ((tid & 31) == 0) f.bits[p / 32] = (unsigned)(tid & 32 ? m >> 32 : m);
+    }
+    __syncthreads();
+    if (tid < WORDS) n[0] = __popc(f.bits[tid]);
+    block_scan<W>(n, f.sums, before, released);
+    if (tid < WORDS) f.fronts[tid] = before[0];
+    __syncthreads();
+  } else {
+    const int words = (a.pages + 31) / 32, per = (words + T - 1) / T;
+    const int w0 = min(words, tid * per), w1 = min(words, w0 + per);
+    auto each_released = [&](auto&& found) __attribute__((always_inline)) {
+      for (int w = w0; w < w1; ++w)
+        for (unsigned m = a.bits[w]; m != 0; m &= m - 1) {
+          const int p = 32 * w + __builtin_ctz(m);
+          if (a.shares[p] < 0) found(p);
+        }
+    };
+    each_released([&](int) { ++n[0]; });
+    block_scan<W>(n, f.sums, before, released);
+    int at = start + min(copies, a.F - start) - released[0] + before[0];
+    each_released([&](int p) {
+      a.shares[p] = 0;
+      if (at >= 0) a.free_pages[at] = p;
+      ++at;
+    });
+  }
+  const int first = start + min(copies, a.F - start) - released[0];
+  if (tid == 0) a.free_out[0] = max(first, 0);
+  if (a.bits) return;
+#pragma unroll
+  for (int i = 0; i < kForkPages / T; ++i) {
+    const int p = T * i + tid;
+    if (p >= a.pages) break;
+    const unsigned word = f.bits[p / 32];
+    if (!(word >> (p & 31) & 1)) continue;
+    const int k = first + f.fronts[p / 32] + __popc(word & ((1u << (p & 31)) - 1));
+    a.shares[p] = 0;
+    if (k >= 0) a.free_pages[k] = p;
+  }
+}
+
 // Block 0: the copies and the lists. Block 1 + b + B y: part y of row b's columns.
 __global__ __launch_bounds__(1024) void fork_finish_kernel(ForkArgs a) {
   constexpr int W = 16, T = 64 * W;
   __shared__ int sums[2][W][1];
+  __shared__ ForkFound found;
   const int tid = threadIdx.x;
   int last, begun;
   if (blockIdx.x > 0) {
@@ -146,26 +209,75 @@ __global__ __launch_bounds__(1024) void fork_finish_kernel(ForkArgs a) {
     }
     copies += all[0];
   }
-  __syncthreads();  // the list's pages are read; scratch is free
-  // The released pages, a run of the bitmap's words a thread.
-  const int words = (a.pages + 31) / 32, per = (words + T - 1) / T;
-  const int w0 = min(words, tid * per), w1 = min(words, w0 + per);
-  int count[1] = {0}, before[1], released[1];
-  for (int w = w0; w < w1; ++w)
-    for (unsigned m = a.bits[w]; m != 0; m &= m - 1)
-      count[0] += a.shares[32 * w + __builtin_ctz(m)] < 0;
-  block_scan<W>(count, sums[0], before, released);
-  const int first = start + min(copies, a.F - start) - released[0];
-  int at = first + before[0];
-  for (int w = w0; w < w1; ++w)
-    for (unsigned m = a.bits[w]; m != 0; m &= m - 1) {
-      const int p = 32 * w + __builtin_ctz(m);
-      if (a.shares[p] >= 0) continue;
-      a.shares[p] = 0;
-      if (at >= 0) a.free_pages[at] = p;
-      ++at;
-    }
-  if (tid == 0) a.free_out[0] = max(first, 0);
+  __syncthreads();  // the list's pages are read
+  fork_release(a, start, copies, found);
+}
+
+// All of it in one block, where that has few entries to walk over.
+constexpr int kForkSmall = 1 << 13;  // most table entries
+constexpr int kForkRows = 1024;      // and rows, one a thread
+
+__global__ __launch_bounds__(1024) void fork_small_kernel(ForkArgs a) {
+  constexpr int W = 16, T = 64 * W;
+  __shared__ int parent[kForkRows], children[kForkRows], keeper[kForkRows], rows[kForkSmall];
+  __shared__ int held_s[kForkRows], begun_s[kForkRows], sums[W][1];
+  __shared__ ForkFound found;
+  const int tid = threadIdx.x, entries = a.B * a.M;
+  int len = 0;
+  if (tid < a.B) {
+    const int x = a.parents[tid];
+    len = a.lengths[tid];
+    parent[tid] = x >= 0 && x < a.B ? x : -1;
+    held_s[tid] = fork_held(a, len, &begun_s[tid]);
+    children[tid] = 0;
+    keeper[tid] = INT32_MAX;
+  }
+#pragma unroll
+  for (int i = 0; i < kForkSmall / T; ++i) {
+    const int t = T * i + tid, b = t / a.M;
+    if (t < entries) rows[t] = a.table[b * a.table_stride + (t - b * a.M)];
+  }
+  int start = a.free_start ? a.free_start[0] : 0;
+  start = min(max(start, 0), a.F);
+  __syncthreads();
+  const int par = tid < a.B ? parent[tid] : -1;
+  if (par >= 0) {
+    atomicAdd(children + par, 1);
+    atomicMin(keeper + par, par == tid ? -1 : tid);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kForkSmall / T; ++i) {
+    const int t = T * i + tid, b = t / a.M, j = t - b * a.M;
+    if (t >= entries || j >= held_s[b]) continue;
+    const int n = begun_s[b] && j == held_s[b] - 1 ? min(children[b], 1) : children[b];
+    if (n != 1 && fork_page(a, rows[t])) atomicAdd(a.shares + rows[t], n - 1);
+  }
+  // The copies: child tid of par.
+  const int last = par >= 0 ? held_s[par] - 1 : -1;
+  const int source = last >= 0 ? rows[par * a.M + last] : -1;
+  const int kept_by = par >= 0 && keeper[par] != -1 ? keeper[par] : par;
+  const bool copy = par >= 0 && begun_s[par] > 0 && kept_by != tid && fork_page(a, source);
+  int x[1] = {copy}, before[1], copies[1];
+  block_scan<W>(x, sums, before, copies);
+  int target = -1;
+  if (copy && (int64_t)start + before[0] < a.F) target = a.free_pages[start + before[0]];
+  if (tid < a.B) {
+    a.sources[tid] = copy ? source : -1;
+    a.targets[tid] = target;
+    a.tokens[tid] = copy ? begun_s[par] : 0;
+    a.lengths_out[tid] = par >= 0 ? max(a.lengths[par], 0) : 0;
+  }
+#pragma unroll
+  for (int i = 0; i < kForkSmall / T; ++i) {
+    const int t = T * i + tid, b = t / a.M, j = t - b * a.M;
+    if (t >= entries) break;
+    const int p = parent[b];
+    if (p >= 0 && p != b && j < held_s[p]) a.table[b * a.table_stride + j] = rows[p * a.M + j];
+  }
+  __syncthreads();  // the counts are whole, and the copied pages' entries come last
+  if (copy) a.table[tid * a.table_stride + last] = target;
+  fork_release(a, start, copies[0], found);
 }
 
 int64_t fork_workspace_bytes(int64_t B, int64_t M, int64_t pages) {
@@ -179,7 +291,15 @@ hipError_t launch_fork(const ForkArgs& args, void* workspace, hipStream_t stream
   a.bits = reinterpret_cast<unsigned*>(a.keeper + a.B);
   a.rows = reinterpret_cast<int*>(a.bits + words);
   a.parts = std::min((a.M + 1023) / 1024, 16);  // four entries a thread, one
-  hipError_t e = zero_words(a.bits, words, stream);
+  // A few counts a thread are read sooner than the bitmap is cleared by a launch of its own.
+  hipError_t e = hipSuccess;
+  if (a.pages <= kForkPages && a.B <= kForkRows && (int64_t)a.B * a.M <= kForkSmall) {
+    a.bits = nullptr;
+    hipLaunchKernelGGL(fork_small_kernel, dim3(1), dim3(1024), 0, stream, a);
+    return hipGetLastError();
+  }
+  if (a.pages <= kForkPages) a.bits = nullptr;
+  else e = zero_words(a.bits, words, stream);
   if (e != hipSuccess) return e;
   if (a.B > 0) {
     hipLaunchKernelGGL(fork_count_kernel, dim3((unsigned)a.B, (unsigned)a.parts), dim3(256), 0, stream, a);
@@ -193,9 +313,8 @@ hipError_t launch_fork(const ForkArgs& args, void* workspace, hipStream_t stream
 // ---- copy -------------------------------------------------------------------------------
 // Rows 0 .. tokens[i] - 1 of page targets[i] become those of page sources[i], keys and values,
 // in 16-byte pieces: bound by memory. A pair's pieces are numbered along the memory, heads of a
-// row or rows of a head inside, whichever lie closer; a block takes 256 U of them.
-
-template <int U>
+// row or rows of a head inside, whichever lie closer; a thread takes one, past the caches. (More a
+// thread, or through the caches, are slower: 1792 pages of 64 tokens, H8 D128, 0.94 GB in all.)
 __global__ __launch_bounds__(256) void page_copy_kernel(CopyArgs a) {
   const unsigned pair = blockIdx.x / a.blocks;
   const int from = a.sources[pair], to = a.targets[pair];
@@ -203,26 +322,14 @@ __global__ __launch_bounds__(256) void page_copy_kernel(CopyArgs a) {
   const int rows = a.tokens ? min(max(a.tokens[pair], 0), a.S) : a.S;
   const unsigned inner = a.rows_inside ? rows : a.H, outer = a.rows_inside ? a.H : rows;
   const unsigned run = inner * a.chunks;  // pieces that lie together
-  const unsigned all = 2 * run * outer;
-  const unsigned first = (blockIdx.x - pair * a.blocks) * (256 * U) + threadIdx.x;
-  if (first >= all) return;
+  const unsigned t = (blockIdx.x - pair * a.blocks) * 256 + threadIdx.x;
+  if (t >= 2 * run * outer) return;
+  const unsigned r = t / run, x = t - r * run, side = r >= outer, y = a.together ? 0 : x / a.chunks;
   const int64_t in = a.rows_inside ? a.ks[2] : a.ks[1], out = a.rows_inside ? a.ks[1] : a.ks[2];
-  u32x4 v[U];
-  half_t* dst[U];
-#pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const unsigned t = first + 256 * i;
-    if (t >= all) continue;
-    const unsigned r = t / run, side = r >= outer, o = side ? r - outer : r, x = t - r * run;
-    const unsigned y = a.together ? 0 : x / a.chunks;
-    const int64_t off = o * out + y * in + 8 * (int64_t)(x - y * a.chunks);
-    half_t* const base = (side ? a.v : a.k) + off;
-    dst[i] = base + to * a.ks[0];
-    v[i] = *reinterpret_cast<const u32x4*>(base + from * a.ks[0]);
-  }
-#pragma unroll
-  for (int i = 0; i < U; ++i)
-    if (first + 256 * i < all) __builtin_nontemporal_store(v[i], reinterpret_cast<u32x4*>(dst[i]));
+  half_t* const base = (side ? a.v : a.k) + (side ? r - outer : r) * out + y * in +
+                       8 * (int64_t)(x - y * a.chunks);
+  const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(base + from * a.ks[0]));
+  __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(base + to * a.ks[0]));
 }
 
 hipError_t launch_page_copy(const CopyArgs& args, hipStream_t stream) {
@@ -230,9 +337,7 @@ hipError_t launch_page_copy(const CopyArgs& args, hipStream_t stream) {
   a.rows_inside = a.ks[2] <= a.ks[1];
   a.together = (a.rows_inside ? a.ks[2] : a.ks[1]) == 8 * a.chunks;
   const int64_t pieces = 2 * (int64_t)a.H * a.S * a.chunks;
-  const bool small = a.n * pieces <= 256 * 2048;
-  const int64_t each = small ? 256 : 256 * 8;
-  a.blocks = (unsigned)((pieces + each - 1) / each);
+  a.blocks = (unsigned)((pieces + 255) / 256);
   const int64_t most = kMostBlocks / a.blocks;
   for (int64_t i = 0; i < args.n; i += most) {  // pairs past one grid's blocks: another launch
     a.n = std::min(most, args.n - i);
@@ -240,8 +345,7 @@ hipError_t launch_page_copy(const CopyArgs& args, hipStream_t stream) {
     a.targets = args.targets + i;
     if (args.tokens) a.tokens = args.tokens + i;
     const dim3 grid((unsigned)(a.n * a.blocks)), block(256);
-    if (small) hipLaunchKernelGGL(page_copy_kernel<1>, grid, block, 0, stream, a);
-    else hipLaunchKernelGGL(page_copy_kernel<8>, grid, block, 0, stream, a);
+    hipLaunchKernelGGL(page_copy_kernel, grid, block, 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -252,7 +356,8 @@ hipError_t launch_page_copy(const CopyArgs& args, hipStream_t stream) {
 // Pages that the list does not name as free are held: with `used` of them, the k-th held page from
 // place `used` on moves to the k-th free page in front of it. compact_mark_kernel marks the free
 // pages in a bitmap, compact_rank_kernel counts along it (every block for itself, over the words in
-// front of its own), compact_apply_kernel renumbers the table, the counts and the list.
+// front of its own), compact_apply_kernel renumbers the table, the counts and the list;
+// compact_small_kernel does it all for a small cache.
 
 __global__ __launch_bounds__(256) void compact_mark_kernel(CompactArgs a) {
   const int start = a.free_start ? min(max(a.free_start[0], 0), a.F) : 0;
@@ -267,41 +372,62 @@ __device__ __forceinline__ unsigned bits_before(int w, int p) {
   return p >= 32 * w + 32 ? ~0u : p <= 32 * w ? 0u : (1u << (p - 32 * w)) - 1;
 }
 
-// Block i: words 256 i to 256 i + 255, one a thread.
+// Where page p >= used or free moves, or comes from: its place among the moves, given the free pages
+// in front of its word, its word of the bitmap and the moves.
+__device__ __forceinline__ int compact_place(int p, int free_before, unsigned word, int used, int moves) {
+  const int free = free_before + __popc(word & ((1u << (p & 31)) - 1));
+  return p < used ? free : p - free - (used - moves);
+}
+
+// Block i: pages 1024 i to 1024 i + 1023, four a thread.
 __global__ __launch_bounds__(256) void compact_rank_kernel(CompactArgs a) {
-  __shared__ int scratch[2][4], sums[4][1];
+  __shared__ int scratch[2][4], fronts[32];
   const int tid = threadIdx.x, words = (a.pages + 31) / 32;
-  const int w0 = blockIdx.x * 256;
+  const int w0 = blockIdx.x * 32;
   int all = 0, front = 0, moves = 0, low = 0;
-  for (int w = tid; w < words; w += 256) {
-    const int n = __popc(a.bits[w]);
+  // (the words behind the last page's, up to a multiple of 4, are cleared as well)
+  const u32x4* const bits4 = reinterpret_cast<const u32x4*>(a.bits);
+#pragma unroll 4
+  for (int w = 4 * tid; w < words; w += 1024) {
+    const u32x4 m = bits4[w / 4];
+    const int n = __popc(m[0]) + __popc(m[1]) + __popc(m[2]) + __popc(m[3]);
     all += n;
-    if (w < w0) front += n;
+    if (w < w0) front += n;  // w0 is a multiple of 4
   }
   block_sum_min(all, low, scratch);
   block_sum_min(front, low, scratch);
   const int used = a.pages - all;
-  for (int w = tid; w < words && 32 * w < used; w += 256) moves += __popc(a.bits[w] & bits_before(w, used));
+#pragma unroll 4
+  for (int w = 4 * tid; w < words && 32 * w < used; w += 1024) {
+    const u32x4 m = bits4[w / 4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) moves += __popc(m[i] & bits_before(w + i, used));
+  }
   block_sum_min(moves, low, scratch);  // free pages in front of `used`, held ones behind it
   if (blockIdx.x == 0 && tid == 0) {
     a.used[0] = used;
     a.counts[0] = moves;
   }
-  const int w = w0 + tid;
-  const unsigned free = w < words ? a.bits[w] : 0u;
-  int x[1] = {(int)__popc(free)}, before[1], total[1];
-  block_scan<4>(x, sums, before, total);
-  if (w >= words) return;
-  const int free_before = front + before[0];
-  const unsigned in = bits_before(w, used);
-  int k = free_before;
-  for (unsigned m = free & in; m != 0; m &= m - 1) a.targets[k++] = 32 * w + __builtin_ctz(m);
-  for (unsigned m = ~free & ~in & bits_before(w, a.pages); m != 0; m &= m - 1) {
-    const int bit = __builtin_ctz(m), p = 32 * w + bit;
-    // held pages in front of p, less those that stay
-    k = p - free_before - __popc(free & ((1u << bit) - 1)) - (used - moves);
-    a.sources[k] = p;
-    a.place[p] = k;
+  if (tid < 64) {
+    const int n = tid < 32 && w0 + tid < words ? __popc(a.bits[w0 + tid]) : 0;
+    const int incl = wave_scan(n);
+    if (tid < 32) fronts[tid] = front + incl - n;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int p = blockIdx.x * 1024 + 256 * i + tid;
+    if (p >= a.pages) break;
+    const unsigned word = a.bits[p >> 5];
+    const bool free = word >> (p & 31) & 1;
+    if (free != (p < used)) continue;
+    const int k = compact_place(p, fronts[(p >> 5) - w0], word, used, moves);
+    if (free) {
+      a.targets[k] = p;
+    } else {
+      a.sources[k] = p;
+      a.place[p] = k;
+    }
   }
 }
 
@@ -335,13 +461,72 @@ __global__ __launch_bounds__(256) void compact_apply_kernel(CompactArgs a) {
   }
 }
 
-int64_t compact_workspace_bytes(int64_t pages) { return 4 * (1 + (pages + 31) / 32 + pages); }
+// All of it in one block, the bitmap and the free pages in front of each of its words in LDS.
+constexpr int kCompactSmall = 1 << 14;  // most pages, and table entries, pages and list entries
+
+__global__ __launch_bounds__(1024) void compact_small_kernel(CompactArgs a) {
+  constexpr int W = 16, T = 64 * W, WORDS = kCompactSmall / 32;
+  static_assert(WORDS <= T, "a word a thread");
+  __shared__ unsigned bits[WORDS];
+  __shared__ int fronts[WORDS], sums[2][W][1];
+  const int tid = threadIdx.x;
+  if (tid < WORDS) bits[tid] = 0;
+  const int start = a.free_start ? min(max(a.free_start[0], 0), a.F) : 0;
+  __syncthreads();
+  for (int i = start + tid; i < a.F; i += T) {
+    const int p = a.free_pages[i];
+    if (p >= 0 && p < a.pages) atomicOr(bits + (p >> 5), 1u << (p & 31));
+  }
+  __syncthreads();
+  const unsigned mine = tid < WORDS ? bits[tid] : 0u;
+  int x[1] = {(int)__popc(mine)}, before[1], all[1];
+  block_scan<W>(x, sums[0], before, all);
+  if (tid < WORDS) fronts[tid] = before[0];
+  const int used = a.pages - all[0];
+  x[0] = __popc(mine & bits_before(tid, used));
+  block_scan<W>(x, sums[1], before, all);
+  const int moves = all[0];
+  if (tid == 0) a.used[0] = used;
+  auto is_free = [&](int p) __attribute__((always_inline)) { return bits[p >> 5] >> (p & 31) & 1; };
+  auto place = [&](int p) __attribute__((always_inline)) {
+    return compact_place(p, fronts[p >> 5], bits[p >> 5], used, moves);
+  };
+  for (int p = tid; p < a.pages; p += T) {
+    const bool free = is_free(p);
+    if (free && p < used) a.targets[place(p)] = p;
+    else if (!free && p >= used) a.sources[place(p)] = p;
+  }
+  __syncthreads();
+  auto moved = [&](int p) __attribute__((always_inline)) { return p >= used && p < a.pages && !is_free(p); };
+  for (int t = tid; t < a.B * a.M; t += T) {
+    const int b = t / a.M, p = a.table[b * a.table_stride + (t - b * a.M)];
+    a.table_out[t] = moved(p) ? a.targets[place(p)] : p;
+  }
+  for (int p = tid; p < a.pages; p += T) {
+    if (p >= used) a.shares_out[p] = 0;
+    if (moved(p)) a.shares_out[a.targets[place(p)]] = a.shares[p];
+    else if (p < used && !is_free(p)) a.shares_out[p] = a.shares[p];
+  }
+  for (int i = tid; i < a.F; i += T) {
+    const int p = used + (i - start);
+    a.free_pages_out[i] = i < start ? a.free_pages[i] : p < a.pages ? p : -1;
+    if (i >= moves) a.sources[i] = a.targets[i] = -1;
+  }
+}
+
+static int64_t compact_words(int64_t pages) { return (pages + 127) / 128 * 4; }
+int64_t compact_workspace_bytes(int64_t pages) { return 4 * (4 + compact_words(pages) + pages); }
 
 hipError_t launch_compact(const CompactArgs& args, void* workspace, hipStream_t stream) {
   CompactArgs a = args;
-  const int64_t words = ((int64_t)a.pages + 31) / 32;
+  const int64_t words = compact_words(a.pages);
+  const int64_t items = (int64_t)a.B * a.M + a.pages + a.F;
+  if (items <= kCompactSmall) {
+    hipLaunchKernelGGL(compact_small_kernel, dim3(1), dim3(1024), 0, stream, a);
+    return hipGetLastError();
+  }
   a.counts = static_cast<int*>(workspace);
-  a.bits = reinterpret_cast<unsigned*>(a.counts + 1);
+  a.bits = reinterpret_cast<unsigned*>(a.counts + 4);
   a.place = reinterpret_cast<int*>(a.bits + words);
   hipError_t e = zero_words(a.bits, words, stream);
   if (e != hipSuccess) return e;
@@ -351,10 +536,9 @@ hipError_t launch_compact(const CompactArgs& args, void* workspace, hipStream_t 
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(compact_rank_kernel, dim3((unsigned)((words + 255) / 256)), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(compact_rank_kernel, dim3((unsigned)((words + 31) / 32)), dim3(256), 0, stream, a);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int64_t items = (int64_t)a.B * a.M + a.pages + a.F;
   const int64_t blocks = std::min<int64_t>((items + 255) / 256, 4096);
   hipLaunchKernelGGL(compact_apply_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
   return hipGetLastError();

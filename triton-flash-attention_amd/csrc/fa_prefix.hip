@@ -108,10 +108,10 @@ __device__ __forceinline__ PrefixGroup* prefix_groups(const PrefixArgs& a) {
   return reinterpret_cast<PrefixGroup*>(prefix_seqs(a) + a.B);
 }
 
-// Pieces that a triple of `units` units is cut into where a work-group takes L; 0: it is on the line.
-__device__ __forceinline__ int prefix_cuts(int units, int L, bool cut) {
-  const int each = L - kPrefixLead;
-  return cut && each >= kPrefixLead && units >= 2 * each ? (units + each - 1) / each : 0;
+// Whether a prefix of `units` units is cut into pieces instead of lying on the line whose stretches
+// are of L.
+__device__ __forceinline__ bool prefix_long(int units, int L) {
+  return L >= 2 * kPrefixLead && units >= 2 * (L - kPrefixLead);
 }
 
 // A wave's stretch of the sequences' own keys, where a work-group's is L.
@@ -123,7 +123,7 @@ __device__ __forceinline__ PrefixLine prefix_find(const PrefixArgs& a, int* lds,
   constexpr int W = kPrefixWaves, T = 64 * W;
   int(*const found)[12] = reinterpret_cast<int(*)[12]>(lds);    // [W]
   int* const wrongs = lds + 48;                                // [W]
-  int(*const sums)[4] = reinterpret_cast<int(*)[4]>(lds + 52);  // [2 W], used in turn
+  int(*const sums)[1] = reinterpret_cast<int(*)[1]>(lds + 52);  // [W]
   int* const kept_starts = lds + 96;
   int* const kept_prefix = kept_starts + kPrefixKeptGroups;
   int* const kept_lengths = kept_prefix + kPrefixKeptGroups;
@@ -170,49 +170,76 @@ __device__ __forceinline__ PrefixLine prefix_find(const PrefixArgs& a, int* lds,
   };
   auto front_at = [&](int g) __attribute__((always_inline)) { return g >= 0 && g < G ? front_of(g) : 0; };
 
-  // The thread's groups and sequences, and their parts of the work.
-  const int per_g = (G + T - 1) / T, g0 = min(G, tid * per_g), g1 = min(G, g0 + per_g);
+  // A lane's groups, alike in every wave, and a thread's sequences. (One of each is the rule: what is
+  // known of the first is kept.)
+  const int lane = tid & 63;
+  const int per_g = (G + 63) / 64, g0 = min(G, lane * per_g), g1 = min(G, g0 + per_g);
   const int per_b = (a.B + T - 1) / T, b0 = min(a.B, tid * per_b), b1 = min(a.B, b0 + per_b);
   const int HB = a.Hkv * a.blocks, lead = WAVES ? kOwnLead : kPrefixLead;
-  int own = 0;
+  const int g0_keys = g0 < g1 ? front_of(g0) : 0, g0_triples = g0 < g1 ? triples_of(g0) : 0;
+  auto keys_in = [&](int g) __attribute__((always_inline)) { return g == g0 ? g0_keys : front_of(g); };
+  auto triples_in = [&](int g) __attribute__((always_inline)) { return g == g0 ? g0_triples : triples_of(g); };
+  const int b0_group = G > 0 && b0 < b1 ? group_at(b0) : -1;
+  const int b0_front = front_at(b0_group), b0_end = b0 < b1 ? length(b0) : 0;
+  auto group_in = [&](int b) __attribute__((always_inline)) {
+    return b == b0 ? b0_group : G > 0 ? group_at(b) : -1;
+  };
+  auto front_in = [&](int b, int g) __attribute__((always_inline)) { return b == b0 ? b0_front : front_at(g); };
+  auto end_in = [&](int b) __attribute__((always_inline)) { return b == b0 ? b0_end : length(b); };
+  // Units of sequences' own keys and of the prefixes, on the line.
+  int own[1] = {0}, own_before[1], own_all[1];
   for (int b = b0; b < b1; ++b)
-    own += on_line(key_units(G > 0 ? front_at(group_at(b)) : 0, length(b)), lead) * HB;
-  // Sums: long prefixes' pieces; units and triples of the others; units of sequences' own keys.
+    own[0] += on_line(key_units(front_in(b, group_in(b)), end_in(b)), lead) * HB;
+  block_scan<W>(own, sums, own_before, own_all);
+  own_all[0] = uniform(own_all[0]);
+  // Of the lane's groups: pieces of the long prefixes; units and triples of the others on the line;
+  // units of the long ones. And the sums of the lanes before, and all.
   int x[4], before[4], all[4];
-  bool cut = true;
-  int L = 0;
-  for (int round = 0;; ++round) {
-    x[0] = x[1] = x[2] = 0;
-    x[3] = own;
+  auto sum = [&](int i) __attribute__((always_inline)) {
+    const int incl = wave_scan(x[i]);
+    before[i] = incl - x[i];
+    all[i] = __builtin_amdgcn_readlane(incl, 63);
+  };
+  x[1] = 0;
+  for (int g = g0; g < g1; ++g) x[1] += on_line(key_units(0, keys_in(g)), kPrefixLead) * triples_in(g);
+  sum(1);
+  // (The line's two parts end with a stretch of their own each.)
+  const int room = a.grid - 2;
+  const int L = max((all[1] + own_all[0] + room - 1) / room, kPrefixStretch);
+  // Long prefixes are cut by the work-groups that the line leaves: of all[3] units in all, a triple
+  // of u into the whole part of u / all[3] of those. Where the grid would not hold the pieces, they
+  // stay on the line.
+  bool cut = all[1] > 0;
+  int budget = 0;
+  auto cuts_of = [&](int u) __attribute__((always_inline)) {
+    return cut && prefix_long(u, L) ? max(1, (int)((double)u * budget / all[3])) : 0;
+  };
+  x[0] = x[2] = x[3] = 0;
+  sum(0);
+  sum(2);
+  while (all[1] > 0) {
+    x[0] = x[1] = x[2] = x[3] = 0;
     for (int g = g0; g < g1; ++g) {
-      const int u = key_units(0, front_of(g)), t = u > 0 ? triples_of(g) : 0;
-      const int k = prefix_cuts(u, L, cut);
-      if (k > 0) {
-        x[0] += t * k;
+      const int u = key_units(0, keys_in(g)), t = u > 0 ? triples_in(g) : 0;
+      if (cut && prefix_long(u, L)) {
+        x[3] += u * t;
       } else {
         x[1] += on_line(u, kPrefixLead) * t;
         x[2] += t;
       }
     }
-    block_scan<W>(x, sums + W * (round & 1), before, all);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) all[i] = uniform(all[i]);
-    if (round == 0) {  // all of it (L = 0 cuts nothing)
-      L = max((all[1] + all[3] + a.grid - 1) / a.grid, kPrefixStretch);
-      if (all[1] == 0) break;
-      continue;
-    }
-    // Work-groups that it takes: a longer stretch, until the grid holds them.
+    sum(1);
+    sum(2);
+    sum(3);
+    if (all[3] == 0) break;
     const int each = WAVES ? W * own_stretch(L) : L;
-    const int need = (all[0] + 7) / 8 * 8 + (WAVES ? (all[1] + L - 1) / L + (all[3] + each - 1) / each
-                                                   : (all[1] + all[3] + L - 1) / L);
-    if (need <= a.grid) break;
-    if (round < 10) {
-      L += max(max(1, L / 32), (int)((int64_t)L * (need - a.grid) / a.grid));
-    } else {
-      cut = false;
-      L *= 2;
-    }
+    const int rest = WAVES ? (all[1] + L - 1) / L + (own_all[0] + each - 1) / each
+                           : (all[1] + own_all[0] + L - 1) / L;
+    budget = min(a.grid - rest, a.most_pieces) & ~7;
+    for (int g = g0; g < g1; ++g) x[0] += cuts_of(key_units(0, keys_in(g))) * triples_in(g);
+    sum(0);
+    if ((all[0] + 7) / 8 * 8 <= a.grid - rest) break;
+    cut = false;
   }
   line.stretch = L;
   line.pieces = all[0];
@@ -224,26 +251,26 @@ __device__ __forceinline__ PrefixLine prefix_find(const PrefixArgs& a, int* lds,
   line.s = piece ? xcd * each + i : (i - each) * 8 + xcd;
   const int stretches = WAVES ? (all[1] + L - 1) / L : 0;
   line.own = !piece && WAVES && line.s >= stretches;
-  int mine = L, end = WAVES ? all[1] : all[1] + all[3];  // of the line
+  int mine = L, end = WAVES ? all[1] : all[1] + own_all[0];  // of the line
   if (line.own) {
     line.s = (line.s - stretches) * W + (tid >> 6);
     mine = own_stretch(L);
-    end = all[3];
+    end = own_all[0];
   }
   int64_t from = (int64_t)line.s * mine;
   line.left = piece ? (line.s < all[0] ? 1 : 0) : from < end ? (int)min((int64_t)mine, end - from) : 0;
   if (piece) {
-    if (line.s >= before[0] && line.s < before[0] + x[0]) {
+    if (tid < 64 && line.s >= before[0] && line.s < before[0] + x[0]) {
       int at = line.s - before[0];
       for (int g = g0; g < g1; ++g) {
-        const int keys = front_of(g), u = key_units(0, keys), k = prefix_cuts(u, L, true);
-        const int n = k > 0 ? triples_of(g) * k : 0;
+        const int keys = keys_in(g), u = key_units(0, keys), k = cuts_of(u);
+        const int n = triples_in(g) * k;
         if (at >= n) {
           at -= n;
           continue;
         }
         // piece p of head kvh, tile t: place (kvh k + p) tiles + t
-        const int tiles = triples_of(g) / a.Hkv, t = at % tiles, p = at / tiles % k;
+        const int tiles = triples_in(g) / a.Hkv, t = at % tiles, p = at / tiles % k;
         int* const f = found[0];
         f[0] = 2;
         f[1] = g;
@@ -258,11 +285,11 @@ __device__ __forceinline__ PrefixLine prefix_find(const PrefixArgs& a, int* lds,
       }
     }
   } else {
-    if (!line.own && from >= before[1] && from < (int64_t)before[1] + x[1]) {
+    if (!line.own && tid < 64 && from >= before[1] && from < (int64_t)before[1] + x[1]) {
       int at = (int)(from - before[1]), t = before[2];
       for (int g = g0; g < g1; ++g) {
-        const int keys = front_of(g), u = key_units(0, keys);
-        const int n = u > 0 && prefix_cuts(u, L, cut) == 0 ? triples_of(g) : 0;
+        const int keys = keys_in(g), u = key_units(0, keys);
+        const int n = u > 0 && !(cut && prefix_long(u, L)) ? triples_in(g) : 0;
         const int len = on_line(u, kPrefixLead);
         if (at < len * n) {
           int* const f = found[0];
@@ -286,10 +313,10 @@ __device__ __forceinline__ PrefixLine prefix_find(const PrefixArgs& a, int* lds,
       for (int w = 0; w < (WAVES ? W : 1); ++w) {
         if (WAVES) from = (int64_t)((line.s & ~(W - 1)) + w) * mine;
         else from = (int64_t)line.s * mine - all[1];
-        if (from < before[3] || from >= (int64_t)before[3] + own) continue;
-        int at = (int)(from - before[3]);
+        if (from < own_before[0] || from >= (int64_t)own_before[0] + own[0]) continue;
+        int at = (int)(from - own_before[0]);
         for (int b = b0; b < b1; ++b) {
-          const int g = G > 0 ? group_at(b) : -1, keys = front_at(g), stop = length(b);
+          const int g = group_in(b), keys = front_in(b, g), stop = end_in(b);
           const int len = on_line(key_units(keys, stop), lead);
           if (at < len * HB) {
             int* const f = found[w];
@@ -317,17 +344,21 @@ __device__ __forceinline__ PrefixLine prefix_find(const PrefixArgs& a, int* lds,
       a.ws[2] = line.bad;
       a.ws[3] = all[0];
     }
-    int base = (WAVES ? 0 : all[1]) + before[3];
+    int base = (WAVES ? 0 : all[1]) + own_before[0];
     for (int b = b0; b < b1; ++b) {
-      const int g = G > 0 ? group_at(b) : -1, u = key_units(front_at(g), length(b));
+      const int g = group_in(b), u = key_units(front_in(b, g), end_in(b));
       const bool in = g >= 0 && g < G;
-      prefix_seqs(a)[b] = {base, u, in ? g : -1, in ? b - start(g) : 0};
+      PrefixSeq* const q = prefix_seqs(a) + b;
+      q->own_base = base;
+      q->own_units = u;
+      q->group = in ? g : -1;
+      q->member = in ? b - start(g) : 0;
       base += on_line(u, lead) * HB;
     }
     int pieces = before[0], t = before[2];
     base = before[1];
-    for (int g = g0; g < g1; ++g) {
-      const int u = key_units(0, front_of(g)), n = triples_of(g), k = prefix_cuts(u, L, cut);
+    for (int g = tid < 64 ? g0 : g1; g < g1; ++g) {
+      const int u = key_units(0, keys_in(g)), n = triples_in(g), k = cuts_of(u);
       prefix_groups(a)[g] = {k > 0 ? pieces : base, u, t, n / a.Hkv, k, 0, 0, 0};
       if (k > 0) {
         pieces += n * k;
@@ -429,6 +460,13 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const PrefixJo
   const int ql = lane & 31;
   const int g = lane >> 5;
 
+  // Pages of half units, one a lane, clamped to the last key's, so that the load needs no branch.
+  auto half_key = [&](int i) __attribute__((always_inline)) { return job.k_lo + 32 * i + 16 * lane; };
+  auto fetch = [&](int i) __attribute__((always_inline)) {
+    return job.table[min(half_key(i), job.k_hi - 1) / a.S];
+  };
+  int next_page = fetch(0);
+
   // The lane's row, the keys that it sees, and its query.
   const int r = job.row0 + 32 * wave + ql;
   const bool real = r < job.rows;
@@ -436,7 +474,7 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const PrefixJo
   const int member = r / a.R, rr = r - member * a.R;
   const int h = rr / a.N, n = rr - h * a.N;
   const int b = job.b0 + member;
-  int see = INT32_MAX, len = 0;
+  int see = INT32_MAX;
   half8 qf[NQ];
   {
     const half_t* q = a.q + b * a.qs[0] + (int64_t)(job.kvh * a.group + h) * a.qs[1] + n * a.qs[2];
@@ -446,10 +484,7 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const PrefixJo
       if (real && 16 * kk + 8 * g < a.d) v = *reinterpret_cast<const u32x4*>(q + 16 * kk + 8 * g);
       qf[kk] = __builtin_bit_cast(half8, v);
     }
-    if (real) {
-      len = a.lengths[b];
-      see = min(fitting(a, len) - a.N + n + 1, job.k_hi);
-    }
+    if (real) see = min(fitting(a, a.lengths[b]) - a.N + n + 1, job.k_hi);
   }
   // Units that end below this need no mask.
   int all_see = see;
@@ -476,14 +511,8 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const PrefixJo
   }
 
   // Where the half units from unit iu & ~31 on lie, one a lane: the byte offset of the first of
-  // their rows that exist, and the bytes from it to the end of the last; and the next 32 units'
-  // pages (clamped to the last key's, so that the load needs no branch and none waits for it).
+  // their rows that exist, and the bytes from it to the end of the last.
   int bad_key = INT32_MAX;  // first key of the first page that does not exist
-  auto half_key = [&](int i) __attribute__((always_inline)) { return job.k_lo + 32 * i + 16 * lane; };
-  auto fetch = [&](int i) __attribute__((always_inline)) {
-    return job.table[min(half_key(i), job.k_hi - 1) / a.S];
-  };
-  int next_page = fetch(0);
   int64_t off = 0;
   uint32_t rows_bytes = 0;
   int iu = 0;  // next unit to ask for
@@ -719,7 +748,8 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const PrefixJo
 #pragma unroll
   for (int i = 32; i > 0; i >>= 1) bad_key = min(bad_key, __shfl_xor(bad_key, i, 64));
   float lt = halves_sum(l);
-  if (len > bad_key) lt = __builtin_nanf("");  // the row's sequence needs a page that does not exist
+  // A row whose sequence needs a page that does not exist.
+  if (bad_key != INT32_MAX && real && a.lengths[b] > bad_key) lt = __builtin_nanf("");
   if (real) {
     const float inv = lt == 0.f ? 0.f : 1.0f / lt;
     const int row = 32 * wave + ql;
@@ -1014,7 +1044,7 @@ __global__ __launch_bounds__(64 * kPrefixWaves, PrefixRing<D>::WGS) void prefix_
         at.n = end - at.b0;
         at.k_end = uniform(prefix_keys(a, at.at, at.b0, end));
         units = key_units(0, at.k_end);
-        if (prefix_cuts(units, line.stretch, line.pieces > 0) > 0) units = 0;
+        if (line.pieces > 0 && prefix_long(units, line.stretch)) units = 0;
       }
       if (units > 0) continue;
       if (WAVES) return;
@@ -1028,33 +1058,37 @@ __global__ __launch_bounds__(64 * kPrefixWaves, PrefixRing<D>::WGS) void prefix_
 }
 
 // Joins the pieces of each row: those of its group's prefix, then those of its own keys. A lane
-// holds four columns of a row, a wave 64 / (D / 4) rows, one after the other in the output; a
-// block's four waves take every fourth piece of the same rows and merge through LDS, in a fixed
-// order. A piece weighs exp2 of its log-sum-exp against the others'.
-template <int D, class E>
-__global__ __launch_bounds__(64 * kPrefixWaves) void prefix_join_kernel(PrefixArgs a) {
-  constexpr int W = kPrefixWaves;
+// holds four columns of a row, a wave 64 / (D / 4) rows, one after the other in the output; SPLIT of a
+// block's waves take every SPLIT-th piece of the same rows and merge through LDS, in a fixed order.
+// A piece weighs exp2 of its log-sum-exp against the others'.
+template <int D, class E, int SPLIT>
+__global__ __launch_bounds__(64 * (SPLIT < 4 ? 4 : SPLIT)) void prefix_join_kernel(PrefixArgs a) {
+  constexpr int W = SPLIT < 4 ? 4 : SPLIT;  // waves
   constexpr int COLS = D / 4, RPP = 64 / COLS;
-  constexpr int AHEAD = 4;
+  constexpr int AHEAD = SPLIT == 16 ? 4 : 8;
   // The weight of the largest piece: those of 1024 pieces sum to 1/2, so that sums of values near
   // 2^128 stay in float32.
   constexpr float kWeight = 0x1p-11f;
-  __shared__ __attribute__((aligned(16))) float acc_s[W][64][4];
+  __shared__ __attribute__((aligned(16))) float acc_s[SPLIT > 1 ? W : 1][64][4];
   __shared__ float m_s[W][64], l_s[W][64];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int64_t row = (int64_t)blockIdx.x * RPP + lane / COLS;  // of the output [B, Hq, N]
+  const int part = wave % SPLIT;
+  const unsigned row = (blockIdx.x * (W / SPLIT) + wave / SPLIT) * RPP + lane / COLS;  // of [B, Hq, N]
   const int col = 4 * (lane % COLS);
-  const int64_t seq_rows = (int64_t)a.Hkv * a.R;
+  const unsigned seq_rows = a.Hkv * a.R;
   const bool real = row < a.B * seq_rows;
-  const int64_t rr = real ? row : 0;
-  const int b = (int)(rr / seq_rows), in_seq = (int)(rr - b * seq_rows);
+  const unsigned rr = real ? row : 0;
+  const int b = rr / seq_rows, in_seq = rr - b * seq_rows;
   const int kvh = in_seq / a.R, r = in_seq - kvh * a.R;
   const int stretch = a.ws[0], own_stretch = a.ws[1], cut = a.ws[3];
   const bool bad = a.ws[2] != 0;
   const int len = a.lengths[b];
   const PrefixSeq q = prefix_seqs(a)[b];
+  // (most batches have one group: it is asked for beside the sequence)
   PrefixGroup grp = {0, 0, 0, 1, 0, 0, 0, 0};
-  if (q.group >= 0) grp = prefix_groups(a)[q.group];
+  if (a.G > 0) grp = prefix_groups(a)[0];
+  if (q.group > 0) grp = prefix_groups(a)[q.group];
+  if (q.group < 0) grp = {0, 0, 0, 1, 0, 0, 0, 0};
 
   // Pieces of a triple on the line whose part of it begins at `base`: the first one's stretch, and
   // how many there are.
@@ -1101,10 +1135,10 @@ __global__ __launch_bounds__(64 * kPrefixWaves) void prefix_join_kernel(PrefixAr
   };
   float m = -INFINITY, l = 0.f;
   float4v acc = {0.f, 0.f, 0.f, 0.f};
-  for (int i0 = wave; i0 < count; i0 += W * AHEAD) {
+  for (int i0 = part; i0 < count; i0 += SPLIT * AHEAD) {
     Piece p[AHEAD];
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) p[i] = load(i0 + W * i);
+    for (int i = 0; i < AHEAD; ++i) p[i] = load(i0 + SPLIT * i);
     float mx = m;
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) mx = __builtin_fmaxf(mx, p[i].lse);
@@ -1120,28 +1154,33 @@ __global__ __launch_bounds__(64 * kPrefixWaves) void prefix_join_kernel(PrefixAr
     }
     m = mx;
   }
-  *reinterpret_cast<float4v*>(acc_s[wave][lane]) = acc;
-  m_s[wave][lane] = m;
-  l_s[wave][lane] = l;
-  __syncthreads();
-  if (wave != 0 || !real || col >= a.d) return;
-  float mx = -INFINITY;
+  float lt = l;
+  float4v v = acc;
+  if constexpr (SPLIT > 1) {
+    *reinterpret_cast<float4v*>(acc_s[wave][lane]) = acc;
+    m_s[wave][lane] = m;
+    l_s[wave][lane] = l;
+    __syncthreads();
+    if (part != 0) return;
+    float mx = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < W; ++i) mx = __builtin_fmaxf(mx, m_s[i][lane]);
-  float lt = 0.f;
-  float4v v = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < SPLIT; ++i) mx = __builtin_fmaxf(mx, m_s[wave + i][lane]);
+    lt = 0.f;
+    v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < W; ++i) {
-    const float f = m_s[i][lane] == -INFINITY ? 0.f : exp2_fast(m_s[i][lane] - mx);
-    lt += f * l_s[i][lane];
-    v += *reinterpret_cast<const float4v*>(acc_s[i][lane]) * f;
+    for (int i = 0; i < SPLIT; ++i) {
+      const float f = m_s[wave + i][lane] == -INFINITY ? 0.f : exp2_fast(m_s[wave + i][lane] - mx);
+      lt += f * l_s[wave + i][lane];
+      v += *reinterpret_cast<const float4v*>(acc_s[wave + i][lane]) * f;
+    }
   }
+  if (!real || col >= a.d) return;
   v *= lt == 0.f ? 0.f : 1.0f / lt;  // a row that saw no key is 0
   if (bad || len < 0 || len > a.M * a.S) {
     const float nan = __builtin_nanf("");
     v = {nan, nan, nan, nan};
   }
-  *reinterpret_cast<u32x2*>(a.o + row * a.d + col) = pack4<E>(v[0], v[1], v[2], v[3]);
+  *reinterpret_cast<u32x2*>(a.o + (int64_t)row * a.d + col) = pack4<E>(v[0], v[1], v[2], v[3]);
 }
 
 static int prefix_width(int64_t D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
@@ -1160,12 +1199,26 @@ PrefixSizes prefix_sizes(int64_t B, int64_t G, int64_t Hkv, int64_t R, int64_t D
   // Work-groups that the chip holds at once, at most one for each four units that the tables could
   // hold; as many on each XCD.
   z.grid = (int)std::min((double)most, std::ceil(z.units / kPrefixStretch));
-  z.grid = (z.grid + 7) / 8 * 8;
+  z.grid = std::max((z.grid + 7) / 8 * 8, 16);
+  // Where all rows fit one tile memory bounds a prefix, and a piece's partial is worth four units of
+  // it: no more pieces than it takes to keep the memory busy.
+  z.most_pieces = B * R <= kPrefixTile ? std::min(z.grid, 256) : z.grid;
   z.pslots = triples > 0 ? z.grid + triples : 0;
   z.head_bytes = (64 + B * (int64_t)sizeof(PrefixSeq) + G * (int64_t)sizeof(PrefixGroup) + 63) / 64 * 64;
   const int64_t rows = z.pslots * z.prows + (kPrefixWaves * z.grid + own) * z.srows;
   z.bytes = z.head_bytes + rows * (prefix_width(D) + 4) * 4;
   return z;
+}
+
+// Few rows have many pieces and are joined by more waves each; with many rows the waves are enough.
+template <int D, class E, int SPLIT>
+hipError_t prefix_join_start(const PrefixArgs& a, hipStream_t stream) {
+  constexpr int W = SPLIT < 4 ? 4 : SPLIT;
+  constexpr int RPB = 64 / (D / 4) * (W / SPLIT);
+  const int64_t rows = (int64_t)a.B * a.Hkv * a.R;
+  hipLaunchKernelGGL((prefix_join_kernel<D, E, SPLIT>), dim3((unsigned)((rows + RPB - 1) / RPB)),
+                     dim3(64 * W), 0, stream, a);
+  return hipGetLastError();
 }
 
 template <int D, class E>
@@ -1175,11 +1228,10 @@ hipError_t prefix_start(const PrefixArgs& a, hipStream_t stream) {
   else hipLaunchKernelGGL((prefix_fwd_kernel<D, E, false>), grid, block, 0, stream, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  constexpr int RPP = 64 / (D / 4);
-  const int64_t rows = (int64_t)a.B * a.Hkv * a.R;
-  hipLaunchKernelGGL((prefix_join_kernel<D, E>), dim3((unsigned)((rows + RPP - 1) / RPP)),
-                     dim3(64 * kPrefixWaves), 0, stream, a);
-  return hipGetLastError();
+  const int64_t waves = (int64_t)a.B * a.Hkv * a.R / (64 / (D / 4));
+  return waves >= 1024  ? prefix_join_start<D, E, 2>(a, stream)
+         : waves >= 256 ? prefix_join_start<D, E, 4>(a, stream)
+                        : prefix_join_start<D, E, 16>(a, stream);
 }
 
 hipError_t launch_prefix_fwd(const PrefixArgs& a, int dtype, hipStream_t stream) {
