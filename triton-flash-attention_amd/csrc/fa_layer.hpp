@@ -258,7 +258,10 @@ struct PrefixGroup {
 constexpr int kPrefixTile = 128;   // query rows of a tile
 constexpr int kPrefixLead = 6;     // empty units in front of a triple on the line
 constexpr int kPrefixStretch = 4;  // least units of a work-group
-constexpr int kOwnRows = 32;       // most rows of a sequence whose own keys are a wave's work,
+// Groups (fewer) and sequences whose lengths and starts a work-group keeps in LDS.
+constexpr int kPrefixKeptGroups = 1024, kPrefixKeptSeqs = 2048;
+constexpr int kOwnRows = 64;       // most rows of a sequence whose own keys are a wave's work,
+constexpr int kOwnTile = 32;       // the rows of a tile there,
 constexpr int kOwnLead = 1;        // and the empty units in front of them
 inline __host__ __device__ int prefix_tiles(int64_t sequences, int64_t R) {
   return (int)((sequences * R + kPrefixTile - 1) / kPrefixTile);

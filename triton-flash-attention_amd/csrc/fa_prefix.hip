@@ -24,9 +24,9 @@ namespace fa {
 // and base-2 log-sum-exp of each row, into a slot of its own.
 //
 // Prefixes meet many rows: a work-group's four waves share each unit of 32 keys (prefix_piece). A
-// sequence's own keys meet few, at most 32 in decoding, and come in many short triples: there each
-// wave works on a triple of its own, so that eight are open on a CU (own_piece); with more rows a
-// head they go the prefixes' way (WAVES false).
+// sequence's own keys meet few, rarely more than 32 in decoding, and come in many short triples: there
+// each wave works on a triple of its own, with tiles of 32 rows, so that eight are open on a CU
+// (own_piece); with many rows a head they go the prefixes' way (WAVES false).
 //
 // Units of all triples lie on a line, each triple's behind `lead` empty ones that stand for opening
 // and closing a piece; the line is cut into equal stretches, one a work-group or a wave, found from
@@ -37,7 +37,6 @@ namespace fa {
 // equal pieces, so that no work-group opens two, and the tiles of one range of keys go to
 // neighbouring work-groups of one XCD, whose L2 then reads the keys once for all of them.
 constexpr int kPrefixWaves = 4;
-constexpr int kPrefixKeptGroups = 1024, kPrefixKeptSeqs = 2048;  // whose values are kept in LDS
 
 template <int D>
 struct PrefixRing {
@@ -114,8 +113,9 @@ __device__ __forceinline__ bool prefix_long(int units, int L) {
   return L >= 2 * kPrefixLead && units >= 2 * (L - kPrefixLead);
 }
 
-// A wave's stretch of the sequences' own keys, where a work-group's is L.
-__device__ __forceinline__ int own_stretch(int L) { return max((L + kPrefixWaves - 1) / kPrefixWaves, 2); }
+// A wave's stretch of the sequences' own keys, where a work-group's is L: four waves take three units
+// of them in the time that it takes for two of a prefix.
+__device__ __forceinline__ int own_stretch(int L) { return max((5 * L + 15) / 16, 2); }
 
 // The work-group's place, or the wave's. `lds`: the work-group's memory, free before and after.
 template <bool WAVES>
@@ -205,14 +205,15 @@ __device__ __forceinline__ PrefixLine prefix_find(const PrefixArgs& a, int* lds,
   sum(1);
   // (The line's two parts end with a stretch of their own each.)
   const int room = a.grid - 2;
-  const int L = max((all[1] + own_all[0] + room - 1) / room, kPrefixStretch);
+  const int own_cost = WAVES ? (4 * own_all[0] + 4) / 5 : own_all[0];
+  const int L = max((all[1] + own_cost + room - 1) / room, kPrefixStretch);
   // Long prefixes are cut by the work-groups that the line leaves: of all[3] units in all, a triple
   // of u into the whole part of u / all[3] of those. Where the grid would not hold the pieces, they
   // stay on the line.
   bool cut = all[1] > 0;
   int budget = 0;
   auto cuts_of = [&](int u) __attribute__((always_inline)) {
-    return cut && prefix_long(u, L) ? max(1, (int)((double)u * budget / all[3])) : 0;
+    return cut && prefix_long(u, L) ? max(1, min((int)((double)u * budget / all[3]), u / 16)) : 0;
   };
   x[0] = x[2] = x[3] = 0;
   sum(0);
@@ -770,11 +771,11 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const PrefixJo
 }
 
 // A wave's piece of a sequence's own keys [k_lo, k_hi), of which k_first is the first (k_lo is that
-// rounded down to 16), against the R <= 32 rows of head kvh, as in paged_fwd_kernel: K rows come in
-// the layout of the MFMA operand, V rows go through a tile in LDS (`vt`) for the transposing reads,
-// both asked for a unit ahead.
+// rounded down to 16), against the 32 rows from row0 on that read head kvh, as in paged_fwd_kernel: K
+// rows come in the layout of the MFMA operand, V rows go through a tile in LDS (`vt`) for the
+// transposing reads, both asked for a unit ahead.
 template <int D, class E>
-__device__ __forceinline__ void own_piece(const PrefixArgs& a, int b, int kvh, int k_lo, int k_first,
+__device__ __forceinline__ void own_piece(const PrefixArgs& a, int b, int kvh, int row0, int k_lo, int k_first,
                                           int k_hi, int len, float* slot, half_t* vt) {
   constexpr int KD = D / 32, DD = D / 16, RB = 2;
   constexpr int VI = 32 * D * 2 / 1024, VROWS = 512 / D;  // 1 KiB loads of a unit's V, rows of one
@@ -813,7 +814,7 @@ __device__ __forceinline__ void own_piece(const PrefixArgs& a, int b, int kvh, i
   half8 qf[RB][KD];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    const int r = 16 * rb + c16, h = r / a.N, n = r - h * a.N;
+    const int r = row0 + 16 * rb + c16, h = r / a.N, n = r - h * a.N;
     see[rb] = r < a.R ? min(all_see + n, k_hi) : INT32_MAX;
     const half_t* q = a.q + b * a.qs[0] + (int64_t)(kvh * a.group + h) * a.qs[1] + n * a.qs[2];
 #pragma unroll
@@ -966,7 +967,7 @@ __device__ __forceinline__ void own_piece(const PrefixArgs& a, int b, int kvh, i
     const int r = 16 * rb + c16;
     float lt = quarters_sum(l[rb]);
     if (bad) lt = __builtin_nanf("");
-    if (r >= a.R) continue;
+    if (row0 + r >= a.R) continue;
     const float inv = lt == 0.f ? 0.f : 1.0f / lt;
 #pragma unroll
     for (int dd = 0; dd < DD; ++dd)
@@ -992,8 +993,9 @@ __global__ __launch_bounds__(64 * kPrefixWaves, PrefixRing<D>::WGS) void prefix_
       const int len = units + kOwnLead;
       const int u0 = max(at.unit - kOwnLead, 0);
       const int u1 = left < len - at.unit ? max(at.unit + left - kOwnLead, 0) : units;
+      const int kvh = at.sub / a.blocks;
       if (u1 > u0)
-        own_piece<D, E>(a, at.at, at.sub, k0 + 32 * u0, max(at.k_first, k0 + 32 * u0),
+        own_piece<D, E>(a, at.at, kvh, (at.sub - kvh * a.blocks) * kOwnTile, k0 + 32 * u0, max(at.k_first, k0 + 32 * u0),
                         min(at.k_end, k0 + 32 * u1), at.k_end,
                         own_slot(a, D, (int64_t)line.s + (int64_t)at.at * HB + at.sub), vt);
       left -= len - at.unit;
@@ -1065,7 +1067,7 @@ template <int D, class E, int SPLIT>
 __global__ __launch_bounds__(64 * (SPLIT < 4 ? 4 : SPLIT)) void prefix_join_kernel(PrefixArgs a) {
   constexpr int W = SPLIT < 4 ? 4 : SPLIT;  // waves
   constexpr int COLS = D / 4, RPP = 64 / COLS;
-  constexpr int AHEAD = SPLIT == 16 ? 4 : 8;
+  constexpr int AHEAD = 4;
   // The weight of the largest piece: those of 1024 pieces sum to 1/2, so that sums of values near
   // 2^128 stay in float32.
   constexpr float kWeight = 0x1p-11f;
@@ -1111,8 +1113,9 @@ __global__ __launch_bounds__(64 * (SPLIT < 4 ? 4 : SPLIT)) void prefix_join_kern
                   stretch, &np);
     pslot += (int64_t)cut + grp.first + psub;
   }
-  const int osub = kvh * a.blocks + r / kPrefixTile;
-  const int lead = a.R <= kOwnRows ? kOwnLead : kPrefixLead;
+  const bool waves = a.R <= kOwnRows;
+  const int own_tile = waves ? kOwnTile : kPrefixTile, lead = waves ? kOwnLead : kPrefixLead;
+  const int osub = kvh * a.blocks + r / own_tile;
   int64_t oslot = range(q.own_base + (int64_t)osub * on_line(q.own_units, lead), q.own_units, lead,
                         own_stretch, &no);
   oslot += (int64_t)b * a.Hkv * a.blocks + osub;
@@ -1127,7 +1130,7 @@ __global__ __launch_bounds__(64 * (SPLIT < 4 ? 4 : SPLIT)) void prefix_join_kern
       const bool pre = i < np;
       const float* slot = pre ? prefix_slot(a, D, pslot + (int64_t)i * step)
                               : own_slot(a, D, oslot + (i - np));
-      const int at = pre ? (int)(gr % kPrefixTile) : r % kPrefixTile;
+      const int at = pre ? (int)(gr % kPrefixTile) : r % own_tile;
       p.lse = slot[(int64_t)(pre ? a.prows : a.srows) * D + at];
       p.o = *reinterpret_cast<const float4v*>(slot + (int64_t)at * D + col);
     }
@@ -1187,9 +1190,10 @@ static int prefix_width(int64_t D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
 PrefixSizes prefix_sizes(int64_t B, int64_t G, int64_t Hkv, int64_t R, int64_t D, int64_t keys) {
   PrefixSizes z;
-  z.blocks = prefix_tiles(R, 1);
-  z.prows = std::min<int64_t>(kPrefixTile, B * R);
-  z.srows = std::min<int64_t>(kPrefixTile, R);
+  const int64_t own_tile = R <= kOwnRows ? kOwnTile : kPrefixTile;
+  z.blocks = (int)((R + own_tile - 1) / own_tile);
+  z.prows = (int)std::min<int64_t>(kPrefixTile, B * R);
+  z.srows = (int)std::min(own_tile, R);
   // Groups of two sequences or more have prefixes, in at most so many tiles.
   const int64_t groups = std::min(G, B / 2), own = B * Hkv * z.blocks;
   const int64_t triples = groups > 0 ? Hkv * (B * R / kPrefixTile + groups) : 0;
@@ -1229,9 +1233,8 @@ hipError_t prefix_start(const PrefixArgs& a, hipStream_t stream) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int64_t waves = (int64_t)a.B * a.Hkv * a.R / (64 / (D / 4));
-  return waves >= 1024  ? prefix_join_start<D, E, 2>(a, stream)
-         : waves >= 256 ? prefix_join_start<D, E, 4>(a, stream)
-                        : prefix_join_start<D, E, 16>(a, stream);
+  return waves >= 256 ? prefix_join_start<D, E, 4>(a, stream)
+                      : prefix_join_start<D, E, 16>(a, stream);
 }
 
 hipError_t launch_prefix_fwd(const PrefixArgs& a, int dtype, hipStream_t stream) {
