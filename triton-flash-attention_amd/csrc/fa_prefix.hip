@@ -113,8 +113,8 @@ __device__ __forceinline__ bool prefix_long(int units, int L) {
   return L >= 2 * kPrefixLead && units >= 2 * (L - kPrefixLead);
 }
 
-// A wave's stretch of the sequences' own keys, where a work-group's is L: four waves take three units
-// of them in the time that it takes for two of a prefix.
+// A wave's stretch of the sequences' own keys, where a work-group's is L: four waves take five units
+// of them in the time that it takes for four of a prefix.
 __device__ __forceinline__ int own_stretch(int L) { return max((5 * L + 15) / 16, 2); }
 
 // The work-group's place, or the wave's. `lds`: the work-group's memory, free before and after.
@@ -205,7 +205,7 @@ __device__ __forceinline__ PrefixLine prefix_find(const PrefixArgs& a, int* lds,
   sum(1);
   // (The line's two parts end with a stretch of their own each.)
   const int room = a.grid - 2;
-  const int own_cost = WAVES ? (4 * own_all[0] + 4) / 5 : own_all[0];
+  const int own_cost = WAVES ? own_all[0] - own_all[0] / 5 : own_all[0];
   const int L = max((all[1] + own_cost + room - 1) / room, kPrefixStretch);
   // Long prefixes are cut by the work-groups that the line leaves: of all[3] units in all, a triple
   // of u into the whole part of u / all[3] of those. Where the grid would not hold the pieces, they
@@ -424,13 +424,53 @@ struct PrefixJob {
   int slot_rows;
 };
 
-// What issue_kv_unit asks of a wave's share of a unit.
+// A wave's share of a unit: one or two of the 1 KiB pieces of its K rows and of its V rows.
 template <int P>
 struct PrefixDma {
-  static constexpr int PER_WAVE = P;
+  static_assert(P == 1 || P == 2, "one or two pieces");
   uint32_t voff[P];  // byte offsets in the page's half of the unit
-  uint32_t row_bytes;
 };
+// Moves the share to the LDS tiles at `base` (K) and base + TILE_BYTES (V); `back` bytes are taken
+// off the offsets. The descriptors' words come from v_readlane, and a load may read such a register
+// five wait states later at the earliest: the compiler does not look into the block for it, so the
+// block waits.
+template <int TILE_BYTES, int P>
+__device__ __forceinline__ void issue_unit(const PrefixDma<P>& dma, int4v r_k, int4v r_v, uint32_t back,
+                                           uint32_t base) {
+  const uint32_t v0 = dma.voff[0] - back;
+  uint32_t saved;
+  if constexpr (P == 1) {
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_nop 2\n\t"
+        "s_mov_b32 m0, %4\n\t"
+        "buffer_load_dwordx4 %1, %2, 0 offen lds\n\t"
+        "s_mov_b32 m0, %5\n\t"
+        "buffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "v"(v0), "s"(r_k), "s"(r_v), "s"(base), "s"(base + TILE_BYTES)
+        : "memory");
+  } else {
+    const uint32_t v1 = dma.voff[1] - back;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_nop 2\n\t"
+        "s_mov_b32 m0, %5\n\t"
+        "buffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
+        "s_mov_b32 m0, %6\n\t"
+        "buffer_load_dwordx4 %2, %3, 0 offen lds\n\t"
+        "s_mov_b32 m0, %7\n\t"
+        "buffer_load_dwordx4 %1, %4, 0 offen lds\n\t"
+        "s_mov_b32 m0, %8\n\t"
+        "buffer_load_dwordx4 %2, %4, 0 offen lds\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "v"(v0), "v"(v1), "s"(r_k), "s"(r_v), "s"(base), "s"(base + 1024u), "s"(base + TILE_BYTES),
+          "s"(base + TILE_BYTES + 1024u)
+        : "memory");
+  }
+}
 
 template <int I, int N, typename F>
 __device__ __forceinline__ void each(F&& f) {
@@ -455,7 +495,9 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const PrefixJo
   constexpr int NS = T::NS;
   constexpr int IPU = 2 * T::PER_WAVE;
   constexpr int NQ = D / 16;
-  const int tid = threadIdx.x;
+  // (from an asm statement, so that what follows from it is not kept from one piece to the next)
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
   const int lane = tid & 63;
   const int wave = uniform(tid >> 6);
   const int ql = lane & 31;
@@ -502,7 +544,6 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const PrefixJo
   PrefixDma<T::PER_WAVE> dma;
   const int piece0 = T::INSTR >= kPrefixWaves ? wave * T::PER_WAVE : wave % T::INSTR;
   const int e = piece0 * 1024 / (D * 2) / 16;
-  dma.row_bytes = (uint32_t)row_bytes;
 #pragma unroll
   for (int i = 0; i < T::PER_WAVE; ++i) {
     const int byte = (piece0 + i) * 1024 + lane * 16;
@@ -533,8 +574,9 @@ __device__ __forceinline__ void prefix_piece(const PrefixArgs& a, const PrefixJo
     const uint64_t o = (uint32_t)__builtin_amdgcn_readlane((int)off, at) |
                        (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(off >> 32), at) << 32;
     const uint32_t n = __builtin_amdgcn_readlane(rows_bytes, at);
-    issue_kv_unit<T::TILE * 2>(dma, make_rsrc_words(k_head + o, n), make_rsrc_words(v_head + o, n),
-                               -skip, lds0 + (uint32_t)slot * (T::STAGE * 2u) + (uint32_t)piece0 * 1024u);
+    issue_unit<T::TILE * 2>(dma, make_rsrc_words(k_head + o, n), make_rsrc_words(v_head + o, n),
+                            (uint32_t)(skip * row_bytes),
+                            lds0 + (uint32_t)slot * (T::STAGE * 2u) + (uint32_t)piece0 * 1024u);
     ++iu;
   };
 

@@ -95,6 +95,12 @@ def _defaults() -> tuple[str, ...]:
                   for r in (1, 2) for s in ("false", "true")]
         names += [f"fa::paged_join_kernel<{d}, {e}>" for d in (32, 64, 128)]
         names.append(f"fa::rope_reduce_kernel<{e}>")
+        names += [f"fa::prefix_fwd_kernel<{d}, {e}, {w}>" for d in (32, 64, 128)
+                  for w in ("false", "true")]
+        names += [f"fa::prefix_join_kernel<{d}, {e}, {w}>" for d in (32, 64, 128) for w in (4, 16)]
+    names += [f"fa::{k}_kernel" for k in ("fork_small", "fork_count", "fork_finish", "page_copy",
+                                          "compact_small", "compact_mark", "compact_rank",
+                                          "compact_apply")]
     names += ["fa::paged_plan_kernel<1>", "fa::paged_plan_kernel<2>"]
     names += [f"fa::paged_store_kernel<{w}>" for w in (32, 64, 128, 256)]
     names += [f"fa::{k}_kernel<128, false, 4, 32, {e}>" for k in ("dq", "dkdv")
@@ -107,8 +113,14 @@ DEFAULT_KERNELS = _defaults()
 # short-query dK/dV at D = 128 asks for two waves per SIMD (256 registers) and
 # reloads two 16-byte values per 32-query unit; with them it is 13-15 % faster
 # than the pipelined kernel at one wave per SIMD for 4-64 queries (select_dkdv,
-# csrc/fa_capi.hip). Any other spill, or a larger one, fails --strict.
+# csrc/fa_capi.hip). The attention over shared prefixes at D = 64 keeps up to
+# three values of a work-group's place in scratch while it works on a piece of
+# a prefix: they are stored and read outside the loops over keys, and three
+# work-groups a CU are worth more. Any other spill, or a larger one, fails
+# --strict.
 ALLOWED_SPILLS = {f"fa::dkdv_kernel<128, false, 4, 32, {e}>": 52 for e in ("fa::F16", "fa::BF16")}
+ALLOWED_SPILLS |= {f"fa::prefix_fwd_kernel<64, {e}, {w}>": 16 for e in ("fa::F16", "fa::BF16")
+                   for w in ("false", "true")}
 # The same table as (kernel kind, head_dim, causal) -> default variant index,
 # for the test that keeps this list in step with kDefault (kinds: 0 fwd,
 # 1 dK/dV, 2 dQ).

@@ -17,7 +17,9 @@ from .attention import Backend, _forward_ad_active
 from .paged import (_attention_reason, _check_attention, _check_ints, _scaled_query)
 from .rotary import _binding, _check_backend, _check_tensor, _falls_back
 
-_TILE = 128  # query rows of a tile (fa_layer.hpp kPrefixTile)
+# Query rows of a tile: of a prefix, and of a sequence's own keys where it has at most _OWN_ROWS
+# (fa_layer.hpp kPrefixTile, kOwnTile, kOwnRows).
+_TILE, _OWN_TILE, _OWN_ROWS = 128, 32, 64
 
 
 def _prefixes(lengths, group_starts, prefix_lengths, capacity):
@@ -101,9 +103,8 @@ def paged_prefix_attention(
     sequence that is shorter.
 
     The gfx950 kernels serve what those of ``paged_attention`` serve. They work on tiles of 128
-    of the rows that share a prefix and a key/value head, so besides groups they suit several
-    newest tokens a sequence; for one token each of sequences that share nothing
-    ``paged_attention`` is faster. They have no backward.
+    of the rows that share a prefix and a key/value head; for sequences that share nothing
+    ``paged_attention`` is faster, which has less to find out first. They have no backward.
     """
     native = _binding(backend)
     if native is not None and not _forward_ad_active():
@@ -121,7 +122,9 @@ def paged_prefix_attention(
     _check_ints("group_starts", group_starts, (G + 1,), query.device)
     softmax_scale = float(scale) if scale is not None else D ** -0.5
     rows = Hq // H * N
-    tiles = B * H * -(-rows // _TILE) + (H * (B * rows // _TILE + min(G, B // 2)) if B > 1 else 0)
+    tiles = B * H * -(-rows // (_OWN_TILE if rows <= _OWN_ROWS else _TILE))
+    if G > 0 and B > 1:
+        tiles += H * (B * rows // _TILE + min(G, B // 2))
     too_many = Hq >= 1 << 20 or N >= 1 << 20 or G >= 1 << 30 or B * Hq * N >= 1 << 24 or (
         tiles * (-(-page_table.shape[1] * S // 32) + 24) >= 1 << 30)
     reason, served = _attention_reason(backend, query, key_cache, value_cache, softmax_scale, too_many)
