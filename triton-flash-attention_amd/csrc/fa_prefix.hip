@@ -220,6 +220,7 @@ __device__ __forceinline__ PrefixLine prefix_find(const PrefixArgs& a, int* lds,
   sum(2);
   while (all[1] > 0) {
     x[0] = x[1] = x[2] = x[3] = 0;
+    before[0] = all[0] = 0;
     for (int g = g0; g < g1; ++g) {
       const int u = key_units(0, keys_in(g)), t = u > 0 ? triples_in(g) : 0;
       if (cut && prefix_long(u, L)) {
