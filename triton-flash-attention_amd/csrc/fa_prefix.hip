@@ -210,7 +210,8 @@ __device__ __forceinline__ PrefixLine prefix_find(const PrefixArgs& a, int* lds,
   // Long prefixes are cut by the work-groups that the line leaves: of all[3] units in all, a triple
   // of u into the whole part of u / all[3] of those. Where the grid would not hold the pieces, they
   // stay on the line.
-  bool cut = all[1] > 0;
+  const bool any = all[1] > 0;
+  bool cut = any;
   int budget = 0;
   auto cuts_of = [&](int u) __attribute__((always_inline)) {
     return cut && prefix_long(u, L) ? max(1, min((int)((double)u * budget / all[3]), u / 16)) : 0;
@@ -218,7 +219,7 @@ __device__ __forceinline__ PrefixLine prefix_find(const PrefixArgs& a, int* lds,
   x[0] = x[2] = x[3] = 0;
   sum(0);
   sum(2);
-  while (all[1] > 0) {
+  while (any) {
     x[0] = x[1] = x[2] = x[3] = 0;
     before[0] = all[0] = 0;
     for (int g = g0; g < g1; ++g) {
