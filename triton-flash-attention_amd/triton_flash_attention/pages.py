@@ -16,6 +16,8 @@ A step of beam search, where row b of the next step continues row ``parents[b]``
     lengths, free_start = fork.lengths, fork.free_start
 
 Samples of one prompt are rows with the same parent; a sequence ends where its row's parent is -1.
+A begun page, the last of a sequence that does not fill it, has to be held by one row alone, as it is
+after forks and plans: a program that shortens a row into a shared page copies this page first.
 The rows of a fork share whole pages, which :func:`.prefix.paged_prefix_attention` reads once.
 
 No counterpart in the reference. Names, checks and the choice of a backend follow :mod:`.paged`.
