@@ -57,6 +57,11 @@ struct PrefixRing {
   static_assert(WGS * HALVES * 2 <= 160 * 1024, "LDS of a CU");
 };
 
+// Work-groups that the chip holds, and pieces of one row: one a work-group of its group's prefix, and
+// one a wave of its own keys.
+constexpr int kPrefixMostGrid = 256 * PrefixRing<64>::WGS;
+constexpr int kPrefixMostPieces = kPrefixMostGrid * (1 + kPrefixWaves);
+
 // As in fa_paged.hip: the reference of a row's probabilities is 2^7 below the max for fp16 and 2^16
 // above it, or above the sum, for bf16, whose probabilities so far are held to 1/4 a lane, 1/2 a row.
 template <class E>
@@ -1116,9 +1121,6 @@ __global__ __launch_bounds__(64 * (SPLIT < 4 ? 4 : SPLIT)) void prefix_join_kern
   constexpr int W = SPLIT < 4 ? 4 : SPLIT;  // waves
   constexpr int COLS = D / 4, RPP = 64 / COLS;
   constexpr int AHEAD = 4;
-  // The weight of the largest piece: those of 1024 pieces sum to 1/2, so that sums of values near
-  // 2^128 stay in float32.
-  constexpr float kWeight = 0x1p-11f;
   __shared__ __attribute__((aligned(16))) float acc_s[SPLIT > 1 ? W : 1][64][4];
   __shared__ float m_s[W][64], l_s[W][64];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -1168,6 +1170,10 @@ __global__ __launch_bounds__(64 * (SPLIT < 4 ? 4 : SPLIT)) void prefix_join_kern
                         own_stretch, &no);
   oslot += (int64_t)b * a.Hkv * a.blocks + osub;
   const int count = real ? np + no : 0;
+  // The weight of the largest piece: those of a row sum to 1/2 at most, so that sums of values near
+  // 2^128 stay in float32. (Up to 1024 pieces the weight is larger, which leaves small values more bits.)
+  static_assert(kPrefixMostPieces <= 4096, "weights of 2^-13");
+  const float weight = count <= 1024 ? 0x1p-11f : 0x1p-13f;
   struct Piece {
     float lse;
     float4v o;
@@ -1199,7 +1205,7 @@ __global__ __launch_bounds__(64 * (SPLIT < 4 ? 4 : SPLIT)) void prefix_join_kern
     acc *= keep;
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
-      const float f = p[i].lse == -INFINITY ? 0.f : exp2_fast(p[i].lse - ref) * kWeight;
+      const float f = p[i].lse == -INFINITY ? 0.f : exp2_fast(p[i].lse - ref) * weight;
       l += f;
       acc += p[i].o * f;
     }
@@ -1247,7 +1253,7 @@ PrefixSizes prefix_sizes(int64_t B, int64_t G, int64_t Hkv, int64_t R, int64_t D
   const int64_t triples = groups > 0 ? Hkv * (B * R / kPrefixTile + groups) : 0;
   const double each = (double)((keys + 31) / 32 + 1 + kPrefixLead);
   z.units = each * ((double)triples + (double)own);
-  const int64_t most = 256 * (prefix_width(D) == 128 ? 2 : 3);
+  const int64_t most = prefix_width(D) == 128 ? PrefixRing<128>::WGS * 256 : kPrefixMostGrid;
   // Work-groups that the chip holds at once, at most one for each four units that the tables could
   // hold; as many on each XCD.
   z.grid = (int)std::min((double)most, std::ceil(z.units / kPrefixStretch));
