@@ -30,7 +30,7 @@ from typing import NamedTuple
 import torch
 
 from . import _ops
-from .attention import Backend
+from .attention import Backend, _forward_ad_active
 from .paged import _PAGE_MULTIPLE, _cache_reason, _check_caches, _check_ints, _check_table
 from .rotary import _binding, _check_backend, _check_tensor, _falls_back, _gpu_reason
 
@@ -213,10 +213,11 @@ def paged_cache_copy(
     ``tokens[i]`` rows (int32, taken into [0, page_size]); the target's other rows stay as they
     were. Pairs of which one names no page (-1) are left out. The targets must differ from each
     other and from all sources. Gradients are not recorded: the call raises where one would have
-    to be.
+    to be. Tangents move along: inside a forward-mode level the call runs in PyTorch under
+    ``backend="auto"``.
     """
     native = _binding(backend)
-    if native is not None and native.paged_copy(
+    if native is not None and not _forward_ad_active() and native.paged_copy(
             key_cache, value_cache, sources, targets, tokens):
         return
     _check_backend(backend)
@@ -242,6 +243,8 @@ def paged_cache_copy(
                   else _cache_reason(key_cache, value_cache) or _gpu_reason(key_cache))
         if reason is None and key_cache[0].numel() >= 1 << 33:
             reason = "the pages are too large for one launch"
+        elif reason is None and _forward_ad_active():
+            reason = "the copying kernel moves no tangents"
     if _falls_back(backend, reason):
         kept = (sources >= 0) & (sources < pages) & (targets >= 0) & (targets < pages)
         source, target = sources[kept].long(), targets[kept].long()
