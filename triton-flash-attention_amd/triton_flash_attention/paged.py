@@ -222,10 +222,12 @@ def paged_cache_store(
     slot s is row ``s % page_size`` of page ``s // page_size``. Negative slots and slots behind
     the last page are left out; the others must differ from each other. Rows of the cache that
     no slot names stay as they were. key and value must not share memory with the cache.
-    Gradients are not recorded: the call raises where one would have to be.
+    Gradients are not recorded: the call raises where one would have to be. Tangents are written
+    along: inside a forward-mode level the call runs in PyTorch under ``backend="auto"``.
     """
     native = _binding(backend)
-    if native is not None and native.paged_store(key, value, key_cache, value_cache, slots):
+    if native is not None and not _forward_ad_active() and native.paged_store(
+            key, value, key_cache, value_cache, slots):
         return
     _check_backend(backend)
     for name, t in (("key", key), ("value", value)):
@@ -258,6 +260,8 @@ def paged_cache_store(
     if backend != "torch":
         reason = (_gpu_reason(key_cache) if key_cache.device.type != "cuda"
                   else _cache_reason(key_cache, value_cache) or _gpu_reason(key_cache))
+        if reason is None and _forward_ad_active():
+            reason = "the storing kernel writes no tangents"
     if _falls_back(backend, reason):
         kept = torch.nonzero((slots >= 0) & (slots < pages * S)).squeeze(1)
         page, row = slots[kept] // S, slots[kept] % S
