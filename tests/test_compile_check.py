@@ -40,6 +40,14 @@ def test_resource_report_parsing():
     assert "fa::dkdv_pipe_kernel<64, true, 4, fa::BF16>" in missing
 
 
+def test_resource_report_with_the_place_behind_the_word():
+    """As the compiler words it where it keeps the assembly."""
+    lines = [f"remark: {place}: {rest}" for place, rest in
+             (line.split(": remark: ") for line in REMARKS.splitlines())]
+    assert compile_check.parse_resource_usage("\n".join(lines)) == \
+        compile_check.parse_resource_usage(REMARKS)
+
+
 def test_spill_allowance_is_per_kernel_and_capped():
     """A default kernel listed in ALLOWED_SPILLS may spill up to its measured
     bytes per lane and no more; every other default kernel may not spill."""
@@ -83,3 +91,46 @@ def test_unsupported_arch_is_rejected():
 def test_library_compiles_for_gfx950_without_spills_in_the_defaults(capsys):
     assert compile_check.main(["--strict"]) == 0
     assert "compile check passed for gfx950" in capsys.readouterr().out
+
+
+ASSEMBLY = """\
+	.globl	_ZN2fa5tile_kernelE
+_ZN2fa5tile_kernelE:                    ; @_ZN2fa5tile_kernelE
+; %bb.0:
+	v_readlane_b32 s6, v3, 2
+	s_mov_b32 s7, 0x20000
+	{first}
+	s_cbranch_scc1 .LBB0_2
+; %bb.1:
+	s_add_u32 s4, s4, 64
+.LBB0_2:                                ; =>This Inner Loop Header: Depth=1
+	;;#ASMSTART
+	s_mov_b32 s9, m0
+	s_mov_b32 m0, s8
+	{second}
+	buffer_load_dwordx4 v1, s[4:7], 0 offen lds
+	s_mov_b32 m0, s9
+	;;#ASMEND
+	s_cbranch_vccnz .LBB0_2
+	s_endpgm
+.Lfunc_end0:
+"""
+
+
+@pytest.mark.parametrize(("first", "second", "found"), [
+    ("", "s_nop 0", []),                       # five states behind the readlane, one behind M0
+    ("s_nop 0", "", ["m0"]),
+    ("s_nop 7", "", ["m0"]),
+    ("", "", ["m0", "readlane"]),
+    ("s_cmp_eq_u32 s2, 0", "s_nop 0", []),
+    ("s_mov_b32 s6, 0", "", ["m0"]),           # the descriptor's word is a scalar instruction's by then
+    ("v_readlane_b32 s4, v3, 1", "s_nop 0", ["readlane"]),  # on the path past the addition
+    ("v_add_co_u32 v2, s[4:5], v2, v4", "s_nop 0", ["v_add_co"]),
+    ("v_add_co_u32 v2, s[4:5], v2, v4", "s_nop 1", []),
+    ("v_add_f32 v2, s4, v4", "s_nop 0", []),
+])
+def test_missing_wait_states_are_found(first, second, found):
+    faults = compile_check.wait_state_faults(ASSEMBLY.format(first=first, second=second))
+    assert len(faults) == len(found)
+    for word in found:
+        assert any(word in f.split("behind")[1] for f in faults), faults

@@ -378,12 +378,15 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 }
 
 // 16 bytes per lane from byte offset `voff` of the buffer to LDS[m0 + 16 lane].
-// M0 is reserved by the compiler, so the block restores it before returning.
+// M0 is reserved by the compiler, so the block restores it before returning. A load that
+// goes to LDS may read M0 one wait state behind its write at the earliest: the compiler
+// does not look into the block for that, so each block waits.
 __device__ __forceinline__ void dma_b128(int4v rsrc, uint32_t voff, uint32_t lds_base) {
   uint32_t saved;
   asm volatile(
       "s_mov_b32 %0, m0\n\t"
       "s_mov_b32 m0, %3\n\t"
+      "s_nop 0\n\t"
       "buffer_load_dwordx4 %1, %2, 0 offen lds\n\t"
       "s_mov_b32 m0, %0"
       : "=&s"(saved)
@@ -397,6 +400,7 @@ __device__ __forceinline__ void dma_b32(int4v rsrc, uint32_t voff, uint32_t lds_
   asm volatile(
       "s_mov_b32 %0, m0\n\t"
       "s_mov_b32 m0, %3\n\t"
+      "s_nop 0\n\t"
       "buffer_load_dword %1, %2, 0 offen lds\n\t"
       "s_mov_b32 m0, %0"
       : "=&s"(saved)
@@ -467,8 +471,10 @@ __device__ __forceinline__ void issue_kv_unit(const Dma& dma, int4v r_k, int4v r
     asm volatile(
         "s_mov_b32 %0, m0\n\t"
         "s_mov_b32 m0, %4\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dwordx4 %1, %2, 0 offen lds\n\t"
         "s_mov_b32 m0, %5\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
         "s_mov_b32 m0, %0"
         : "=&s"(saved)
@@ -479,12 +485,16 @@ __device__ __forceinline__ void issue_kv_unit(const Dma& dma, int4v r_k, int4v r
     asm volatile(
         "s_mov_b32 %0, m0\n\t"
         "s_mov_b32 m0, %5\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
         "s_mov_b32 m0, %6\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dwordx4 %2, %3, 0 offen lds\n\t"
         "s_mov_b32 m0, %7\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dwordx4 %1, %4, 0 offen lds\n\t"
         "s_mov_b32 m0, %8\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dwordx4 %2, %4, 0 offen lds\n\t"
         "s_mov_b32 m0, %0"
         : "=&s"(saved)
@@ -508,10 +518,13 @@ __device__ __forceinline__ void issue_q_unit(const Dma& dma, int4v r_q, int4v r_
     asm volatile(
         "s_mov_b32 %0, m0\n\t"
         "s_mov_b32 m0, %6\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
         "s_mov_b32 m0, %7\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dwordx4 %1, %4, 0 offen lds\n\t"
         "s_mov_b32 m0, %8\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dword %2, %5, 0 offen lds\n\t"
         "s_mov_b32 m0, %0"
         : "=&s"(saved)
@@ -523,14 +536,19 @@ __device__ __forceinline__ void issue_q_unit(const Dma& dma, int4v r_q, int4v r_
     asm volatile(
         "s_mov_b32 %0, m0\n\t"
         "s_mov_b32 m0, %7\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dwordx4 %1, %4, 0 offen lds\n\t"
         "s_mov_b32 m0, %8\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dwordx4 %2, %4, 0 offen lds\n\t"
         "s_mov_b32 m0, %9\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dwordx4 %1, %5, 0 offen lds\n\t"
         "s_mov_b32 m0, %10\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dwordx4 %2, %5, 0 offen lds\n\t"
         "s_mov_b32 m0, %11\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dword %3, %6, 0 offen lds\n\t"
         "s_mov_b32 m0, %0"
         : "=&s"(saved)

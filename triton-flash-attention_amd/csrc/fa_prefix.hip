@@ -443,8 +443,8 @@ struct PrefixDma {
 };
 // Moves the share to the LDS tiles at `base` (K) and base + TILE_BYTES (V); `back` bytes are taken
 // off the offsets. The descriptors' words come from v_readlane, and a load may read such a register
-// five wait states later at the earliest: the compiler does not look into the block for it, so the
-// block waits.
+// five wait states later at the earliest, and M0 one behind its write: the compiler does not look into
+// the block for either, so the block waits.
 template <int TILE_BYTES, int P>
 __device__ __forceinline__ void issue_unit(const PrefixDma<P>& dma, int4v r_k, int4v r_v, uint32_t back,
                                            uint32_t base) {
@@ -453,10 +453,11 @@ __device__ __forceinline__ void issue_unit(const PrefixDma<P>& dma, int4v r_k, i
   if constexpr (P == 1) {
     asm volatile(
         "s_mov_b32 %0, m0\n\t"
-        "s_nop 2\n\t"
         "s_mov_b32 m0, %4\n\t"
+        "s_nop 2\n\t"
         "buffer_load_dwordx4 %1, %2, 0 offen lds\n\t"
         "s_mov_b32 m0, %5\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
         "s_mov_b32 m0, %0"
         : "=&s"(saved)
@@ -466,14 +467,17 @@ __device__ __forceinline__ void issue_unit(const PrefixDma<P>& dma, int4v r_k, i
     const uint32_t v1 = dma.voff[1] - back;
     asm volatile(
         "s_mov_b32 %0, m0\n\t"
-        "s_nop 2\n\t"
         "s_mov_b32 m0, %5\n\t"
+        "s_nop 2\n\t"
         "buffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
         "s_mov_b32 m0, %6\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dwordx4 %2, %3, 0 offen lds\n\t"
         "s_mov_b32 m0, %7\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dwordx4 %1, %4, 0 offen lds\n\t"
         "s_mov_b32 m0, %8\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dwordx4 %2, %4, 0 offen lds\n\t"
         "s_mov_b32 m0, %0"
         : "=&s"(saved)

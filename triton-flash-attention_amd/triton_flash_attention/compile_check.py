@@ -8,7 +8,9 @@ temporary file, no GPU or driver needed, and reads the compiler's per-kernel
 resource report (VGPRs, AGPRs, scratch, occupancy, LDS). With ``--strict`` it
 also fails when a kernel the default tiling table selects spills registers to
 scratch memory: a spill reload inside a pipelined loop is a vector-memory load,
-and waiting for it drains the kernel's DMA ring.
+and waiting for it drains the kernel's DMA ring. It also reads the assembly of
+every kernel for wait states that the hardware wants and inline assembly leaves
+out (wait_state_faults), and fails where one is missing.
 
     python -m triton_flash_attention.compile_check [--arch gfx950] [--report] [--strict]
 """
@@ -144,14 +146,16 @@ class KernelUsage:
     lds: int = -1
 
 
+# (with -save-temps the source's place stands behind the word)
+_REMARK = r"remark:\s+(?:\S+:\d+:\d+:\s+)?"
 _FIELDS = (
-    ("vgprs", re.compile(r"remark:\s+VGPRs: (\d+)")),
-    ("agprs", re.compile(r"remark:\s+AGPRs: (\d+)")),
-    ("scratch", re.compile(r"remark:\s+ScratchSize \[bytes/lane\]: (\d+)")),
-    ("occupancy", re.compile(r"remark:\s+Occupancy \[waves/SIMD\]: (\d+)")),
-    ("lds", re.compile(r"remark:\s+LDS Size \[bytes/block\]: (\d+)")),
+    ("vgprs", re.compile(_REMARK + r"VGPRs: (\d+)")),
+    ("agprs", re.compile(_REMARK + r"AGPRs: (\d+)")),
+    ("scratch", re.compile(_REMARK + r"ScratchSize \[bytes/lane\]: (\d+)")),
+    ("occupancy", re.compile(_REMARK + r"Occupancy \[waves/SIMD\]: (\d+)")),
+    ("lds", re.compile(_REMARK + r"LDS Size \[bytes/block\]: (\d+)")),
 )
-_NAME = re.compile(r"remark: Function Name: (\S+)")
+_NAME = re.compile(_REMARK + r"Function Name: (\S+)")
 
 
 _MANGLED = re.compile(r"^_ZN2fa(\d+)")
@@ -210,16 +214,110 @@ def parse_resource_usage(text: str) -> list[KernelUsage]:
     return kernels
 
 
-def compile_library(arch: str = "gfx950") -> tuple[list[KernelUsage], str]:
-    """Compile the library into a temporary file; returns (kernels, diagnostics)."""
+# ---- wait states ------------------------------------------------------------------------
+#
+# The compiler keeps instructions apart that the hardware does not, but looks into no block of
+# inline assembly. Two such rules of gfx950 meet the blocks that move tiles to LDS:
+M0_WAIT = 1    # from a scalar write of M0 to a load that goes to LDS through it
+SGPR_WAIT = 5  # from a vector instruction that writes a scalar register to a memory access that reads it
+
+_FUNCTION = re.compile(r"^(\w+):\s*; @")
+_LABEL = re.compile(r"^([.\w$]+):")
+_SCALARS = re.compile(r"(?<![\w\[:.])(?:s\[(\d+):(\d+)\]|s(\d+)\b|(vcc|m0)\b)")
+
+
+def _scalars(operands: str) -> frozenset:
+    found = set()
+    for lo, hi, one, name in _SCALARS.findall(operands):
+        found |= {name} if name else {int(one)} if one else set(range(int(lo), int(hi) + 1))
+    return frozenset(found)
+
+
+def _functions(assembly: str):
+    """(name, instructions, labels) of each function: ("op", "operands") in order, and the place that
+    a label stands for."""
+    name = None
+    for line in assembly.splitlines():
+        line = line.strip()
+        m = _FUNCTION.match(line)
+        if m:
+            name, code, labels = m.group(1), [], {}
+            continue
+        if name is None:
+            continue
+        if line.startswith(".Lfunc_end"):
+            yield name, code, labels
+            name = None
+            continue
+        line = line.split(";")[0].strip()
+        if not line:
+            continue
+        m = _LABEL.match(line)
+        if m:
+            labels[m.group(1)] = len(code)
+        elif not line.startswith("."):
+            op, _, operands = line.partition(" ")
+            code.append((op, operands.strip()))
+
+
+def wait_state_faults(assembly: str) -> list[str]:
+    """Instructions of gfx950 assembly that follow what they read too soon (M0_WAIT, SGPR_WAIT), along
+    every path to them."""
+    faults = []
+    for name, code, labels in _functions(assembly):
+        before = [[] for _ in range(len(code) + 1)]
+        for i, (op, operands) in enumerate(code):
+            if op == "s_branch" or op.startswith("s_cbranch"):
+                before[labels[operands]].append(i)
+            if op not in ("s_branch", "s_endpgm", "s_setpc_b64"):
+                before[i + 1].append(i)
+        for i, (op, operands) in enumerate(code):
+            if not op.startswith(("buffer_", "global_", "scratch_", "flat_")):
+                continue
+            reads = _scalars(operands)
+            if operands.split()[-1] == "lds":
+                reads |= {"m0"}
+            todo, seen = [(p, 0, reads) for p in before[i]], set()
+            while todo:
+                state = todo.pop()
+                p, waited, left = state
+                if waited >= SGPR_WAIT or not left or state in seen:
+                    continue
+                seen.add(state)
+                by, args = code[p]
+                to = args.split(",")
+                if by.startswith("v_"):
+                    two = "_co_" in by or by.startswith(("v_div_scale", "v_mad_u64", "v_mad_i64"))
+                    if _scalars(",".join(to[:2 if two else 1])) & left:
+                        faults.append(f"{name}: '{op} {operands}' {waited} wait states behind "
+                                      f"'{by} {args}', not {SGPR_WAIT}")
+                        continue
+                elif by.startswith("s_") and not by.startswith(("s_cmp", "s_bitcmp", "s_wait", "s_nop")):
+                    written = _scalars(to[0])
+                    if "m0" in written & left and waited < M0_WAIT:
+                        faults.append(f"{name}: '{op} {operands}' {waited} wait states behind "
+                                      f"'{by} {args}', not {M0_WAIT}")
+                    left -= written
+                waited += int(args, 0) + 1 if by == "s_nop" else 1
+                todo += [(q, waited, left) for q in before[p]]
+    return faults
+
+
+def compile_library(arch: str = "gfx950",
+                    faults: list[str] | None = None) -> tuple[list[KernelUsage], str]:
+    """Compile the library into a temporary file; returns (kernels, diagnostics). ``faults`` takes
+    what wait_state_faults finds in the kernels' assembly."""
     if arch not in SUPPORTED_ARCHS:
         raise ValueError(f"unsupported arch {arch!r}: the kernels are written for {SUPPORTED_ARCHS}")
     with tempfile.TemporaryDirectory() as tmp:
-        jobs = _build.object_commands(Path(tmp),
-                                      extra=("-Rpass-analysis=kernel-resource-usage",))
+        jobs = _build.object_commands(Path(tmp), extra=(
+            "-Rpass-analysis=kernel-resource-usage",
+            *(() if faults is None else ("-save-temps=obj",))))
         procs = [subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
                  for _, cmd in jobs]
         results = [(p.returncode, err) for p in procs for _, err in [p.communicate()]]
+        for path in () if faults is None else sorted(Path(tmp).glob(f"*-amdgcn-*{arch}.s")):
+            faults += wait_state_faults(path.read_text())
     stderr = "\n".join(err or "" for _, err in results)
     diag = "\n".join(ln for ln in stderr.splitlines()
                      if "packed-fp32-ops" not in ln and "remark:" not in ln)
@@ -245,10 +343,12 @@ def main(argv: list[str] | None = None) -> int:
     parser.add_argument("--arch", default="gfx950", help="offload target (only gfx950)")
     parser.add_argument("--report", action="store_true", help="print every kernel's resource usage")
     parser.add_argument("--strict", action="store_true",
-                        help="fail if a default-tiling kernel spills to scratch")
+                        help="fail if a default-tiling kernel spills to scratch, or a wait state "
+                             "is missing")
     args = parser.parse_args(argv)
+    faults: list[str] = []
     try:
-        kernels, _ = compile_library(args.arch)
+        kernels, _ = compile_library(args.arch, faults if args.strict else None)
     except (ValueError, RuntimeError) as e:
         print(f"compile check FAILED: {e}", file=sys.stderr)
         return 1
@@ -257,7 +357,9 @@ def main(argv: list[str] | None = None) -> int:
         for k in kernels:
             print(f"{k.name[:58]:58s} {k.vgprs:5d} {k.agprs:5d} {k.scratch:7d} {k.occupancy:10d} {k.lds:7d}")
     spills, missing = spilling_defaults(kernels)
-    if args.strict and (spills or missing):
+    if args.strict and (spills or missing or faults):
+        for line in faults:
+            print(f"missing wait state: {line}", file=sys.stderr)
         for k in spills:
             print(f"default kernel spills {k.scratch} bytes/lane to scratch: {k.name}", file=sys.stderr)
         for name in missing:
