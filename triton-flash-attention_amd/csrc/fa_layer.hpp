@@ -215,6 +215,7 @@ struct CompactArgs {
   // the workspace, filled in by the launcher
   int* counts;            // [1], moves
   unsigned* bits;         // free pages
+  int* chunks;            // [pages / 1024 + 1], the free pages in front of each 1024, and all
   int* place;             // [pages], a moved page's place among the moves
 };
 int64_t compact_workspace_bytes(int64_t pages);

@@ -355,9 +355,16 @@ hipError_t launch_page_copy(const CopyArgs& args, hipStream_t stream) {
 // ---- compact ----------------------------------------------------------------------------
 // Pages that the list does not name as free are held: with `used` of them, the k-th held page from
 // place `used` on moves to the k-th free page in front of it. compact_mark_kernel marks the free
-// pages in a bitmap, compact_rank_kernel counts along it (every block for itself, over the words in
-// front of its own), compact_apply_kernel renumbers the table, the counts and the list;
-// compact_small_kernel does it all for a small cache.
+// pages in a bitmap, compact_rank_kernel counts along it, compact_apply_kernel renumbers the table,
+// the counts and the list; compact_small_kernel does it all for a small cache.
+//
+// Up to kCompactCounted pages each block of compact_rank_kernel counts the whole bitmap for itself,
+// which saves two launches; that work grows with the square of the pages, so in larger caches
+// compact_count_kernel counts it once, by chunks of 1024 pages, and compact_scan_kernel sums the counts.
+// (Half of the pages free, in any order: 2^19 pages 36 us without the counts and 39 with them, 2^20
+// 52 and 48, 2^22 259 and 131, 2^26 44600 and 1800.)
+constexpr int kChunk = 1024;  // pages of a chunk
+constexpr int kCompactCounted = 1 << 19;
 
 __global__ __launch_bounds__(256) void compact_mark_kernel(CompactArgs a) {
   const int start = a.free_start ? min(max(a.free_start[0], 0), a.F) : 0;
@@ -365,6 +372,34 @@ __global__ __launch_bounds__(256) void compact_mark_kernel(CompactArgs a) {
     const int p = a.free_pages[i];
     if (p >= 0 && p < a.pages) atomicOr(a.bits + (p >> 5), 1u << (p & 31));
   }
+}
+
+// Free pages of each chunk, 32 threads a chunk.
+__global__ __launch_bounds__(256) void compact_count_kernel(CompactArgs a) {
+  static_assert(kChunk == 32 * 32, "a word a thread");
+  const int w = blockIdx.x * 256 + threadIdx.x;
+  int n = w < (a.pages + 31) / 32 ? __popc(a.bits[w]) : 0;
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) n += __shfl_xor(n, i, 32);
+  if (w % 32 == 0 && w / 32 < (a.pages + kChunk - 1) / kChunk) a.chunks[w / 32] = n;
+}
+
+// Free pages of the chunks in front of each, and of all behind the last.
+__global__ __launch_bounds__(1024) void compact_scan_kernel(CompactArgs a) {
+  constexpr int W = 16, T = 64 * W;
+  __shared__ int sums[W][1];
+  const int tid = threadIdx.x, n = (a.pages + kChunk - 1) / kChunk;
+  const int per = (n + T - 1) / T, c0 = min(n, tid * per), c1 = min(n, c0 + per);
+  int x[1] = {0}, before[1], all[1];
+  for (int c = c0; c < c1; ++c) x[0] += a.chunks[c];
+  block_scan<W>(x, sums, before, all);
+  int front = before[0];
+  for (int c = c0; c < c1; ++c) {
+    const int here = a.chunks[c];
+    a.chunks[c] = front;
+    front += here;
+  }
+  if (tid == 0) a.chunks[n] = all[0];
 }
 
 // The bits of word w whose pages lie in front of page p.
@@ -380,30 +415,41 @@ __device__ __forceinline__ int compact_place(int p, int free_before, unsigned wo
 }
 
 // Block i: pages 1024 i to 1024 i + 1023, four a thread.
+template <bool COUNTED>
 __global__ __launch_bounds__(256) void compact_rank_kernel(CompactArgs a) {
   __shared__ int scratch[2][4], fronts[32];
   const int tid = threadIdx.x, words = (a.pages + 31) / 32;
   const int w0 = blockIdx.x * 32;
-  int all = 0, front = 0, moves = 0, low = 0;
-  // (the words behind the last page's, up to a multiple of 4, are cleared as well)
-  const u32x4* const bits4 = reinterpret_cast<const u32x4*>(a.bits);
+  int all = 0, front = 0, moves = 0, low = 0, used;  // moves: free pages in front of `used`
+  if constexpr (COUNTED) {
+    all = a.chunks[gridDim.x];
+    front = a.chunks[blockIdx.x];
+    used = a.pages - all;
+    const int c = used / kChunk, w = c * (kChunk / 32) + tid;  // of the chunk that `used` lies in
+    if (tid < kChunk / 32 && w < words) moves = __popc(a.bits[w] & bits_before(w, used));
+    block_sum_min(moves, low, scratch);
+    moves += a.chunks[c];
+  } else {
+    // (the words behind the last page's, up to a multiple of 4, are cleared as well)
+    const u32x4* const bits4 = reinterpret_cast<const u32x4*>(a.bits);
 #pragma unroll 4
-  for (int w = 4 * tid; w < words; w += 1024) {
-    const u32x4 m = bits4[w / 4];
-    const int n = __popc(m[0]) + __popc(m[1]) + __popc(m[2]) + __popc(m[3]);
-    all += n;
-    if (w < w0) front += n;  // w0 is a multiple of 4
-  }
-  block_sum_min(all, low, scratch);
-  block_sum_min(front, low, scratch);
-  const int used = a.pages - all;
+    for (int w = 4 * tid; w < words; w += 1024) {
+      const u32x4 m = bits4[w / 4];
+      const int n = __popc(m[0]) + __popc(m[1]) + __popc(m[2]) + __popc(m[3]);
+      all += n;
+      if (w < w0) front += n;  // w0 is a multiple of 4
+    }
+    block_sum_min(all, low, scratch);
+    block_sum_min(front, low, scratch);
+    used = a.pages - all;
 #pragma unroll 4
-  for (int w = 4 * tid; w < words && 32 * w < used; w += 1024) {
-    const u32x4 m = bits4[w / 4];
+    for (int w = 4 * tid; w < words && 32 * w < used; w += 1024) {
+      const u32x4 m = bits4[w / 4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) moves += __popc(m[i] & bits_before(w + i, used));
+      for (int i = 0; i < 4; ++i) moves += __popc(m[i] & bits_before(w + i, used));
+    }
+    block_sum_min(moves, low, scratch);
   }
-  block_sum_min(moves, low, scratch);  // free pages in front of `used`, held ones behind it
   if (blockIdx.x == 0 && tid == 0) {
     a.used[0] = used;
     a.counts[0] = moves;
@@ -515,7 +561,10 @@ __global__ __launch_bounds__(1024) void compact_small_kernel(CompactArgs a) {
 }
 
 static int64_t compact_words(int64_t pages) { return (pages + 127) / 128 * 4; }
-int64_t compact_workspace_bytes(int64_t pages) { return 4 * (4 + compact_words(pages) + pages); }
+static int64_t compact_chunks(int64_t pages) { return (pages + kChunk - 1) / kChunk; }
+int64_t compact_workspace_bytes(int64_t pages) {
+  return 4 * (4 + compact_words(pages) + compact_chunks(pages) + 1 + pages);
+}
 
 hipError_t launch_compact(const CompactArgs& args, void* workspace, hipStream_t stream) {
   CompactArgs a = args;
@@ -527,16 +576,29 @@ hipError_t launch_compact(const CompactArgs& args, void* workspace, hipStream_t 
   }
   a.counts = static_cast<int*>(workspace);
   a.bits = reinterpret_cast<unsigned*>(a.counts + 4);
-  a.place = reinterpret_cast<int*>(a.bits + words);
+  a.chunks = reinterpret_cast<int*>(a.bits + words);
+  a.place = a.chunks + compact_chunks(a.pages) + 1;
+  const bool counted = a.pages > kCompactCounted;
+  const dim3 block(256), chunks((unsigned)compact_chunks(a.pages));
   hipError_t e = zero_words(a.bits, words, stream);
   if (e != hipSuccess) return e;
   if (a.F > 0) {
-    const int64_t blocks = std::min<int64_t>(((int64_t)a.F + 255) / 256, 2048);
-    hipLaunchKernelGGL(compact_mark_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    const dim3 grid((unsigned)std::min<int64_t>(((int64_t)a.F + 255) / 256, 2048));
+    hipLaunchKernelGGL(compact_mark_kernel, grid, block, 0, stream, a);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(compact_rank_kernel, dim3((unsigned)((words + 31) / 32)), dim3(256), 0, stream, a);
+  if (counted) {
+    hipLaunchKernelGGL(compact_count_kernel, dim3((chunks.x + 7) / 8), block, 0, stream, a);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(compact_scan_kernel, dim3(1), dim3(1024), 0, stream, a);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(compact_rank_kernel<true>, chunks, block, 0, stream, a);
+  } else {
+    hipLaunchKernelGGL(compact_rank_kernel<false>, chunks, block, 0, stream, a);
+  }
   e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int64_t blocks = std::min<int64_t>((items + 255) / 256, 4096);

@@ -101,8 +101,9 @@ def _defaults() -> tuple[str, ...]:
                   for w in ("false", "true")]
         names += [f"fa::prefix_join_kernel<{d}, {e}, {w}>" for d in (32, 64, 128) for w in (4, 16)]
     names += [f"fa::{k}_kernel" for k in ("fork_small", "fork_count", "fork_finish", "page_copy",
-                                          "compact_small", "compact_mark", "compact_rank",
-                                          "compact_apply")]
+                                          "compact_small", "compact_mark", "compact_count",
+                                          "compact_scan", "compact_apply")]
+    names += [f"fa::compact_rank_kernel<{c}>" for c in ("false", "true")]
     names += ["fa::paged_plan_kernel<1>", "fa::paged_plan_kernel<2>"]
     names += [f"fa::paged_store_kernel<{w}>" for w in (32, 64, 128, 256)]
     names += [f"fa::{k}_kernel<128, false, 4, 32, {e}>" for k in ("dq", "dkdv")
