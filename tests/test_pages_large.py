@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from triton_flash_attention import paged_cache_compact
+from triton_flash_attention import paged_cache_compact, paged_cache_fork
 
 GPU = dict(device="cuda", dtype=torch.int32)
 
@@ -71,3 +71,49 @@ def test_compact_kernel_takes_no_time_that_grows_with_the_square():
     out = [torch.empty_like(t) for t in (table, names, shares)]
     copies = microseconds(lambda: [a.copy_(b) for a, b in zip(out, (table, names, shares))])
     assert microseconds(lambda: paged_cache_compact(table, names, shares, backend="triton")) < 100 * copies
+
+
+def rows(B, M, pages, parents, seed=0):
+    """Rows of any pages of which several may be the same, with counts that cover them."""
+    gen = torch.Generator("cuda").manual_seed(seed)
+    table = torch.randint(-1, pages, (B, M), generator=gen, **GPU)
+    lengths = torch.randint(0, 16 * M + 9, (B,), generator=gen, **GPU)
+    par = torch.randint(-1, B, (B,), generator=gen, **GPU)
+    if isinstance(parents, int):
+        par[:] = parents
+    elif parents is not None:  # neighbours with one parent, which one of them may be itself
+        n, which = parents
+        par = (torch.arange(B, **GPU) // n * n + which).clamp(max=B - 1)
+    shares = torch.randint(0, 40, (pages,), generator=gen, **GPU)
+    names = torch.randperm(pages, generator=gen, device="cuda").int()
+    return table, lengths, par, names, shares
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pages", [8000, 70000])
+@pytest.mark.parametrize(("B", "M", "parents"), [
+    (4096, 3, None), (4097, 3, None), (4097, 1500, 9), (30001, 2, None), (131071, 1, None), (131071, 2, 70000),
+    (20000, 2, -1), (5000, 2, (8, 0)), (5000, 2, (100, 37)), (5001, 2, (200, 150)), (5001, 2, (64, 64)),
+])
+def test_fork_kernel_of_many_rows(B, M, parents, pages):
+    outs = []
+    for backend in ("triton", "torch"):
+        table, lengths, par, names, shares = rows(B, M, pages, parents, seed=B + M)
+        fork = paged_cache_fork(table, lengths, par, names, shares, page_size=16,
+                                free_start=torch.tensor([pages // 2], **GPU), backend=backend)
+        outs.append(dict(fork._asdict(), table=table, names=names, shares=shares))
+    for name in outs[0]:
+        assert torch.equal(outs[0][name], outs[1][name]), name
+
+
+@pytest.mark.gpu
+def test_fork_kernel_takes_no_time_that_grows_with_the_square():
+    """16 times the rows in less than 32 times the time (78 times where each row looks through all
+    parents)."""
+    times = []
+    for B in (8191, 131071):
+        table, lengths, par, names, shares = rows(B, 1, 8000, None)
+        shares += 1 << 20
+        times.append(microseconds(lambda: paged_cache_fork(
+            table, lengths, par, names, shares, page_size=16, backend="triton")))
+    assert times[1] < 32 * times[0]

@@ -176,6 +176,7 @@ struct ForkArgs {
   // the workspace, and blocks a row, filled in by the launcher
   int* keeper;            // [B], the child that goes on in the row's begun page
   unsigned* bits;         // pages whose count fell below zero
+  int* children;          // [B], and [B] that say which comes first (fork_children_kernel)
   int* rows;              // [B, M], the new rows
   int parts;
 };

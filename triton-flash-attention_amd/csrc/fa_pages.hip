@@ -55,6 +55,11 @@ __device__ __forceinline__ void block_sum_min(int& sum, int& low, int (*scratch)
 // Counts do not depend on it. The released pages return in ascending order, so that the result does
 // not either: one block looks through the counts for them or, in a large cache, through a bitmap
 // that is marked beside the counts. What bounds it is the chain behind each launch.
+//
+// Up to kForkCounted rows each block of fork_count_kernel looks through all parents for its row's
+// children, which saves a launch; that work grows with the square of the rows, so for more of them
+// fork_children_kernel counts the children of all. (Rows of a page, any parents: 4096 rows 29 us without
+// the counts, 4097 30 with them, 8192 58 and 45, 32768 413 and 140, 131071 4520 and 521.)
 
 // A row's pages, and the tokens of the last one if it has begun (0: it is full).
 __device__ __forceinline__ int fork_held(const ForkArgs& a, int len, int* begun) {
@@ -65,18 +70,43 @@ __device__ __forceinline__ int fork_held(const ForkArgs& a, int len, int* begun)
 }
 __device__ __forceinline__ bool fork_page(const ForkArgs& a, int p) { return p >= 0 && p < a.pages; }
 
+// Each row's children, and the one that comes first: B + 1 for the row itself, B - x for child x, so
+// that the largest is the keeper and 0 stands for none. The first lane adds for all of its wave that
+// have the same parent, since atomics on one address follow one another: many rows with one parent are
+// the samples of a prompt.
+__global__ __launch_bounds__(256) void fork_children_kernel(ForkArgs a) {
+  const int x = blockIdx.x * 256 + threadIdx.x;
+  if (x >= a.B) return;
+  const int par = a.parents[x];
+  if (par < 0 || par >= a.B) return;
+  const bool same = par == __builtin_amdgcn_readfirstlane(par);
+  const int n = __popcll(__builtin_amdgcn_ballot_w64(same));
+  const bool itself = __builtin_amdgcn_ballot_w64(same && x == par) != 0;
+  const bool first = x == __builtin_amdgcn_readfirstlane(x);  // of those with a parent: of `same` too
+  if (same && !first) return;
+  atomicAdd(a.children + par, first ? n : 1);
+  atomicMax(a.children + a.B + par, (first ? itself : x == par) ? a.B + 1 : a.B - x);
+}
+
 // Block (b, y): part y of row b's columns.
+template <bool COUNTED>
 __global__ __launch_bounds__(256) void fork_count_kernel(ForkArgs a) {
   __shared__ int scratch[2][4];
   const int b = blockIdx.x, tid = threadIdx.x;
   int children = 0, keeper = INT32_MAX;
-  for (int x = tid; x < a.B; x += 256)
-    if (a.parents[x] == b) {
-      ++children;
-      keeper = min(keeper, x == b ? -1 : x);
-    }
-  block_sum_min(children, keeper, scratch);
-  if (keeper == -1) keeper = b;
+  if constexpr (COUNTED) {
+    children = a.children[b];
+    const int first = a.children[a.B + b];
+    if (first > 0) keeper = first > a.B ? b : a.B - first;
+  } else {
+    for (int x = tid; x < a.B; x += 256)
+      if (a.parents[x] == b) {
+        ++children;
+        keeper = min(keeper, x == b ? -1 : x);
+      }
+    block_sum_min(children, keeper, scratch);
+    if (keeper == -1) keeper = b;
+  }
   if (blockIdx.y == 0 && tid == 0) a.keeper[b] = keeper;
   const int step = (int)gridDim.y * 256;
   int begun;
@@ -216,6 +246,7 @@ __global__ __launch_bounds__(1024) void fork_finish_kernel(ForkArgs a) {
 // All of it in one block, where that has few entries to walk over.
 constexpr int kForkSmall = 1 << 13;  // most table entries
 constexpr int kForkRows = 1024;      // and rows, one a thread
+constexpr int kForkCounted = 1 << 12;
 
 __global__ __launch_bounds__(1024) void fork_small_kernel(ForkArgs a) {
   constexpr int W = 16, T = 64 * W;
@@ -281,7 +312,7 @@ __global__ __launch_bounds__(1024) void fork_small_kernel(ForkArgs a) {
 }
 
 int64_t fork_workspace_bytes(int64_t B, int64_t M, int64_t pages) {
-  return 4 * (B + (pages + 31) / 32 + B * M);
+  return 4 * (3 * B + (pages + 31) / 32 + B * M);
 }
 
 hipError_t launch_fork(const ForkArgs& args, void* workspace, hipStream_t stream) {
@@ -289,20 +320,33 @@ hipError_t launch_fork(const ForkArgs& args, void* workspace, hipStream_t stream
   const int64_t words = (a.pages + 31) / 32;
   a.keeper = static_cast<int*>(workspace);
   a.bits = reinterpret_cast<unsigned*>(a.keeper + a.B);
-  a.rows = reinterpret_cast<int*>(a.bits + words);
+  a.children = reinterpret_cast<int*>(a.bits + words);
+  a.rows = a.children + 2 * a.B;
   a.parts = std::min((a.M + 1023) / 1024, 16);  // four entries a thread, one
-  // A few counts a thread are read sooner than the bitmap is cleared by a launch of its own.
-  hipError_t e = hipSuccess;
   if (a.pages <= kForkPages && a.B <= kForkRows && (int64_t)a.B * a.M <= kForkSmall) {
     a.bits = nullptr;
     hipLaunchKernelGGL(fork_small_kernel, dim3(1), dim3(1024), 0, stream, a);
     return hipGetLastError();
   }
-  if (a.pages <= kForkPages) a.bits = nullptr;
-  else e = zero_words(a.bits, words, stream);
-  if (e != hipSuccess) return e;
+  // A few counts a thread are read sooner than the bitmap is cleared by a launch of its own.
+  const bool marked = a.pages > kForkPages, counted = a.B > kForkCounted;
+  hipError_t e = hipSuccess;
+  if (marked || counted) {
+    unsigned* const from = marked ? a.bits : reinterpret_cast<unsigned*>(a.children);
+    e = zero_words(from, (marked ? words : 0) + (counted ? 2 * (int64_t)a.B : 0), stream);
+    if (e != hipSuccess) return e;
+  }
+  if (!marked) a.bits = nullptr;
   if (a.B > 0) {
-    hipLaunchKernelGGL(fork_count_kernel, dim3((unsigned)a.B, (unsigned)a.parts), dim3(256), 0, stream, a);
+    const dim3 grid((unsigned)a.B, (unsigned)a.parts), block(256);
+    if (counted) {
+      hipLaunchKernelGGL(fork_children_kernel, dim3((unsigned)(a.B + 255) / 256), block, 0, stream, a);
+      e = hipGetLastError();
+      if (e != hipSuccess) return e;
+      hipLaunchKernelGGL(fork_count_kernel<true>, grid, block, 0, stream, a);
+    } else {
+      hipLaunchKernelGGL(fork_count_kernel<false>, grid, block, 0, stream, a);
+    }
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }

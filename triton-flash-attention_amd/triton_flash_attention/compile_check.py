@@ -100,10 +100,10 @@ def _defaults() -> tuple[str, ...]:
         names += [f"fa::prefix_fwd_kernel<{d}, {e}, {w}>" for d in (32, 64, 128)
                   for w in ("false", "true")]
         names += [f"fa::prefix_join_kernel<{d}, {e}, {w}>" for d in (32, 64, 128) for w in (4, 16)]
-    names += [f"fa::{k}_kernel" for k in ("fork_small", "fork_count", "fork_finish", "page_copy",
+    names += [f"fa::{k}_kernel" for k in ("fork_small", "fork_children", "fork_finish", "page_copy",
                                           "compact_small", "compact_mark", "compact_count",
                                           "compact_scan", "compact_apply")]
-    names += [f"fa::compact_rank_kernel<{c}>" for c in ("false", "true")]
+    names += [f"fa::{k}_kernel<{c}>" for k in ("fork_count", "compact_rank") for c in ("false", "true")]
     names += ["fa::paged_plan_kernel<1>", "fa::paged_plan_kernel<2>"]
     names += [f"fa::paged_store_kernel<{w}>" for w in (32, 64, 128, 256)]
     names += [f"fa::{k}_kernel<128, false, 4, 32, {e}>" for k in ("dq", "dkdv")
