@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+from test_prefix_work import Workspaces
 
 from triton_flash_attention import paged_cache_compact, paged_cache_fork
 
@@ -117,3 +118,29 @@ def test_fork_kernel_takes_no_time_that_grows_with_the_square():
         times.append(microseconds(lambda: paged_cache_fork(
             table, lengths, par, names, shares, page_size=16, backend="triton")))
     assert times[1] < 32 * times[0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize(("B", "pages"), [
+    (9, 500), (900, 8192), (1500, 8000), (1500, 8193), (37, 100001), (5000, 4000), (5000, 50000),
+])
+def test_pages_kernels_stay_inside_their_workspaces(B, pages, monkeypatch):
+    """Workspaces of exactly the bytes that the calls ask for, between guards."""
+    kept = Workspaces(monkeypatch)
+    table, lengths, par, names, shares = rows(B, 5, pages, None)
+    state = [t.clone() for t in (table, names, shares)]
+    got = paged_cache_fork(state[0], lengths, par, state[1], state[2], page_size=16, backend="triton")
+    kept.last()
+    want = paged_cache_fork(table, lengths, par, names, shares, page_size=16, backend="torch")
+    assert all(torch.equal(a, b) for a, b in zip((*got, *state), (*want, table, names, shares)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize(("B", "pages"), [(9, 500), (9, 14001), (900, 16000), (37, 100001), (5, 600001)])
+def test_compact_kernels_stay_inside_their_workspaces(B, pages, monkeypatch):
+    kept = Workspaces(monkeypatch)
+    table, names, shares = cache(pages, pages // 3, B, 5)
+    got = paged_cache_compact(table, names, shares, backend="triton")
+    kept.last()
+    want = paged_cache_compact(table, names, shares, backend="torch")
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
