@@ -477,13 +477,14 @@ int fa_paged_fwd_bf16(const fa_half_t* q, const fa_half_t* k_cache, const fa_hal
                       void* workspace, int64_t workspace_bytes, void* stream);
 
 /* The same where groups of sequences share a prefix, whose keys are read once for a group. Group g
- * holds the sequences group_starts[g] .. group_starts[g + 1] - 1 (G + 1 values that ascend within
- * [0, B]; otherwise all rows are NaN; sequences outside all groups share nothing). Its prefix is the
- * first prefix_lengths[g] keys of its first sequence, at most that sequence's length (none where
- * this is not in [0, M * S]): keys j below it lie in the pages of the first sequence for all the
- * group's sequences, the others in each one's own pages, and a sequence's own table entries in
- * front of them are not read (of a group of one all keys are its own). Which keys a query sees, and
- * the rows that are 0 or NaN, are as above. The workspace is needed for every call. */
+ * (G below 2^24) holds the sequences group_starts[g] .. group_starts[g + 1] - 1 (G + 1 values that
+ * ascend within [0, B]; otherwise all rows are NaN; sequences outside all groups share nothing).
+ * Its prefix is the first prefix_lengths[g] keys of its first sequence, at most that sequence's
+ * length (none where this is not in [0, M * S]): keys j below it lie in the pages of the first
+ * sequence for all the group's sequences, the others in each one's own pages, and a sequence's own
+ * table entries in front of them are not read (of a group of one all keys are its own). Which keys
+ * a query sees, and the rows that are 0 or NaN, are as above. The workspace is needed for every
+ * call. */
 int64_t fa_paged_prefix_fwd_workspace_bytes(int64_t B, int64_t G, int64_t Hq, int64_t Hkv, int64_t N,
                                             int64_t D, int64_t M, int64_t S);
 int fa_paged_prefix_fwd(const fa_half_t* q, const fa_half_t* k_cache, const fa_half_t* v_cache,

@@ -11,7 +11,7 @@ from test_paged import F32, HALF
 from test_prefix import make_shared, within
 from test_prefix_line import Line
 
-from triton_flash_attention import _native, _ops, paged_prefix_attention
+from triton_flash_attention import _lib, _native, _ops, paged_prefix_attention
 
 
 def ints(v):
@@ -214,3 +214,25 @@ def test_short_prefixes_stay_inside_their_workspaces(case, monkeypatch):
     got, want = places(kept.last(), Line(sizes, prefix, lengths, Hkv, Hq // Hkv * N, D, table.shape[1] * S))
     assert got == want and got[0][3] == 0
     within(o, *reference_on_gpu(q, dense, D ** -0.5, dtype), dtype)
+
+
+def test_too_many_groups_are_refused():
+    """A work-group looks through all groups, the empty ones too."""
+    size = _lib.load().fa_paged_prefix_fwd_workspace_bytes
+    assert size(2, (1 << 24) - 1, 4, 2, 1, 64, 100, 16) > 0
+    assert size(2, 1 << 24, 4, 2, 1, 64, 100, 16) == _lib.FA_ERR_TOO_LARGE
+    assert "too many" in _lib.last_error()
+
+
+@pytest.mark.gpu
+def test_too_many_groups_run_in_pytorch():
+    views, table, _, dense = make_shared([2], [20], [40, 33], 2, 16, 32, F16, device="cuda", fill=0.0)
+    q = torch.randn(2, 4, 1, 32, generator=torch.Generator().manual_seed(1)).half().cuda()
+    starts = torch.zeros((1 << 24) + 1, dtype=torch.int32, device="cuda")
+    starts[-1] = 2
+    prefix = torch.full((1 << 24,), 20, dtype=torch.int32, device="cuda")
+    args = (q, *views, table, ints([40, 33]), starts, prefix)
+    with pytest.raises(RuntimeError, match="too many"):
+        paged_prefix_attention(*args, enable_gqa=True, backend="triton")
+    within(paged_prefix_attention(*args, enable_gqa=True),
+           *reference_on_gpu(q, dense, 32 ** -0.5, F16), F16)

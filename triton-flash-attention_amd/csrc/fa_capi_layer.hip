@@ -345,8 +345,9 @@ int check_prefix(const char* name, int64_t B, int64_t G, int64_t Hq, int64_t Hkv
   if (G < 0) return capi_fail(FA_ERR_BAD_SHAPE, "%s: G must not be negative", name);
   const int64_t R = Hq / Hkv * N;
   // Rows that read a head and units of the line are counted in 32 bits; two rows or more of the
-  // output are a block of the join, whose grid's threads are too.
-  if (G >= (int64_t)1 << 30 || R >= (int64_t)1 << 25 || B * Hkv * R > 2 * fa::kMostBlocks ||
+  // output are a block of the join, whose grid's threads are too. Every work-group looks through all
+  // groups, which takes 20 ms for 2^20 of them, however empty.
+  if (G >= (int64_t)1 << 24 || R >= (int64_t)1 << 25 || B * Hkv * R > 2 * fa::kMostBlocks ||
       fa::prefix_sizes(B, G, Hkv, R, D, M * S).units >= (double)((int64_t)1 << 30))
     return capi_fail(FA_ERR_TOO_LARGE,
                      "%s: %lld sequences of up to %lld keys in %lld groups are too many for one call",

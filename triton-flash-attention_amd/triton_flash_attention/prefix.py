@@ -102,7 +102,7 @@ def paged_prefix_attention(
     infinity in the values of a prefix's token reaches all rows of its group, also those of a
     sequence that is shorter.
 
-    The gfx950 kernels serve what those of ``paged_attention`` serve. They work on tiles of 128
+    The gfx950 kernels serve what those of ``paged_attention`` serve, in up to 2^24 groups. They work on tiles of 128
     of the rows that share a prefix and a key/value head; for sequences that share nothing
     ``paged_attention`` is faster, which has less to find out first. They have no backward.
     """
@@ -125,7 +125,7 @@ def paged_prefix_attention(
     tiles = B * H * -(-rows // (_OWN_TILE if rows <= _OWN_ROWS else _TILE))
     if G > 0 and B > 1:
         tiles += H * (B * rows // _TILE + min(G, B // 2))
-    too_many = Hq >= 1 << 20 or N >= 1 << 20 or G >= 1 << 30 or B * Hq * N >= 1 << 24 or (
+    too_many = Hq >= 1 << 20 or N >= 1 << 20 or G >= 1 << 24 or B * Hq * N >= 1 << 24 or (
         tiles * (-(-page_table.shape[1] * S // 32) + 24) >= 1 << 30)
     reason, served = _attention_reason(backend, query, key_cache, value_cache, softmax_scale, too_many)
     if _falls_back(backend, reason):
