@@ -259,12 +259,17 @@ struct PrefixGroup {
 };
 constexpr int kPrefixTile = 128;   // query rows of a tile
 constexpr int kPrefixLead = 6;     // empty units in front of a triple on the line
-constexpr int kPrefixStretch = 4;  // least units of a work-group
+// Least units of a work-group. (4 beams over 512 shared keys, Hq32 Hkv8 D128: 16.4 us, with 2 16.9, with 8
+// 17.6.)
+constexpr int kPrefixStretch = 4;
 // Groups (fewer) and sequences whose lengths and starts a work-group keeps in LDS.
 constexpr int kPrefixKeptGroups = 1024, kPrefixKeptSeqs = 2048;
-constexpr int kOwnRows = 64;       // most rows of a sequence whose own keys are a wave's work,
-constexpr int kOwnTile = 32;       // the rows of a tile there,
-constexpr int kOwnLead = 1;        // and the empty units in front of them
+// Most rows of a sequence whose own keys are a wave's work, the rows of a tile there, and the empty units
+// in front of a triple. (From 33 rows on the keys are read once a tile; the other way is a work-group for
+// up to 128 rows. Which is faster goes by the keys, Hkv4 D128 bf16, this and the other: 100 sequences of
+// 48 rows and up to 100 keys of their own 79 us and 85; 24 of 40 rows and 300 keys 44 and 43; 32 of 40 rows
+// and 2000 keys 54 and 40; 24 of 72 rows and 300 keys 57 and 60, 32 of 72 and 2000 keys 75 and 48.)
+constexpr int kOwnRows = 64, kOwnTile = 32, kOwnLead = 1;
 inline __host__ __device__ int prefix_tiles(int64_t sequences, int64_t R) {
   return (int)((sequences * R + kPrefixTile - 1) / kPrefixTile);
 }

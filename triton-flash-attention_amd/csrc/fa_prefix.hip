@@ -123,7 +123,9 @@ __device__ __forceinline__ bool prefix_long(int units, int L) {
 }
 
 // A wave's stretch of the sequences' own keys, where a work-group's is L: four waves take five units
-// of them in the time that it takes for four of a prefix.
+// of them in the time that it takes for four of a prefix. (Hq32 Hkv8 D128 bf16; 64 sequences over 4096
+// shared keys, 8 groups of 8 with up to 2000 keys of their own: 43.7 and 100 us; 4 for 4 43.7 and 98; 6 for
+// 4 45.5 and 101. Of 5 tokens and 8192 shared keys: 44.4, 44.5 and 43.7.)
 __device__ __forceinline__ int own_stretch(int L) { return max((5 * L + 15) / 16, 2); }
 
 // The work-group's place, or the wave's. `lds`: the work-group's memory, free before and after.
@@ -217,8 +219,9 @@ __device__ __forceinline__ PrefixLine prefix_find(const PrefixArgs& a, int* lds,
   const int own_cost = WAVES ? own_all[0] - own_all[0] / 5 : own_all[0];
   const int L = max((all[1] + own_cost + room - 1) / room, kPrefixStretch);
   // Long prefixes are cut by the work-groups that the line leaves: of all[3] units in all, a triple
-  // of u into the whole part of u / all[3] of those. Where the grid would not hold the pieces, they
-  // stay on the line.
+  // of u into the whole part of u / all[3] of those, but of 16 units at least. (32 sequences, Hq32 Hkv8 D128,
+  // four groups over 2048 keys each, or 40 over 8192: 35.5 and 32 us; of 8 at least 36 and 34, of 32 41 and
+  // 36.) Where the grid would not hold the pieces, they stay on the line.
   const bool any = all[1] > 0;
   bool cut = any;
   int budget = 0;
@@ -1262,8 +1265,9 @@ PrefixSizes prefix_sizes(int64_t B, int64_t G, int64_t Hkv, int64_t R, int64_t D
   // hold; as many on each XCD.
   z.grid = (int)std::min((double)most, std::ceil(z.units / kPrefixStretch));
   z.grid = std::max((z.grid + 7) / 8 * 8, 16);
-  // Where all rows fit one tile memory bounds a prefix, and a piece's partial is worth four units of
-  // it: no more pieces than it takes to keep the memory busy.
+  // Where all rows fit one tile memory bounds a prefix, and 256 pieces keep it busy. (4 sequences over
+  // 65536 and 262144 keys, Hq32 Hkv8 D128: 58 and 197 us; 128 pieces 77 and 263; 512, with twice the
+  // partials, 56 and 198.)
   z.most_pieces = B * R <= kPrefixTile ? std::min(z.grid, 256) : z.grid;
   z.pslots = triples > 0 ? z.grid + triples : 0;
   z.head_bytes = (64 + B * (int64_t)sizeof(PrefixSeq) + G * (int64_t)sizeof(PrefixGroup) + 63) / 64 * 64;
@@ -1273,6 +1277,8 @@ PrefixSizes prefix_sizes(int64_t B, int64_t G, int64_t Hkv, int64_t R, int64_t D
 }
 
 // Few rows have many pieces and are joined by more waves each; with many rows the waves are enough.
+// (Whole calls over 4096 shared keys, Hq32 Hkv8 D128: 128 waves of rows 20.0 us with sixteen for each and
+// 21.7 with four; 256 23.1 and 24.6; 384 27.9 and 26.5.)
 template <int D, class E, int SPLIT>
 hipError_t prefix_join_start(const PrefixArgs& a, hipStream_t stream) {
   constexpr int W = SPLIT < 4 ? 4 : SPLIT;

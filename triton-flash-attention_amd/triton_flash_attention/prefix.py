@@ -102,9 +102,13 @@ def paged_prefix_attention(
     infinity in the values of a prefix's token reaches all rows of its group, also those of a
     sequence that is shorter.
 
-    The gfx950 kernels serve what those of ``paged_attention`` serve, in up to 2^24 groups. They work on tiles of 128
-    of the rows that share a prefix and a key/value head; for sequences that share nothing
-    ``paged_attention`` is faster, which has less to find out first. They have no backward.
+    The gfx950 kernels serve what those of ``paged_attention`` serve, in fewer than 2^24 groups, and
+    have no backward. They work on tiles of 128 of the rows that share a prefix and a key/value head,
+    and take about 15 us before the keys count. Where the rows of ``page_table`` name the shared pages
+    themselves (as forks leave them), ``paged_attention`` gives the same rows, and sooner for short
+    prefixes: with 32 query heads on 8 and D = 128, up to some 1000 shared keys (6 us against 16 at
+    128), 2000 for four sequences or less; over 8192 keys 32 sequences take 33 us here and 85 there.
+    For sequences that share nothing ``paged_attention`` is faster as well.
     """
     native = _binding(backend)
     if native is not None and not _forward_ad_active():
