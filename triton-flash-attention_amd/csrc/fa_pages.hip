@@ -245,9 +245,10 @@ __global__ __launch_bounds__(1024) void fork_finish_kernel(ForkArgs a) {
   fork_release(a, start, copies, found);
 }
 
-// All of it in one block, where that has few entries to walk over. (Rows x pages, one launch and more:
-// 64 x 16 6.5 us and 9.7, 64 x 64 10.5 and 11.3, 1024 x 2 9.3 and 13.0; 64 x 128 13.6 and 11.3.)
-constexpr int kForkSmall = 1 << 12;  // most table entries
+// All of it in one block, where that has few entries to walk over. (One launch and two: 64 rows of beams,
+// 17 to 1100 tokens in tables of 70 pages, 6.9 us and 9.6. Rows x pages, the tables more than half full:
+// 64 x 16 6.5 and 9.7, 64 x 64 10.5 and 11.3, 1024 x 2 9.3 and 13.0; 64 x 128 13.6 and 11.3.)
+constexpr int kForkSmall = 1 << 13;  // most table entries
 constexpr int kForkRows = 1024;      // and rows, one a thread
 constexpr int kForkCounted = 1 << 12;
 
