@@ -246,7 +246,7 @@ __global__ __launch_bounds__(1024) void fork_finish_kernel(ForkArgs a) {
 }
 
 // All of it in one block, where that has few entries to walk over. (One launch and two: 64 rows of beams,
-// 17 to 1100 tokens in tables of 70 pages, 6.9 us and 9.6. Rows x pages, the tables more than half full:
+// 112 to 1086 tokens in tables of 68 pages, 6.8 us and 9.6. Rows x pages, three quarters full:
 // 64 x 16 6.5 and 9.7, 64 x 64 10.5 and 11.3, 1024 x 2 9.3 and 13.0; 64 x 128 13.6 and 11.3.)
 constexpr int kForkSmall = 1 << 13;  // most table entries
 constexpr int kForkRows = 1024;      // and rows, one a thread

@@ -38,7 +38,7 @@ namespace fa {
 // neighbouring work-groups of one XCD, whose L2 then reads the keys once for all of them.
 //
 // Measured (Hq32 Hkv8 D128): 64 sequences over 4096 shared keys and up to 1024 of their own, bf16, 154 MB:
-// 37 us and 7 for the join; 128 sequences over 32768 shared keys, fp16, 70 GFLOP: 114-146 and 11. About 6 us
+// 37 us and 7 for the join; 128 sequences over 32768 shared keys, fp16, 70 GFLOP: 114-160 and 12. About 6 us
 // go into finding the work and 5 until the first keys arrive.
 constexpr int kPrefixWaves = 4;
 

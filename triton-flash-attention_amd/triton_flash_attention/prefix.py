@@ -107,8 +107,8 @@ def paged_prefix_attention(
     and take about 15 us before the keys count. Where the rows of ``page_table`` name the shared pages
     themselves (as forks leave them), ``paged_attention`` gives the same rows, and sooner for short
     prefixes: with 32 query heads on 8 and D = 128, up to some 1000 shared keys (6 us against 16 at
-    128), 2000 for four sequences or less; over 8192 keys 32 sequences take 33 us here and 85 there.
-    For sequences that share nothing ``paged_attention`` is faster as well.
+    128), 2000 for four sequences and 8000 for two; over 8192 keys 32 sequences take 33 us here and
+    84 there. For sequences that share nothing ``paged_attention`` is faster as well.
     """
     native = _binding(backend)
     if native is not None and not _forward_ad_active():
