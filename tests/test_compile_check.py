@@ -134,3 +134,9 @@ def test_missing_wait_states_are_found(first, second, found):
     assert len(faults) == len(found)
     for word in found:
         assert any(word in f.split("behind")[1] for f in faults), faults
+
+
+def test_memory_instructions_without_operands_are_read():
+    """Cache maintenance between a write of M0 and the load is one wait state; it reads nothing."""
+    text = ASSEMBLY.format(first="buffer_inv", second="buffer_wbl2")
+    assert compile_check.wait_state_faults(text) == []

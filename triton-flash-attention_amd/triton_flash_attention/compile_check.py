@@ -276,7 +276,7 @@ def wait_state_faults(assembly: str) -> list[str]:
             if not op.startswith(("buffer_", "global_", "scratch_", "flat_")):
                 continue
             reads = _scalars(operands)
-            if operands.split()[-1] == "lds":
+            if operands.endswith(" lds"):
                 reads |= {"m0"}
             todo, seen = [(p, 0, reads) for p in before[i]], set()
             while todo:
